@@ -15,6 +15,7 @@ LIBRARY = Path(__file__).resolve().parent / "libcxlsparse_b200.so"
 OK, ERR_INVALID, ERR_CUDA, ERR_CAPACITY, ERR_REGISTRATION, ERR_UNSUPPORTED = range(6)
 # Device error word bits.
 DEVICE_ERR_READY_TIMEOUT, DEVICE_ERR_COPY_TIMEOUT, DEVICE_ERR_BAD_BLOCK = 1, 2, 4
+DEVICE_ERR_BAD_LENGTH = 8
 ORDER_PHYSICAL, ORDER_DEPTH, ORDER_DEPTH_SHARED = 0, 1, 2
 READ_ORDERS = {
     "physical": ORDER_PHYSICAL,
@@ -90,6 +91,31 @@ class AttendBuffers(ctypes.Structure):
     _fields_ = [(name, c_vp) for name in ATTEND_BUFFER_FIELDS]
 
 
+class CacheCall(ctypes.Structure):
+    _fields_ = [(name, c_vp) for name in (
+        "codes", "scales", "table", "lengths", "offsets", "error")] + [
+        ("table_stride", c_i64)] + [(name, c_i32) for name in (
+            "pages", "kv_heads", "dim", "page_size", "format", "users", "width", "tokens",
+            "max_tokens", "type")]
+
+
+class CacheAttendCall(ctypes.Structure):
+    _fields_ = [("cache", CacheCall)] + [(name, c_vp) for name in (
+        "query", "out", "lse", "workspace")] + [(name, c_i64) for name in (
+            "workspace_bytes", "q_token_stride", "q_head_stride")] + [
+        (name, c_i32) for name in ("heads", "causal", "window")] + [("scale", ctypes.c_float)]
+
+
+class RotaryCall(ctypes.Structure):
+    _fields_ = [(name, c_vp) for name in (
+        "q", "k", "q_out", "k_out", "positions", "steps")] + [(name, c_i64) for name in (
+            "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+            "q_out_token_stride", "q_out_head_stride", "k_out_token_stride",
+            "k_out_head_stride")] + [(name, c_i32) for name in (
+                "tokens", "heads", "kv_heads", "dim", "rotary_dim", "layout", "type",
+                "transpose", "wide_positions")] + [("magnitude", ctypes.c_float)]
+
+
 _lib = None
 
 
@@ -159,6 +185,13 @@ def lib():
             "cxs_ipc_close": (c_i32, [c_vp]),
             "cxs_exchange_barrier": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_vp,
                                              c_vp]),
+            "cxs_cache_append": (c_i32, [ctypes.POINTER(CacheCall), c_vp, c_i64, c_i64, c_vp,
+                                         c_i64, c_i64, c_vp]),
+            "cxs_cache_read": (c_i32, [ctypes.POINTER(CacheCall), c_vp, c_vp, c_vp]),
+            "cxs_cache_attend": (c_i32, [ctypes.POINTER(CacheAttendCall), c_vp]),
+            "cxs_cache_attend_workspace": (c_i32, [ctypes.POINTER(CacheAttendCall),
+                                                   ctypes.POINTER(c_i64)]),
+            "cxs_rotary": (c_i32, [ctypes.POINTER(RotaryCall), c_vp]),
         }
         for name, (restype, argtypes) in sigs.items():
             fn = getattr(handle, name)
@@ -200,4 +233,5 @@ def exported_symbols():
             "cxs_qkv_rope", "cxs_qkv_rope_segments", "cxs_silu_mul", "cxs_compress_windows",
             "cxs_device_alloc",
             "cxs_device_free", "cxs_ipc_get_handle", "cxs_ipc_open_handle", "cxs_ipc_close",
-            "cxs_exchange_barrier")
+            "cxs_exchange_barrier", "cxs_cache_append", "cxs_cache_read", "cxs_cache_attend",
+            "cxs_cache_attend_workspace", "cxs_rotary")

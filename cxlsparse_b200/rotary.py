@@ -1,0 +1,148 @@
+"""Rotary positions over the C ABI (``cxs_rotary``).
+
+The glue kernel of the extend model rotates whole bf16 heads of 64 in the half
+layout. ``Rotary`` covers the other forms: interleaved pairs, part of the
+head, frequencies scaled for long contexts, bf16 / fp16 / fp32, strided and
+in-place tensors, and the transposed rotation, which is the gradient. The
+reference has only the first form (models/tensor_ops.py:14-26).
+"""
+
+import math
+
+import torch
+
+from . import _lib
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def frequencies(rotary_dim, theta=10000.0, scaling=None):
+    """Radians per position of every channel pair (fp64, on the CPU) and the
+    factor on the rotated values. ``scaling``:
+
+    - None: theta ** (-2 i / rotary_dim);
+    - ``dict(type="linear", factor=s)``: positions divided by s;
+    - ``dict(type="ntk", factor=s)``: theta raised so that the slowest pair is
+      stretched s times and the fastest is kept;
+    - ``dict(type="yarn", factor=s, original=n, fast=32, slow=1)`` (Peng et al.
+      2023): pairs that make fewer than ``slow`` turns over ``n`` positions are
+      stretched s times, those with more than ``fast`` are kept, a linear ramp
+      over the pair index between; values times 0.1 ln(s) + 1 (or ``magnitude``).
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even")
+    if not theta > 1:
+        raise ValueError("theta must be above 1")
+    scaling = dict(scaling or {"type": "none"})
+    kind = scaling.pop("type", None)
+    fields = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+              "yarn": ("factor", "original", "fast", "slow", "magnitude")}
+    if kind not in fields:
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    unknown = set(scaling) - set(fields[kind])
+    if unknown:
+        raise ValueError(f"unknown fields of rotary scaling {kind!r}: {sorted(unknown)}")
+    factor = float(scaling.get("factor", 1.0))
+    if not factor > 0:
+        raise ValueError("the scaling factor must be positive")
+    if kind == "ntk" and rotary_dim > 2:
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    index = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    f = theta ** (-index / rotary_dim)
+    if kind == "linear":
+        return f / factor, 1.0
+    if kind == "yarn":
+        if "original" not in scaling or not scaling["original"] > 0:
+            raise ValueError("yarn scaling needs the original context length")
+        original = scaling["original"]
+
+        def pair(turns):  # the pair index that makes `turns` turns over `original` positions
+            return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low = max(0, math.floor(pair(scaling.get("fast", 32))))
+        high = min(rotary_dim - 1, math.ceil(pair(scaling.get("slow", 1))))
+        ramp = ((index / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+        magnitude = scaling.get("magnitude", 0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
+        return f / factor * ramp + f * (1 - ramp), float(magnitude)
+    return f, 1.0
+
+
+class Rotary:
+    """The rotation of one head geometry: ``apply(q, k, positions)``.
+
+    ``steps`` holds each pair's turns per position as a 64-bit fraction, so a
+    phase is exact at any position before its sine and cosine are taken."""
+
+    def __init__(self, dim, *, rotary_dim=None, theta=10000.0, layout="half", scaling=None,
+                 device="cuda"):
+        rotary_dim = dim if rotary_dim is None else rotary_dim
+        if dim < 2 or dim % 2 or dim > 512:
+            raise ValueError("dim must be even and at most 512")
+        if rotary_dim > dim:
+            raise ValueError("rotary_dim must be at most dim")
+        if layout not in LAYOUTS:
+            raise ValueError(f"unknown rotary layout {layout!r}")
+        self.dim, self.rotary_dim, self.layout = dim, rotary_dim, layout
+        f, self.magnitude = frequencies(rotary_dim, theta, scaling)
+        # Fractions of 2^62 doubled twice: a full turn per position stays in
+        # range, and the product with a position wraps modulo one turn.
+        steps = (f / (2 * math.pi) * 2.0 ** 62).round().to(torch.int64) << 2
+        self.steps = steps.to(device)
+
+    def _check(self, name, x, like=None):
+        if x.ndim != 3 or x.shape[-1] != self.dim or x.stride(-1) != 1:
+            raise ValueError(f"{name} must be [tokens, heads, {self.dim}] with contiguous channels")
+        if x.dtype not in TYPES:
+            raise ValueError(f"{name} must be bf16, fp16 or fp32")
+        if x.device != self.steps.device:
+            raise ValueError(f"{name} must be on {self.steps.device}")
+        if like is not None and x.dtype != like.dtype:
+            raise ValueError(f"{name} must have the type of the other tensor")
+
+    def apply(self, q, k, positions, *, transpose=False, out=None):
+        """Rotated ``(q, k)`` for q [tokens, heads, dim], k [tokens, kv_heads,
+        dim] (either may be None) and positions [tokens] int32 or int64, in one
+        launch on the current stream. ``transpose`` turns the other way: given
+        the gradients of the outputs it returns those of the inputs (and, for
+        magnitude 1, undoes the rotation). ``out=(q_out, k_out)`` receives the
+        result and may be the inputs themselves."""
+        first = q if q is not None else k
+        if first is None:
+            raise ValueError("q or k is needed")
+        for name, x in (("q", q), ("k", k)):
+            if x is not None:
+                self._check(name, x, first)
+        tokens = len(first)
+        if (k is not None and len(k) != tokens) or positions.shape != (tokens,):
+            raise ValueError("q, k and positions must have as many tokens")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != first.device:
+            raise ValueError("positions must be int32 or int64 on the device of q and k")
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        if out is None:
+            q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        else:
+            q_out, k_out = out
+            for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+                if (x is None) != (y is None):
+                    raise ValueError(f"out must have a tensor for {name} exactly when {name} is given")
+                if y is not None:
+                    self._check(f"out of {name}", y, first)
+                    if y.shape != x.shape:
+                        raise ValueError(f"out of {name} must have its shape")
+        qs = (0, 0, 0) if q is None else q.stride()
+        ks = (0, 0, 0) if k is None else k.stride()
+        qo = (0, 0, 0) if q is None else q_out.stride()
+        ko = (0, 0, 0) if k is None else k_out.stride()
+        call = _lib.RotaryCall(
+            _lib.ptr(q), _lib.ptr(k), _lib.ptr(q_out), _lib.ptr(k_out), positions.data_ptr(),
+            self.steps.data_ptr(), qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1],
+            tokens, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], self.dim,
+            self.rotary_dim, LAYOUTS[self.layout], TYPES[first.dtype], int(bool(transpose)),
+            int(positions.dtype == torch.int64), self.magnitude)
+        with torch.cuda.device(first.device):
+            _lib.check(_lib.lib().cxs_rotary(
+                call, torch.cuda.current_stream(first.device).cuda_stream))
+        return q_out, k_out

@@ -475,6 +475,129 @@ int cxs_compress_windows(const void* records, const int64_t* rows, int32_t windo
 /* out[r, c] = bf16(silu(gate_up[r, c])) * gate_up[r, ffn + c] (SwiGLU). */
 int cxs_silu_mul(const void* gate_up, int32_t rows, int32_t ffn, void* out, void* stream);
 
+/* --------------------------------------------- dense 8-bit cache (HBM) ---
+ * No counterpart in the reference, whose history lives in 16 bits in the
+ * backing pool. A user's whole history is kept in HBM at 8 bits a channel:
+ * half the bytes of a bf16 replica, read by dense attention (decode steps and
+ * suffixes) and brought back to 16 bits where another branch needs records.
+ *
+ * One layer's cache is codes [pages, kv_heads, 2 (K, V), page_size, dim], one
+ * byte each, and scales [pages, kv_heads, 2] fp32: a value is code * scale.
+ * Token t of user b lies in page table[b, t / page_size], slot t % page_size;
+ * pages of different users may be shared for reading.
+ *
+ * New tokens are packed rows: user b's are rows offsets[b] .. offsets[b + 1]
+ * and its last tokens, at positions lengths[b] - new[b] .. lengths[b] - 1
+ * (lengths counts them). offsets == NULL: one new token for every user.
+ *
+ * What the device finds wrong is reported in `error` (bits, never cleared by
+ * the calls) and skipped: CXS_DEVICE_ERR_BAD_BLOCK for a page id outside
+ * [0, pages), CXS_DEVICE_ERR_BAD_LENGTH for lengths or offsets that reach
+ * past the table, the packed rows or max_tokens.
+ */
+#define CXS_DEVICE_ERR_BAD_LENGTH 8
+
+enum cxs_type { CXS_TYPE_BF16 = 0, CXS_TYPE_F16 = 1, CXS_TYPE_F32 = 2 };
+enum cxs_cache_format {
+  CXS_FORMAT_E4M3 = 0, /* 8-bit floats (4 exponent, 3 mantissa bits), largest 448 */
+  CXS_FORMAT_INT8 = 1  /* integers -127 .. 127 */
+};
+enum cxs_rotary_layout {
+  CXS_ROTARY_HALF = 0,       /* pair i is channels (i, i + rotary_dim / 2) */
+  CXS_ROTARY_INTERLEAVED = 1 /* pair i is channels (2 i, 2 i + 1) */
+};
+
+typedef struct cxs_cache_call {
+  void* codes;             /* [pages, kv_heads, 2, page_size, dim], 16-byte aligned */
+  float* scales;           /* [pages, kv_heads, 2] */
+  const int32_t* table;    /* [users, width], rows table_stride apart */
+  const int32_t* lengths;  /* [users] tokens, the new ones included (read: first position) */
+  const int32_t* offsets;  /* [users + 1] packed rows of each user, or NULL */
+  int32_t* error;          /* device error word, or NULL */
+  int64_t table_stride;
+  int32_t pages, kv_heads, dim, page_size; /* dim 64 or 128; page_size 16, 32 or 64 */
+  int32_t format;          /* CXS_FORMAT_* */
+  int32_t users, width;
+  int32_t tokens;          /* packed rows */
+  int32_t max_tokens;      /* most rows of one user (bounds the launch) */
+  int32_t type;            /* CXS_TYPE_* of the 16- or 32-bit side */
+} cxs_cache_call;
+
+/* Quantise the new tokens' keys and values [tokens, kv_heads, dim] (channels
+ * contiguous, strides in elements) into their pages. For each page that gets
+ * new tokens, head and part, with A the largest finite magnitude among that
+ * page's new tokens and Q the format's largest code:
+ *   s = max(A * fl(1 / Q), 2^-64, the page's scale if it holds older tokens),
+ *   code = x * fl(1 / s) saturated to +-Q and rounded to nearest even,
+ * and, where s exceeds the older scale, older codes c become c * fl(old / s)
+ * rounded again. All in fp32. Infinities saturate; NaN is kept by e4m3 and
+ * becomes 0 in int8. Slots past lengths[b] keep their bytes. A page that gets
+ * new tokens must belong to one user only. */
+int cxs_cache_append(const cxs_cache_call* call, const void* k, int64_t k_token_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                     int64_t v_head_stride, void* stream);
+
+/* Values code * scale of consecutive tokens of each user, rounded once to
+ * `type`, into k and v [tokens, kv_heads, dim] (contiguous): row offsets[b] + i
+ * is position lengths[b] + i (lengths holds the first position here). Tokens
+ * of a page that is not there come back as 0, with the error bit. */
+int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream);
+
+/* Attention of the new tokens' queries [tokens, heads, dim] (bf16 or fp16,
+ * channels contiguous, strides in elements; query head h reads KV head
+ * h / (heads / kv_heads)) over the cached tokens of their user:
+ *   out = softmax(scale * q . k over the visible tokens) . v   [tokens, heads, dim]
+ *   lse = log of the softmax's sum (natural, fp32), or NULL    [tokens, heads]
+ * The row at position p sees positions <= p (causal) or < lengths[b], and with
+ * window > 0 only positions > p - window. A row that sees nothing gets out = 0
+ * and lse = -infinity. Bytes of slots past lengths[b], and pages not in the
+ * table's used part, are never part of a result, whatever they hold. Scales
+ * below 2^-64 count as 2^-64. */
+typedef struct cxs_cache_attend_call {
+  cxs_cache_call cache;
+  const void* query;
+  void* out;
+  float* lse;
+  void* workspace;         /* cxs_cache_attend_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t q_token_stride, q_head_stride;
+  int32_t heads;
+  int32_t causal;
+  int32_t window;          /* 0: no window */
+  float scale;
+} cxs_cache_attend_call;
+int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream);
+/* Scratch bytes of a cxs_cache_attend call (pointers are not looked at). The
+ * scratch needs no initialisation and keeps nothing between calls; calls that
+ * may overlap need their own. */
+int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes);
+
+/* Rotary positions of queries and keys in one launch. Pair i of a head at
+ * position p turns by the angle p * f_i:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin),
+ * channels from rotary_dim on are copied. transpose = 1 turns the other way,
+ * which is the gradient. steps[i] = f_i / (2 pi) as a 64-bit fraction of a
+ * turn (modulo 2^64), so the phase of any position is exact before its sine
+ * and cosine are taken in fp32. Outputs may be the inputs. */
+typedef struct cxs_rotary_call {
+  const void* q;             /* [tokens, heads, dim], channels contiguous, or NULL */
+  const void* k;             /* [tokens, kv_heads, dim], or NULL */
+  void* q_out;
+  void* k_out;
+  const void* positions;     /* [tokens] int32, or int64 when wide_positions */
+  const int64_t* steps;      /* [rotary_dim / 2] */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  int32_t tokens, heads, kv_heads, dim; /* dim even, at most 512 */
+  int32_t rotary_dim;        /* even, 2 .. dim */
+  int32_t layout;            /* CXS_ROTARY_* */
+  int32_t type;              /* CXS_TYPE_* */
+  int32_t transpose;
+  int32_t wide_positions;
+  float magnitude;
+} cxs_rotary_call;
+int cxs_rotary(const cxs_rotary_call* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
