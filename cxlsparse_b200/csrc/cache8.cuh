@@ -84,9 +84,8 @@ __device__ __forceinline__ Rows user_rows(const cxs_cache_call& c, int user, int
   }
   if (lo < 0 || hi < lo || hi > c.tokens || hi - lo > c.max_tokens) {
     *bad = 1;
-    if (lo < 0 || hi < lo) return {0, 0};
     if (hi > c.tokens) hi = c.tokens;
-    if (hi < lo) return {0, 0};
+    if (lo < 0 || hi < lo) return {kInt32Max, 0};
     if (hi - lo > c.max_tokens) hi = lo + c.max_tokens;
   }
   return {static_cast<int>(lo), static_cast<int>(hi - lo)};
