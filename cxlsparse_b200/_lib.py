@@ -7,7 +7,10 @@ stream from ``torch.cuda.current_stream().cuda_stream``.
 """
 
 import ctypes
+import struct
 from pathlib import Path
+
+import torch
 
 LIBRARY = Path(__file__).resolve().parent / "libcxlsparse_b200.so"
 
@@ -116,7 +119,26 @@ class RotaryCall(ctypes.Structure):
                 "transpose", "wide_positions")] + [("magnitude", ctypes.c_float)]
 
 
+def _packer(cls):
+    """Packs the fields of a ctypes structure (nested ones flattened, null
+    pointers as 0) into bytes with the C layout, at a fraction of the cost of
+    filling the structure: the calls below are made for every layer and step."""
+    codes = {c_vp: "P", c_i64: "q", c_i32: "i", ctypes.c_float: "f"}
+
+    def fields(c):
+        return "".join(fields(t) if issubclass(t, ctypes.Structure) else codes[t]
+                       for _, t in c._fields_)
+
+    packer = struct.Struct("@" + fields(cls) + "0q")  # 0q: the trailing padding
+    assert packer.size == ctypes.sizeof(cls)
+    return packer.pack
+
+
+pack_cache_call, pack_cache_attend_call, pack_rotary_call = map(
+    _packer, (CacheCall, CacheAttendCall, RotaryCall))
+
 _lib = None
+_packed = None
 
 
 def lib():
@@ -200,6 +222,41 @@ def lib():
             raise ImportError("cxlsparse_b200 ABI version mismatch")
         _lib = handle
     return _lib
+
+
+class _Packed:
+    """Entry points that take their structure as packed bytes."""
+
+    def __init__(self, handle):
+        for name, argtypes in (
+                ("cxs_cache_append", [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp]),
+                ("cxs_cache_read", [c_vp, c_vp, c_vp, c_vp]),
+                ("cxs_cache_attend", [c_vp, c_vp]),
+                ("cxs_cache_attend_workspace", [c_vp, ctypes.POINTER(c_i64)]),
+                ("cxs_rotary", [c_vp, c_vp])):
+            fn = handle[name]  # a function object of its own
+            fn.restype, fn.argtypes = c_i32, argtypes
+            setattr(self, name, fn)
+
+
+def packed():
+    """``lib()`` with the structures of the cache and rotary calls as bytes."""
+    global _packed
+    if _packed is None:
+        _packed = _Packed(lib())
+    return _packed
+
+
+def on_device(index, fn, *args):
+    """``fn(*args, stream)`` on the current stream of CUDA device ``index``,
+    raising for a failure status."""
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
 def check(status):

@@ -43,8 +43,28 @@ namespace {
 
 using namespace cxs::cache8;
 
-// One page, head and part (K or V) per CTA: the page's new tokens' largest
-// magnitude, the scale, and one pass that writes codes.
+// Sixteen consecutive values, 16 bytes at a time where `wide` allows it.
+template <typename T>
+__device__ __forceinline__ void load16(float (&x)[16], const T* from, bool wide) {
+  alignas(16) T in[16];
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i)
+      reinterpret_cast<uint4*>(in)[i] = reinterpret_cast<const uint4*>(from)[i];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) in[e] = from[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = to_float(in[e]);
+}
+
+// One page, head and part (K or V) per CTA, 16 channels of a slot per thread:
+// the values are read once, kept in registers while the CTA finds the largest
+// magnitude, then written as codes, 16 bytes a thread. Memory-bound (2 or 4
+// bytes in, 1 out): a page's CTA has all its loads in flight at once, and
+// several CTAs share an SM, so one's reduction hides under the others' loads.
+// Older codes are touched only where the page's scale grows.
 template <int FORMAT, typename T>
 __global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
                               long long k_token, long long k_head, const T* __restrict__ v,
@@ -54,7 +74,7 @@ __global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
   const int head = blockIdx.y, part = blockIdx.z;
   int bad = 0;
   const Rows rows = user_rows(c, user, &bad);
-  long long start = (long long)c.lengths[user] - rows.count;
+  const long long start = (long long)c.lengths[user] - rows.count;
   const long long end = start + rows.count;
   const long long most = (long long)c.width * c.page_size;
   if (start < 0 || end > most) bad = 1;
@@ -63,47 +83,73 @@ __global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
   const long long from = start > 0 ? start : 0, to = end < most ? end : most;
   const long long low = (from / c.page_size + step) * c.page_size;  // position of slot 0
   if (from >= to || low >= to) return;
+  const int fill = from > low ? (int)(from - low) : 0;  // slots of older tokens
+  const int stop = to - low < c.page_size ? (int)(to - low) : c.page_size;
+  const int chunks = c.dim / 16, slot = threadIdx.x / chunks, channel = threadIdx.x % chunks * 16;
+  const bool fresh = slot >= fill && slot < stop, old = slot < fill;
+
+  float x[16];
+  float size = 0.f;
+  if (fresh) {
+    const T* row = part ? v + head * v_head : k + head * k_head;
+    row += (rows.first + (low - start) + slot) * (part ? v_token : k_token) + channel;
+    load16(x, row, ((uintptr_t)row & 15) == 0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float a = fabsf(x[e]);
+      if (a < INFINITY) size = fmaxf(size, a);  // neither infinity nor NaN
+    }
+  }
   const int page = c.table[user * c.table_stride + low / c.page_size];
   if (page < 0 || page >= c.pages) {
     if (head == 0 && part == 0 && threadIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
     return;
   }
-  const int fill = from > low ? (int)(from - low) : 0;  // slots of older tokens
-  const int stop = to - low < c.page_size ? (int)(to - low) : c.page_size;
-  const T* x = part ? v + head * v_head : k + head * k_head;
-  const long long x_token = part ? v_token : k_token;
-  x += (rows.first + low - start) * x_token;  // slot 0's row (slots below `fill` are not read)
   const long long cell = ((long long)page * c.kv_heads + head) * 2 + part;
-  uint8_t* codes = (uint8_t*)c.codes + cell * c.page_size * c.dim;
-
-  __shared__ float partial[32];
-  float size = 0.f;
-  for (int i = fill * c.dim + threadIdx.x; i < stop * c.dim; i += blockDim.x) {
-    const float a = fabsf(to_float(x[(i / c.dim) * x_token + i % c.dim]));
-    if (a < INFINITY) size = fmaxf(size, a);  // neither infinity nor NaN
-  }
+  uint4* codes = (uint4*)((uint8_t*)c.codes + cell * c.page_size * c.dim) + threadIdx.x;
+  const float before = fill ? c.scales[cell] : 0.f;
+  __shared__ float partial[16];
   for (int o = 16; o; o >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
   if (threadIdx.x % 32 == 0) partial[threadIdx.x / 32] = size;
-  __syncthreads();
+  __syncthreads();  // and every thread has read the older scale
   for (int w = 0; w < blockDim.x / 32; ++w) size = fmaxf(size, partial[w]);
-  const float before = fill ? c.scales[cell] : 0.f;
   const float scale = fmaxf(fmaxf(size * C::kInverseTop, kLeastScale), before);
-  const float inverse = 1.f / scale;
-  for (int i = fill * c.dim + threadIdx.x; i < stop * c.dim; i += blockDim.x)
-    codes[i] = C::encode(to_float(x[(i / c.dim) * x_token + i % c.dim]) * inverse);
-  if (fill && scale > before) {
-    const float ratio = before / scale;
-    for (int i = threadIdx.x; i < fill * c.dim; i += blockDim.x)
-      codes[i] = C::encode(C::decode(codes[i]) * ratio);
-  }
-  __syncthreads();  // every thread has read the older scale
   if (threadIdx.x == 0) c.scales[cell] = scale;
+  float factor;
+  if (fresh) {
+    factor = 1.f / scale;
+  } else if (old && scale > before) {
+    factor = before / scale;
+    const uint4 w = *codes;
+    float y[4];
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      C::decode4(in[i], y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
+    }
+  } else {
+    return;
+  }
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y[4] = {x[4 * i] * factor, x[4 * i + 1] * factor, x[4 * i + 2] * factor,
+                        x[4 * i + 3] * factor};
+    out[i] = C::encode4(y);
+  }
+  *codes = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// One page and head per CTA.
+// One page and head per CTA: K and V of a page are one run of bytes, read 16
+// a thread with kUnroll reads in flight, multiplied, rounded and written to
+// the two outputs. Memory-bound: 1 byte in, 2 or 4 out.
+constexpr int kReadThreads = 128, kUnroll = 4;
+
 template <int FORMAT, typename T>
-__global__ void read_kernel(const cxs_cache_call c, T* __restrict__ k, T* __restrict__ v,
-                            int reach) {
+__global__ void __launch_bounds__(kReadThreads)
+    read_kernel(const cxs_cache_call c, T* __restrict__ k, T* __restrict__ v, int reach) {
   using C = Code<FORMAT>;
   const int user = blockIdx.x / reach, step = blockIdx.x % reach, head = blockIdx.y;
   int bad = 0;
@@ -128,15 +174,40 @@ __global__ void read_kernel(const cxs_cache_call c, T* __restrict__ k, T* __rest
       if (head == 0 && threadIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
     }
   }
-  for (int part = 0; part < 2; ++part) {
-    const long long cell = ((long long)page * c.kv_heads + head) * 2 + part;
-    const uint8_t* codes = (const uint8_t*)c.codes + cell * c.page_size * c.dim;
-    const float scale = page < 0 ? 0.f : c.scales[cell];
-    T* out = part ? v : k;
-    for (int i = fill * c.dim + threadIdx.x; i < stop * c.dim; i += blockDim.x) {
-      const long long row = rows.first + low + i / c.dim - start;
-      out[(row * c.kv_heads + head) * c.dim + i % c.dim] =
-          from_float<T>(page < 0 ? 0.f : C::decode(codes[i]) * scale);
+  const long long cell = ((long long)(page < 0 ? 0 : page) * c.kv_heads + head) * 2;
+  const float scale_k = page < 0 ? 0.f : c.scales[cell];
+  const float scale_v = page < 0 ? 0.f : c.scales[cell + 1];
+  const uint4* codes = (const uint4*)((const uint8_t*)c.codes + cell * c.page_size * c.dim);
+  const int chunks = c.dim / 16, half = c.page_size * chunks;
+  const long long row0 = rows.first + (low - start);
+  for (int base = threadIdx.x; base < 2 * half; base += kReadThreads * kUnroll) {
+    uint4 w[kUnroll];
+    bool live[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int n = base + i * kReadThreads, slot = n % half / chunks;
+      live[i] = n < 2 * half && slot >= fill && slot < stop;
+      w[i] = live[i] && page >= 0 ? __ldcs(codes + n) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (!live[i]) continue;
+      const int n = base + i * kReadThreads;
+      const bool second = n >= half;
+      const int slot = n % half / chunks, channel = n % chunks * 16;
+      const float scale = second ? scale_v : scale_k;
+      alignas(16) T out[16];
+      const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[4];
+        C::decode4(in[j], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * j + e] = from_float<T>(x[e] * scale);
+      }
+      uint4* to = (uint4*)((second ? v : k) + ((row0 + slot) * c.kv_heads + head) * c.dim + channel);
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T); ++j) to[j] = reinterpret_cast<const uint4*>(out)[j];
     }
   }
 }
@@ -156,9 +227,10 @@ extern "C" int cxs_cache_append(const cxs_cache_call* call, const void* k, int64
   if ((long long)call->users * reach > 0x7fffffffll)
     return set_error(CXS_ERR_CAPACITY, "cache append: too many pages in one call");
   const dim3 grid(call->users * reach, call->kv_heads, 2);
+  const int threads = call->page_size * call->dim / 16;
   CXS_CACHE_FORMAT(call->format, F,
                    CXS_CACHE_TYPE(call->type, T,
-                                  (append_kernel<F, T><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                                  (append_kernel<F, T><<<grid, threads, 0, (cudaStream_t)stream>>>(
                                       *call, (const T*)k, k_token_stride, k_head_stride,
                                       (const T*)v, v_token_stride, v_head_stride, reach))));
   CXS_LAUNCH_CHECK("cache append");
@@ -172,6 +244,8 @@ extern "C" int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void
   status = cxs_host::check_cache_pointers(call, "cache read");
   if (status != CXS_OK) return status;
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache read: null output");
+  if ((uintptr_t)k % 16 || (uintptr_t)v % 16)
+    return set_error(CXS_ERR_INVALID, "cache read: outputs must be 16-byte aligned");
   const int reach = (call->max_tokens + call->page_size - 2) / call->page_size + 1;
   if ((long long)call->users * reach > 0x7fffffffll)
     return set_error(CXS_ERR_CAPACITY, "cache read: too many pages in one call");
@@ -179,7 +253,7 @@ extern "C" int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void
   CXS_CACHE_FORMAT(
       call->format, F,
       CXS_CACHE_TYPE(call->type, T,
-                     (read_kernel<F, T><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                     (read_kernel<F, T><<<grid, kReadThreads, 0, (cudaStream_t)stream>>>(
                          *call, (T*)k, (T*)v, reach))));
   CXS_LAUNCH_CHECK("cache read");
   return CXS_OK;

@@ -12,7 +12,7 @@ namespace cache8 {
 
 constexpr float kLeastScale = 5.421010862427522e-20f;  // 2^-64
 
-// Codes of a format: the largest one, decoding and rounding.
+// Codes of a format: the largest one, decoding and rounding of four at once.
 template <int FORMAT>
 struct Code;
 
@@ -20,14 +20,17 @@ template <>
 struct Code<CXS_FORMAT_E4M3> {
   static constexpr float kTop = 448.f;
   static constexpr float kInverseTop = 1.f / 448.f;
-  static __device__ __forceinline__ float decode(uint8_t c) {
-    __nv_fp8_e4m3 v;
-    v.__x = c;
-    return static_cast<float>(v);
+  static __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+    __nv_fp8x4_e4m3 v;
+    v.__x = w;
+    const float4 f = static_cast<float4>(v);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
   }
-  // Nearest code, ties to even, saturated; NaN stays NaN.
-  static __device__ __forceinline__ uint8_t encode(float x) {
-    return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  // Nearest codes, ties to even, saturated; NaN stays NaN.
+  static __device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
   }
 };
 
@@ -35,14 +38,20 @@ template <>
 struct Code<CXS_FORMAT_INT8> {
   static constexpr float kTop = 127.f;
   static constexpr float kInverseTop = 1.f / 127.f;
-  static __device__ __forceinline__ float decode(uint8_t c) {
-    return static_cast<float>(static_cast<int8_t>(c));
+  static __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
   }
-  // Nearest code, ties to even, saturated; NaN becomes 0.
-  static __device__ __forceinline__ uint8_t encode(float x) {
-    if (!(x == x)) return 0;
-    return static_cast<uint8_t>(
-        static_cast<int8_t>(__float2int_rn(fminf(fmaxf(x, -kTop), kTop))));
+  // Nearest codes, ties to even, saturated; NaN becomes 0. Adding 1.5 * 2^23
+  // leaves the integer, rounded, in the low bits of the sum.
+  static __device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = x[e] == x[e] ? fminf(fmaxf(x[e], -kTop), kTop) : 0.f;
+      b[e] = __float_as_uint(__fadd_rn(y, 12582912.f));
+    }
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
 };
 

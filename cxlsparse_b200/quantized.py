@@ -63,6 +63,9 @@ class QuantizedCache:
         self.format = CODE_TYPES[codes.dtype]
         self.device = codes.device
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._codes, self._scales, self._error = (
+            t.data_ptr() for t in (codes, scales, self.error))
+        self._workspace = {}
 
     # -- checks ------------------------------------------------------------
     def check(self):
@@ -77,66 +80,79 @@ class QuantizedCache:
             raise _lib.CxsError(_lib.ERR_INVALID, "cache call met " + " and ".join(what))
 
     def _call(self, table, lengths, offsets, tokens, max_tokens, type_):
-        if table.ndim != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+        """The fields of ``cxs_cache_call``."""
+        shape, stride = table.shape, table.stride()
+        if len(shape) != 2 or table.dtype != torch.int32 or stride[1] != 1:
             raise ValueError("table must be [users, width] int32 with contiguous rows")
-        users, width = table.shape
+        users, width = shape
         if lengths.shape != (users,) or lengths.dtype != torch.int32 \
                 or not lengths.is_contiguous():
             raise ValueError("lengths must be [users] int32, contiguous")
-        if offsets is not None and (offsets.shape != (users + 1,)
-                                    or offsets.dtype != torch.int32
-                                    or not offsets.is_contiguous()):
-            raise ValueError("offsets must be [users + 1] int32, contiguous")
-        if offsets is None and tokens != users:
-            raise ValueError("without offsets every user has one row")
-        for t in (table, lengths) if offsets is None else (table, lengths, offsets):
-            if t.device != self.device:
-                raise ValueError(f"table, lengths and offsets must be on {self.device}")
-        if max_tokens is None:
-            max_tokens = 1 if offsets is None else tokens
-        if max_tokens < 0:
-            raise ValueError("max_tokens must not be negative")
-        return _lib.CacheCall(
-            self.codes.data_ptr(), self.scales.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-            _lib.ptr(offsets), self.error.data_ptr(), table.stride(0), self.pages, self.kv_heads,
-            self.dim, self.page_size, self.format, users, width, tokens,
-            min(max_tokens, tokens), type_)
+        if table.device != self.device or lengths.device != self.device:
+            raise ValueError(f"table and lengths must be on {self.device}")
+        if offsets is None:
+            if tokens != users:
+                raise ValueError("without offsets every user has one row")
+            at, most = 0, 1
+        else:
+            if offsets.shape != (users + 1,) or offsets.dtype != torch.int32 \
+                    or not offsets.is_contiguous() or offsets.device != self.device:
+                raise ValueError(f"offsets must be [users + 1] int32, contiguous, on {self.device}")
+            at, most = offsets.data_ptr(), tokens
+        if max_tokens is not None:
+            if max_tokens < 0:
+                raise ValueError("max_tokens must not be negative")
+            most = min(most, max_tokens)
+        return (self._codes, self._scales, table.data_ptr(), lengths.data_ptr(), at, self._error,
+                stride[0], self.pages, self.kv_heads, self.dim, self.page_size, self.format,
+                users, width, tokens, most, type_)
 
-    def _rows(self, name, x, heads=None):
-        if x.ndim != 3 or x.shape[-1] != self.dim or x.stride(-1) != 1 \
-                or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.dim}] with "
-                             "contiguous channels")
+    def _rows(self, name, x):
+        """(shape, strides) of a [tokens, heads, dim] tensor."""
+        shape, stride = x.shape, x.stride()
+        if len(shape) != 3 or shape[2] != self.dim or stride[2] != 1:
+            raise ValueError(f"{name} must be [tokens, heads, {self.dim}] with contiguous channels")
         if x.device != self.device:
             raise ValueError(f"{name} must be on {self.device}")
+        return shape, stride
+
+    def _workspace_bytes(self, common, heads):
+        """Scratch of an attend call, kept by (heads, most rows of one user)."""
+        size = _lib.c_i64(0)
+        _lib.check(_lib.packed().cxs_cache_attend_workspace(
+            _lib.pack_cache_attend_call(*common, 0, 0, 0, 0, 0, 0, 0, heads, 1, 0, 1.0), size))
+        if len(self._workspace) >= 4096:
+            self._workspace.clear()
+        self._workspace[heads, common[15]] = size.value
+        return size.value
 
     # -- operators ---------------------------------------------------------
     def append(self, k, v, table, lengths, offsets=None, *, max_tokens=None):
         """Quantise the new tokens' keys and values [tokens, kv_heads, dim]
         (bf16, fp16 or fp32) into their pages. ``max_tokens``: most new tokens
         of one user, if known on the host (it bounds the launch)."""
-        self._rows("k", k, self.kv_heads)
-        self._rows("v", v, self.kv_heads)
-        if k.dtype not in TYPES or v.dtype != k.dtype or len(v) != len(k):
-            raise ValueError("k and v must be bf16, fp16 or fp32, of one type and length")
-        call = self._call(table, lengths, offsets, len(k), max_tokens, TYPES[k.dtype])
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().cxs_cache_append(
-                call, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                v.stride(1), torch.cuda.current_stream(self.device).cuda_stream))
+        (shape, ks), (v_shape, vs) = self._rows("k", k), self._rows("v", v)
+        if shape[1] != self.kv_heads or v_shape != shape:
+            raise ValueError(f"k and v must both be [tokens, {self.kv_heads}, {self.dim}]")
+        dtype = k.dtype
+        if dtype not in TYPES or v.dtype != dtype:
+            raise ValueError("k and v must be bf16, fp16 or fp32, of one type")
+        call = _lib.pack_cache_call(
+            *self._call(table, lengths, offsets, shape[0], max_tokens, TYPES[dtype]))
+        _lib.on_device(self.device.index, _lib.packed().cxs_cache_append, call, k.data_ptr(),
+                       ks[0], ks[1], v.data_ptr(), vs[0], vs[1])
 
     def read(self, table, starts, offsets, *, total, max_tokens=None, dtype=torch.bfloat16):
         """``(k, v)`` [total, kv_heads, dim] of consecutive tokens: row
         offsets[b] + i is user b's token starts[b] + i."""
         if dtype not in TYPES:
             raise ValueError("dtype must be bf16, fp16 or fp32")
-        call = self._call(table, starts, offsets, total, max_tokens, TYPES[dtype])
+        call = _lib.pack_cache_call(
+            *self._call(table, starts, offsets, total, max_tokens, TYPES[dtype]))
         k = torch.empty((total, self.kv_heads, self.dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().cxs_cache_read(
-                call, k.data_ptr(), v.data_ptr(),
-                torch.cuda.current_stream(self.device).cuda_stream))
+        _lib.on_device(self.device.index, _lib.packed().cxs_cache_read, call, k.data_ptr(),
+                       v.data_ptr())
         return k, v
 
     def attend(self, q, table, lengths, offsets=None, *, max_tokens=None, causal=True, window=0,
@@ -147,10 +163,11 @@ class QuantizedCache:
         row also sees only the last ``window`` positions up to its own. Returns
         [tokens, heads, dim], with ``return_lse`` also the softmax's log-sum
         [tokens, heads] fp32 (for joining with attention over other keys)."""
-        self._rows("q", q)
-        if q.dtype not in (torch.bfloat16, torch.float16):
+        shape, stride = self._rows("q", q)
+        dtype = q.dtype
+        if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("q must be bf16 or fp16")
-        tokens, heads = q.shape[:2]
+        tokens, heads = shape[0], shape[1]
         if heads < 1 or heads % self.kv_heads:
             raise ValueError("heads must be a multiple of kv_heads")
         scale = self.dim ** -0.5 if scale is None else float(scale)
@@ -158,20 +175,16 @@ class QuantizedCache:
             raise ValueError("scale must be finite")
         if window < 0:
             raise ValueError("window must not be negative")
-        out = torch.empty((tokens, heads, self.dim), dtype=q.dtype, device=self.device)
+        common = self._call(table, lengths, offsets, tokens, max_tokens, TYPES[dtype])
+        size = self._workspace.get((heads, common[15]))
+        if size is None:
+            size = self._workspace_bytes(common, heads)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) \
             if return_lse else None
-        call = _lib.CacheAttendCall(
-            self._call(table, lengths, offsets, tokens, max_tokens, TYPES[q.dtype]),
-            q.data_ptr(), out.data_ptr(), _lib.ptr(lse), None, 0, q.stride(0), q.stride(1),
-            heads, int(bool(causal)), window, scale)
-        with torch.cuda.device(self.device):
-            lib = _lib.lib()
-            size = _lib.c_i64(0)
-            _lib.check(lib.cxs_cache_attend_workspace(call, size))
-            if size.value:
-                workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device)
-                call.workspace, call.workspace_bytes = workspace.data_ptr(), size.value
-            _lib.check(lib.cxs_cache_attend(
-                call, torch.cuda.current_stream(self.device).cuda_stream))
+        workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        call = _lib.pack_cache_attend_call(
+            *common, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            workspace.data_ptr(), size, stride[0], stride[1], heads, bool(causal), window, scale)
+        _lib.on_device(self.device.index, _lib.packed().cxs_cache_attend, call)
         return (out, lse) if return_lse else out

@@ -89,16 +89,19 @@ class Rotary:
         # range, and the product with a position wraps modulo one turn.
         steps = (f / (2 * math.pi) * 2.0 ** 62).round().to(torch.int64) << 2
         self.steps = steps.to(device)
+        self.device = self.steps.device
+        self._steps = self.steps.data_ptr()
 
-    def _check(self, name, x, like=None):
-        if x.ndim != 3 or x.shape[-1] != self.dim or x.stride(-1) != 1:
+    def _check(self, name, x, dtype):
+        """(heads, token stride, head stride) of a [tokens, heads, dim] tensor."""
+        shape, stride = x.shape, x.stride()
+        if len(shape) != 3 or shape[2] != self.dim or stride[2] != 1:
             raise ValueError(f"{name} must be [tokens, heads, {self.dim}] with contiguous channels")
-        if x.dtype not in TYPES:
-            raise ValueError(f"{name} must be bf16, fp16 or fp32")
-        if x.device != self.steps.device:
-            raise ValueError(f"{name} must be on {self.steps.device}")
-        if like is not None and x.dtype != like.dtype:
-            raise ValueError(f"{name} must have the type of the other tensor")
+        if x.dtype != dtype:
+            raise ValueError("the tensors must have one type")
+        if x.device != self.device:
+            raise ValueError(f"{name} must be on {self.device}")
+        return shape, stride
 
     def apply(self, q, k, positions, *, transpose=False, out=None):
         """Rotated ``(q, k)`` for q [tokens, heads, dim], k [tokens, kv_heads,
@@ -106,43 +109,50 @@ class Rotary:
         launch on the current stream. ``transpose`` turns the other way: given
         the gradients of the outputs it returns those of the inputs (and, for
         magnitude 1, undoes the rotation). ``out=(q_out, k_out)`` receives the
-        result and may be the inputs themselves."""
+        result; each may be its input itself, and must not overlap an input in
+        another way."""
         first = q if q is not None else k
         if first is None:
             raise ValueError("q or k is needed")
-        for name, x in (("q", q), ("k", k)):
-            if x is not None:
-                self._check(name, x, first)
-        tokens = len(first)
-        if (k is not None and len(k) != tokens) or positions.shape != (tokens,):
-            raise ValueError("q, k and positions must have as many tokens")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != first.device:
-            raise ValueError("positions must be int32 or int64 on the device of q and k")
+        dtype, tokens = first.dtype, first.shape[0]
+        if dtype not in TYPES:
+            raise ValueError("q and k must be bf16, fp16 or fp32")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
+                or positions.device != self.device:
+            raise ValueError(f"positions must be [tokens] int32 or int64 on {self.device}")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        if out is None:
-            q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        else:
-            q_out, k_out = out
-            for name, x, y in (("q", q, q_out), ("k", k, k_out)):
-                if (x is None) != (y is None):
-                    raise ValueError(f"out must have a tensor for {name} exactly when {name} is given")
-                if y is not None:
-                    self._check(f"out of {name}", y, first)
-                    if y.shape != x.shape:
-                        raise ValueError(f"out of {name} must have its shape")
-        qs = (0, 0, 0) if q is None else q.stride()
-        ks = (0, 0, 0) if k is None else k.stride()
-        qo = (0, 0, 0) if q is None else q_out.stride()
-        ko = (0, 0, 0) if k is None else k_out.stride()
-        call = _lib.RotaryCall(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(q_out), _lib.ptr(k_out), positions.data_ptr(),
-            self.steps.data_ptr(), qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1],
-            tokens, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], self.dim,
-            self.rotary_dim, LAYOUTS[self.layout], TYPES[first.dtype], int(bool(transpose)),
-            int(positions.dtype == torch.int64), self.magnitude)
-        with torch.cuda.device(first.device):
-            _lib.check(_lib.lib().cxs_rotary(
-                call, torch.cuda.current_stream(first.device).cuda_stream))
-        return q_out, k_out
+        if out is not None and ((out[0] is None) != (q is None) or (out[1] is None) != (k is None)):
+            raise ValueError("out must have a tensor for each of q and k that is given")
+        made, pointers, strides, heads = [], [], [], []
+        for i, (name, x) in enumerate((("q", q), ("k", k))):
+            if x is None:
+                made.append(None)
+                pointers.append((0, 0))
+                strides.append((0, 0, 0, 0))
+                heads.append(0)
+                continue
+            shape, stride = self._check(name, x, dtype)
+            if shape[0] != tokens:
+                raise ValueError("q, k and positions must have as many tokens")
+            if out is None:
+                y = torch.empty_like(x, memory_format=torch.contiguous_format)
+                to = (shape[1] * self.dim, self.dim)
+            else:
+                y = out[i]
+                out_shape, to = self._check(f"out of {name}", y, dtype)
+                if out_shape != shape:
+                    raise ValueError(f"out of {name} must have its shape")
+            made.append(y)
+            pointers.append((x.data_ptr(), y.data_ptr()))
+            strides.append((stride[0], stride[1], to[0], to[1]))
+            heads.append(shape[1])
+        (qp, qo), (kp, ko) = pointers
+        qs, ks = strides
+        call = _lib.pack_rotary_call(
+            qp, kp, qo, ko, positions.data_ptr(), self._steps, qs[0], qs[1], ks[0], ks[1],
+            qs[2], qs[3], ks[2], ks[3], tokens, heads[0], heads[1], self.dim, self.rotary_dim,
+            LAYOUTS[self.layout], TYPES[dtype], bool(transpose), positions.dtype == torch.int64,
+            self.magnitude)
+        _lib.on_device(self.device.index, _lib.packed().cxs_rotary, call)
+        return tuple(made)

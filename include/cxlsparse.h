@@ -538,7 +538,7 @@ int cxs_cache_append(const cxs_cache_call* call, const void* k, int64_t k_token_
                      int64_t v_head_stride, void* stream);
 
 /* Values code * scale of consecutive tokens of each user, rounded once to
- * `type`, into k and v [tokens, kv_heads, dim] (contiguous): row offsets[b] + i
+ * `type`, into k and v [tokens, kv_heads, dim] (contiguous, 16-byte aligned): row offsets[b] + i
  * is position lengths[b] + i (lengths holds the first position here). Tokens
  * of a page that is not there come back as 0, with the error bit. */
 int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream);
