@@ -13,7 +13,7 @@ from pathlib import Path
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 SOURCES = ["capi.cu", "planner.cu", "attend.cu", "select.cu", "glue.cu", "exchange.cu",
-           "rotary.cu", "cache8.cu", "cache8_attend.cu"]
+           "rotary.cu", "cache8.cu", "cache8_attend.cu", "cache8_tile.cu"]
 LIBRARY = PACKAGE / "libcxlsparse_b200.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -104,6 +104,20 @@ __device__ __forceinline__ Rows user_rows(const cxs_cache_call& c, int user, int
 }  // namespace cxs
 
 namespace cxs_host {
+// Runs a step (a function attribute, say) once for each device.
+struct OncePerDevice {
+  static constexpr int kDevices = 64;
+  int done[kDevices];
+  template <typename F>
+  int run(F step) {
+    int device = 0;
+    CXS_CUDA(cudaGetDevice(&device));
+    if (device < kDevices && __atomic_load_n(&done[device], __ATOMIC_ACQUIRE)) return CXS_OK;
+    const int status = step();
+    if (status == CXS_OK && device < kDevices) __atomic_store_n(&done[device], 1, __ATOMIC_RELEASE);
+    return status;
+  }
+};
 constexpr long long kMaxPositions = 1ll << 30;  // positions of one table row
 // CXS_OK, or what is wrong with the sizes / the pointers every cache call shares.
 int check_cache(const cxs_cache_call* call, const char* what);

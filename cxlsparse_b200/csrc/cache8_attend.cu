@@ -1,61 +1,14 @@
-// Attention over the dense 8-bit cache.
-//
-// Mathematics. With codes c and scales s_k, s_v constant over a page, a score
-// in base-2 units is x = scale log2(e) s_k (q . c_k), and
-//   out = sum 2^x s_v c_v / sum 2^x = sum p c_v / sum p / s_v,
-//   p = 2^(x + log2 s_v - M),  M = running max of x + log2 s_v.
-// Folding s_v into the exponent keeps p <= 1 whatever the pages' scales, so p
-// is rounded to fp16 (11 bits) and multiplied with the codes themselves, which
-// fp16 holds exactly (e4m3 and integers to 128); the denominator divides each
-// page's sum of p by its s_v in fp32. Queries are scaled by a power of two per
-// row so that fp16 holds them: exact for fp16 inputs, and for bf16 (8 bits of
-// mantissa) but for parts 2^-28 below the row's largest element, which lose
-// less than 2^-39 of it.
+// Attention over the dense 8-bit cache: few query rows a KV head, the joining
+// of partial results, and the entry points.
 #include <cuda_pipeline_primitives.h>
 
-#include "cache8.cuh"
+#include "cache8_attend.cuh"
 
 using cxs_host::set_error;
 
 namespace {
 
 using namespace cxs::cache8;
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kInf = INFINITY;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// ------------------------------------------------------ code conversion ---
-
-// Two codes (the low or high half of `w`) as fp16, exact.
-template <int FORMAT>
-__device__ __forceinline__ uint32_t half2_of(uint32_t w, int high);
-template <>
-__device__ __forceinline__ uint32_t half2_of<CXS_FORMAT_E4M3>(uint32_t w, int high) {
-  uint32_t r;
-  asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, %2;}"
-      : "=r"(r)
-      : "r"(w), "h"((unsigned short)(high ? w >> 16 : w & 0xffffu)));
-  return r;
-}
-// An integer v as 1024 + 128 + v (its bits in an fp16 mantissa), minus 1152.
-template <>
-__device__ __forceinline__ uint32_t half2_of<CXS_FORMAT_INT8>(uint32_t w, int high) {
-  const uint32_t biased = __byte_perm(w ^ 0x80808080u, 0x64646464u, high ? 0x4342 : 0x4140);
-  __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
 
 // D += A B, 16x8x16, fp16 in, fp32 out.
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -65,116 +18,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// ----------------------------------------------------------------- items ---
-//
-// An item is one user's tile of query rows (a row is a new token and one of
-// the KV head's query heads: row r is token r / group, head r % group) with
-// one KV head. Its work is a run of key tiles. All items' tiles, in order,
-// are cut into equal shares, one for each CTA, whatever the users' lengths;
-// an item whose tiles fall into several shares leaves a partial result (O, M,
-// l) in each, which combine_kernel joins in the order of the keys.
-
-constexpr int kSlice = 2048;  // users of one launch (their tile counts sit in shared memory)
-
-struct Shape {
-  int group;      // query heads of a KV head
-  int user0;      // first user of this launch (table, lengths and offsets point at it)
-  int users;
-  int last;       // the launch holds the last user
-  int grid;       // most CTAs
-  int min_tiles;  // fewest tiles worth a CTA
-};
-
-// One user's positions. Visible to some row: [begin, end).
-struct Span {
-  int first, count;     // packed rows
-  int start;            // position of the first row (negative: more rows than tokens)
-  int length;           // tokens, cut to the table
-  int begin;
-};
-
-__device__ __forceinline__ Span user_span(const cxs_cache_attend_call& a, const Shape& z, int user,
-                                          int* bad) {
-  const cxs_cache_call& c = a.cache;
-  Span s;
-  Rows rows;
-  if (c.offsets) {
-    rows = user_rows(c, user, bad);
-  } else {
-    rows = {z.user0 + user, 1};
-  }
-  const int most = c.width * c.page_size;
-  s.first = rows.first;
-  s.count = rows.count;
-  s.length = c.lengths[user];
-  if (s.length < 0) s.length = 0, *bad = 1;
-  s.start = s.length - rows.count;
-  if (s.length > most) s.length = most, *bad = 1;
-  s.begin = a.window > 0 && s.start >= a.window ? min(s.start - a.window + 1, s.length) : 0;
-  return s;
-}
-
-// Row r of a user sees positions [x, y).
-__device__ __forceinline__ int2 row_range(const cxs_cache_attend_call& a, const Span& s,
-                                          int token) {
-  const int position = s.start + token;
-  int hi = s.length, lo = 0;
-  if (a.causal && position + 1 < hi) hi = position + 1;
-  if (a.window > 0 && position >= a.window) lo = position - a.window + 1;
-  return make_int2(lo, hi);
-}
-
-// Shares: CTA c of n takes tiles [total c / n, total (c + 1) / n) (without the
-// product's overflow).
-__device__ __forceinline__ long long share(long long total, int c, int n) {
-  return total / n * c + total % n * c / n;
-}
-// The CTA whose share holds tile `tile` (total >= n).
-__device__ __forceinline__ int share_of(long long total, long long tile, int n) {
-  const long long guess = tile / (total / n);
-  int c = guess < n - 1 ? (int)guess : n - 1;
-  while (share(total, c, n) > tile) --c;
-  while (share(total, c + 1, n) <= tile) ++c;
-  return c;
-}
-
-struct alignas(16) Partial {  // the item that starts in a CTA's share and goes on past it
-  int parts;      // CTAs it falls into; 0: none
-  int first, rows, row0, kv_head;  // the item's packed first row, user's rows, first row, head
-};
-
-// Rows of no user (before the first offset, past the last, or more than
-// max_tokens of one user): zero, and nothing in the sum.
-template <typename T, int D>
-__device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int cta, int ctas) {
-  const cxs_cache_call& c = a.cache;
-  if (!c.offsets) return;
-  for (int b = cta - 1; b <= z.users; b += ctas) {
-    long long low, high;
-    if (b < 0) {
-      low = z.user0 == 0 ? 0 : 1;
-      high = z.user0 == 0 ? c.offsets[0] : 0;
-    } else if (b < z.users) {
-      int bad = 0;
-      const Rows rows = user_rows(c, b, &bad);
-      if (!bad) continue;
-      low = (long long)rows.first + rows.count;
-      high = c.offsets[b + 1];
-    } else {
-      low = z.last ? c.offsets[z.users] : 1;
-      high = z.last ? c.tokens : 0;
-    }
-    if (low < 0) low = 0;
-    if (high > c.tokens) high = c.tokens;
-    if (low >= high) continue;
-    for (long long i = low * a.heads * D + threadIdx.x; i < high * a.heads * D; i += blockDim.x)
-      ((T*)a.out)[i] = from_float<T>(0.f);
-    if (a.lse)
-      for (long long i = low * a.heads + threadIdx.x; i < high * a.heads; i += blockDim.x)
-        a.lse[i] = -kInf;
-  }
 }
 
 // ------------------------------------------------- few rows: one warp, 16 ---
@@ -670,19 +513,19 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   __pipeline_wait_prior(0);
 }
 
-// Joins the partial results of the item that starts in share blockIdx.x and
-// goes on into later ones: one thread per four channels of a row, in the
-// order of the shares.
-template <typename T, int D>
+// Joins the partial results of the item (of ROWS rows) that starts in share
+// blockIdx.x and goes on into later ones: 16 rows a CTA, one thread per four
+// channels of a row, in the order of the shares.
+template <typename T, int D, int ROWS>
 __global__ void combine_kernel(const cxs_cache_attend_call a, const Shape z) {
-  constexpr int kRows = Decode<D>::kRows, kSize = kRows * (D + 2);
+  constexpr int kRows = ROWS, kSize = kRows * (D + 2);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Partial* partials = reinterpret_cast<const Partial*>(a.workspace);
   const Partial item = partials[blockIdx.x];
   if (item.parts == 0) return;
   const float* scratch =
       reinterpret_cast<const float*>(partials + z.grid) + (long long)blockIdx.x * 2 * kSize;
-  const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const int r = 16 * blockIdx.y + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   const int row = item.row0 + r;
   if (row >= item.rows) return;
   auto part = [&](int i) { return scratch + (i == 0 ? kSize : 2 * i * kSize); };
@@ -730,65 +573,70 @@ int check_attend(const cxs_cache_attend_call* a) {
   return CXS_OK;
 }
 
-constexpr int kMaxDevices = 64;
-
 // SMs of the current device (looked up once).
 int sm_count(int* sms) {
-  static int known[kMaxDevices];
-  int device = 0;
-  CXS_CUDA(cudaGetDevice(&device));
-  int n = device < kMaxDevices ? __atomic_load_n(&known[device], __ATOMIC_RELAXED) : 0;
-  if (!n) {
+  static int known;
+  static cxs_host::OncePerDevice looked;
+  const int status = looked.run([] {
+    int device = 0, n = 0;
+    CXS_CUDA(cudaGetDevice(&device));
     CXS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
-    if (device < kMaxDevices) __atomic_store_n(&known[device], n, __ATOMIC_RELAXED);
-  }
-  *sms = n;
-  return CXS_OK;
+    __atomic_store_n(&known, n, __ATOMIC_RELAXED);
+    return (int)CXS_OK;
+  });
+  *sms = __atomic_load_n(&known, __ATOMIC_RELAXED);
+  return status;
 }
 
-// Largest grid a call uses: one CTA per SM. Counted without a device as the
-// B200's 148, so that the workspace's size does not depend on one.
+// Largest grid a call uses: one CTA per SM of a B200. A constant, so that the
+// workspace's size does not depend on the device.
 constexpr int kMostCtas = 148;
 
+// Most rows of a user and KV head for which the mma.sync kernel runs.
+constexpr int kFewRows = 64;
+
+bool few_rows(const cxs_cache_attend_call& a) {
+  return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= kFewRows;
+}
+
 long long workspace_bytes(const cxs_cache_attend_call& a) {
-  const int d = a.cache.dim;
-  return (long long)kMostCtas * (sizeof(Partial) + 2ll * 16 * (d + 2) * sizeof(float));
+  const long long rows = few_rows(a) ? 16 : kTileRows;
+  return kMostCtas * (sizeof(Partial) + 2 * rows * (a.cache.dim + 2) * (long long)sizeof(float));
 }
 
 template <int FORMAT, typename T, int D>
-int launch_decode(const cxs_cache_attend_call& call, int grid, cudaStream_t stream) {
+int launch_decode(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream) {
   using K = Decode<D>;
-  static int ready[kMaxDevices];
-  int device = 0;
-  CXS_CUDA(cudaGetDevice(&device));
-  if (device >= kMaxDevices || !__atomic_load_n(&ready[device], __ATOMIC_RELAXED)) {
+  static cxs_host::OncePerDevice ready;
+  const int status = ready.run([] {
     CXS_CUDA(cudaFuncSetAttribute(decode_kernel<FORMAT, T, D>,
                                   cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes));
-    if (device < kMaxDevices) __atomic_store_n(&ready[device], 1, __ATOMIC_RELAXED);
-  }
-  const int group = call.heads / call.cache.kv_heads;
-  for (int user0 = 0; user0 < call.cache.users; user0 += kSlice) {
-    cxs_cache_attend_call a = call;
-    const int left = call.cache.users - user0;
-    Shape z{group, user0, left < kSlice ? left : kSlice, left <= kSlice, grid, K::kWarps};
-    a.cache.table += user0 * call.cache.table_stride;
-    a.cache.lengths += user0;
-    if (a.cache.offsets) a.cache.offsets += user0;
-    decode_kernel<FORMAT, T, D><<<grid, K::kThreads, K::kBytes, stream>>>(a, z);
-    CXS_LAUNCH_CHECK("cache attend");
-    // The join starts while the last CTAs finish and waits for them on the device.
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(K::kRows * D / 4);
-    config.stream = stream;
-    cudaLaunchAttribute early = {};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D>, a, z));
-    CXS_LAUNCH_CHECK("cache attend join");
-  }
+    return (int)CXS_OK;
+  });
+  if (status != CXS_OK) return status;
+  decode_kernel<FORMAT, T, D><<<z.grid, K::kThreads, K::kBytes, stream>>>(a, z);
+  CXS_LAUNCH_CHECK("cache attend");
+  return CXS_OK;
+}
+
+template <typename T, int D>
+int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cudaStream_t stream) {
+  // Its CTAs may start while the last CTAs before finish; they wait for them
+  // on the device.
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(z.grid, few ? 1 : kTileRows / 16);
+  config.blockDim = dim3(16 * D / 4);
+  config.stream = stream;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  if (few)
+    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, 16>, a, z));
+  else
+    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, kTileRows>, a, z));
+  CXS_LAUNCH_CHECK("cache attend join");
   return CXS_OK;
 }
 
@@ -818,12 +666,36 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
   status = sm_count(&sms);
   if (status != CXS_OK) return status;
   const int grid = sms < kMostCtas ? sms : kMostCtas;
+  const bool few = few_rows(*call);
   cudaStream_t s = (cudaStream_t)stream;
-  CXS_CACHE_FORMAT(c.format, F, {
+  for (int user0 = 0; user0 < c.users; user0 += kSlice) {
+    cxs_cache_attend_call a = *call;
+    const int left = c.users - user0;
+    const Shape z{call->heads / c.kv_heads, user0, left < kSlice ? left : kSlice, left <= kSlice,
+                  grid, few ? Decode<64>::kWarps : 2};
+    a.cache.table += user0 * c.table_stride;
+    a.cache.lengths += user0;
+    if (a.cache.offsets) a.cache.offsets += user0;
+    if (few) {
+      CXS_CACHE_FORMAT(c.format, F, {
+        if (c.type == CXS_TYPE_BF16)
+          status = c.dim == 64 ? launch_decode<F, __nv_bfloat16, 64>(a, z, s)
+                               : launch_decode<F, __nv_bfloat16, 128>(a, z, s);
+        else
+          status = c.dim == 64 ? launch_decode<F, __half, 64>(a, z, s)
+                               : launch_decode<F, __half, 128>(a, z, s);
+      });
+    } else {
+      status = launch_tile(a, z, s);
+    }
+    if (status != CXS_OK) return status;
     if (c.type == CXS_TYPE_BF16)
-      return c.dim == 64 ? launch_decode<F, __nv_bfloat16, 64>(*call, grid, s)
-                         : launch_decode<F, __nv_bfloat16, 128>(*call, grid, s);
-    return c.dim == 64 ? launch_decode<F, __half, 64>(*call, grid, s)
-                       : launch_decode<F, __half, 128>(*call, grid, s);
-  });
+      status = c.dim == 64 ? launch_combine<__nv_bfloat16, 64>(a, z, few, s)
+                           : launch_combine<__nv_bfloat16, 128>(a, z, few, s);
+    else
+      status = c.dim == 64 ? launch_combine<__half, 64>(a, z, few, s)
+                           : launch_combine<__half, 128>(a, z, few, s);
+    if (status != CXS_OK) return status;
+  }
+  return CXS_OK;
 }

@@ -1,0 +1,173 @@
+// Attention over the dense 8-bit cache: what its kernels share.
+//
+// Mathematics. With codes c and scales s_k, s_v constant over a page, a score
+// in base-2 units is x = scale log2(e) s_k (q . c_k), and
+//   out = sum 2^x s_v c_v / sum 2^x = sum p c_v / sum p / s_v,
+//   p = 2^(x + log2 s_v - M),  M = running max of x + log2 s_v.
+// Folding s_v into the exponent keeps p <= 1 whatever the pages' scales, so p
+// is rounded to fp16 (11 bits) and multiplied with the codes themselves, which
+// fp16 holds exactly (e4m3 and integers to 128); the denominator divides each
+// page's sum of p by its s_v in fp32. Queries are scaled by a power of two per
+// row so that fp16 holds them: exact for fp16 inputs, and for bf16 (8 bits of
+// mantissa) but for parts 2^-28 below the row's largest element, which lose
+// less than 2^-39 of it.
+#pragma once
+
+#include "cache8.cuh"
+
+namespace cxs {
+namespace cache8 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kInf = INFINITY;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------ code conversion ---
+
+// Two codes (the low or high half of `w`) as fp16, exact.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t half2_of(uint32_t w, int high);
+template <>
+__device__ __forceinline__ uint32_t half2_of<CXS_FORMAT_E4M3>(uint32_t w, int high) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
+      : "=r"(r)
+      : "h"((unsigned short)(high ? w >> 16 : w & 0xffffu)));
+  return r;
+}
+// An integer v as 1024 + 128 + v (its bits in an fp16 mantissa), minus 1152.
+template <>
+__device__ __forceinline__ uint32_t half2_of<CXS_FORMAT_INT8>(uint32_t w, int high) {
+  const uint32_t biased = __byte_perm(w ^ 0x80808080u, 0x64646464u, high ? 0x4342 : 0x4140);
+  __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// ----------------------------------------------------------------- items ---
+//
+// An item is one user's tile of query rows (a row is a new token and one of
+// the KV head's query heads: row r is token r / group, head r % group) with
+// one KV head. Its work is a run of key tiles. All items' tiles, in order,
+// are cut into equal shares, one for each CTA, whatever the users' lengths;
+// an item whose tiles fall into several shares leaves a partial result (O, M,
+// l) in each, which combine_kernel joins in the order of the keys.
+
+constexpr int kSlice = 2048;  // users of one launch (their tile counts sit in shared memory)
+
+struct Shape {
+  int group;      // query heads of a KV head
+  int user0;      // first user of this launch (table, lengths and offsets point at it)
+  int users;
+  int last;       // the launch holds the last user
+  int grid;       // most CTAs
+  int min_tiles;  // fewest tiles worth a CTA
+};
+
+// One user's positions. Visible to some row: [begin, end).
+struct Span {
+  int first, count;     // packed rows
+  int start;            // position of the first row (negative: more rows than tokens)
+  int length;           // tokens, cut to the table
+  int begin;
+};
+
+__device__ __forceinline__ Span user_span(const cxs_cache_attend_call& a, const Shape& z, int user,
+                                          int* bad) {
+  const cxs_cache_call& c = a.cache;
+  Span s;
+  Rows rows;
+  if (c.offsets) {
+    rows = user_rows(c, user, bad);
+  } else {
+    rows = {z.user0 + user, 1};
+  }
+  const int most = c.width * c.page_size;
+  s.first = rows.first;
+  s.count = rows.count;
+  s.length = c.lengths[user];
+  if (s.length < 0) s.length = 0, *bad = 1;
+  s.start = s.length - rows.count;
+  if (s.length > most) s.length = most, *bad = 1;
+  s.begin = a.window > 0 && s.start >= a.window ? min(s.start - a.window + 1, s.length) : 0;
+  return s;
+}
+
+// Row r of a user sees positions [x, y).
+__device__ __forceinline__ int2 row_range(const cxs_cache_attend_call& a, const Span& s,
+                                          int token) {
+  const int position = s.start + token;
+  int hi = s.length, lo = 0;
+  if (a.causal && position + 1 < hi) hi = position + 1;
+  if (a.window > 0 && position >= a.window) lo = position - a.window + 1;
+  return make_int2(lo, hi);
+}
+
+// Shares: CTA c of n takes tiles [total c / n, total (c + 1) / n) (without the
+// product's overflow).
+__device__ __forceinline__ long long share(long long total, int c, int n) {
+  return total / n * c + total % n * c / n;
+}
+// The CTA whose share holds tile `tile` (total >= n).
+__device__ __forceinline__ int share_of(long long total, long long tile, int n) {
+  const long long guess = tile / (total / n);
+  int c = guess < n - 1 ? (int)guess : n - 1;
+  while (share(total, c, n) > tile) --c;
+  while (share(total, c + 1, n) <= tile) ++c;
+  return c;
+}
+
+struct alignas(16) Partial {  // the item that starts in a CTA's share and goes on past it
+  int parts;      // CTAs it falls into; 0: none
+  int first, rows, row0, kv_head;  // the item's packed first row, user's rows, first row, head
+};
+
+// Rows of no user (before the first offset, past the last, or more than
+// max_tokens of one user): zero, and nothing in the sum.
+template <typename T, int D>
+__device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int cta, int ctas) {
+  const cxs_cache_call& c = a.cache;
+  if (!c.offsets) return;
+  for (int b = cta - 1; b <= z.users; b += ctas) {
+    long long low, high;
+    if (b < 0) {
+      low = z.user0 == 0 ? 0 : 1;
+      high = z.user0 == 0 ? c.offsets[0] : 0;
+    } else if (b < z.users) {
+      int bad = 0;
+      const Rows rows = user_rows(c, b, &bad);
+      if (!bad) continue;
+      low = (long long)rows.first + rows.count;
+      high = c.offsets[b + 1];
+    } else {
+      low = z.last ? c.offsets[z.users] : 1;
+      high = z.last ? c.tokens : 0;
+    }
+    if (low < 0) low = 0;
+    if (high > c.tokens) high = c.tokens;
+    if (low >= high) continue;
+    for (long long i = low * a.heads * D + threadIdx.x; i < high * a.heads * D; i += blockDim.x)
+      ((T*)a.out)[i] = from_float<T>(0.f);
+    if (a.lse)
+      for (long long i = low * a.heads + threadIdx.x; i < high * a.heads; i += blockDim.x)
+        a.lse[i] = -kInf;
+  }
+}
+
+constexpr int kTileRows = 256;  // query rows of an item of the tile kernel
+
+// One launch of the tile kernel over z.users users (cache8_tile.cu).
+int launch_tile(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream);
+
+}  // namespace cache8
+}  // namespace cxs

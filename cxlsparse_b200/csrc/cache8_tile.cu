@@ -1,0 +1,712 @@
+// Attention over the dense 8-bit cache: many query rows a KV head (suffixes,
+// prefills), on tcgen05 with TMEM accumulators.
+//
+// An item is 256 query rows (two groups of 128) of one user and KV head; its
+// keys come in tiles of 128. One CTA per SM, 13 warps:
+//   warps 0-3, 4-7  softmax of group 0 and 1, one row a thread: reads S from
+//                   TMEM twice (maximum, then p = 2^(x - M)), writes p as fp16
+//                   over S, rescales O when M grows by more than 2^8
+//   warps 8-11      conversion: K and V codes global -> registers (one tile
+//                   ahead) -> fp16 in shared memory, shared by both groups
+//   warp 12         one thread issues every MMA: S = Q K^T (Q, K in shared
+//                   memory), O += P V (P in TMEM, V in shared memory)
+// While one group's softmax runs, the tensor core works for the other. The
+// MMAs of one thread complete in order, so S of the next tile may be issued
+// over P right after the P V that reads it, and a commit after S also tells
+// that the group's previous P V is done (O may be rescaled).
+// Waits are bounded: a wait that runs out sets the error word and an abort
+// flag that ends every role.
+#include "cache8_attend.cuh"
+#include "tile_tc.cuh"
+
+namespace {
+
+using namespace cxs::cache8;
+namespace tc = cxs::tc;
+
+constexpr int kKeys = 128;              // of a tile
+constexpr int kThreads = 13 * 32;
+constexpr int kConvertWarp = 8, kMmaWarp = 12;
+constexpr int kPanel = 128 * 128;       // bytes: 128 rows (queries or keys) of 64 channels, swizzled
+constexpr int kRuns = kKeys / 16;       // runs of 16 keys: each within one page
+constexpr int kTmem = 512;              // columns: S/P of two groups (128 each), O of two groups
+constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
+
+struct Run {     // what the softmax needs of a run of 16 keys
+  float factor;  // |scale| log2(e) s_k
+  float lift;    // log2 s_v
+  float per;     // 1 / s_v
+  int missing;   // no page: no row sees it
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kPanels = D / 64;
+  static constexpr int kQ = 0;                                   // [2 groups][panels]
+  static constexpr int kK = kQ + 2 * kPanels * kPanel;           // [2 stages][panels]
+  static constexpr int kV = kK + 2 * kPanels * kPanel;           // [2 stages][panels]
+  static constexpr int kRunsAt = kV + 2 * kPanels * kPanel;      // [4][kRuns]
+  static constexpr int kBars = kRunsAt + 4 * kRuns * (int)sizeof(Run);
+  static constexpr int kPrefix = kBars + 256;
+  static constexpr int kBytes = kPrefix + (kSlice + 1) * 8 + 1024;  // and the 1024-byte alignment
+};
+
+struct Bars {
+  uint64_t k_full[2], v_full[2], k_free[2], v_free[2];  // by stage
+  uint64_t s_full[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
+  uint64_t drain;
+  int abort;
+  uint32_t tmem;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+// Bounded wait on a barrier phase; false: some role of the CTA gave up.
+__device__ __forceinline__ bool wait(uint64_t* bar, int phase, Bars* b, int* error) {
+  if (cxs::mbar_try_wait(bar, phase & 1)) return true;
+  const long long start = clock64();
+  while (!cxs::mbar_try_wait(bar, phase & 1)) {
+    if (*(volatile int*)&b->abort) return false;
+    if (clock64() - start > kSpinLimit) {
+      report(error, CXS_DEVICE_ERR_COPY_TIMEOUT);
+      *(volatile int*)&b->abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// The same for a whole warp: every lane gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, int phase, Bars* b, int* error) {
+  return __all_sync(0xffffffffu, wait(bar, phase, b, error));
+}
+
+// Arrive for a warp whose lanes have all written what the barrier guards.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) cxs::mbar_arrive(bar);
+}
+
+// kind::f16 with fp16 operands and fp32 accumulation.
+__device__ __forceinline__ uint32_t idesc_f16(int m, int n, int b_mn_major) {
+  return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+// D += A B with A in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       int accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// An item and where its tiles lie among all tiles of the launch.
+struct Item {
+  int user, tile_row, kv_head;   // rows kTileRows * tile_row ..
+  long long begin, end;
+  Span span;
+  int rows;                      // of the user with this KV head
+  int first;                     // its first tile of keys
+};
+
+// Tiles of keys that some row of a row tile sees; at least one, so that rows
+// that see nothing are written.
+__device__ __forceinline__ int key_tiles(const cxs_cache_attend_call& a, const Shape& z,
+                                         const Span& s, int rows, int tile_row, int* first) {
+  const int row0 = tile_row * kTileRows, row1 = min(rows, row0 + kTileRows) - 1;
+  const int lo = row_range(a, s, row0 / z.group).x, hi = row_range(a, s, row1 / z.group).y;
+  *first = lo / kKeys;
+  const int n = (hi + kKeys - 1) / kKeys - *first;
+  return hi > 0 && n > 0 ? n : 1;
+}
+
+template <int FORMAT, typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    tile_kernel(const cxs_cache_attend_call a, const Shape z) {
+  using L = Layout<D>;
+  const cxs_cache_call& c = a.cache;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem =
+      (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Bars* const bars = (Bars*)(smem + L::kBars);
+  Run* const runs = (Run*)(smem + L::kRunsAt);
+  long long* const prefix = (long long*)(smem + L::kPrefix);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      cxs::mbar_init(&bars->k_full[i], 4);
+      cxs::mbar_init(&bars->v_full[i], 4);
+      cxs::mbar_init(&bars->k_free[i], 1);
+      cxs::mbar_init(&bars->v_free[i], 1);
+      cxs::mbar_init(&bars->s_full[i], 1);
+      cxs::mbar_init(&bars->p_full[i], 4);
+      cxs::mbar_init(&bars->q_full[i], 4);
+      cxs::mbar_init(&bars->o_done[i], 1);
+      cxs::mbar_init(&bars->o_free[i], 4);
+    }
+    cxs::mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    cxs::fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     cxs::smem_addr(&bars->tmem)),
+                 "r"(kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // Tiles before each user: a warp adds up a user's row tiles, one warp scans.
+  for (int b = warp; b < z.users; b += kThreads / 32) {
+    int bad = 0;
+    const Span s = user_span(a, z, b, &bad);
+    const int rows = s.count * z.group;
+    long long n = 0;
+    for (int r = lane; r * kTileRows < rows; r += 32) {
+      int first;
+      n += key_tiles(a, z, s, rows, r, &first);
+    }
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) {
+      prefix[b + 1] = n * c.kv_heads;
+      if (bad && blockIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long base = 0;
+    if (lane == 0) prefix[0] = 0;
+    for (int b0 = 0; b0 < z.users; b0 += 32) {
+      const int b = b0 + lane;
+      long long sum = b < z.users ? prefix[b + 1] : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      if (b < z.users) prefix[b + 1] = base + sum;
+      base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = bars->tmem;
+  const long long total = prefix[z.users];
+  const long long wanted = (total + z.min_tiles - 1) / z.min_tiles;
+  const int ctas = wanted < z.grid ? (int)wanted : z.grid;
+  Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
+  Partial& mine = partials[blockIdx.x];
+  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) mine.parts = 0;
+  const bool busy = (int)blockIdx.x < ctas;
+  const long long lo = busy ? share(total, blockIdx.x, ctas) : 0;
+  const long long hi = busy ? share(total, blockIdx.x + 1, ctas) : 0;
+  float* const scratch = reinterpret_cast<float*>(partials + z.grid) +
+                         (long long)blockIdx.x * 2 * kTileRows * (D + 2);
+
+  // The item that holds the share's first tile; every warp finds it.
+  Item item = {};
+  if (lo < hi) {
+    int l = 0, h = z.users - 1;
+    while (l < h) {
+      const int m = (l + h) / 2;
+      if (prefix[m + 1] > lo) h = m; else l = m + 1;
+    }
+    int bad = 0;
+    item.user = l;
+    item.span = user_span(a, z, l, &bad);
+    item.rows = item.span.count * z.group;
+    long long before = prefix[l];  // tiles before row tile r0
+    for (int r0 = 0;; r0 += 32) {
+      const int r = r0 + lane;
+      int first = 0;
+      const int n = r * kTileRows < item.rows ? key_tiles(a, z, item.span, item.rows, r, &first) : 0;
+      long long sum = (long long)n * c.kv_heads;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > lo);
+      if (past || (r0 + 32) * (long long)kTileRows >= item.rows) {
+        const int at = past ? __ffs(past) - 1 : 31;
+        const int tiles = __shfl_sync(0xffffffffu, n, at);
+        const long long start = before + __shfl_sync(0xffffffffu, sum, at) -
+                                (long long)tiles * c.kv_heads;
+        item.tile_row = r0 + at;
+        item.first = __shfl_sync(0xffffffffu, first, at);
+        item.kv_head = (int)((lo - start) / tiles);
+        item.begin = start + (long long)item.kv_head * tiles;
+        item.end = item.begin + tiles;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  // The item after `p` (there is one: its tiles end before the share does).
+  auto next = [&](Item& p) {
+    const long long n = p.end - p.begin;
+    p.begin = p.end;
+    if (++p.kv_head < c.kv_heads) {
+      p.end = p.begin + n;
+      return;
+    }
+    p.kv_head = 0;
+    ++p.tile_row;
+    if ((long long)p.tile_row * kTileRows >= p.rows) {
+      do ++p.user;
+      while (prefix[p.user + 1] <= p.begin);
+      int bad = 0;
+      p.span = user_span(a, z, p.user, &bad);
+      p.rows = p.span.count * z.group;
+      p.tile_row = 0;
+    }
+    p.end = p.begin + key_tiles(a, z, p.span, p.rows, p.tile_row, &p.first);
+  };
+  // Whether the item has rows for group g.
+  auto active = [&](const Item& p, int g) { return p.rows - p.tile_row * kTileRows > 128 * g; };
+
+  if (warp < kConvertWarp) {
+    // ------------------------------------------------------------ softmax ---
+    const int g = warp / 4, r = threadIdx.x % 128;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t s_at = tmem + lanes + 128 * g, o_at = tmem + lanes + 256 + D * g;
+    uint8_t* const q_panels = smem + L::kQ + g * L::kPanels * kPanel;
+    int tiles = 0;    // of the share
+    int mine_s = 0;   // tiles of this group
+    int mine_i = 0;   // items of this group
+    float back = 1.f, back_next = 1.f;
+
+    // The row's query, scaled by a power of two (and the scale's sign), into
+    // the group's Q panels. Returns the power's inverse.
+    auto load_query = [&](const Item& p) -> float {
+      const int row = p.tile_row * kTileRows + 128 * g + r;
+      const bool live = row < p.rows;
+      const T* from = (const T*)a.query;
+      if (live)
+        from += (long long)(p.span.first + row / z.group) * a.q_token_stride +
+                (long long)(p.kv_head * z.group + row % z.group) * a.q_head_stride;
+      const bool wide = ((uintptr_t)from & 15) == 0;
+      auto eight = [&](T (&x)[8], int i) {
+        if (wide) {
+          *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = from[8 * i + j];
+        }
+      };
+      // Twice: once for the largest element, once (from L1) for the values,
+      // rather than a row in registers.
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        alignas(16) T x[8];
+        eight(x, i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = fabsf(to_float(x[j]));
+          if (v < kInf) top = fmaxf(top, v);
+        }
+      }
+      int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+      if (e < -100) e = -100;
+      if (top == 0.f) e = 14;
+      float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      if (a.scale < 0.f) up = -up;
+      if (a.scale == 0.f) up = 0.f;  // every score is 0
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        alignas(16) T x[8];
+        eight(x, i);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = live ? to_float(x[j]) * up : 0.f;
+        *reinterpret_cast<uint4*>(q_panels + i / 8 * kPanel + tc::sw128_chunk(r, i % 8)) =
+            make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
+                       pack_half2(v[6], v[7]));
+      }
+      cxs::fence_proxy_async_shared();
+      warp_arrive(&bars->q_full[g], lane);
+      return __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    };
+
+    bool loaded = false;
+    for (long long tile = lo; tile < hi;) {
+      const long long until = item.end < hi ? item.end : hi;
+      const int count = (int)(until - tile);
+      const bool more = until < hi;
+      if (!active(item, g)) {
+        tiles += count;
+        tile = until;
+        if (more) next(item);
+        continue;
+      }
+      if (!loaded) back_next = load_query(item);
+      back = back_next;
+      loaded = false;
+      const int row = item.tile_row * kTileRows + 128 * g + r;
+      const int2 see = row < item.rows ? row_range(a, item.span, row / z.group)
+                                       : make_int2(0, item.span.length);
+      float m = -kInf, l = 0.f;
+      int key0 = (item.first + (int)(tile - item.begin)) * kKeys;
+      for (int i = 0; i < count; ++i, ++tiles, ++mine_s, key0 += kKeys) {
+        // (The runs were written before the K that S was computed from.)
+        if (!warp_wait(&bars->s_full[g], mine_s, bars, c.error)) goto done;
+        tc::fence_after();
+        const Run* const run = runs + (tiles & 3) * kRuns;
+        const int from = see.x - key0, to = see.y - key0;  // visible columns
+        bool whole = from <= 0 && to >= kKeys;
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) whole = whole && !run[u].missing;
+        const bool masked = !__all_sync(0xffffffffu, whole);
+        auto hide = [&](float (&x)[32], int at) {  // columns at .. at + 31
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (at + e < from || at + e >= to || run[(at + e) / 16].missing) x[e] = -kInf;
+        };
+        // Never 0, which times a hidden score would be NaN (scores that small
+        // are 0 either way); NaN stays NaN.
+        auto factor_of = [&](const Run& u) {
+          const float f = u.factor * back;
+          return f < 1.2e-38f ? 1.2e-38f : f;
+        };
+        float top = -kInf;
+#pragma unroll
+        for (int q = 0; q < kKeys / 32; ++q) {
+          float x[32];
+          tc::ld32(s_at + 32 * q, x);
+          if (masked) hide(x, 32 * q);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float t = x[16 * h];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) t = fmaxf(t, x[16 * h + e]);
+            const Run& u = run[2 * q + h];
+            top = fmaxf(top, fmaf(t, factor_of(u), u.lift));
+          }
+        }
+        // M moves when a score passes it by 2^8: p stays below 2^8, exact in
+        // fp16's range, and most tiles leave O as it is.
+        const bool grows = top > m + 8.f;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float fresh = grows ? top : m;
+          const float f = grows ? (m == -kInf ? 0.f : ex2(m - fresh)) : 1.f;
+          m = fresh;
+          l *= f;
+          if (i > 0) {
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              float o[32];
+              tc::ld32(o_at + 32 * q, o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tc::st32(o_at + 32 * q, o);
+            }
+          }
+        }
+        const float base = m == -kInf ? 0.f : m;
+#pragma unroll
+        for (int q = 0; q < kKeys / 32; ++q) {
+          float x[32];
+          tc::ld32(s_at + 32 * q, x);
+          if (masked) hide(x, 32 * q);
+          uint32_t p[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const Run& u = run[2 * q + h];
+            const float f = factor_of(u), shift = u.lift - base;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float p0 = ex2(fmaf(x[16 * h + e], f, shift));
+              const float p1 = ex2(fmaf(x[16 * h + e + 1], f, shift));
+              s0 += p0;
+              s1 += p1;
+              p[8 * h + e / 2] = pack_half2(p0, p1);
+            }
+            l = fmaf(s0 + s1, u.per, l);
+          }
+          st16(s_at + 16 * q, p);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        warp_arrive(&bars->p_full[g], lane);
+      }
+      // Load the next item's queries (its S may start while this one ends).
+      const Item ended = item;
+      const long long started = tile;
+      tile = until;
+      if (more) {
+        next(item);
+        if (active(item, g)) {
+          back_next = load_query(item);
+          loaded = true;
+        }
+      }
+      if (!warp_wait(&bars->o_done[g], mine_i, bars, c.error)) goto done;
+      ++mine_i;
+      tc::fence_after();
+      const bool complete = started == ended.begin && until == ended.end;
+      float* const part = scratch + (started == ended.begin ? kTileRows * (D + 2) : 0);
+      const bool some = !(l == 0.f);
+      const float inv = some ? 1.f / l : 0.f;
+      const long long head = (long long)(ended.span.first + row / z.group) * a.heads +
+                             ended.kv_head * z.group + row % z.group;
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        float o[32];
+        __syncwarp();
+        tc::ld32(o_at + 32 * q, o);
+        if (row < ended.rows && complete) {
+          T* out = (T*)a.out + head * D + 32 * q;
+          alignas(16) T y[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = from_float<T>(some ? o[e] * inv : 0.f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            reinterpret_cast<uint4*>(out)[e] = reinterpret_cast<const uint4*>(y)[e];
+        } else if (row < ended.rows) {
+          float4* out = reinterpret_cast<float4*>(part + (128 * g + r) * D + 32 * q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            out[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+      tc::fence_before();
+      warp_arrive(&bars->o_free[g], lane);
+      if (row < ended.rows) {
+        if (complete) {
+          if (a.lse) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+        } else {
+          part[kTileRows * D + 2 * (128 * g + r)] = m;
+          part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
+        }
+      }
+      if (!complete && started == ended.begin && g == 0 && r == 0) {
+        const int last = share_of(total, ended.end - 1, ctas);
+        mine.first = ended.span.first;
+        mine.rows = ended.rows;
+        mine.row0 = ended.tile_row * kTileRows;
+        mine.kv_head = ended.kv_head;
+        mine.parts = last - (int)blockIdx.x + 1;
+      }
+    }
+  } else if (warp < kMmaWarp) {
+    // --------------------------------------------------------- conversion ---
+    constexpr int kChunks = D / 16;             // 16-byte chunks of a key
+    constexpr int kStep = 128 / kChunks;        // keys of one pass of the 128 threads
+    constexpr int kPasses = kKeys / kStep;
+    const int i = threadIdx.x - 32 * kConvertWarp, key = i / kChunks, chunk = i % kChunks;
+    const int entries = kKeys / c.page_size;
+    const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+    const int page_bits = __ffs(c.page_size) - 1;
+    uint4 kc[kPasses], vc[kPasses];
+    float sk = 0.f, sv = 0.f;
+    int gone = 0;
+    long long next_tile = lo;                   // the tile to load next
+    int ids = -1;
+    // Lane e: the page of the e-th page of the tile to load next.
+    auto look_up = [&]() {
+      ids = -1;
+      if (next_tile >= hi) return;
+      const int at = (item.first + (int)(next_tile - item.begin)) * kKeys + lane * c.page_size;
+      if (lane < entries && at < item.span.length && at + c.page_size > item.span.begin) {
+        ids = c.table[item.user * c.table_stride + (at >> page_bits)];
+        if (ids < 0 || ids >= c.pages) {
+          ids = -1;
+          report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
+        }
+      }
+    };
+    // part 0: K and the scales, part 1: V, of the tile to load next.
+    auto load = [&](uint4 (&to)[kPasses], int part) {
+      const int key0 = (item.first + (int)(next_tile - item.begin)) * kKeys;
+#pragma unroll
+      for (int j = 0; j < kPasses; ++j) {
+        const int at = j * kStep + key;
+        const int id = __shfl_sync(0xffffffffu, ids, at >> page_bits);
+        const bool live = id >= 0 && key0 + at < item.span.length;
+        const long long cell = ((long long)id * c.kv_heads + item.kv_head) * 2 + part;
+        const uint8_t* from = (const uint8_t*)c.codes +
+                              (cell * c.page_size + (at & (c.page_size - 1))) * D + chunk * 16;
+        to[j] = live ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+      }
+      if (part == 0 && warp == kConvertWarp) {
+        const int id = __shfl_sync(0xffffffffu, ids, lane % kRuns * 16 >> page_bits);
+        gone = id < 0;
+        const float* from = c.scales + ((long long)id * c.kv_heads + item.kv_head) * 2;
+        sk = gone || lane >= kRuns ? 1.f : from[0];
+        sv = gone || lane >= kRuns ? 1.f : from[1];
+      }
+    };
+    auto advance = [&]() {
+      ++next_tile;
+      if (next_tile >= hi) return;
+      if (next_tile >= item.end) next(item);
+      look_up();
+    };
+    auto convert = [&](const uint4 (&from)[kPasses], uint8_t* panels) {
+#pragma unroll
+      for (int j = 0; j < kPasses; ++j) {
+        const int at = j * kStep + key, first = chunk % 4 * 2, swap = chunk / 4 & 1;
+        const uint4 w = from[j];
+        const uint4 a0 = make_uint4(half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1),
+                                    half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
+        const uint4 a1 = make_uint4(half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1),
+                                    half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
+        uint8_t* const to = panels + chunk / 4 * kPanel;
+        // Lanes of the second panel write their halves in the other order:
+        // eight lanes then cover all banks.
+        *reinterpret_cast<uint4*>(to + tc::sw128_chunk(at, first + swap)) = swap ? a1 : a0;
+        *reinterpret_cast<uint4*>(to + tc::sw128_chunk(at, first + 1 - swap)) = swap ? a0 : a1;
+      }
+    };
+    if (lo < hi) {
+      look_up();
+      load(kc, 0);
+      load(vc, 1);
+      const long long n = hi - lo;
+      advance();
+      for (int t = 0; t < n; ++t) {
+        const int stage = t & 1;
+        const bool more = next_tile < hi;
+        if (!warp_wait(&bars->k_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
+        convert(kc, smem + L::kK + stage * L::kPanels * kPanel);
+        if (warp == kConvertWarp && lane < kRuns) {
+          Run u;
+          u.factor = usable_scale(sk) * unit;
+          u.lift = __log2f(usable_scale(sv));
+          u.per = __frcp_rn(usable_scale(sv));
+          u.missing = gone;
+          runs[(t & 3) * kRuns + lane] = u;
+        }
+        cxs::fence_proxy_async_shared();
+        warp_arrive(&bars->k_full[stage], lane);
+        if (more) load(kc, 0);
+        if (!warp_wait(&bars->v_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
+        convert(vc, smem + L::kV + stage * L::kPanels * kPanel);
+        cxs::fence_proxy_async_shared();
+        warp_arrive(&bars->v_full[stage], lane);
+        if (more) {
+          load(vc, 1);
+          advance();
+        }
+      }
+    }
+  } else if (lane == 0 && lo < hi) {
+    // ---------------------------------------------------------------- MMAs ---
+    const uint32_t base = cxs::smem_addr(smem);
+    const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, 64, 1);
+    struct Place {
+      Item item;
+      long long tile;
+      int n;        // tiles since the share's start
+      int items[2]; // items started, by group
+    };
+    Place s{item, lo, 0, {0, 0}}, p{item, lo, 0, {0, 0}};
+    int n_p[2] = {0, 0};
+    bool fine = true;
+    auto step = [&](Place& x) {  // to the next tile
+      ++x.tile;
+      ++x.n;
+      if (x.tile < hi && x.tile >= x.item.end) next(x.item);
+    };
+    auto starts = [&](const Place& x) { return x.tile == x.item.begin || x.tile == lo; };
+    auto issue_s = [&](int g) {
+      if (starts(s)) {
+        if (!(fine = wait(&bars->q_full[g], s.items[g], bars, c.error))) return;
+        ++s.items[g];
+      }
+      if (!(fine = wait(&bars->k_full[s.n & 1], s.n >> 1, bars, c.error))) return;
+      tc::fence_after();
+      const uint32_t q = base + L::kQ + g * L::kPanels * kPanel;
+      const uint32_t k = base + L::kK + (s.n & 1) * L::kPanels * kPanel;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        tc::mma(tmem + 128 * g, tc::desc_sw128(q + i / 4 * kPanel + 32 * (i % 4), 16, 1024),
+                tc::desc_sw128(k + i / 4 * kPanel + 32 * (i % 4), 16, 1024), id_s, i > 0);
+      tc::commit(&bars->s_full[g]);
+      if (g == 1 || !active(s.item, 1)) tc::commit(&bars->k_free[s.n & 1]);
+    };
+    auto issue_o = [&](int g) {
+      const bool first = starts(p);
+      if (!(fine = wait(&bars->p_full[g], n_p[g], bars, c.error))) return;
+      ++n_p[g];
+      if (!(fine = wait(&bars->v_full[p.n & 1], p.n >> 1, bars, c.error))) return;
+      if (first) {
+        if (p.items[g] > 0 && !(fine = wait(&bars->o_free[g], p.items[g] - 1, bars, c.error))) return;
+        ++p.items[g];
+      }
+      tc::fence_after();
+      const uint32_t v = base + L::kV + (p.n & 1) * L::kPanels * kPanel;
+#pragma unroll
+      for (int h = 0; h < L::kPanels; ++h)
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_ts(tmem + 256 + D * g + 64 * h, tmem + 128 * g + 8 * i,
+                 tc::desc_sw128(v + h * kPanel + 2048 * i, 16, 1024), id_o, !first || i > 0);
+      if (g == 1 || !active(p.item, 1)) tc::commit(&bars->v_free[p.n & 1]);
+      if (p.tile + 1 == hi || p.tile + 1 == p.item.end) tc::commit(&bars->o_done[g]);
+    };
+    issue_s(0);
+    if (fine && active(s.item, 1)) issue_s(1);
+    step(s);
+    while (fine && p.tile < hi) {
+      const bool more = s.tile < hi;
+      issue_o(0);
+      if (fine && more) issue_s(0);
+      if (fine && active(p.item, 1)) issue_o(1);
+      if (fine && more && active(s.item, 1)) issue_s(1);
+      if (more) step(s);
+      step(p);
+    }
+    if (!fine) {  // let the MMAs in flight end before TMEM is freed
+      tc::commit(&bars->drain);
+      const long long start = clock64();
+      while (!cxs::mbar_try_wait(&bars->drain, 0) && clock64() - start < kSpinLimit) {
+      }
+    }
+  }
+done:
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
+}
+
+template <int FORMAT, typename T, int D>
+int launch(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream) {
+  static cxs_host::OncePerDevice ready;
+  const int status = ready.run([] {
+    CXS_CUDA(cudaFuncSetAttribute(tile_kernel<FORMAT, T, D>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes));
+    return (int)CXS_OK;
+  });
+  if (status != CXS_OK) return status;
+  tile_kernel<FORMAT, T, D><<<z.grid, kThreads, Layout<D>::kBytes, stream>>>(a, z);
+  CXS_LAUNCH_CHECK("cache attend");
+  return CXS_OK;
+}
+
+}  // namespace
+
+int cxs::cache8::launch_tile(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream) {
+  CXS_CACHE_FORMAT(a.cache.format, F, {
+    if (a.cache.type == CXS_TYPE_BF16)
+      return a.cache.dim == 64 ? launch<F, __nv_bfloat16, 64>(a, z, stream)
+                               : launch<F, __nv_bfloat16, 128>(a, z, stream);
+    return a.cache.dim == 64 ? launch<F, __half, 64>(a, z, stream)
+                             : launch<F, __half, 128>(a, z, stream);
+  });
+}
