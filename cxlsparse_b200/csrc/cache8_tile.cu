@@ -2,10 +2,10 @@
 // prefills), on tcgen05 with TMEM accumulators.
 //
 // An item is 256 query rows (two groups of 128) of one user and KV head; its
-// keys come in tiles of 128. One CTA per SM, 13 warps:
+// keys come in tiles of 128. One CTA per SM, 16 warps:
 //   warps 0-3, 4-7  softmax of group 0 and 1, one row a thread: reads S from
-//                   TMEM twice (maximum, then p = 2^(x - M)), writes p as fp16
-//                   over S, rescales O when M grows by more than 2^8
+//                   TMEM, writes p = 2^(x - M) as fp16 over S, rescales O when
+//                   M grows by more than 2^8
 //   warps 8-11      conversion: K and V codes global -> registers (one tile
 //                   ahead) -> fp16 in shared memory, shared by both groups
 //   warp 12         one thread issues every MMA: S = Q K^T (Q, K in shared
@@ -25,12 +25,31 @@ using namespace cxs::cache8;
 namespace tc = cxs::tc;
 
 constexpr int kKeys = 128;              // of a tile
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;  // the last three warps only share the setup
 constexpr int kConvertWarp = 8, kMmaWarp = 12;
 constexpr int kPanel = 128 * 128;       // bytes: 128 rows (queries or keys) of 64 channels, swizzled
 constexpr int kRuns = kKeys / 16;       // runs of 16 keys: each within one page
 constexpr int kTmem = 512;              // columns: S/P of two groups (128 each), O of two groups
 constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
+
+// What the MMA warp needs of a tile.
+constexpr int kFirst = 1, kLast = 2, kTwo = 4;  // of its item here; rows for group 1
+
+// Registers a thread by role: twice the softmax's, the conversion's and the
+// MMA warp's, times 128, are the 64 K that 512 threads of 128 are launched with.
+template <int D>
+struct Registers {
+  static constexpr int kSoftmax = D == 64 ? 160 : 144, kConvert = D == 64 ? 128 : 160, kMma = 64;
+  static_assert(2 * kSoftmax + kConvert + kMma == 4 * 128, "all of the block's registers");
+};
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct Run {     // what the softmax needs of a run of 16 keys
   float factor;  // |scale| log2(e) s_k
@@ -57,6 +76,7 @@ struct Bars {
   uint64_t drain;
   int abort;
   uint32_t tmem;
+  int flags[4];  // of the tiles in work
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
 
@@ -92,13 +112,51 @@ __device__ __forceinline__ uint32_t idesc_f16(int m, int n, int b_mn_major) {
          ((uint32_t)(m >> 4) << 24);
 }
 
-// D += A B with A in TMEM.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       int accumulate) {
+// D (+)= A B; A in shared memory, or (mma_ts) in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((int)accumulate));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((int)accumulate));
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one;
+}
+
+// 64 fp32 columns of this warp's 32 lanes (the wait is part of the statement:
+// nothing can use, move or spill the registers before they are written).
+__device__ __forceinline__ void ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,"
+      "%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]),
+        "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]),
+        "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
 }
 
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -141,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Bars* const bars = (Bars*)(smem + L::kBars);
   Run* const runs = (Run*)(smem + L::kRunsAt);
   long long* const prefix = (long long*)(smem + L::kPrefix);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // (Broadcast: uniform across the warp also for the compiler.)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -199,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
   const long long total = prefix[z.users];
   const long long wanted = (total + z.min_tiles - 1) / z.min_tiles;
   const int ctas = wanted < z.grid ? (int)wanted : z.grid;
@@ -277,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kConvertWarp) {
     // ------------------------------------------------------------ softmax ---
+    more_registers<Registers<D>::kSoftmax>();
     const int g = warp / 4, r = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + 128 * g, o_at = tmem + lanes + 256 + D * g;
@@ -284,80 +344,127 @@ __global__ void __launch_bounds__(kThreads, 1)
     int tiles = 0;    // of the share
     int mine_s = 0;   // tiles of this group
     int mine_i = 0;   // items of this group
-    float back = 1.f, back_next = 1.f;
-
-    // The row's query, scaled by a power of two (and the scale's sign), into
-    // the group's Q panels. Returns the power's inverse.
-    auto load_query = [&](const Item& p) -> float {
-      const int row = p.tile_row * kTileRows + 128 * g + r;
-      const bool live = row < p.rows;
-      const T* from = (const T*)a.query;
-      if (live)
-        from += (long long)(p.span.first + row / z.group) * a.q_token_stride +
-                (long long)(p.kv_head * z.group + row % z.group) * a.q_head_stride;
-      const bool wide = ((uintptr_t)from & 15) == 0;
-      auto eight = [&](T (&x)[8], int i) {
-        if (wide) {
-          *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i];
-        } else {
+    float m = -kInf, l = 0.f, back = 1.f;
+    bool pending = false;  // an item whose O is still in TMEM:
+    Item ended = {};
+    long long started = lo;
+    long long tile = lo;
+    while (true) {
+      for (; tile < hi && !active(item, g);) {  // items without rows for this group
+        const long long until = item.end < hi ? item.end : hi;
+        tiles += (int)(until - tile);
+        tile = until;
+        if (until < hi) next(item);
+      }
+      if (tile < hi) {
+        // The row's query, scaled by a power of two (and the scale's sign),
+        // into the group's Q panels, before the last item's O is written: S
+        // of this item may start meanwhile. Twice: once for the largest
+        // element, once (from L1) for the values.
+        const int row = item.tile_row * kTileRows + 128 * g + r;
+        const bool live = row < item.rows;
+        const T* from = (const T*)a.query;
+        if (live)
+          from += (long long)(item.span.first + row / z.group) * a.q_token_stride +
+                  (long long)(item.kv_head * z.group + row % z.group) * a.q_head_stride;
+        const bool wide = ((uintptr_t)from & 15) == 0;
+        float top = 0.f, up = 1.f;
+#pragma unroll 1
+        for (int i = 0; i < D / 4; ++i) {
+          alignas(16) T x[8];
+          if (wide) {
+            *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i % (D / 8)];
+          } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = from[8 * i + j];
+            for (int j = 0; j < 8; ++j) x[j] = from[8 * (i % (D / 8)) + j];
+          }
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = live ? to_float(x[j]) : 0.f;
+          if (i < D / 8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (fabsf(v[j]) < kInf) top = fmaxf(top, fabsf(v[j]));
+            if (i == D / 8 - 1) {
+              int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+              if (e < -100) e = -100;
+              if (top == 0.f) e = 14;
+              up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+              if (a.scale < 0.f) up = -up;
+              if (a.scale == 0.f) up = 0.f;  // every score is 0
+              back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+            }
+          } else {
+            const int k = i - D / 8;
+            *reinterpret_cast<uint4*>(q_panels + k / 8 * kPanel + tc::sw128_chunk(r, k % 8)) =
+                make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
+                           pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
+          }
         }
-      };
-      // Twice: once for the largest element, once (from L1) for the values,
-      // rather than a row in registers.
-      float top = 0.f;
+        cxs::fence_proxy_async_shared();
+        warp_arrive(&bars->q_full[g], lane);
+      }
+      if (pending) {
+        // The ended item's O: the result, or this share's part of it.
+        if (!warp_wait(&bars->o_done[g], mine_i, bars, c.error)) goto done;
+        ++mine_i;
+        tc::fence_after();
+        const long long until = ended.end < hi ? ended.end : hi;
+        const bool complete = started == ended.begin && until == ended.end;
+        float* const part = scratch + (started == ended.begin ? kTileRows * (D + 2) : 0);
+        const bool some = !(l == 0.f);
+        const float inv = some ? 1.f / l : 0.f;
+        const int row = ended.tile_row * kTileRows + 128 * g + r;
+        const bool live = row < ended.rows;
+        const long long head = (long long)(ended.span.first + row / z.group) * a.heads +
+                               ended.kv_head * z.group + row % z.group;
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          float o[32];
+          __syncwarp();
+          tc::ld32(o_at + 32 * q, o);
+          if (live && complete) {
+            alignas(16) T y[32];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        alignas(16) T x[8];
-        eight(x, i);
+            for (int e = 0; e < 32; ++e) y[e] = from_float<T>(some ? o[e] * inv : 0.f);
+            uint4* out = reinterpret_cast<uint4*>((T*)a.out + head * D + 32 * q);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = fabsf(to_float(x[j]));
-          if (v < kInf) top = fmaxf(top, v);
+            for (int e = 0; e < 4; ++e) out[e] = reinterpret_cast<const uint4*>(y)[e];
+          } else if (live) {
+            float4* out = reinterpret_cast<float4*>(part + (128 * g + r) * D + 32 * q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              out[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        tc::fence_before();
+        warp_arrive(&bars->o_free[g], lane);
+        if (live && complete) {
+          if (a.lse) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+        } else if (live) {
+          part[kTileRows * D + 2 * (128 * g + r)] = m;
+          part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
+        }
+        if (!complete && started == ended.begin && g == 0 && r == 0) {
+          const int last = share_of(total, ended.end - 1, ctas);
+          mine.first = ended.span.first;
+          mine.rows = ended.rows;
+          mine.row0 = ended.tile_row * kTileRows;
+          mine.kv_head = ended.kv_head;
+          mine.parts = last - (int)blockIdx.x + 1;
         }
       }
-      int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-      if (e < -100) e = -100;
-      if (top == 0.f) e = 14;
-      float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-      if (a.scale < 0.f) up = -up;
-      if (a.scale == 0.f) up = 0.f;  // every score is 0
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        alignas(16) T x[8];
-        eight(x, i);
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = live ? to_float(x[j]) * up : 0.f;
-        *reinterpret_cast<uint4*>(q_panels + i / 8 * kPanel + tc::sw128_chunk(r, i % 8)) =
-            make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
-                       pack_half2(v[6], v[7]));
-      }
-      cxs::fence_proxy_async_shared();
-      warp_arrive(&bars->q_full[g], lane);
-      return __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-    };
+      if (tile >= hi) break;
 
-    bool loaded = false;
-    for (long long tile = lo; tile < hi;) {
       const long long until = item.end < hi ? item.end : hi;
       const int count = (int)(until - tile);
-      const bool more = until < hi;
-      if (!active(item, g)) {
-        tiles += count;
-        tile = until;
-        if (more) next(item);
-        continue;
-      }
-      if (!loaded) back_next = load_query(item);
-      back = back_next;
-      loaded = false;
       const int row = item.tile_row * kTileRows + 128 * g + r;
       const int2 see = row < item.rows ? row_range(a, item.span, row / z.group)
                                        : make_int2(0, item.span.length);
-      float m = -kInf, l = 0.f;
+      m = -kInf;
+      l = 0.f;
       int key0 = (item.first + (int)(tile - item.begin)) * kKeys;
+#pragma unroll 1
       for (int i = 0; i < count; ++i, ++tiles, ++mine_s, key0 += kKeys) {
         // (The runs were written before the K that S was computed from.)
         if (!warp_wait(&bars->s_full[g], mine_s, bars, c.error)) goto done;
@@ -368,185 +475,160 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int u = 0; u < kRuns; ++u) whole = whole && !run[u].missing;
         const bool masked = !__all_sync(0xffffffffu, whole);
-        auto hide = [&](float (&x)[32], int at) {  // columns at .. at + 31
+        // Columns 32 q .. 32 q + 31 of S in x become probabilities over S. M
+        // moves when a score passes it by 2^8 (p then stays below 2^8, well
+        // inside fp16's range): rare, so S is read once and what was computed
+        // with the older M (O, l, the tile's earlier probabilities) follows it.
+        auto chunk = [&](uint32_t* x, int q) {
+          if (masked) {  // what the row does not see becomes -infinity
+            const int low = min(max(from - 32 * q, 0), 32), high = min(max(to - 32 * q, 0), 32);
+            unsigned seen =
+                (high == 32 ? ~0u : (1u << high) - 1) & ~(low == 32 ? ~0u : (1u << low) - 1);
+            if (run[2 * q].missing) seen &= 0xffff0000u;
+            if (run[2 * q + 1].missing) seen &= 0x0000ffffu;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (at + e < from || at + e >= to || run[(at + e) / 16].missing) x[e] = -kInf;
-        };
-        // Never 0, which times a hidden score would be NaN (scores that small
-        // are 0 either way); NaN stays NaN.
-        auto factor_of = [&](const Run& u) {
-          const float f = u.factor * back;
-          return f < 1.2e-38f ? 1.2e-38f : f;
-        };
-        float top = -kInf;
-#pragma unroll
-        for (int q = 0; q < kKeys / 32; ++q) {
-          float x[32];
-          tc::ld32(s_at + 32 * q, x);
-          if (masked) hide(x, 32 * q);
+            for (int e = 0; e < 32; ++e) x[e] = seen >> e & 1 ? x[e] : 0xff800000u;
+          }
+          float factor[2], lift[2], per[2], top = -kInf;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float t = x[16 * h];
+            const Run u = run[2 * q + h];
+            // Never 0, which times a hidden score would be NaN (scores that
+            // small are 0 either way); NaN stays NaN.
+            const float f = u.factor * back;
+            factor[h] = f < 1.2e-38f ? 1.2e-38f : f;
+            lift[h] = u.lift;
+            per[h] = u.per;
+            float t = __uint_as_float(x[16 * h]);
 #pragma unroll
-            for (int e = 1; e < 16; ++e) t = fmaxf(t, x[16 * h + e]);
-            const Run& u = run[2 * q + h];
-            top = fmaxf(top, fmaf(t, factor_of(u), u.lift));
+            for (int e = 1; e < 15; e += 2)
+              t = fmaxf(fmaxf(t, __uint_as_float(x[16 * h + e])), __uint_as_float(x[16 * h + e + 1]));
+            t = fmaxf(t, __uint_as_float(x[16 * h + 15]));
+            top = fmaxf(top, fmaf(t, factor[h], lift[h]));
           }
-        }
-        // M moves when a score passes it by 2^8: p stays below 2^8, exact in
-        // fp16's range, and most tiles leave O as it is.
-        const bool grows = top > m + 8.f;
-        if (__any_sync(0xffffffffu, grows)) {
-          const float fresh = grows ? top : m;
-          const float f = grows ? (m == -kInf ? 0.f : ex2(m - fresh)) : 1.f;
-          m = fresh;
-          l *= f;
-          if (i > 0) {
+          const bool grows = top > m + 8.f;
+          if (__any_sync(0xffffffffu, grows)) {
+            const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
+            if (grows) m = top;
+            l *= f;
+            tc::wait_st();
+            if (i > 0) {
+#pragma unroll 1
+              for (int d = 0; d < D; d += 16) {
+                float o[16];
+                tc::ld16(o_at + d, o);
 #pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              float o[32];
-              tc::ld32(o_at + 32 * q, o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tc::st32(o_at + 32 * q, o);
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                tc::st16(o_at + d, o);
+              }
             }
-          }
-        }
-        const float base = m == -kInf ? 0.f : m;
+#pragma unroll 1
+            for (int d = 0; d < 16 * q; d += 16) {
+              float o[16];
+              uint32_t p[16];
+              tc::ld16(s_at + d, o);
 #pragma unroll
-        for (int q = 0; q < kKeys / 32; ++q) {
-          float x[32];
-          tc::ld32(s_at + 32 * q, x);
-          if (masked) hide(x, 32 * q);
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t bits = __float_as_uint(o[e]);
+                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&bits));
+                p[e] = pack_half2(y.x * f, y.y * f);
+              }
+              st16(s_at + d, p);
+            }
+            tc::wait_st();
+          }
+          const float base = m == -kInf ? 0.f : m;
           uint32_t p[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const Run& u = run[2 * q + h];
-            const float f = factor_of(u), shift = u.lift - base;
-            float s0 = 0.f, s1 = 0.f;
+            const float shift = lift[h] - base;
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float p0 = ex2(fmaf(x[16 * h + e], f, shift));
-              const float p1 = ex2(fmaf(x[16 * h + e + 1], f, shift));
-              s0 += p0;
-              s1 += p1;
-              p[8 * h + e / 2] = pack_half2(p0, p1);
+            for (int e = 16 * h; e < 16 * h + 16; e += 2) {
+              float2 y = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])),
+                                    make_float2(factor[h], factor[h]), make_float2(shift, shift));
+              y = make_float2(ex2(y.x), ex2(y.y));
+              sum = __fadd2_rn(sum, y);
+              p[e / 2] = pack_half2(y.x, y.y);
             }
-            l = fmaf(s0 + s1, u.per, l);
+            l = fmaf(sum.x + sum.y, per[h], l);
           }
           st16(s_at + 16 * q, p);
+        };
+#pragma unroll 1
+        for (int q = 0; q < kKeys / 32; q += 2) {
+          uint32_t x[64];
+          ld64(s_at + 32 * q, x);
+          chunk(x, q);
+          chunk(x + 32, q + 1);
         }
         tc::wait_st();
         tc::fence_before();
         warp_arrive(&bars->p_full[g], lane);
       }
-      // Load the next item's queries (its S may start while this one ends).
-      const Item ended = item;
-      const long long started = tile;
+      pending = true;
+      ended = item;
+      started = tile;
       tile = until;
-      if (more) {
-        next(item);
-        if (active(item, g)) {
-          back_next = load_query(item);
-          loaded = true;
-        }
-      }
-      if (!warp_wait(&bars->o_done[g], mine_i, bars, c.error)) goto done;
-      ++mine_i;
-      tc::fence_after();
-      const bool complete = started == ended.begin && until == ended.end;
-      float* const part = scratch + (started == ended.begin ? kTileRows * (D + 2) : 0);
-      const bool some = !(l == 0.f);
-      const float inv = some ? 1.f / l : 0.f;
-      const long long head = (long long)(ended.span.first + row / z.group) * a.heads +
-                             ended.kv_head * z.group + row % z.group;
-#pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        float o[32];
-        __syncwarp();
-        tc::ld32(o_at + 32 * q, o);
-        if (row < ended.rows && complete) {
-          T* out = (T*)a.out + head * D + 32 * q;
-          alignas(16) T y[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = from_float<T>(some ? o[e] * inv : 0.f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(out)[e] = reinterpret_cast<const uint4*>(y)[e];
-        } else if (row < ended.rows) {
-          float4* out = reinterpret_cast<float4*>(part + (128 * g + r) * D + 32 * q);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            out[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
-      }
-      tc::fence_before();
-      warp_arrive(&bars->o_free[g], lane);
-      if (row < ended.rows) {
-        if (complete) {
-          if (a.lse) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
-        } else {
-          part[kTileRows * D + 2 * (128 * g + r)] = m;
-          part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
-        }
-      }
-      if (!complete && started == ended.begin && g == 0 && r == 0) {
-        const int last = share_of(total, ended.end - 1, ctas);
-        mine.first = ended.span.first;
-        mine.rows = ended.rows;
-        mine.row0 = ended.tile_row * kTileRows;
-        mine.kv_head = ended.kv_head;
-        mine.parts = last - (int)blockIdx.x + 1;
-      }
+      if (until < hi) next(item);
     }
   } else if (warp < kMmaWarp) {
     // --------------------------------------------------------- conversion ---
+    if constexpr (Registers<D>::kConvert > 128) more_registers<Registers<D>::kConvert>();
     constexpr int kChunks = D / 16;             // 16-byte chunks of a key
     constexpr int kStep = 128 / kChunks;        // keys of one pass of the 128 threads
     constexpr int kPasses = kKeys / kStep;
     const int i = threadIdx.x - 32 * kConvertWarp, key = i / kChunks, chunk = i % kChunks;
-    const int entries = kKeys / c.page_size;
+    const int page_bits = __ffs(c.page_size) - 1, entries = kKeys >> page_bits;
+    const int page_bytes = c.page_size * D;
     const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-    const int page_bits = __ffs(c.page_size) - 1;
     uint4 kc[kPasses], vc[kPasses];
     float sk = 0.f, sv = 0.f;
     int gone = 0;
     long long next_tile = lo;                   // the tile to load next
-    int ids = -1;
-    // Lane e: the page of the e-th page of the tile to load next.
+    const uint8_t* pages = nullptr;             // lane e: its e-th page's K codes of the head
+    long long cell = 0;                         // and the index of its scales
     auto look_up = [&]() {
-      ids = -1;
+      pages = nullptr;
       if (next_tile >= hi) return;
-      const int at = (item.first + (int)(next_tile - item.begin)) * kKeys + lane * c.page_size;
+      const int at = (item.first + (int)(next_tile - item.begin)) * kKeys + (lane << page_bits);
       if (lane < entries && at < item.span.length && at + c.page_size > item.span.begin) {
-        ids = c.table[item.user * c.table_stride + (at >> page_bits)];
-        if (ids < 0 || ids >= c.pages) {
-          ids = -1;
+        const int id = c.table[item.user * c.table_stride + (at >> page_bits)];
+        if (id < 0 || id >= c.pages) {
           report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
+        } else {
+          cell = ((long long)id * c.kv_heads + item.kv_head) * 2;
+          pages = (const uint8_t*)c.codes + cell * page_bytes;
         }
       }
     };
     // part 0: K and the scales, part 1: V, of the tile to load next.
     auto load = [&](uint4 (&to)[kPasses], int part) {
-      const int key0 = (item.first + (int)(next_tile - item.begin)) * kKeys;
+      const int left = item.span.length - (item.first + (int)(next_tile - item.begin)) * kKeys;
+      const int offset = part * page_bytes + chunk * 16;
 #pragma unroll
       for (int j = 0; j < kPasses; ++j) {
         const int at = j * kStep + key;
-        const int id = __shfl_sync(0xffffffffu, ids, at >> page_bits);
-        const bool live = id >= 0 && key0 + at < item.span.length;
-        const long long cell = ((long long)id * c.kv_heads + item.kv_head) * 2 + part;
-        const uint8_t* from = (const uint8_t*)c.codes +
-                              (cell * c.page_size + (at & (c.page_size - 1))) * D + chunk * 16;
-        to[j] = live ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+        const uint8_t* from =
+            (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)pages, at >> page_bits);
+        const bool live = from && at < left;
+        to[j] = make_uint4(0, 0, 0, 0);
+        if (live)
+          to[j] = __ldg(reinterpret_cast<const uint4*>(from + offset + (at & (c.page_size - 1)) * D));
       }
       if (part == 0 && warp == kConvertWarp) {
-        const int id = __shfl_sync(0xffffffffu, ids, lane % kRuns * 16 >> page_bits);
-        gone = id < 0;
-        const float* from = c.scales + ((long long)id * c.kv_heads + item.kv_head) * 2;
-        sk = gone || lane >= kRuns ? 1.f : from[0];
-        sv = gone || lane >= kRuns ? 1.f : from[1];
+        const int e = (lane % kRuns * 16) >> page_bits;
+        const bool here = __shfl_sync(0xffffffffu, pages != nullptr, e);
+        const float* from = c.scales + __shfl_sync(0xffffffffu, cell, e);
+        gone = !here;
+        sk = here ? from[0] : 1.f;
+        sv = here ? from[1] : 1.f;
       }
+    };
+    auto flags_of = [&]() {  // of the tile to load next
+      const bool first = next_tile == item.begin || next_tile == lo;
+      const bool last = next_tile + 1 == item.end || next_tile + 1 == hi;
+      return (first ? kFirst : 0) | (last ? kLast : 0) | (active(item, 1) ? kTwo : 0);
     };
     auto advance = [&]() {
       ++next_tile;
@@ -570,15 +652,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<uint4*>(to + tc::sw128_chunk(at, first + 1 - swap)) = swap ? a0 : a1;
       }
     };
-    if (lo < hi) {
-      look_up();
-      load(kc, 0);
-      load(vc, 1);
-      const long long n = hi - lo;
-      advance();
-      for (int t = 0; t < n; ++t) {
-        const int stage = t & 1;
-        const bool more = next_tile < hi;
+    look_up();
+    const int n = (int)(hi - lo);
+    int flags = 0;
+#pragma unroll 1
+    for (int t = lo < hi ? -1 : 0; t < n; ++t) {  // tile t is converted, tile t + 1 loaded
+      const int stage = t & 1;
+      const bool more = next_tile < hi;
+      if (t >= 0) {
         if (!warp_wait(&bars->k_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
         convert(kc, smem + L::kK + stage * L::kPanels * kPanel);
         if (warp == kConvertWarp && lane < kRuns) {
@@ -588,91 +669,104 @@ __global__ void __launch_bounds__(kThreads, 1)
           u.per = __frcp_rn(usable_scale(sv));
           u.missing = gone;
           runs[(t & 3) * kRuns + lane] = u;
+          if (lane == 0) bars->flags[t & 3] = flags;
         }
         cxs::fence_proxy_async_shared();
         warp_arrive(&bars->k_full[stage], lane);
-        if (more) load(kc, 0);
+      }
+      if (more) load(kc, 0);
+      if (t >= 0) {
         if (!warp_wait(&bars->v_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
         convert(vc, smem + L::kV + stage * L::kPanels * kPanel);
         cxs::fence_proxy_async_shared();
         warp_arrive(&bars->v_full[stage], lane);
-        if (more) {
-          load(vc, 1);
-          advance();
-        }
+      }
+      if (more) {
+        load(vc, 1);
+        flags = flags_of();
+        advance();
       }
     }
-  } else if (lane == 0 && lo < hi) {
+  } else {
     // ---------------------------------------------------------------- MMAs ---
-    const uint32_t base = cxs::smem_addr(smem);
-    const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, 64, 1);
-    struct Place {
-      Item item;
-      long long tile;
-      int n;        // tiles since the share's start
-      int items[2]; // items started, by group
-    };
-    Place s{item, lo, 0, {0, 0}}, p{item, lo, 0, {0, 0}};
-    int n_p[2] = {0, 0};
-    bool fine = true;
-    auto step = [&](Place& x) {  // to the next tile
-      ++x.tile;
-      ++x.n;
-      if (x.tile < hi && x.tile >= x.item.end) next(x.item);
-    };
-    auto starts = [&](const Place& x) { return x.tile == x.item.begin || x.tile == lo; };
-    auto issue_s = [&](int g) {
-      if (starts(s)) {
-        if (!(fine = wait(&bars->q_full[g], s.items[g], bars, c.error))) return;
-        ++s.items[g];
+    fewer_registers<Registers<D>::kMma>();
+    // The whole warp walks the tiles, so that what the MMAs need stays in
+    // uniform registers; one elected lane issues them.
+    if (warp == kMmaWarp && lo < hi) {
+      const uint32_t base = cxs::smem_addr(smem);
+      constexpr uint32_t kPanel16 = kPanel / 16;  // descriptors count 16-byte units
+      const uint64_t dq = tc::desc_sw128(base + L::kQ, 16, 1024);
+      const uint64_t dk = tc::desc_sw128(base + L::kK, 16, 1024);
+      // V is read channel-major: 64-channel panels kPanel apart, 8 keys 1024.
+      const uint64_t dv = tc::desc_sw128(base + L::kV, kPanel, 1024);
+      const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, D, 1);
+      const int count = (int)(hi - lo);
+      int s_items[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
+      // S of tile n for group g; `flags` are the tile's.
+      auto issue_s = [&](int g, int n, int flags) -> bool {
+        if (flags & kFirst) {
+          if (!warp_wait(&bars->q_full[g], s_items[g], bars, c.error)) return false;
+          ++s_items[g];
+        }
+        tc::fence_after();
+        const uint64_t q = dq + g * L::kPanels * kPanel16;
+        const uint64_t k = dk + (n & 1) * L::kPanels * kPanel16;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            mma_ss(tmem + 128 * g, q + i / 4 * kPanel16 + 2 * (i % 4),
+                   k + i / 4 * kPanel16 + 2 * (i % 4), id_s, i > 0);
+          tc::commit(&bars->s_full[g]);
+          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->k_free[n & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // O of tile n for group g.
+      auto issue_o = [&](int g, int n, int flags) -> bool {
+        if (!warp_wait(&bars->p_full[g], o_tiles[g], bars, c.error)) return false;
+        ++o_tiles[g];
+        if (!warp_wait(&bars->v_full[n & 1], n >> 1, bars, c.error)) return false;
+        if (flags & kFirst) {
+          if (o_items[g] > 0 && !warp_wait(&bars->o_free[g], o_items[g] - 1, bars, c.error))
+            return false;
+          ++o_items[g];
+        }
+        tc::fence_after();
+        const uint64_t v = dv + (n & 1) * L::kPanels * kPanel16;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tmem + 256 + D * g, tmem + 128 * g + 8 * i, v + 128 * i, id_o,
+                   !(flags & kFirst) || i > 0);
+          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->v_free[n & 1]);
+          if (flags & kLast) tc::commit(&bars->o_done[g]);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool fine = warp_wait(&bars->k_full[0], 0, bars, c.error);
+      int ahead = fine ? bars->flags[0] : 0;
+      fine = fine && issue_s(0, 0, ahead);
+      if (ahead & kTwo) fine = fine && issue_s(1, 0, ahead);
+      for (int n = 0; fine && n < count; ++n) {
+        const int flags = ahead;
+        const bool more = n + 1 < count;
+        fine = issue_o(0, n, flags);
+        if (fine && more) {
+          fine = warp_wait(&bars->k_full[(n + 1) & 1], (n + 1) >> 1, bars, c.error);
+          ahead = bars->flags[(n + 1) & 3];
+          fine = fine && issue_s(0, n + 1, ahead);
+        }
+        if (fine && (flags & kTwo)) fine = issue_o(1, n, flags);
+        if (fine && more && (ahead & kTwo)) fine = issue_s(1, n + 1, ahead);
       }
-      if (!(fine = wait(&bars->k_full[s.n & 1], s.n >> 1, bars, c.error))) return;
-      tc::fence_after();
-      const uint32_t q = base + L::kQ + g * L::kPanels * kPanel;
-      const uint32_t k = base + L::kK + (s.n & 1) * L::kPanels * kPanel;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        tc::mma(tmem + 128 * g, tc::desc_sw128(q + i / 4 * kPanel + 32 * (i % 4), 16, 1024),
-                tc::desc_sw128(k + i / 4 * kPanel + 32 * (i % 4), 16, 1024), id_s, i > 0);
-      tc::commit(&bars->s_full[g]);
-      if (g == 1 || !active(s.item, 1)) tc::commit(&bars->k_free[s.n & 1]);
-    };
-    auto issue_o = [&](int g) {
-      const bool first = starts(p);
-      if (!(fine = wait(&bars->p_full[g], n_p[g], bars, c.error))) return;
-      ++n_p[g];
-      if (!(fine = wait(&bars->v_full[p.n & 1], p.n >> 1, bars, c.error))) return;
-      if (first) {
-        if (p.items[g] > 0 && !(fine = wait(&bars->o_free[g], p.items[g] - 1, bars, c.error))) return;
-        ++p.items[g];
-      }
-      tc::fence_after();
-      const uint32_t v = base + L::kV + (p.n & 1) * L::kPanels * kPanel;
-#pragma unroll
-      for (int h = 0; h < L::kPanels; ++h)
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_ts(tmem + 256 + D * g + 64 * h, tmem + 128 * g + 8 * i,
-                 tc::desc_sw128(v + h * kPanel + 2048 * i, 16, 1024), id_o, !first || i > 0);
-      if (g == 1 || !active(p.item, 1)) tc::commit(&bars->v_free[p.n & 1]);
-      if (p.tile + 1 == hi || p.tile + 1 == p.item.end) tc::commit(&bars->o_done[g]);
-    };
-    issue_s(0);
-    if (fine && active(s.item, 1)) issue_s(1);
-    step(s);
-    while (fine && p.tile < hi) {
-      const bool more = s.tile < hi;
-      issue_o(0);
-      if (fine && more) issue_s(0);
-      if (fine && active(p.item, 1)) issue_o(1);
-      if (fine && more && active(s.item, 1)) issue_s(1);
-      if (more) step(s);
-      step(p);
-    }
-    if (!fine) {  // let the MMAs in flight end before TMEM is freed
-      tc::commit(&bars->drain);
-      const long long start = clock64();
-      while (!cxs::mbar_try_wait(&bars->drain, 0) && clock64() - start < kSpinLimit) {
+      if (!fine) {  // let the MMAs in flight end before TMEM is freed
+        if (elect_one()) tc::commit(&bars->drain);
+        __syncwarp();
+        const long long start = clock64();
+        while (!cxs::mbar_try_wait(&bars->drain, 0) && clock64() - start < kSpinLimit) {
+        }
       }
     }
   }
