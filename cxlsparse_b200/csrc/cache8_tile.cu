@@ -6,10 +6,12 @@
 //   warps 0-3, 4-7  softmax of group 0 and 1, one row a thread: reads S from
 //                   TMEM, writes p = 2^(x - M) as fp16 over S, rescales O when
 //                   M grows by more than 2^8
-//   warps 8-11      conversion: K and V codes global -> registers (one tile
-//                   ahead) -> fp16 in shared memory, shared by both groups
+//   warps 8-11      conversion of K and V codes to fp16 operand tiles in shared
+//                   memory, which both groups use
 //   warp 12         one thread issues every MMA: S = Q K^T (Q, K in shared
 //                   memory), O += P V (P in TMEM, V in shared memory)
+//   warp 13         loads: bulk copies of the tiles' pages into shared memory,
+//                   their scales, and what the others need to know of a tile
 // While one group's softmax runs, the tensor core works for the other. The
 // MMAs of one thread complete in order, so S of the next tile may be issued
 // over P right after the P V that reads it, and a commit after S also tells
@@ -25,23 +27,18 @@ using namespace cxs::cache8;
 namespace tc = cxs::tc;
 
 constexpr int kKeys = 128;              // of a tile
-constexpr int kThreads = 16 * 32;  // the last three warps only share the setup
-constexpr int kConvertWarp = 8, kMmaWarp = 12;
+constexpr int kThreads = 16 * 32;  // the last two warps only share the setup
+constexpr int kConvertWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
 constexpr int kPanel = 128 * 128;       // bytes: 128 rows (queries or keys) of 64 channels, swizzled
 constexpr int kRuns = kKeys / 16;       // runs of 16 keys: each within one page
+constexpr int kRing = 8;                // tiles whose Tile is kept: more than are ever in work
 constexpr int kTmem = 512;              // columns: S/P of two groups (128 each), O of two groups
 constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
 
-// What the MMA warp needs of a tile.
-constexpr int kFirst = 1, kLast = 2, kTwo = 4;  // of its item here; rows for group 1
-
 // Registers a thread by role: twice the softmax's, the conversion's and the
-// MMA warp's, times 128, are the 64 K that 512 threads of 128 are launched with.
-template <int D>
-struct Registers {
-  static constexpr int kSoftmax = D == 64 ? 160 : 144, kConvert = D == 64 ? 128 : 160, kMma = 64;
-  static_assert(2 * kSoftmax + kConvert + kMma == 4 * 128, "all of the block's registers");
-};
+// rest's, times 128, are the 64 K that 512 threads of 128 are launched with.
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 80, kOtherRegs = 64;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs == 4 * 128, "the block's registers");
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -51,34 +48,49 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-struct Run {     // what the softmax needs of a run of 16 keys
-  float factor;  // |scale| log2(e) s_k
-  float lift;    // log2 s_v
-  float per;     // 1 / s_v
-  int missing;   // no page: no row sees it
+constexpr int kFirst = 1, kLast = 2, kTwo = 4;  // of its item here; rows for group 1
+
+struct Tile {                // what the roles need of a tile of keys
+  float4 runs[kRuns];        // of 16 keys: |scale| log2(e) s_k, log2 s_v, 1 / s_v, unused
+  unsigned missing;          // bit u: run u has no page, no row sees it
+  int left;                  // keys of the tile that hold tokens (may be negative or above kKeys)
+  int flags;
+  int unused;
 };
 
+// Shared memory. K has one operand stage where two do not fit (D = 128): the
+// next K is converted while the softmax of this tile runs.
 template <int D>
 struct Layout {
   static constexpr int kPanels = D / 64;
+  static constexpr int kKStages = D == 64 ? 2 : 1, kVStages = 2, kRawStages = D == 64 ? 2 : 1;
+  static constexpr int kRawPart = kKeys * D;                     // bytes of K or V codes
   static constexpr int kQ = 0;                                   // [2 groups][panels]
-  static constexpr int kK = kQ + 2 * kPanels * kPanel;           // [2 stages][panels]
-  static constexpr int kV = kK + 2 * kPanels * kPanel;           // [2 stages][panels]
-  static constexpr int kRunsAt = kV + 2 * kPanels * kPanel;      // [4][kRuns]
-  static constexpr int kBars = kRunsAt + 4 * kRuns * (int)sizeof(Run);
+  static constexpr int kK = kQ + 2 * kPanels * kPanel;           // [stages][panels]
+  static constexpr int kV = kK + kKStages * kPanels * kPanel;    // [stages][panels]
+  static constexpr int kRaw = kV + kVStages * kPanels * kPanel;  // [stages][K, V]
+  static constexpr int kTiles = kRaw + kRawStages * 2 * kRawPart;  // [kRing]
+  static constexpr int kBars = kTiles + kRing * (int)sizeof(Tile);
   static constexpr int kPrefix = kBars + 256;
   static constexpr int kBytes = kPrefix + (kSlice + 1) * 8 + 1024;  // and the 1024-byte alignment
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
 struct Bars {
-  uint64_t k_full[2], v_full[2], k_free[2], v_free[2];  // by stage
+  uint64_t raw_full[2][2], raw_free[2][2];          // by raw stage and part
+  uint64_t k_full[2], v_full[2], k_free[2], v_free[2];  // by operand stage
   uint64_t s_full[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
   uint64_t drain;
   int abort;
   uint32_t tmem;
-  int flags[4];  // of the tiles in work
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
+
+// Stage of use n of a ring of N and the parity of its n-th phase.
+template <int N>
+__device__ __forceinline__ int stage_of(int n) { return N == 1 ? 0 : n & 1; }
+template <int N>
+__device__ __forceinline__ int phase_of(int n) { return N == 1 ? n : n >> 1; }
 
 // Bounded wait on a barrier phase; false: some role of the CTA gave up.
 __device__ __forceinline__ bool wait(uint64_t* bar, int phase, Bars* b, int* error) {
@@ -137,7 +149,7 @@ __device__ __forceinline__ bool elect_one() {
 
 // 64 fp32 columns of this warp's 32 lanes (the wait is part of the statement:
 // nothing can use, move or spill the registers before they are written).
-__device__ __forceinline__ void ld64(uint32_t taddr, uint32_t (&r)[64]) {
+__device__ __forceinline__ void ld64(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
@@ -197,13 +209,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const smem =
       (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   Bars* const bars = (Bars*)(smem + L::kBars);
-  Run* const runs = (Run*)(smem + L::kRunsAt);
+  Tile* const ring = (Tile*)(smem + L::kTiles);
   long long* const prefix = (long long*)(smem + L::kPrefix);
   // (Broadcast: uniform across the warp also for the compiler.)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
+      for (int part = 0; part < 2; ++part) {
+        cxs::mbar_init(&bars->raw_full[i][part], 1);
+        cxs::mbar_init(&bars->raw_free[i][part], 4);
+      }
       cxs::mbar_init(&bars->k_full[i], 4);
       cxs::mbar_init(&bars->v_full[i], 4);
       cxs::mbar_init(&bars->k_free[i], 1);
@@ -336,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kConvertWarp) {
     // ------------------------------------------------------------ softmax ---
-    more_registers<Registers<D>::kSoftmax>();
+    more_registers<kSoftmaxRegs>();
     const int g = warp / 4, r = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + lanes + 128 * g, o_at = tmem + lanes + 256 + D * g;
@@ -466,101 +482,85 @@ __global__ void __launch_bounds__(kThreads, 1)
       int key0 = (item.first + (int)(tile - item.begin)) * kKeys;
 #pragma unroll 1
       for (int i = 0; i < count; ++i, ++tiles, ++mine_s, key0 += kKeys) {
-        // (The runs were written before the K that S was computed from.)
+        // (Tile t was described before the K that S was computed from came.)
         if (!warp_wait(&bars->s_full[g], mine_s, bars, c.error)) goto done;
         tc::fence_after();
-        const Run* const run = runs + (tiles & 3) * kRuns;
+        const Tile& tile_info = ring[tiles % kRing];
         const int from = see.x - key0, to = see.y - key0;  // visible columns
-        bool whole = from <= 0 && to >= kKeys;
+        const unsigned missing = tile_info.missing;
+        uint32_t x[kKeys];
+        ld64(s_at, x);
+        ld64(s_at + 64, x + 64);
+        if (!__all_sync(0xffffffffu, from <= 0 && to >= kKeys && missing == 0)) {
+          // What the row does not see becomes -infinity.
 #pragma unroll
-        for (int u = 0; u < kRuns; ++u) whole = whole && !run[u].missing;
-        const bool masked = !__all_sync(0xffffffffu, whole);
-        // Columns 32 q .. 32 q + 31 of S in x become probabilities over S. M
-        // moves when a score passes it by 2^8 (p then stays below 2^8, well
-        // inside fp16's range): rare, so S is read once and what was computed
-        // with the older M (O, l, the tile's earlier probabilities) follows it.
-        auto chunk = [&](uint32_t* x, int q) {
-          if (masked) {  // what the row does not see becomes -infinity
+          for (int q = 0; q < kKeys / 32; ++q) {
             const int low = min(max(from - 32 * q, 0), 32), high = min(max(to - 32 * q, 0), 32);
             unsigned seen =
                 (high == 32 ? ~0u : (1u << high) - 1) & ~(low == 32 ? ~0u : (1u << low) - 1);
-            if (run[2 * q].missing) seen &= 0xffff0000u;
-            if (run[2 * q + 1].missing) seen &= 0x0000ffffu;
+            if (missing >> (2 * q) & 1) seen &= 0xffff0000u;
+            if (missing >> (2 * q + 1) & 1) seen &= 0x0000ffffu;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = seen >> e & 1 ? x[e] : 0xff800000u;
+            for (int e = 0; e < 32; ++e) x[32 * q + e] = seen >> e & 1 ? x[32 * q + e] : 0xff800000u;
           }
-          float factor[2], lift[2], per[2], top = -kInf;
+        }
+        // A run's factor; never 0, which times a hidden score would be NaN
+        // (scores that small are 0 either way); NaN stays NaN.
+        auto factor_of = [&](float run) {
+          const float f = run * back;
+          return f < 1.2e-38f ? 1.2e-38f : f;
+        };
+        float top = -kInf;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const Run u = run[2 * q + h];
-            // Never 0, which times a hidden score would be NaN (scores that
-            // small are 0 either way); NaN stays NaN.
-            const float f = u.factor * back;
-            factor[h] = f < 1.2e-38f ? 1.2e-38f : f;
-            lift[h] = u.lift;
-            per[h] = u.per;
-            float t = __uint_as_float(x[16 * h]);
+        for (int u = 0; u < kRuns; ++u) {
+          const float2 run = *reinterpret_cast<const float2*>(&tile_info.runs[u]);
+          float t0 = __uint_as_float(x[16 * u]), t1 = __uint_as_float(x[16 * u + 1]);
 #pragma unroll
-            for (int e = 1; e < 15; e += 2)
-              t = fmaxf(fmaxf(t, __uint_as_float(x[16 * h + e])), __uint_as_float(x[16 * h + e + 1]));
-            t = fmaxf(t, __uint_as_float(x[16 * h + 15]));
-            top = fmaxf(top, fmaf(t, factor[h], lift[h]));
+          for (int e = 2; e < 16; e += 2) {
+            t0 = fmaxf(t0, __uint_as_float(x[16 * u + e]));
+            t1 = fmaxf(t1, __uint_as_float(x[16 * u + e + 1]));
           }
-          const bool grows = top > m + 8.f;
-          if (__any_sync(0xffffffffu, grows)) {
-            const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
-            if (grows) m = top;
-            l *= f;
-            tc::wait_st();
-            if (i > 0) {
+          top = fmaxf(top, fmaf(fmaxf(t0, t1), factor_of(run.x), run.y));
+        }
+        // M moves when a score passes it by 2^8: p stays below 2^8, well inside
+        // fp16's range, and most tiles leave O as it is.
+        const bool grows = top > m + 8.f;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
+          if (grows) m = top;
+          l *= f;
+          if (i > 0) {
 #pragma unroll 1
-              for (int d = 0; d < D; d += 16) {
-                float o[16];
-                tc::ld16(o_at + d, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= f;
-                tc::st16(o_at + d, o);
-              }
-            }
-#pragma unroll 1
-            for (int d = 0; d < 16 * q; d += 16) {
+            for (int d = 0; d < D; d += 16) {
               float o[16];
-              uint32_t p[16];
-              tc::ld16(s_at + d, o);
+              tc::ld16(o_at + d, o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const uint32_t bits = __float_as_uint(o[e]);
-                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&bits));
-                p[e] = pack_half2(y.x * f, y.y * f);
-              }
-              st16(s_at + d, p);
+              for (int e = 0; e < 16; ++e) o[e] *= f;
+              tc::st16(o_at + d, o);
             }
-            tc::wait_st();
           }
-          const float base = m == -kInf ? 0.f : m;
+        }
+        const float base = m == -kInf ? 0.f : m;
+#pragma unroll
+        for (int q = 0; q < kKeys / 32; ++q) {
           uint32_t p[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float shift = lift[h] - base;
+            const float4 run = tile_info.runs[2 * q + h];
+            const float factor = factor_of(run.x), shift = run.y - base;
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int e = 16 * h; e < 16 * h + 16; e += 2) {
-              float2 y = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])),
-                                    make_float2(factor[h], factor[h]), make_float2(shift, shift));
+            for (int e = 0; e < 16; e += 2) {
+              const uint32_t* const s2 = x + 32 * q + 16 * h + e;
+              float2 y = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])),
+                                    make_float2(factor, factor), make_float2(shift, shift));
               y = make_float2(ex2(y.x), ex2(y.y));
               sum = __fadd2_rn(sum, y);
-              p[e / 2] = pack_half2(y.x, y.y);
+              p[8 * h + e / 2] = pack_half2(y.x, y.y);
             }
-            l = fmaf(sum.x + sum.y, per[h], l);
+            l = fmaf(sum.x + sum.y, run.z, l);
           }
           st16(s_at + 16 * q, p);
-        };
-#pragma unroll 1
-        for (int q = 0; q < kKeys / 32; q += 2) {
-          uint32_t x[64];
-          ld64(s_at + 32 * q, x);
-          chunk(x, q);
-          chunk(x + 32, q + 1);
         }
         tc::wait_st();
         tc::fence_before();
@@ -574,122 +574,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < kMmaWarp) {
     // --------------------------------------------------------- conversion ---
-    if constexpr (Registers<D>::kConvert > 128) more_registers<Registers<D>::kConvert>();
+    fewer_registers<kConvertRegs>();
     constexpr int kChunks = D / 16;             // 16-byte chunks of a key
     constexpr int kStep = 128 / kChunks;        // keys of one pass of the 128 threads
-    constexpr int kPasses = kKeys / kStep;
     const int i = threadIdx.x - 32 * kConvertWarp, key = i / kChunks, chunk = i % kChunks;
-    const int page_bits = __ffs(c.page_size) - 1, entries = kKeys >> page_bits;
-    const int page_bytes = c.page_size * D;
-    const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-    uint4 kc[kPasses], vc[kPasses];
-    float sk = 0.f, sv = 0.f;
-    int gone = 0;
-    long long next_tile = lo;                   // the tile to load next
-    const uint8_t* pages = nullptr;             // lane e: its e-th page's K codes of the head
-    long long cell = 0;                         // and the index of its scales
-    auto look_up = [&]() {
-      pages = nullptr;
-      if (next_tile >= hi) return;
-      const int at = (item.first + (int)(next_tile - item.begin)) * kKeys + (lane << page_bits);
-      if (lane < entries && at < item.span.length && at + c.page_size > item.span.begin) {
-        const int id = c.table[item.user * c.table_stride + (at >> page_bits)];
-        if (id < 0 || id >= c.pages) {
-          report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
-        } else {
-          cell = ((long long)id * c.kv_heads + item.kv_head) * 2;
-          pages = (const uint8_t*)c.codes + cell * page_bytes;
-        }
-      }
-    };
-    // part 0: K and the scales, part 1: V, of the tile to load next.
-    auto load = [&](uint4 (&to)[kPasses], int part) {
-      const int left = item.span.length - (item.first + (int)(next_tile - item.begin)) * kKeys;
-      const int offset = part * page_bytes + chunk * 16;
-#pragma unroll
-      for (int j = 0; j < kPasses; ++j) {
-        const int at = j * kStep + key;
-        const uint8_t* from =
-            (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)pages, at >> page_bits);
-        const bool live = from && at < left;
-        to[j] = make_uint4(0, 0, 0, 0);
-        if (live)
-          to[j] = __ldg(reinterpret_cast<const uint4*>(from + offset + (at & (c.page_size - 1)) * D));
-      }
-      if (part == 0 && warp == kConvertWarp) {
-        const int e = (lane % kRuns * 16) >> page_bits;
-        const bool here = __shfl_sync(0xffffffffu, pages != nullptr, e);
-        const float* from = c.scales + __shfl_sync(0xffffffffu, cell, e);
-        gone = !here;
-        sk = here ? from[0] : 1.f;
-        sv = here ? from[1] : 1.f;
-      }
-    };
-    auto flags_of = [&]() {  // of the tile to load next
-      const bool first = next_tile == item.begin || next_tile == lo;
-      const bool last = next_tile + 1 == item.end || next_tile + 1 == hi;
-      return (first ? kFirst : 0) | (last ? kLast : 0) | (active(item, 1) ? kTwo : 0);
-    };
-    auto advance = [&]() {
-      ++next_tile;
-      if (next_tile >= hi) return;
-      if (next_tile >= item.end) next(item);
-      look_up();
-    };
-    auto convert = [&](const uint4 (&from)[kPasses], uint8_t* panels) {
-#pragma unroll
-      for (int j = 0; j < kPasses; ++j) {
-        const int at = j * kStep + key, first = chunk % 4 * 2, swap = chunk / 4 & 1;
-        const uint4 w = from[j];
+    const int first = chunk % 4 * 2, swap = chunk / 4 & 1;
+    // Codes -> fp16 in the operand's layout; keys without a token become 0 (a
+    // probability of 0 times whatever their bytes hold could be NaN).
+    auto convert = [&](const uint8_t* raw, uint8_t* panels, const Tile& tile) {
+      panels += chunk / 4 * kPanel;
+      const unsigned missing = tile.missing;
+      const int left = tile.left;
+#pragma unroll 2
+      for (int at = key; at < kKeys; at += kStep) {
+        uint4 w = *reinterpret_cast<const uint4*>(raw + at * D + chunk * 16);
+        if (at >= left || missing >> (at / 16) & 1) w = make_uint4(0, 0, 0, 0);
         const uint4 a0 = make_uint4(half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1),
                                     half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
         const uint4 a1 = make_uint4(half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1),
                                     half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
-        uint8_t* const to = panels + chunk / 4 * kPanel;
         // Lanes of the second panel write their halves in the other order:
         // eight lanes then cover all banks.
-        *reinterpret_cast<uint4*>(to + tc::sw128_chunk(at, first + swap)) = swap ? a1 : a0;
-        *reinterpret_cast<uint4*>(to + tc::sw128_chunk(at, first + 1 - swap)) = swap ? a0 : a1;
+        *reinterpret_cast<uint4*>(panels + tc::sw128_chunk(at, first + swap)) = swap ? a1 : a0;
+        *reinterpret_cast<uint4*>(panels + tc::sw128_chunk(at, first + 1 - swap)) = swap ? a0 : a1;
       }
     };
-    look_up();
     const int n = (int)(hi - lo);
-    int flags = 0;
 #pragma unroll 1
-    for (int t = lo < hi ? -1 : 0; t < n; ++t) {  // tile t is converted, tile t + 1 loaded
-      const int stage = t & 1;
-      const bool more = next_tile < hi;
-      if (t >= 0) {
-        if (!warp_wait(&bars->k_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
-        convert(kc, smem + L::kK + stage * L::kPanels * kPanel);
-        if (warp == kConvertWarp && lane < kRuns) {
-          Run u;
-          u.factor = usable_scale(sk) * unit;
-          u.lift = __log2f(usable_scale(sv));
-          u.per = __frcp_rn(usable_scale(sv));
-          u.missing = gone;
-          runs[(t & 3) * kRuns + lane] = u;
-          if (lane == 0) bars->flags[t & 3] = flags;
-        }
+    for (int t = 0; t < n; ++t) {
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int raw = stage_of<L::kRawStages>(t);
+        const int to = part ? stage_of<L::kVStages>(t) : stage_of<L::kKStages>(t);
+        const int use = part ? phase_of<L::kVStages>(t) : phase_of<L::kKStages>(t);
+        if (!warp_wait(&bars->raw_full[raw][part], phase_of<L::kRawStages>(t), bars, c.error)) goto done;
+        if (!warp_wait(part ? &bars->v_free[to] : &bars->k_free[to], use + 1, bars, c.error)) goto done;
+        convert(smem + L::kRaw + (2 * raw + part) * L::kRawPart,
+                smem + (part ? L::kV : L::kK) + to * L::kPanels * kPanel, ring[t % kRing]);
         cxs::fence_proxy_async_shared();
-        warp_arrive(&bars->k_full[stage], lane);
-      }
-      if (more) load(kc, 0);
-      if (t >= 0) {
-        if (!warp_wait(&bars->v_free[stage], (t >> 1) + 1, bars, c.error)) goto done;
-        convert(vc, smem + L::kV + stage * L::kPanels * kPanel);
-        cxs::fence_proxy_async_shared();
-        warp_arrive(&bars->v_full[stage], lane);
-      }
-      if (more) {
-        load(vc, 1);
-        flags = flags_of();
-        advance();
+        warp_arrive(part ? &bars->v_full[to] : &bars->k_full[to], lane);
+        if (lane == 0) cxs::mbar_arrive(&bars->raw_free[raw][part]);
       }
     }
   } else {
     // ---------------------------------------------------------------- MMAs ---
-    fewer_registers<Registers<D>::kMma>();
+    fewer_registers<kOtherRegs>();
     // The whole warp walks the tiles, so that what the MMAs need stays in
     // uniform registers; one elected lane issues them.
     if (warp == kMmaWarp && lo < hi) {
@@ -710,14 +639,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::fence_after();
         const uint64_t q = dq + g * L::kPanels * kPanel16;
-        const uint64_t k = dk + (n & 1) * L::kPanels * kPanel16;
+        const int stage = stage_of<L::kKStages>(n);
+        const uint64_t k = dk + stage * L::kPanels * kPanel16;
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
             mma_ss(tmem + 128 * g, q + i / 4 * kPanel16 + 2 * (i % 4),
                    k + i / 4 * kPanel16 + 2 * (i % 4), id_s, i > 0);
           tc::commit(&bars->s_full[g]);
-          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->k_free[n & 1]);
+          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->k_free[stage]);
         }
         __syncwarp();
         return true;
@@ -746,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       bool fine = warp_wait(&bars->k_full[0], 0, bars, c.error);
-      int ahead = fine ? bars->flags[0] : 0;
+      int ahead = fine ? ring[0].flags : 0;
       fine = fine && issue_s(0, 0, ahead);
       if (ahead & kTwo) fine = fine && issue_s(1, 0, ahead);
       for (int n = 0; fine && n < count; ++n) {
@@ -754,8 +684,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = n + 1 < count;
         fine = issue_o(0, n, flags);
         if (fine && more) {
-          fine = warp_wait(&bars->k_full[(n + 1) & 1], (n + 1) >> 1, bars, c.error);
-          ahead = bars->flags[(n + 1) & 3];
+          fine = warp_wait(&bars->k_full[stage_of<L::kKStages>(n + 1)],
+                           phase_of<L::kKStages>(n + 1), bars, c.error);
+          ahead = ring[(n + 1) % kRing].flags;
           fine = fine && issue_s(0, n + 1, ahead);
         }
         if (fine && (flags & kTwo)) fine = issue_o(1, n, flags);
@@ -766,6 +697,86 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         const long long start = clock64();
         while (!cxs::mbar_try_wait(&bars->drain, 0) && clock64() - start < kSpinLimit) {
+        }
+      }
+    } else if (warp == kLoadWarp) {
+      // -------------------------------------------------------------- loads ---
+      const int page_bits = __ffs(c.page_size) - 1, entries = kKeys >> page_bits;
+      const int page_bytes = c.page_size * D;
+      const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+      const int n = (int)(hi - lo);
+      long long tile = lo;
+      // Lane e: the id of the e-th page of the tile at `tile` (looked up one
+      // tile early), -1 where it has no token or none that a row sees.
+      auto look_up = [&]() {
+        const int at = (item.first + (int)(tile - item.begin)) * kKeys + (lane << page_bits);
+        const bool needed = lane < entries && at < item.span.length &&
+                            at + c.page_size > item.span.begin;
+        return needed ? __ldg(c.table + item.user * c.table_stride + (at >> page_bits)) : -2;
+      };
+      int id = n > 0 ? look_up() : -2;
+#pragma unroll 1
+      for (int t = 0; t < n; ++t) {
+        if (id != -2 && (id < 0 || id >= c.pages)) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
+        if (id < 0 || id >= c.pages) id = -1;
+        const long long cell = ((long long)id * c.kv_heads + item.kv_head) * 2;
+        const unsigned pages = __ballot_sync(0xffffffffu, id >= 0);
+        // Lane u: the scales of run u of 16 keys.
+        const int e = (lane % kRuns * 16) >> page_bits;
+        const long long its = __shfl_sync(0xffffffffu, cell, e);
+        const bool here = pages >> e & 1;
+        float sk = 1.f, sv = 1.f;
+        if (here && lane < kRuns) {
+          sk = __ldg(c.scales + its);
+          sv = __ldg(c.scales + its + 1);
+        }
+        const unsigned missing = __ballot_sync(0xffffffffu, lane < kRuns && !here);
+        const bool first = tile == item.begin || t == 0, last = tile + 1 == item.end || t + 1 == n;
+        const int flags = (first ? kFirst : 0) | (last ? kLast : 0) | (active(item, 1) ? kTwo : 0);
+        const int left = item.span.length - (item.first + (int)(tile - item.begin)) * kKeys;
+        const uint8_t* from = (const uint8_t*)c.codes + cell * page_bytes;
+        ++tile;
+        if (t + 1 < n) {
+          if (tile >= item.end) next(item);
+          id = look_up();
+        }
+        const int raw = stage_of<L::kRawStages>(t);
+        uint8_t* const to = smem + L::kRaw + 2 * raw * L::kRawPart + lane * page_bytes;
+        const uint32_t bytes = __popc(pages) * page_bytes;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          if (!warp_wait(&bars->raw_free[raw][part], phase_of<L::kRawStages>(t) + 1, bars, c.error)) {
+            // Copies in flight end before the CTA does (of each barrier, the
+            // last use issued: one that has ended is not waited for).
+            for (int k = 0; k < 2 * L::kRawStages; ++k) {
+              const int use = 2 * t + part - 1 - k;  // of K and V of all tiles, in order
+              if (use < 0) break;
+              const long long start = clock64();
+              while (!cxs::mbar_try_wait(&bars->raw_full[stage_of<L::kRawStages>(use / 2)][use & 1],
+                                         phase_of<L::kRawStages>(use / 2) & 1) &&
+                     clock64() - start < kSpinLimit) {
+              }
+            }
+            goto done;
+          }
+          if (part == 0) {
+            // K's arrival also tells the other roles that the tile is described.
+            Tile& about = ring[t % kRing];
+            if (lane < kRuns)
+              about.runs[lane] = make_float4(usable_scale(sk) * unit, __log2f(usable_scale(sv)),
+                                             __frcp_rn(usable_scale(sv)), 0.f);
+            if (lane == 0) {
+              about.missing = missing;
+              about.left = left;
+              about.flags = flags;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) cxs::mbar_expect_tx(&bars->raw_full[raw][part], bytes);
+          __syncwarp();
+          if (pages >> lane & 1)
+            cxs::bulk_g2s(to + part * L::kRawPart, from + part * page_bytes, page_bytes,
+                          &bars->raw_full[raw][part]);
         }
       }
     }
