@@ -63,6 +63,10 @@ struct Tile {                // what the roles need of a tile of keys
 template <int D>
 struct Layout {
   static constexpr int kPanels = D / 64;
+  // TMEM columns: S of two groups, P (over S where nothing else is left), O.
+  static constexpr bool kApart = D == 64;  // P has its own columns
+  static constexpr int kP = kApart ? 256 : 0, kPStep = kApart ? 64 : 128;
+  static constexpr int kO = kApart ? 384 : 256;
   static constexpr int kKStages = D == 64 ? 2 : 1, kVStages = 2, kRawStages = D == 64 ? 2 : 1;
   static constexpr int kRawPart = kKeys * D;                     // bytes of K or V codes
   static constexpr int kQ = 0;                                   // [2 groups][panels]
@@ -79,7 +83,7 @@ struct Layout {
 struct Bars {
   uint64_t raw_full[2][2], raw_free[2][2];          // by raw stage and part
   uint64_t k_full[2], v_full[2], k_free[2], v_free[2];  // by operand stage
-  uint64_t s_full[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
+  uint64_t s_full[2], s_free[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
   uint64_t drain;
   int abort;
   uint32_t tmem;
@@ -91,6 +95,17 @@ template <int N>
 __device__ __forceinline__ int stage_of(int n) { return N == 1 ? 0 : n & 1; }
 template <int N>
 __device__ __forceinline__ int phase_of(int n) { return N == 1 ? n : n >> 1; }
+
+// Whether a barrier's phase has completed, without waiting.
+__device__ __forceinline__ bool test_wait(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(cxs::smem_addr(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
 
 // Bounded wait on a barrier phase; false: some role of the CTA gave up.
 __device__ __forceinline__ bool wait(uint64_t* bar, int phase, Bars* b, int* error) {
@@ -171,13 +186,13 @@ __device__ __forceinline__ void ld64(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
+// (No memory clobber: loads of what a tile's next columns need move ahead.)
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
       "%13,%14,%15,%16};" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));
 }
 
 // An item and where its tiles lie among all tiles of the launch.
@@ -225,6 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       cxs::mbar_init(&bars->k_free[i], 1);
       cxs::mbar_init(&bars->v_free[i], 1);
       cxs::mbar_init(&bars->s_full[i], 1);
+      cxs::mbar_init(&bars->s_free[i], 4);
       cxs::mbar_init(&bars->p_full[i], 4);
       cxs::mbar_init(&bars->q_full[i], 4);
       cxs::mbar_init(&bars->o_done[i], 1);
@@ -355,11 +371,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     more_registers<kSoftmaxRegs>();
     const int g = warp / 4, r = threadIdx.x % 128;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t s_at = tmem + lanes + 128 * g, o_at = tmem + lanes + 256 + D * g;
+    const uint32_t s_at = tmem + lanes + 128 * g, p_at = tmem + lanes + L::kP + L::kPStep * g;
+    const uint32_t o_at = tmem + lanes + L::kO + D * g;
     uint8_t* const q_panels = smem + L::kQ + g * L::kPanels * kPanel;
     int tiles = 0;    // of the share
     int mine_s = 0;   // tiles of this group
-    int mine_i = 0;   // items of this group
     float m = -kInf, l = 0.f, back = 1.f;
     bool pending = false;  // an item whose O is still in TMEM:
     Item ended = {};
@@ -384,46 +400,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           from += (long long)(item.span.first + row / z.group) * a.q_token_stride +
                   (long long)(item.kv_head * z.group + row % z.group) * a.q_head_stride;
         const bool wide = ((uintptr_t)from & 15) == 0;
-        float top = 0.f, up = 1.f;
-#pragma unroll 1
-        for (int i = 0; i < D / 4; ++i) {
+        auto eight = [&](float (&v)[8], int i) {  // channels 8 i ..
           alignas(16) T x[8];
           if (wide) {
-            *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i % (D / 8)];
+            *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i];
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = from[8 * (i % (D / 8)) + j];
+            for (int j = 0; j < 8; ++j) x[j] = from[8 * i + j];
           }
-          float v[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = live ? to_float(x[j]) : 0.f;
-          if (i < D / 8) {
+        };
+        float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (fabsf(v[j]) < kInf) top = fmaxf(top, fabsf(v[j]));
-            if (i == D / 8 - 1) {
-              int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-              if (e < -100) e = -100;
-              if (top == 0.f) e = 14;
-              up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-              if (a.scale < 0.f) up = -up;
-              if (a.scale == 0.f) up = 0.f;  // every score is 0
-              back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-            }
-          } else {
-            const int k = i - D / 8;
-            *reinterpret_cast<uint4*>(q_panels + k / 8 * kPanel + tc::sw128_chunk(r, k % 8)) =
-                make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
-                           pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
-          }
+        for (int i = 0; i < D / 8; ++i) {  // all loads in flight
+          float v[8];
+          eight(v, i);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (fabsf(v[j]) < kInf) top = fmaxf(top, fabsf(v[j]));
+        }
+        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+        if (e < -100) e = -100;
+        if (top == 0.f) e = 14;
+        float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        if (a.scale < 0.f) up = -up;
+        if (a.scale == 0.f) up = 0.f;  // every score is 0
+        back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+#pragma unroll 2
+        for (int i = 0; i < D / 8; ++i) {
+          float v[8];
+          eight(v, i);
+          *reinterpret_cast<uint4*>(q_panels + i / 8 * kPanel + tc::sw128_chunk(r, i % 8)) =
+              make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
+                         pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
         }
         cxs::fence_proxy_async_shared();
         warp_arrive(&bars->q_full[g], lane);
       }
       if (pending) {
         // The ended item's O: the result, or this share's part of it.
-        if (!warp_wait(&bars->o_done[g], mine_i, bars, c.error)) goto done;
-        ++mine_i;
+        if (!warp_wait(&bars->o_done[g], mine_s - 1, bars, c.error)) goto done;
         tc::fence_after();
         const long long until = ended.end < hi ? ended.end : hi;
         const bool complete = started == ended.begin && until == ended.end;
@@ -491,6 +508,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t x[kKeys];
         ld64(s_at, x);
         ld64(s_at + 64, x + 64);
+        if (L::kApart) {  // S of the next tile may come
+          tc::fence_before();
+          warp_arrive(&bars->s_free[g], lane);
+        }
         if (!__all_sync(0xffffffffu, from <= 0 && to >= kKeys && missing == 0)) {
           // What the row does not see becomes -infinity.
 #pragma unroll
@@ -525,6 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // M moves when a score passes it by 2^8: p stays below 2^8, well inside
         // fp16's range, and most tiles leave O as it is.
         const bool grows = top > m + 8.f;
+        // The last tile's P V is done: O may be rescaled and P overwritten.
+        // (With P over S, S of this tile came after it.)
+        if (L::kApart && mine_s > 0) {
+          if (!warp_wait(&bars->o_done[g], mine_s - 1, bars, c.error)) goto done;
+          tc::fence_after();
+        }
         if (__any_sync(0xffffffffu, grows)) {
           const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
           if (grows) m = top;
@@ -560,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             l = fmaf(sum.x + sum.y, run.z, l);
           }
-          st16(s_at + 16 * q, p);
+          st16(p_at + 16 * q, p);
         }
         tc::wait_st();
         tc::fence_before();
@@ -575,28 +602,41 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < kMmaWarp) {
     // --------------------------------------------------------- conversion ---
     fewer_registers<kConvertRegs>();
-    constexpr int kChunks = D / 16;             // 16-byte chunks of a key
-    constexpr int kStep = 128 / kChunks;        // keys of one pass of the 128 threads
-    const int i = threadIdx.x - 32 * kConvertWarp, key = i / kChunks, chunk = i % kChunks;
-    const int first = chunk % 4 * 2, swap = chunk / 4 & 1;
+    // A thread's 16 codes: chunk `chunk` of 64 channels (a panel), key `key` of
+    // each pass. Eight neighbouring lanes take four chunks of two keys, for
+    // D = 128 of different panels: their reads and their writes then each
+    // cover all banks.
+    const int i = threadIdx.x - 32 * kConvertWarp, chunk = i % 4;
+    const int panel = D == 64 ? 0 : (i / 8 % 2) ^ (i / 4 % 2);
+    const int key = D == 64 ? i / 4 : i / 16 * 2 + i / 4 % 2;
+    constexpr int kStep = 128 * 16 / D;         // keys of one pass of the 128 threads
+    const int from = key * D + panel * 64 + chunk * 16;
+    const int to0 = panel * kPanel + tc::sw128_chunk(key, 2 * chunk);
+    const int to1 = panel * kPanel + tc::sw128_chunk(key, 2 * chunk + 1);
     // Codes -> fp16 in the operand's layout; keys without a token become 0 (a
     // probability of 0 times whatever their bytes hold could be NaN).
     auto convert = [&](const uint8_t* raw, uint8_t* panels, const Tile& tile) {
-      panels += chunk / 4 * kPanel;
       const unsigned missing = tile.missing;
       const int left = tile.left;
-#pragma unroll 2
-      for (int at = key; at < kKeys; at += kStep) {
-        uint4 w = *reinterpret_cast<const uint4*>(raw + at * D + chunk * 16);
-        if (at >= left || missing >> (at / 16) & 1) w = make_uint4(0, 0, 0, 0);
-        const uint4 a0 = make_uint4(half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1),
-                                    half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
-        const uint4 a1 = make_uint4(half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1),
-                                    half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
-        // Lanes of the second panel write their halves in the other order:
-        // eight lanes then cover all banks.
-        *reinterpret_cast<uint4*>(panels + tc::sw128_chunk(at, first + swap)) = swap ? a1 : a0;
-        *reinterpret_cast<uint4*>(panels + tc::sw128_chunk(at, first + 1 - swap)) = swap ? a0 : a1;
+      auto pass = [&](int at, uint4 w) {
+        *reinterpret_cast<uint4*>(panels + to0 + at * 128) =
+            make_uint4(half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1),
+                       half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
+        *reinterpret_cast<uint4*>(panels + to1 + at * 128) =
+            make_uint4(half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1),
+                       half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
+      };
+      if (left >= kKeys && missing == 0) {
+#pragma unroll 4
+        for (int at = 0; at < kKeys; at += kStep)
+          pass(at, *reinterpret_cast<const uint4*>(raw + from + at * D));
+      } else {
+#pragma unroll 1
+        for (int at = 0; at < kKeys; at += kStep) {
+          const bool here = key + at < left && !(missing >> ((key + at) / 16) & 1);
+          pass(at, here ? *reinterpret_cast<const uint4*>(raw + from + at * D)
+                        : make_uint4(0, 0, 0, 0));
+        }
       }
     };
     const int n = (int)(hi - lo);
@@ -630,67 +670,93 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dv = tc::desc_sw128(base + L::kV, kPanel, 1024);
       const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, D, 1);
       const int count = (int)(hi - lo);
-      int s_items[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
-      // S of tile n for group g; `flags` are the tile's.
-      auto issue_s = [&](int g, int n, int flags) -> bool {
-        if (flags & kFirst) {
-          if (!warp_wait(&bars->q_full[g], s_items[g], bars, c.error)) return false;
-          ++s_items[g];
+      // Next tile and uses of the barriers so far, by group.
+      int s_next[2] = {0, 0}, s_items[2] = {0, 0}, s_tiles[2] = {0, 0};
+      int o_next[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
+      auto ready = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, test_wait(bar, phase & 1));
+      };
+      // S of group g's next tile, if what it needs is there: K, the item's
+      // queries, and its columns (read, or with P over S: their P V issued).
+      auto try_s = [&](int g) -> bool {
+        const int n = s_next[g], stage = stage_of<L::kKStages>(n);
+        if (n >= count || (!L::kApart && n > o_next[g])) return false;
+        if (!ready(&bars->k_full[stage], phase_of<L::kKStages>(n))) return false;
+        const int flags = ring[n % kRing].flags;
+        if (g == 1 && !(flags & kTwo)) {  // not for this group
+          ++s_next[1];
+          if (o_next[1] == n) ++o_next[1];
+          return true;
         }
+        if ((flags & kFirst) && !ready(&bars->q_full[g], s_items[g])) return false;
+        if (L::kApart && s_tiles[g] > 0 && !ready(&bars->s_free[g], s_tiles[g] - 1)) return false;
+        s_items[g] += flags & kFirst ? 1 : 0;
+        ++s_tiles[g];
+        ++s_next[g];
         tc::fence_after();
         const uint64_t q = dq + g * L::kPanels * kPanel16;
-        const int stage = stage_of<L::kKStages>(n);
         const uint64_t k = dk + stage * L::kPanels * kPanel16;
+        // The last to use this K: the other group has, or has no rows.
+        const bool last = !(flags & kTwo) || s_next[1 - g] > n;
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
             mma_ss(tmem + 128 * g, q + i / 4 * kPanel16 + 2 * (i % 4),
                    k + i / 4 * kPanel16 + 2 * (i % 4), id_s, i > 0);
           tc::commit(&bars->s_full[g]);
-          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->k_free[stage]);
+          if (last) tc::commit(&bars->k_free[stage]);
         }
         __syncwarp();
         return true;
       };
-      // O of tile n for group g.
-      auto issue_o = [&](int g, int n, int flags) -> bool {
-        if (!warp_wait(&bars->p_full[g], o_tiles[g], bars, c.error)) return false;
-        ++o_tiles[g];
-        if (!warp_wait(&bars->v_full[n & 1], n >> 1, bars, c.error)) return false;
-        if (flags & kFirst) {
-          if (o_items[g] > 0 && !warp_wait(&bars->o_free[g], o_items[g] - 1, bars, c.error))
-            return false;
-          ++o_items[g];
+      // O of group g's next tile, if its P and V are there (and, for an item's
+      // first tile, the last item's O has been read).
+      auto try_o = [&](int g) -> bool {
+        const int n = o_next[g];
+        if (n >= s_next[g]) return false;
+        const int flags = ring[n % kRing].flags;
+        if (g == 1 && !(flags & kTwo)) {
+          ++o_next[1];
+          return true;
         }
+        if (!ready(&bars->p_full[g], o_tiles[g])) return false;
+        if (!ready(&bars->v_full[n & 1], n >> 1)) return false;
+        if ((flags & kFirst) && o_items[g] > 0 && !ready(&bars->o_free[g], o_items[g] - 1))
+          return false;
+        o_items[g] += flags & kFirst ? 1 : 0;
+        ++o_tiles[g];
+        ++o_next[g];
         tc::fence_after();
         const uint64_t v = dv + (n & 1) * L::kPanels * kPanel16;
+        const bool last = !(flags & kTwo) || o_next[1 - g] > n;
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < kKeys / 16; ++i)
-            mma_ts(tmem + 256 + D * g, tmem + 128 * g + 8 * i, v + 128 * i, id_o,
+            mma_ts(tmem + L::kO + D * g, tmem + L::kP + L::kPStep * g + 8 * i, v + 128 * i, id_o,
                    !(flags & kFirst) || i > 0);
-          if (g == 1 || !(flags & kTwo)) tc::commit(&bars->v_free[n & 1]);
-          if (flags & kLast) tc::commit(&bars->o_done[g]);
+          tc::commit(&bars->o_done[g]);
+          if (last) tc::commit(&bars->v_free[n & 1]);
         }
         __syncwarp();
         return true;
       };
-      bool fine = warp_wait(&bars->k_full[0], 0, bars, c.error);
-      int ahead = fine ? ring[0].flags : 0;
-      fine = fine && issue_s(0, 0, ahead);
-      if (ahead & kTwo) fine = fine && issue_s(1, 0, ahead);
-      for (int n = 0; fine && n < count; ++n) {
-        const int flags = ahead;
-        const bool more = n + 1 < count;
-        fine = issue_o(0, n, flags);
-        if (fine && more) {
-          fine = warp_wait(&bars->k_full[stage_of<L::kKStages>(n + 1)],
-                           phase_of<L::kKStages>(n + 1), bars, c.error);
-          ahead = ring[(n + 1) % kRing].flags;
-          fine = fine && issue_s(0, n + 1, ahead);
+      // Whatever is ready, P V first: a group's softmax waits for it longest.
+      bool fine = true;
+      long long since = clock64();
+      while (o_next[0] < count || o_next[1] < count) {
+        bool some = try_o(0);
+        some |= try_o(1);
+        some |= try_s(0);
+        some |= try_s(1);
+        if (some) {
+          since = clock64();
+        } else if (__any_sync(0xffffffffu, *(volatile int*)&bars->abort ||
+                                               clock64() - since > kSpinLimit)) {
+          if (!*(volatile int*)&bars->abort) report(c.error, CXS_DEVICE_ERR_COPY_TIMEOUT);
+          *(volatile int*)&bars->abort = 1;
+          fine = false;
+          break;
         }
-        if (fine && (flags & kTwo)) fine = issue_o(1, n, flags);
-        if (fine && more && (ahead & kTwo)) fine = issue_s(1, n + 1, ahead);
       }
       if (!fine) {  // let the MMAs in flight end before TMEM is freed
         if (elect_one()) tc::commit(&bars->drain);
