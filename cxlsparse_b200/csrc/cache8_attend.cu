@@ -20,6 +20,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 2^(x f + shift) of two scores.
+__device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float shift) {
+  const float2 e =
+      __ffma2_rn(make_float2(x, y), make_float2(f, f), make_float2(shift, shift));
+  return make_float2(ex2(e.x), ex2(e.y));
+}
+
 // ------------------------------------------------- few rows: one warp, 16 ---
 
 // One CTA of 8 warps per SM. A warp takes a tile of keys at a time with all
@@ -32,19 +39,21 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // byte permutes. No transposition passes through shared memory.
 template <int D>
 struct Decode {
-  static constexpr int kWarps = 8, kThreads = 32 * kWarps;
+  static constexpr int kWarps = 12, kThreads = 32 * kWarps;
   static constexpr int kTile = D == 64 ? 64 : 32;     // keys
   static constexpr int kPart = kTile * D;             // bytes of K or V
-  static constexpr int kStages = 3;
-  static constexpr int kStage = 2 * kPart;            // 8 KB; also holds a warp's O (16 x D fp32)
+  static constexpr int kStages = 2;
+  static constexpr int kStage = 2 * kPart;            // also holds a warp's O (16 x D fp32)
   static constexpr int kGroups = kTile / 16;          // runs of 16 keys: within one page
   static constexpr int kRows = 16;
   static_assert(kStage >= kRows * D * 4, "a stage holds a warp's O");
   // Shared memory: stages, then scales, page flags, row statistics, prefix.
   static constexpr int kScales = kWarps * kStages * kStage;
   static constexpr int kBad = kScales + kWarps * kStages * 2 * kGroups * 4;
-  static constexpr int kStats = kBad + kWarps * kStages * 4;
-  static constexpr int kPrefix = (kStats + kWarps * kRows * 2 * 4 + 15) / 16 * 16;
+  static constexpr int kStats = kBad + kWarps * kStages * 4;      // [row][warp] M, l; then factors
+  static constexpr int kQuery = (kStats + kRows * kWarps * 2 * 4 + 15) / 16 * 16;  // fp16 rows
+  static constexpr int kBack = kQuery + kRows * D * 2;            // a row's inverse power of two
+  static constexpr int kPrefix = (kBack + kRows * 4 + 15) / 16 * 16;
   static constexpr int kBytes = kPrefix + (kSlice + 1) * 8;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
@@ -68,6 +77,21 @@ struct Cursor {  // a tile of the CTA's share: its item and place
   int user, kv_head, row0;
   Span span;               // of the user
 };
+
+// Four channels of a row's result, and its log-sum.
+template <typename T>
+__device__ __forceinline__ void write_row(const cxs_cache_attend_call& a, const Shape& z, int first,
+                                          int kv_head, int row, int dim, int d, float4 sum, float m,
+                                          float l) {
+  const bool some = !(l == 0.f);
+  const float inv = some ? 1.f / l : 0.f;
+  const long long head =
+      (long long)(first + row / z.group) * a.heads + kv_head * z.group + row % z.group;
+  alignas(8) T y[4] = {from_float<T>(some ? sum.x * inv : 0.f), from_float<T>(some ? sum.y * inv : 0.f),
+                       from_float<T>(some ? sum.z * inv : 0.f), from_float<T>(some ? sum.w * inv : 0.f)};
+  *reinterpret_cast<uint2*>((T*)a.out + head * dim + d) = *reinterpret_cast<const uint2*>(y);
+  if (a.lse && d == 0) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+}
 
 template <int D>
 __device__ __forceinline__ int item_tiles(const Span& s) {
@@ -121,15 +145,18 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   }
   __syncthreads();
   const long long total = prefix[z.users];
-  const long long wanted = (total + z.min_tiles - 1) / z.min_tiles;
+  const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
   const int ctas = wanted < z.grid ? (int)wanted : z.grid;
   Partial* partials = reinterpret_cast<Partial*>(a.workspace);
   Partial& mine = partials[blockIdx.x];
-  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) mine.parts = 0;
-  if ((int)blockIdx.x >= ctas) return;
-  const long long lo = share(total, blockIdx.x, ctas), hi = share(total, blockIdx.x + 1, ctas);
+  if ((int)blockIdx.x >= ctas) {
+    clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
+    return;
+  }
+  const Shares shares(total, ctas);
+  const long long lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
   float* scratch = reinterpret_cast<float*>(partials + z.grid) +
                    (long long)blockIdx.x * 2 * K::kRows * (D + 2);
 
@@ -149,140 +176,187 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     int bad = 0;
     const Span s = user_span(a, z, u, &bad);
     const int n = item_tiles<D>(s);
-    const long long item = (p.tile - prefix[u]) / n;
+    const long long item = divide(p.tile - prefix[u], n);
     p.user = u;
     p.span = s;
     p.item_begin = prefix[u] + item * n;
     p.item_end = p.item_begin + n;
-    p.kv_head = (int)(item % c.kv_heads);
-    p.row0 = (int)(item / c.kv_heads) * K::kRows;
+    const int rows16 = (int)divide(item, c.kv_heads);
+    p.kv_head = (int)(item - (long long)rows16 * c.kv_heads);
+    p.row0 = rows16 * K::kRows;
   };
 
-  // Copies of the tile at `p` into a stage (commits a group in any case).
   uint8_t* const stages = smem + warp * K::kStages * K::kStage;
   float* const scales = reinterpret_cast<float*>(smem + K::kScales) + warp * K::kStages * 2 * K::kGroups;
   int* const bads = reinterpret_cast<int*>(smem + K::kBad) + warp * K::kStages;
-  auto fetch = [&](const Cursor& p, int stage) {
+  const int page_bits = __ffs(c.page_size) - 1;
+  // A lane's places in a tile (rows 8 apart have the same permutation).
+  constexpr int kChunks = D / 16, kStep = 32 / kChunks;  // copies: rows of one instruction
+  const int copy_row = lane / kChunks, copy_chunk = lane % kChunks;
+  int copy_to[16 / kStep];
+#pragma unroll
+  for (int j = 0; j < 16 / kStep; ++j) copy_to[j] = chunk_at<D>(j * kStep + copy_row, copy_chunk);
+  int k_at[D / 64], v_at[2];
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) k_at[j] = chunk_at<D>(key_of_column(g), t + 4 * j);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    v_at[i] = D == 64 ? chunk_at<D>(i ? 4 + (t ^ 1) : t, g / 2) + (g & 1) * 8
+                      : chunk_at<D>(i ? 4 + (t ^ 1) : t, g);
+  // The page of run u of 16 keys of the tile at `p` (lane u), one tile before
+  // its copies are issued; -2 where it holds no token that a row sees.
+  auto look_up = [&](Cursor& p) -> int {
+    if (p.tile >= hi) return -2;
+    seek(p);
+    const int at = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile + 16 * lane;
+    if (lane >= K::kGroups || at >= p.span.length || at + 16 <= p.span.begin) return -2;
+    return __ldg(c.table + p.user * c.table_stride + (at >> page_bits));
+  };
+  // Copies of the tile at `p` into a stage (commits a group in any case).
+  auto fetch = [&](const Cursor& p, int stage, int id) {
     if (p.tile < hi) {
       const Span& s = p.span;
-      const int tile = s.begin / K::kTile + (int)(p.tile - p.item_begin);
-      const int key0 = tile * K::kTile;
-      // Lane u < groups: the page of run u of 16 keys.
-      int page = -1;
-      if (lane < K::kGroups) {
-        const int at = key0 + 16 * lane;
-        if (at < s.length && at + 16 > s.begin) {
-          page = c.table[p.user * c.table_stride + at / c.page_size];
-          if (page < 0 || page >= c.pages) {
-            page = -1;
-            report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
-          }
-        }
-      }
+      const int key0 = (s.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile;
+      const int page = id >= 0 && id < c.pages ? id : -1;
+      if (page < 0 && id != -2) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
       const unsigned missing = __ballot_sync(0xffffffffu, lane < K::kGroups && page < 0);
       if (lane == 0) bads[stage] = missing;
       uint8_t* const dst = stages + stage * K::kStage;
-      constexpr int kChunks = D / 16, kStep = 32 / kChunks;  // rows of one instruction
-      const int row = lane / kChunks, chunk = lane % kChunks;
+      if (missing == 0 && key0 + K::kTile <= s.length) {
 #pragma unroll
-      for (int u = 0; u < K::kGroups; ++u) {
-        const int pg = __shfl_sync(0xffffffffu, page, u);
-        const long long cell = ((long long)(pg < 0 ? 0 : pg) * c.kv_heads + p.kv_head) * 2;
-        const uint8_t* src = (const uint8_t*)c.codes + cell * c.page_size * D;
-        const int slot0 = (key0 + 16 * u) & (c.page_size - 1);
+        for (int u = 0; u < K::kGroups; ++u) {
+          const int pg = __shfl_sync(0xffffffffu, page, u);
+          const long long cell = ((long long)pg * c.kv_heads + p.kv_head) * 2;
+          const int slot = ((key0 + 16 * u) & (c.page_size - 1)) + copy_row;
+          const uint8_t* src =
+              (const uint8_t*)c.codes + (cell * c.page_size + slot) * D + copy_chunk * 16;
+          const uint8_t* src_v = src + c.page_size * D;
 #pragma unroll
-        for (int j = 0; j < 16 / kStep; ++j) {
-          const int r = j * kStep + row;                       // key of the run
-          const int key = key0 + 16 * u + r;
-          const bool live = pg >= 0 && key < s.length;
-          const uint8_t* from = src + (live ? (slot0 + r) * D + chunk * 16 : 0);
-          const int to = chunk_at<D>(16 * u + r, chunk);
-          __pipeline_memcpy_async(dst + to, from, 16, live ? 0 : 16);
-          __pipeline_memcpy_async(dst + K::kPart + to,
-                                  from + (live ? c.page_size * D : 0), 16, live ? 0 : 16);
+          for (int j = 0; j < 16 / kStep; ++j) {
+            uint8_t* const to = dst + 16 * u * D + copy_to[j];
+            __pipeline_memcpy_async(to, src + j * kStep * D, 16);
+            __pipeline_memcpy_async(to + K::kPart, src_v + j * kStep * D, 16);
+          }
+          if (lane < 2)
+            __pipeline_memcpy_async(scales + (stage * K::kGroups + u) * 2 + lane,
+                                    c.scales + cell + lane, 4);
         }
-        if (lane < 2)
-          __pipeline_memcpy_async(scales + (stage * K::kGroups + u) * 2 + lane,
-                                  c.scales + cell + lane, 4, pg < 0 ? 4 : 0);
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < K::kGroups; ++u) {
+          const int pg = __shfl_sync(0xffffffffu, page, u);
+          const long long cell = ((long long)(pg < 0 ? 0 : pg) * c.kv_heads + p.kv_head) * 2;
+          const uint8_t* src = (const uint8_t*)c.codes + cell * c.page_size * D;
+          const int slot0 = (key0 + 16 * u) & (c.page_size - 1);
+#pragma unroll 1
+          for (int j = 0; j < 16 / kStep; ++j) {
+            const int r = j * kStep + copy_row;                  // key of the run
+            const bool live = pg >= 0 && key0 + 16 * u + r < s.length;
+            const uint8_t* from = src + (live ? (slot0 + r) * D + copy_chunk * 16 : 0);
+            const int to = chunk_at<D>(16 * u + r, copy_chunk);
+            __pipeline_memcpy_async(dst + to, from, 16, live ? 0 : 16);
+            __pipeline_memcpy_async(dst + K::kPart + to, from + (live ? c.page_size * D : 0), 16,
+                                    live ? 0 : 16);
+          }
+          if (lane < 2)
+            __pipeline_memcpy_async(scales + (stage * K::kGroups + u) * 2 + lane,
+                                    c.scales + cell + lane, 4, pg < 0 ? 4 : 0);
+        }
       }
     }
     __pipeline_commit();
   };
 
-  Cursor ahead{lo + warp, -1, -1, 0, 0, 0, {}}, item{lo, -1, -1, 0, 0, 0, {}};
+  // The first item is found, and its queries asked for, before the copies:
+  // loads issued after them wait until they have arrived.
+  Cursor item{lo, -1, -1, 0, 0, 0, {}};
+  seek(item);
+  // A thread's 8 channels of one of the item's rows.
+  constexpr int kLanes = D / 8;  // of a row
+  auto load_queries = [&]() {
+    const int row = item.row0 + threadIdx.x / kLanes;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x >= K::kRows * kLanes || row >= item.span.count * z.group) return x;
+    const T* from = (const T*)a.query + 8 * (threadIdx.x % kLanes) +
+                    (long long)(item.span.first + row / z.group) * a.q_token_stride +
+                    (long long)(item.kv_head * z.group + row % z.group) * a.q_head_stride;
+    if (((uintptr_t)from & 15) == 0) return *reinterpret_cast<const uint4*>(from);
+    alignas(16) T in[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) in[e] = from[e];
+    return *reinterpret_cast<const uint4*>(in);
+  };
+  uint4 raw = load_queries();
+  Cursor ahead = item;
+  ahead.tile = lo + warp;
   long long here = lo + warp;  // the next tile this warp takes
-  int fill = 0;
-#pragma unroll 1
-  for (; fill < K::kStages - 1; ++fill) {
-    seek(ahead);
-    fetch(ahead, fill);
+  int fill = 0, ahead_id = look_up(ahead);
+  auto fetch_next = [&]() {
+    fetch(ahead, fill, ahead_id);
+    fill = fill + 1 == K::kStages ? 0 : fill + 1;
     ahead.tile += K::kWarps;
-  }
+    ahead_id = look_up(ahead);
+  };
+#pragma unroll 1
+  for (int i = 0; i < K::kStages - 1; ++i) fetch_next();
   int use = 0;
 
   float o[D / 8][4], m0, m1, l0, l1;  // rows g and g + 8
-  while (item.tile < hi) {
-    seek(item);
+  while (true) {
     const long long item_hi = item.item_end < hi ? item.item_end : hi;
     const Span& s = item.span;
     const int rows = s.count * z.group;
     const int first_tile = s.begin / K::kTile;
-    // The rows' queries as operands, scaled by a power of two per row.
-    uint32_t q[D / 16][4];
-    float back0, back1;
-    int2 see0 = make_int2(0, 0), see1 = make_int2(0, 0);
-    {
-      float v[2][D / 4];
+    // The rows' queries, scaled by a power of two per row (and the scale's
+    // sign), as fp16 in shared memory: 8 channels a thread. (The last item's
+    // join ended with a barrier: nobody reads the last ones any more.)
+    __half* const queries = reinterpret_cast<__half*>(smem + K::kQuery);
+    float* const backs = reinterpret_cast<float*>(smem + K::kBack);
+    if (threadIdx.x < K::kRows * kLanes) {
+      const int r = threadIdx.x / kLanes, i = threadIdx.x % kLanes;
+      alignas(16) T in[8];
+      *reinterpret_cast<uint4*>(in) = raw;
+      float v[8];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = item.row0 + g + 8 * half;
-        const bool live = r < rows;
-        const T* from = (const T*)a.query;
-        if (live) {
-          from += (long long)(s.first + r / z.group) * a.q_token_stride +
-                  (long long)(item.kv_head * z.group + r % z.group) * a.q_head_stride;
-          const int2 see = row_range(a, s, r / z.group);
-          if (half) see1 = see; else see0 = see;
-        }
-        float top = 0.f;
-        const bool wide = ((uintptr_t)from & 15) == 0;
+      for (int e = 0; e < 8; ++e) v[e] = to_float(in[e]);
+      float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          alignas(16) T in[16];
-          if (wide) {
-            reinterpret_cast<uint4*>(in)[0] = reinterpret_cast<const uint4*>(from + 64 * j + 16 * t)[0];
-            reinterpret_cast<uint4*>(in)[1] = reinterpret_cast<const uint4*>(from + 64 * j + 16 * t)[1];
-          } else {
+      for (int e = 0; e < 8; ++e)
+        if (fabsf(v[e]) < kInf) top = fmaxf(top, fabsf(v[e]));
 #pragma unroll
-            for (int e = 0; e < 16; ++e) in[e] = from[64 * j + 16 * t + e];
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float x = live ? to_float(in[e]) : 0.f;
-            v[half][16 * j + e] = x;
-            if (fabsf(x) < kInf) top = fmaxf(top, fabsf(x));
-          }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-        if (e < -100) e = -100;
-        if (top == 0.f) e = 14;
-        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-        if (half) back1 = down; else back0 = down;
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i) v[half][i] *= up;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        q[i][0] = pack_half2(v[0][4 * i], v[0][4 * i + 1]);
-        q[i][1] = pack_half2(v[1][4 * i], v[1][4 * i + 1]);
-        q[i][2] = pack_half2(v[0][4 * i + 2], v[0][4 * i + 3]);
-        q[i][3] = pack_half2(v[1][4 * i + 2], v[1][4 * i + 3]);
-      }
+      for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+      if (e < -100) e = -100;
+      if (top == 0.f) e = 14;
+      float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      if (a.scale < 0.f) up = -up;
+      if (a.scale == 0.f) up = 0.f;  // every score is 0
+      if (i == 0) backs[r] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      *reinterpret_cast<uint4*>(queries + r * D + 8 * i) =
+          make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
+                     pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
     }
-    const float unit = a.scale * kLog2e;
+    __syncthreads();
+    // This lane's rows g and g + 8: what they see, and their operands (its 16
+    // channels of each 64 are four steps' operand elements).
+    int2 see0 = make_int2(0, 0), see1 = make_int2(0, 0);
+    if (item.row0 + g < rows) see0 = row_range(a, s, (item.row0 + g) / z.group);
+    if (item.row0 + g + 8 < rows) see1 = row_range(a, s, (item.row0 + g + 8) / z.group);
+    const float back0 = backs[g], back1 = backs[g + 8];
+    uint32_t q[D / 16][4];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = *reinterpret_cast<const uint4*>(queries + g * D + 64 * j + 16 * t + 8 * h);
+        const uint4 y =
+            *reinterpret_cast<const uint4*>(queries + (g + 8) * D + 64 * j + 16 * t + 8 * h);
+        q[4 * j + 2 * h][0] = x.x, q[4 * j + 2 * h][2] = x.y;
+        q[4 * j + 2 * h + 1][0] = x.z, q[4 * j + 2 * h + 1][2] = x.w;
+        q[4 * j + 2 * h][1] = y.x, q[4 * j + 2 * h][3] = y.y;
+        q[4 * j + 2 * h + 1][1] = y.z, q[4 * j + 2 * h + 1][3] = y.w;
+      }
+    const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -301,10 +375,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     for (; here < item_hi; here += K::kWarps) {
       // The stage consumed in the previous round is free: fetch ahead into it.
       __syncwarp();
-      seek(ahead);
-      fetch(ahead, fill);
-      ahead.tile += K::kWarps;
-      fill = fill + 1 == K::kStages ? 0 : fill + 1;
+      fetch_next();
       __pipeline_wait_prior(K::kStages - 1);
       __syncwarp();
       const uint8_t* ks = stages + use * K::kStage;
@@ -319,33 +390,16 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
 #pragma unroll
       for (int n = 0; n < K::kTile / 8; ++n) {
         x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
-        const int r = 8 * n + key_of_column(g);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(ks + chunk_at<D>(r, t + 4 * j));
+          const uint4 w = *reinterpret_cast<const uint4*>(ks + 8 * n * D + k_at[j]);
           mma16816(x[n], q[4 * j + 0], half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1));
           mma16816(x[n], q[4 * j + 1], half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
           mma16816(x[n], q[4 * j + 2], half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1));
           mma16816(x[n], q[4 * j + 3], half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
         }
       }
-      // x = scale log2(e) s_k q.c + log2 s_v; -inf where a row does not see the key.
-      float per[K::kGroups];  // 1 / s_v
-#pragma unroll
-      for (int u = 0; u < K::kGroups; ++u) {
-        const float sk = usable_scale(sc[2 * u]) * unit, sv = usable_scale(sc[2 * u + 1]);
-        const float lift = __log2f(sv);
-        per[u] = __frcp_rn(sv);
-        const float f0 = sk * back0, f1 = sk * back1;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float(&y)[4] = x[2 * u + h];
-          y[0] = fmaf(y[0], f0, lift);
-          y[1] = fmaf(y[1], f0, lift);
-          y[2] = fmaf(y[2], f1, lift);
-          y[3] = fmaf(y[3], f1, lift);
-        }
-      }
+      // -infinity where a row does not see the key.
       if (missing || key0 < all.x || key0 + K::kTile > all.y) {
 #pragma unroll
         for (int n = 0; n < K::kTile / 8; ++n) {
@@ -357,21 +411,39 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
           if (gone || kb < see1.x || kb >= see1.y) x[n][3] = -kInf;
         }
       }
+      // A score is x f + lift: f = scale log2(e) s_k (and the row's power of
+      // two), lift = log2 s_v, per = 1 / s_v.
+      float f0[K::kGroups], f1[K::kGroups], lift[K::kGroups], per[K::kGroups];
       float t0 = -kInf, t1 = -kInf;
+      // (Lane u works them out for run u.)
+      const float2 scale = *reinterpret_cast<const float2*>(sc + 2 * (lane % K::kGroups));
+      const float my_f = usable_scale(scale.x) * unit;
+      const float my_lift = __log2f(usable_scale(scale.y)), my_per = ex2(-my_lift);
 #pragma unroll
-      for (int n = 0; n < K::kTile / 8; ++n) {
-        t0 = fmaxf(t0, fmaxf(x[n][0], x[n][1]));
-        t1 = fmaxf(t1, fmaxf(x[n][2], x[n][3]));
+      for (int u = 0; u < K::kGroups; ++u) {
+        const float sk = __shfl_sync(0xffffffffu, my_f, u);
+        lift[u] = __shfl_sync(0xffffffffu, my_lift, u);
+        per[u] = __shfl_sync(0xffffffffu, my_per, u);
+        // Never 0, which times a hidden score would be NaN; NaN stays NaN.
+        f0[u] = sk * back0 < 1.2e-38f ? 1.2e-38f : sk * back0;
+        f1[u] = sk * back1 < 1.2e-38f ? 1.2e-38f : sk * back1;
+        const float(&ya)[4] = x[2 * u];
+        const float(&yb)[4] = x[2 * u + 1];
+        t0 = fmaxf(t0, fmaf(fmaxf(fmaxf(ya[0], ya[1]), fmaxf(yb[0], yb[1])), f0[u], lift[u]));
+        t1 = fmaxf(t1, fmaf(fmaxf(fmaxf(ya[2], ya[3]), fmaxf(yb[2], yb[3])), f1[u], lift[u]));
       }
       t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
       t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
       t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
       t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-      if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1)) {
-        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-        const float c0 = m0 == -kInf ? 0.f : ex2(m0 - n0), c1 = m1 == -kInf ? 0.f : ex2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
+      // M moves when a score passes it by 2^8: p stays below 2^8, well inside
+      // fp16's range, and most tiles leave O as it is.
+      const bool g0 = t0 > m0 + 8.f, g1 = t1 > m1 + 8.f;
+      if (__any_sync(0xffffffffu, g0 || g1)) {
+        const float c0 = !g0 ? 1.f : m0 == -kInf ? 0.f : ex2(m0 - t0);
+        const float c1 = !g1 ? 1.f : m1 == -kInf ? 0.f : ex2(m1 - t1);
+        if (g0) m0 = t0;
+        if (g1) m1 = t1;
         l0 *= c0;
         l1 *= c1;
 #pragma unroll
@@ -387,27 +459,26 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
       for (int u = 0; u < K::kGroups; ++u) {
         float(&ya)[4] = x[2 * u];
         float(&yb)[4] = x[2 * u + 1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ya[e] = ex2(ya[e] - (e < 2 ? b0 : b1));
-          yb[e] = ex2(yb[e] - (e < 2 ? b0 : b1));
-        }
-        l0 = fmaf((ya[0] + ya[1]) + (yb[0] + yb[1]), per[u], l0);
-        l1 = fmaf((ya[2] + ya[3]) + (yb[2] + yb[3]), per[u], l1);
-        const uint32_t p[4] = {pack_half2(ya[0], ya[1]), pack_half2(ya[2], ya[3]),
-                               pack_half2(yb[0], yb[1]), pack_half2(yb[2], yb[3])};
+        const float s0 = lift[u] - b0, s1 = lift[u] - b1;
+        const float2 pa0 = exp2_pair(ya[0], ya[1], f0[u], s0), pb0 = exp2_pair(yb[0], yb[1], f0[u], s0);
+        const float2 pa1 = exp2_pair(ya[2], ya[3], f1[u], s1), pb1 = exp2_pair(yb[2], yb[3], f1[u], s1);
+        const float2 sum0 = __fadd2_rn(pa0, pb0), sum1 = __fadd2_rn(pa1, pb1);
+        l0 = fmaf(sum0.x + sum0.y, per[u], l0);
+        l1 = fmaf(sum1.x + sum1.y, per[u], l1);
+        const uint32_t p[4] = {pack_half2(pa0.x, pa0.y), pack_half2(pa1.x, pa1.y),
+                               pack_half2(pb0.x, pb0.y), pack_half2(pb1.x, pb1.y)};
         // Keys of this lane's four operand rows; D / 8 of their channels each.
         constexpr int kWords = D / 32;
         uint32_t w[4][kWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = 16 * u + 8 * (i / 2) + (i & 1 ? 4 + (t ^ 1) : t);
+          const uint8_t* from = vs + (16 * u + 8 * (i / 2)) * D + v_at[i % 2];
           if (D == 64) {
-            const uint2 v = *reinterpret_cast<const uint2*>(vs + chunk_at<D>(r, g / 2) + (g & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(from);
             w[i][0] = v.x;
             w[i][1] = v.y;
           } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(vs + chunk_at<D>(r, g));
+            const uint4 v = *reinterpret_cast<const uint4*>(from);
             w[i][0] = v.x;
             w[i][1] = v.y;
             w[i][kWords - 2] = v.z;
@@ -430,21 +501,19 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
 
     // Join the warps. Each writes O into the stage it consumed last (nothing
     // is in flight there), rows of D fp32, and its rows' M and l.
-    float* const stats = reinterpret_cast<float*>(smem + K::kStats);
+    float2* const stats = reinterpret_cast<float2*>(smem + K::kStats);  // [row][warp]
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    int* const where = reinterpret_cast<int*>(warp_sum);  // stage of each warp, -1: none
+    int* const where = reinterpret_cast<int*>(warp_sum);  // place of each warp's O, -1: none
     __syncwarp();
     if (lane == 0) where[warp] = latest < 0 ? -1 : (warp * K::kStages + latest) * K::kStage;
+    if (t == 0) {
+      stats[g * K::kWarps + warp] = make_float2(m0, l0);
+      stats[(g + 8) * K::kWarps + warp] = make_float2(m1, l1);
+    }
     if (latest >= 0) {
-      if (t == 0) {
-        stats[(warp * K::kRows + g) * 2] = m0;
-        stats[(warp * K::kRows + g) * 2 + 1] = l0;
-        stats[(warp * K::kRows + g + 8) * 2] = m1;
-        stats[(warp * K::kRows + g + 8) * 2 + 1] = l1;
-      }
       float* dst = reinterpret_cast<float*>(stages + latest * K::kStage);
       // Accumulator i, columns 2t, 2t + 1: channels (D / 8) column + i.
 #pragma unroll
@@ -459,20 +528,22 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     // An item that began in an earlier share leaves its partial in slot 0,
     // one that begins here and goes on in slot 1.
     float* const part = scratch + (item.tile == item.item_begin ? K::kRows * (D + 2) : 0);
+    // A thread for each four channels of a row.
     for (int i = threadIdx.x; i < K::kRows * D / 4; i += K::kThreads) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       const int row = item.row0 + r;
       if (row >= rows) continue;
-      float m = -kInf;
-      for (int w = 0; w < K::kWarps; ++w)
-        if (where[w] >= 0) m = fmaxf(m, stats[(w * K::kRows + r) * 2]);
+      const float2* const its = stats + r * K::kWarps;
+      float m = -kInf, l = 0.f;
+#pragma unroll 4
+      for (int w = 0; w < K::kWarps; ++w) m = fmaxf(m, its[w].x);
       const float base = m == -kInf ? 0.f : m;
-      float l = 0.f;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
       for (int w = 0; w < K::kWarps; ++w) {
         if (where[w] < 0) continue;
-        const float f = ex2(stats[(w * K::kRows + r) * 2] - base);
-        l = fmaf(stats[(w * K::kRows + r) * 2 + 1], f, l);
+        const float f = ex2(its[w].x - base);
+        l = fmaf(its[w].y, f, l);
         const float4 v = *reinterpret_cast<const float4*>(smem + where[w] + (r * D + d) * 4);
         sum.x = fmaf(v.x, f, sum.x);
         sum.y = fmaf(v.y, f, sum.y);
@@ -480,37 +551,30 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         sum.w = fmaf(v.w, f, sum.w);
       }
       if (whole) {
-        const bool some = !(l == 0.f);
-        const float inv = some ? 1.f / l : 0.f;
-        const long long head = (long long)(s.first + row / z.group) * a.heads +
-                               item.kv_head * z.group + row % z.group;
-        T* out = (T*)a.out + head * D + d;
-        out[0] = from_float<T>(some ? sum.x * inv : 0.f);
-        out[1] = from_float<T>(some ? sum.y * inv : 0.f);
-        out[2] = from_float<T>(some ? sum.z * inv : 0.f);
-        out[3] = from_float<T>(some ? sum.w * inv : 0.f);
-        if (a.lse && d == 0) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+        write_row<T>(a, z, s.first, item.kv_head, row, D, d, sum, m, l);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = sum;
-        if (d == 0) {
-          part[K::kRows * D + 2 * r] = m;
-          part[K::kRows * D + 2 * r + 1] = l;
-        }
+        if (d == 0)
+          *reinterpret_cast<float2*>(part + K::kRows * D + 2 * r) = make_float2(m, l);
       }
     }
     if (!whole && item.tile == item.item_begin && threadIdx.x == 0) {
       // The last share that holds a tile of the item.
-      const int last = share_of(total, item.item_end - 1, ctas);
+      const int last = shares.of(item.item_end - 1);
       mine.first = s.first;
       mine.rows = rows;
       mine.row0 = item.row0;
       mine.kv_head = item.kv_head;
       mine.parts = last - (int)blockIdx.x + 1;
     }
-    __syncthreads();  // the stages are free again
     item.tile = item_hi;
+    if (item_hi >= hi) break;
+    seek(item);
+    raw = load_queries();
+    __syncthreads();  // the stages are free again
   }
   __pipeline_wait_prior(0);
+  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
 }
 
 // Joins the partial results of the item (of ROWS rows) that starts in share
@@ -529,32 +593,38 @@ __global__ void combine_kernel(const cxs_cache_attend_call a, const Shape z) {
   const int row = item.row0 + r;
   if (row >= item.rows) return;
   auto part = [&](int i) { return scratch + (i == 0 ? kSize : 2 * i * kSize); };
-  float m = -kInf;
-#pragma unroll 8
-  for (int i = 0; i < item.parts; ++i) m = fmaxf(m, part(i)[kRows * D + 2 * r]);
-  const float base = m == -kInf ? 0.f : m;
-  float l = 0.f;
+  // Four shares at a time, all their loads in flight.
+  float m = -kInf, l = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = 0; i < item.parts; ++i) {
-    const float f = ex2(part(i)[kRows * D + 2 * r] - base);
-    l = fmaf(part(i)[kRows * D + 2 * r + 1], f, l);
-    const float4 v = *reinterpret_cast<const float4*>(part(i) + r * D + d);
-    sum.x = fmaf(v.x, f, sum.x);
-    sum.y = fmaf(v.y, f, sum.y);
-    sum.z = fmaf(v.z, f, sum.z);
-    sum.w = fmaf(v.w, f, sum.w);
+  for (int i0 = 0; i0 < item.parts; i0 += 4) {
+    float2 stat[4];
+    float4 v[4];
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* from = part(min(i0 + j, item.parts - 1));
+      stat[j] = *reinterpret_cast<const float2*>(from + kRows * D + 2 * r);
+      v[j] = *reinterpret_cast<const float4*>(from + r * D + d);
+      if (i0 + j >= item.parts) stat[j] = make_float2(-kInf, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, stat[j].x);
+    const float base = top == -kInf ? 0.f : top, old = ex2(m - base);
+    m = top;
+    l *= old;
+    sum.x *= old, sum.y *= old, sum.z *= old, sum.w *= old;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j >= item.parts) break;
+      const float f = ex2(stat[j].x - base);
+      l = fmaf(stat[j].y, f, l);
+      sum.x = fmaf(v[j].x, f, sum.x);
+      sum.y = fmaf(v[j].y, f, sum.y);
+      sum.z = fmaf(v[j].z, f, sum.z);
+      sum.w = fmaf(v[j].w, f, sum.w);
+    }
   }
-  const bool some = !(l == 0.f);
-  const float inv = some ? 1.f / l : 0.f;
-  const long long head =
-      (long long)(item.first + row / z.group) * a.heads + item.kv_head * z.group + row % z.group;
-  T* out = (T*)a.out + head * D + d;
-  out[0] = from_float<T>(some ? sum.x * inv : 0.f);
-  out[1] = from_float<T>(some ? sum.y * inv : 0.f);
-  out[2] = from_float<T>(some ? sum.z * inv : 0.f);
-  out[3] = from_float<T>(some ? sum.w * inv : 0.f);
-  if (a.lse && d == 0) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+  write_row<T>(a, z, item.first, item.kv_head, row, D, d, sum, m, l);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -659,6 +729,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
   status = cxs_host::check_cache_pointers(&c, "cache attend");
   if (status != CXS_OK) return status;
   if (!call->query || !call->out) return set_error(CXS_ERR_INVALID, "cache attend: null query or out");
+  if ((uintptr_t)call->out % 16) return set_error(CXS_ERR_INVALID, "cache attend: out must be 16-byte aligned");
   if (!call->workspace || (uintptr_t)call->workspace % 16 ||
       call->workspace_bytes < workspace_bytes(*call))
     return set_error(CXS_ERR_INVALID, "cache attend: workspace missing, unaligned or too small");
@@ -672,7 +743,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
     cxs_cache_attend_call a = *call;
     const int left = c.users - user0;
     const Shape z{call->heads / c.kv_heads, user0, left < kSlice ? left : kSlice, left <= kSlice,
-                  grid, few ? Decode<64>::kWarps : 2};
+                  grid, !few ? 2 : c.dim == 64 ? Decode<64>::kWarps : Decode<128>::kWarps};
     a.cache.table += user0 * c.table_stride;
     a.cache.lengths += user0;
     if (a.cache.offsets) a.cache.offsets += user0;

@@ -292,16 +292,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
   const long long total = prefix[z.users];
-  const long long wanted = (total + z.min_tiles - 1) / z.min_tiles;
+  const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
   const int ctas = wanted < z.grid ? (int)wanted : z.grid;
   Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
   Partial& mine = partials[blockIdx.x];
-  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) mine.parts = 0;
   const bool busy = (int)blockIdx.x < ctas;
-  const long long lo = busy ? share(total, blockIdx.x, ctas) : 0;
-  const long long hi = busy ? share(total, blockIdx.x + 1, ctas) : 0;
+  const Shares shares(total, ctas > 0 ? ctas : 1);
+  const long long lo = busy ? shares.begin(blockIdx.x) : 0;
+  const long long hi = busy ? shares.begin(blockIdx.x + 1) : 0;
   float* const scratch = reinterpret_cast<float*>(partials + z.grid) +
                          (long long)blockIdx.x * 2 * kTileRows * (D + 2);
 
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 (long long)tiles * c.kv_heads;
         item.tile_row = r0 + at;
         item.first = __shfl_sync(0xffffffffu, first, at);
-        item.kv_head = (int)((lo - start) / tiles);
+        item.kv_head = (int)divide(lo - start, tiles);
         item.begin = start + (long long)item.kv_head * tiles;
         item.end = item.begin + tiles;
         break;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
         }
         if (!complete && started == ended.begin && g == 0 && r == 0) {
-          const int last = share_of(total, ended.end - 1, ctas);
+          const int last = shares.of(ended.end - 1);
           mine.first = ended.span.first;
           mine.rows = ended.rows;
           mine.row0 = ended.tile_row * kTileRows;
@@ -849,6 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 done:
   __syncwarp();
+  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();

@@ -546,7 +546,7 @@ int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream);
 /* Attention of the new tokens' queries [tokens, heads, dim] (bf16 or fp16,
  * channels contiguous, strides in elements; query head h reads KV head
  * h / (heads / kv_heads)) over the cached tokens of their user:
- *   out = softmax(scale * q . k over the visible tokens) . v   [tokens, heads, dim]
+ *   out = softmax(scale * q . k over the visible tokens) . v   [tokens, heads, dim], 16-byte aligned
  *   lse = log of the softmax's sum (natural, fp32), or NULL    [tokens, heads]
  * The row at position p sees positions <= p (causal) or < lengths[b], and with
  * window > 0 only positions > p - window. A row that sees nothing gets out = 0
