@@ -1,7 +1,5 @@
 // Attention over the dense 8-bit cache: few query rows a KV head, the joining
 // of partial results, and the entry points.
-#include <cuda_pipeline_primitives.h>
-
 #include "cache8_attend.cuh"
 
 using cxs_host::set_error;
@@ -29,28 +27,27 @@ __device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float shi
 
 // ------------------------------------------------- few rows: one warp, 16 ---
 
-// One CTA of 8 warps per SM. A warp takes a tile of keys at a time with all
-// 16 rows: K and V codes go global -> shared with 16-byte asynchronous copies
-// (zeros for tokens no row sees), two tiles ahead, then straight into
-// mma.sync fragments: the order of channels within a dot product is free, so
-// a lane's 16 bytes of a key are its fragments of four steps, and the order
-// of keys within a tile is chosen so that the scores' accumulator is the
-// probabilities' operand and a lane's V bytes of four keys pair up by
-// byte permutes. No transposition passes through shared memory.
+// One CTA of 12 warps per SM. A warp takes a tile of keys at a time with all
+// 16 rows: the tile's runs of K and V codes come by bulk copies, one tile
+// ahead, and go from shared memory straight into mma.sync fragments: the
+// order of channels within a dot product is free, so a lane's 16 bytes of a
+// key are its fragments of four steps, and the order of keys within a tile is
+// chosen so that the scores' accumulator is the probabilities' operand and a
+// lane's V bytes of four keys pair up by byte permutes. No transposition
+// passes through shared memory.
 template <int D>
 struct Decode {
   static constexpr int kWarps = 12, kThreads = 32 * kWarps;
   static constexpr int kTile = D == 64 ? 64 : 32;     // keys
   static constexpr int kPart = kTile * D;             // bytes of K or V
-  static constexpr int kStages = 2;
+  static constexpr int kStages = 2;                   // one in work, one coming
   static constexpr int kStage = 2 * kPart;            // also holds a warp's O (16 x D fp32)
   static constexpr int kGroups = kTile / 16;          // runs of 16 keys: within one page
   static constexpr int kRows = 16;
   static_assert(kStage >= kRows * D * 4, "a stage holds a warp's O");
-  // Shared memory: stages, then scales, page flags, row statistics, prefix.
-  static constexpr int kScales = kWarps * kStages * kStage;
-  static constexpr int kBad = kScales + kWarps * kStages * 2 * kGroups * 4;
-  static constexpr int kStats = kBad + kWarps * kStages * 4;      // [row][warp] M, l; then factors
+  // Shared memory: stages, their barriers, row statistics, queries, prefix.
+  static constexpr int kBars = kWarps * kStages * kStage;
+  static constexpr int kStats = kBars + kWarps * kStages * 8;     // [row][warp] M, l
   static constexpr int kQuery = (kStats + kRows * kWarps * 2 * 4 + 15) / 16 * 16;  // fp16 rows
   static constexpr int kBack = kQuery + kRows * D * 2;            // a row's inverse power of two
   static constexpr int kPrefix = (kBack + kRows * 4 + 15) / 16 * 16;
@@ -58,17 +55,8 @@ struct Decode {
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
-// 16-byte chunk c of key row r in a tile. The permutation spreads the rows
-// that one load instruction touches over all banks (rows 0..3 or 4..7 of a
-// run of 8 with two neighbouring chunks for V, rows t and 4 + (t ^ 1) with
-// four chunks for K).
-template <int D>
-__device__ __forceinline__ int chunk_at(int r, int c) {
-  if (D == 64) return r * D + ((c ^ (r & 2)) << 4);
-  return r * D + ((c ^ (2 * ((r ^ ((r >> 1) & 2)) & 3))) << 4);
-}
-
-// Column n of an 8-key score tile is key n / 2, or 4 + (n / 2 ^ 1) for odd n.
+// Column n of an 8-key score tile is key n / 2, or 4 + (n / 2 ^ 1) for odd n:
+// the rows that neighbouring lanes read then lie in different banks (D = 64).
 __device__ __forceinline__ int key_of_column(int n) { return n & 1 ? 4 + ((n >> 1) ^ 1) : n >> 1; }
 
 struct Cursor {  // a tile of the CTA's share: its item and place
@@ -187,84 +175,41 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   };
 
   uint8_t* const stages = smem + warp * K::kStages * K::kStage;
-  float* const scales = reinterpret_cast<float*>(smem + K::kScales) + warp * K::kStages * 2 * K::kGroups;
-  int* const bads = reinterpret_cast<int*>(smem + K::kBad) + warp * K::kStages;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + K::kBars) + warp * K::kStages;
+  if (lane < K::kStages) cxs::mbar_init(bars + lane, 1);
+  cxs::fence_mbar_init();
+  __syncwarp();
+  // A tile's copies: piece_keys keys of one page each, lane 2 i its K, lane
+  // 2 i + 1 its V.
+  const int piece_bits = min(__ffs(c.page_size), __ffs(K::kTile)) - 1;
   const int page_bits = __ffs(c.page_size) - 1;
-  // A lane's places in a tile (rows 8 apart have the same permutation).
-  constexpr int kChunks = D / 16, kStep = 32 / kChunks;  // copies: rows of one instruction
-  const int copy_row = lane / kChunks, copy_chunk = lane % kChunks;
-  int copy_to[16 / kStep];
-#pragma unroll
-  for (int j = 0; j < 16 / kStep; ++j) copy_to[j] = chunk_at<D>(j * kStep + copy_row, copy_chunk);
-  int k_at[D / 64], v_at[2];
-#pragma unroll
-  for (int j = 0; j < D / 64; ++j) k_at[j] = chunk_at<D>(key_of_column(g), t + 4 * j);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    v_at[i] = D == 64 ? chunk_at<D>(i ? 4 + (t ^ 1) : t, g / 2) + (g & 1) * 8
-                      : chunk_at<D>(i ? 4 + (t ^ 1) : t, g);
-  // The page of run u of 16 keys of the tile at `p` (lane u), one tile before
-  // its copies are issued; -2 where it holds no token that a row sees.
+  const int copies = 2 * (K::kTile >> piece_bits), piece_bytes = D << piece_bits;
+  // A copy's page, looked up one tile before the copy is issued; -2 where it
+  // holds no token that a row sees.
   auto look_up = [&](Cursor& p) -> int {
     if (p.tile >= hi) return -2;
     seek(p);
-    const int at = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile + 16 * lane;
-    if (lane >= K::kGroups || at >= p.span.length || at + 16 <= p.span.begin) return -2;
+    const int at = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile +
+                   (lane / 2 << piece_bits);
+    if (lane >= copies || at >= p.span.length || at + (1 << piece_bits) <= p.span.begin) return -2;
     return __ldg(c.table + p.user * c.table_stride + (at >> page_bits));
   };
-  // Copies of the tile at `p` into a stage (commits a group in any case).
-  auto fetch = [&](const Cursor& p, int stage, int id) {
-    if (p.tile < hi) {
-      const Span& s = p.span;
-      const int key0 = (s.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile;
-      const int page = id >= 0 && id < c.pages ? id : -1;
-      if (page < 0 && id != -2) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
-      const unsigned missing = __ballot_sync(0xffffffffu, lane < K::kGroups && page < 0);
-      if (lane == 0) bads[stage] = missing;
-      uint8_t* const dst = stages + stage * K::kStage;
-      if (missing == 0 && key0 + K::kTile <= s.length) {
-#pragma unroll
-        for (int u = 0; u < K::kGroups; ++u) {
-          const int pg = __shfl_sync(0xffffffffu, page, u);
-          const long long cell = ((long long)pg * c.kv_heads + p.kv_head) * 2;
-          const int slot = ((key0 + 16 * u) & (c.page_size - 1)) + copy_row;
-          const uint8_t* src =
-              (const uint8_t*)c.codes + (cell * c.page_size + slot) * D + copy_chunk * 16;
-          const uint8_t* src_v = src + c.page_size * D;
-#pragma unroll
-          for (int j = 0; j < 16 / kStep; ++j) {
-            uint8_t* const to = dst + 16 * u * D + copy_to[j];
-            __pipeline_memcpy_async(to, src + j * kStep * D, 16);
-            __pipeline_memcpy_async(to + K::kPart, src_v + j * kStep * D, 16);
-          }
-          if (lane < 2)
-            __pipeline_memcpy_async(scales + (stage * K::kGroups + u) * 2 + lane,
-                                    c.scales + cell + lane, 4);
-        }
-      } else {
-#pragma unroll 1
-        for (int u = 0; u < K::kGroups; ++u) {
-          const int pg = __shfl_sync(0xffffffffu, page, u);
-          const long long cell = ((long long)(pg < 0 ? 0 : pg) * c.kv_heads + p.kv_head) * 2;
-          const uint8_t* src = (const uint8_t*)c.codes + cell * c.page_size * D;
-          const int slot0 = (key0 + 16 * u) & (c.page_size - 1);
-#pragma unroll 1
-          for (int j = 0; j < 16 / kStep; ++j) {
-            const int r = j * kStep + copy_row;                  // key of the run
-            const bool live = pg >= 0 && key0 + 16 * u + r < s.length;
-            const uint8_t* from = src + (live ? (slot0 + r) * D + copy_chunk * 16 : 0);
-            const int to = chunk_at<D>(16 * u + r, copy_chunk);
-            __pipeline_memcpy_async(dst + to, from, 16, live ? 0 : 16);
-            __pipeline_memcpy_async(dst + K::kPart + to, from + (live ? c.page_size * D : 0), 16,
-                                    live ? 0 : 16);
-          }
-          if (lane < 2)
-            __pipeline_memcpy_async(scales + (stage * K::kGroups + u) * 2 + lane,
-                                    c.scales + cell + lane, 4, pg < 0 ? 4 : 0);
-        }
-      }
-    }
-    __pipeline_commit();
+  // Copies of the tile at `p` into a stage. Returns this lane's scale (of its
+  // copy's page and part) and which copies there are.
+  auto fetch = [&](const Cursor& p, int stage, int id, unsigned* there) -> float {
+    if (p.tile >= hi) return 1.f;
+    const int key0 = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile;
+    const bool mine = id >= 0 && id < c.pages;
+    if (!mine && id != -2) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
+    *there = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) cxs::mbar_expect_tx(bars + stage, __popc(*there) * piece_bytes);
+    __syncwarp();
+    if (!mine) return 1.f;
+    const long long cell = ((long long)id * c.kv_heads + p.kv_head) * 2 + (lane & 1);
+    cxs::bulk_g2s(stages + stage * K::kStage + (lane & 1) * K::kPart + lane / 2 * piece_bytes,
+                  (const uint8_t*)c.codes + (cell * c.page_size + (key0 & (c.page_size - 1))) * D,
+                  piece_bytes, bars + stage);
+    return __ldg(c.scales + cell);
   };
 
   // The first item is found, and its queries asked for, before the copies:
@@ -290,16 +235,16 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   Cursor ahead = item;
   ahead.tile = lo + warp;
   long long here = lo + warp;  // the next tile this warp takes
-  int fill = 0, ahead_id = look_up(ahead);
-  auto fetch_next = [&]() {
-    fetch(ahead, fill, ahead_id);
-    fill = fill + 1 == K::kStages ? 0 : fill + 1;
-    ahead.tile += K::kWarps;
-    ahead_id = look_up(ahead);
-  };
-#pragma unroll 1
-  for (int i = 0; i < K::kStages - 1; ++i) fetch_next();
-  int use = 0;
+  int taken = 0;                // tiles taken so far: stage taken % 2
+  unsigned next_there = 0;      // of the tile that is coming
+  int ahead_id = look_up(ahead);
+  float next_scale = fetch(ahead, 0, ahead_id, &next_there);
+  ahead.tile += K::kWarps;
+  ahead_id = look_up(ahead);
+  // Where this lane reads: its 16 channels of a key, its D / 8 of V.
+  const int k_at = key_of_column(g) * D + 16 * t;
+  const int v_at0 = t * D + D / 8 * g, v_at1 = (4 + (t ^ 1)) * D + D / 8 * g;
+  bool lost = false;  // a copy did not come
 
   float o[D / 8][4], m0, m1, l0, l1;  // rows g and g + 8
   while (true) {
@@ -370,21 +315,41 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     all.x = __reduce_max_sync(0xffffffffu, all.x);
     all.y = __reduce_min_sync(0xffffffffu, all.y);
 
-    int latest = -1;  // the stage this warp consumed last (free until the next fetch)
+    int latest = -1;  // the stage this warp took last (free until the next fetch)
 #pragma unroll 1
     for (; here < item_hi; here += K::kWarps) {
-      // The stage consumed in the previous round is free: fetch ahead into it.
+      // The stage taken in the previous round is free: the next tile's copies.
       __syncwarp();
-      fetch_next();
-      __pipeline_wait_prior(K::kStages - 1);
-      __syncwarp();
-      const uint8_t* ks = stages + use * K::kStage;
-      const uint8_t* vs = ks + K::kPart;
-      const float* sc = scales + use * 2 * K::kGroups;
-      const int missing = bads[use];
-      latest = use;
-      use = use + 1 == K::kStages ? 0 : use + 1;
+      const float scale = next_scale;
+      const unsigned there = next_there;
+      next_scale = fetch(ahead, (taken + 1) % 2, ahead_id, &next_there);
+      ahead.tile += K::kWarps;
+      ahead_id = look_up(ahead);
+      if (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1)) {
+        const long long since = clock64();
+        while (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1) && !lost)
+          lost = clock64() - since > kSpinLimit;
+        if (lost) report(c.error, CXS_DEVICE_ERR_COPY_TIMEOUT);
+      }
+      latest = taken % 2;
+      ++taken;
+      uint8_t* const ks = stages + latest * K::kStage;
+      uint8_t* const vs = ks + K::kPart;
       const int key0 = (first_tile + (int)(here - item.item_begin)) * K::kTile;
+      const bool partial = there != (1u << copies) - 1 || key0 + K::kTile > s.length;
+      if (partial) {
+        // V of keys without a token becomes 0: a probability of 0 times
+        // whatever the bytes hold could be NaN.
+#pragma unroll 1
+        for (int r = lane; r < K::kTile; r += 32) {
+          if (key0 + r < s.length && there >> (r >> piece_bits) * 2 & 1) continue;
+#pragma unroll 1
+          for (int i = 0; i < D; i += 16)
+            *reinterpret_cast<uint4*>(vs + r * D + i) = make_uint4(0, 0, 0, 0);
+        }
+        cxs::fence_proxy_async_shared();
+        __syncwarp();
+      }
 
       float x[K::kTile / 8][4];
 #pragma unroll
@@ -392,7 +357,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(ks + 8 * n * D + k_at[j]);
+          const uint4 w = *reinterpret_cast<const uint4*>(ks + 8 * n * D + k_at + 64 * j);
           mma16816(x[n], q[4 * j + 0], half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1));
           mma16816(x[n], q[4 * j + 1], half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
           mma16816(x[n], q[4 * j + 2], half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1));
@@ -400,11 +365,11 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         }
       }
       // -infinity where a row does not see the key.
-      if (missing || key0 < all.x || key0 + K::kTile > all.y) {
+      if (partial || key0 < all.x || key0 + K::kTile > all.y) {
 #pragma unroll
         for (int n = 0; n < K::kTile / 8; ++n) {
           const int ka = key0 + 8 * n + t, kb = key0 + 8 * n + 4 + (t ^ 1);
-          const bool gone = missing >> (n / 2) & 1;
+          const bool gone = !(there >> (8 * n >> piece_bits) * 2 & 1);
           if (gone || ka < see0.x || ka >= see0.y) x[n][0] = -kInf;
           if (gone || kb < see0.x || kb >= see0.y) x[n][1] = -kInf;
           if (gone || ka < see1.x || ka >= see1.y) x[n][2] = -kInf;
@@ -415,15 +380,15 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
       // two), lift = log2 s_v, per = 1 / s_v.
       float f0[K::kGroups], f1[K::kGroups], lift[K::kGroups], per[K::kGroups];
       float t0 = -kInf, t1 = -kInf;
-      // (Lane u works them out for run u.)
-      const float2 scale = *reinterpret_cast<const float2*>(sc + 2 * (lane % K::kGroups));
-      const float my_f = usable_scale(scale.x) * unit;
-      const float my_lift = __log2f(usable_scale(scale.y)), my_per = ex2(-my_lift);
+      // (Each copy's lane works out its part of them.)
+      const float my_scale = usable_scale(scale), my_f = my_scale * unit;
+      const float my_lift = __log2f(my_scale), my_per = ex2(-my_lift);
 #pragma unroll
       for (int u = 0; u < K::kGroups; ++u) {
-        const float sk = __shfl_sync(0xffffffffu, my_f, u);
-        lift[u] = __shfl_sync(0xffffffffu, my_lift, u);
-        per[u] = __shfl_sync(0xffffffffu, my_per, u);
+        const int from = (16 * u >> piece_bits) * 2;
+        const float sk = __shfl_sync(0xffffffffu, my_f, from);
+        lift[u] = __shfl_sync(0xffffffffu, my_lift, from + 1);
+        per[u] = __shfl_sync(0xffffffffu, my_per, from + 1);
         // Never 0, which times a hidden score would be NaN; NaN stays NaN.
         f0[u] = sk * back0 < 1.2e-38f ? 1.2e-38f : sk * back0;
         f1[u] = sk * back1 < 1.2e-38f ? 1.2e-38f : sk * back1;
@@ -472,7 +437,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         uint32_t w[4][kWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* from = vs + (16 * u + 8 * (i / 2)) * D + v_at[i % 2];
+          const uint8_t* from = vs + (16 * u + 8 * (i / 2)) * D + (i % 2 ? v_at1 : v_at0);
           if (D == 64) {
             const uint2 v = *reinterpret_cast<const uint2*>(from);
             w[i][0] = v.x;
@@ -522,6 +487,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         for (int i = 0; i < D / 8; i += 4)
           *reinterpret_cast<float4*>(dst + (g + 4 * (e & 2)) * D + (D / 8) * (2 * t + (e & 1)) + i) =
               make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
+      cxs::fence_proxy_async_shared();  // before the copies that come here next
     }
     __syncthreads();
     const bool whole = item.tile == item.item_begin && item_hi == item.item_end;
@@ -573,7 +539,6 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     raw = load_queries();
     __syncthreads();  // the stages are free again
   }
-  __pipeline_wait_prior(0);
   clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
 }
 

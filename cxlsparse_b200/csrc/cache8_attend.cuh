@@ -23,6 +23,7 @@ namespace cache8 {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = INFINITY;
+constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -33,7 +33,6 @@ constexpr int kPanel = 128 * 128;       // bytes: 128 rows (queries or keys) of 
 constexpr int kRuns = kKeys / 16;       // runs of 16 keys: each within one page
 constexpr int kRing = 8;                // tiles whose Tile is kept: more than are ever in work
 constexpr int kTmem = 512;              // columns: S/P of two groups (128 each), O of two groups
-constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
 
 // Registers a thread by role: twice the softmax's, the conversion's and the
 // rest's, times 128, are the 64 K that 512 threads of 128 are launched with.
