@@ -27,7 +27,10 @@ __device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float shi
 
 // ------------------------------------------------- few rows: one warp, 16 ---
 
-// One CTA of 12 warps per SM. A warp takes a tile of keys at a time with all
+// One CTA of 12 warps per SM. Each warp works through its own share; the CTA's
+// warps meet once, at the end, to join what they hold of the same items (a
+// meeting at every item cost as much as the tiles of a ragged decode batch). A
+// warp takes a tile of keys at a time with all
 // 16 rows: the tile's runs of K and V codes come by bulk copies, one tile
 // ahead, and go from shared memory straight into mma.sync fragments: the
 // order of channels within a dot product is free, so a lane's 16 bytes of a
@@ -35,22 +38,21 @@ __device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float shi
 // chosen so that the scores' accumulator is the probabilities' operand and a
 // lane's V bytes of four keys pair up by byte permutes. No transposition
 // passes through shared memory.
+constexpr int kDecodeWarps = 12;
+
 template <int D>
 struct Decode {
-  static constexpr int kWarps = 12, kThreads = 32 * kWarps;
+  static constexpr int kWarps = kDecodeWarps, kThreads = 32 * kWarps;
   static constexpr int kTile = D == 64 ? 64 : 32;     // keys
   static constexpr int kPart = kTile * D;             // bytes of K or V
   static constexpr int kStages = 2;                   // one in work, one coming
-  static constexpr int kStage = 2 * kPart;            // also holds a warp's O (16 x D fp32)
+  static constexpr int kStage = 2 * kPart;
   static constexpr int kGroups = kTile / 16;          // runs of 16 keys: within one page
   static constexpr int kRows = 16;
-  static_assert(kStage >= kRows * D * 4, "a stage holds a warp's O");
-  // Shared memory: stages, their barriers, row statistics, queries, prefix.
+  // Shared memory: stages, their barriers, what the warps hold, prefix.
   static constexpr int kBars = kWarps * kStages * kStage;
-  static constexpr int kStats = kBars + kWarps * kStages * 8;     // [row][warp] M, l
-  static constexpr int kQuery = (kStats + kRows * kWarps * 2 * 4 + 15) / 16 * 16;  // fp16 rows
-  static constexpr int kBack = kQuery + kRows * D * 2;            // a row's inverse power of two
-  static constexpr int kPrefix = (kBack + kRows * 4 + 15) / 16 * 16;
+  static constexpr int kPieces = kBars + kWarps * kStages * 8;    // [warp][2]
+  static constexpr int kPrefix = kPieces + kWarps * 2 * 32;
   static constexpr int kBytes = kPrefix + (kSlice + 1) * 8;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
@@ -58,6 +60,15 @@ struct Decode {
 // Column n of an 8-key score tile is key n / 2, or 4 + (n / 2 ^ 1) for odd n:
 // the rows that neighbouring lanes read then lie in different banks (D = 64).
 __device__ __forceinline__ int key_of_column(int n) { return n & 1 ? 4 + ((n >> 1) ^ 1) : n >> 1; }
+
+// A warp's part of an item that began in an earlier share (piece 0) or goes on
+// into the next one (piece 1).
+struct Piece {
+  int state;  // 0: none, 1: the item ends here, 2: it goes on
+  int first, rows, row0, kv_head;
+  long long end;  // of the item's tiles
+};
+static_assert(sizeof(Piece) == 32, "piece");
 
 struct Cursor {  // a tile of the CTA's share: its item and place
   long long tile;          // position among all tiles
@@ -81,12 +92,53 @@ __device__ __forceinline__ void write_row(const cxs_cache_attend_call& a, const 
   if (a.lse && d == 0) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
 }
 
+// The join of partial results for four channels of a row.
+struct Join {
+  float m = -kInf, l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  // Parts k0, k0 + step, ... (four, below `parts`), all loads in flight at once.
+  template <int D, int ROWS, typename F>
+  __device__ __forceinline__ void add4(F part, int k0, int step, int parts, int r, int d) {
+    float2 stat[4];
+    float4 v[4];
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* from = part(min(k0 + j * step, parts - 1));
+      stat[j] = *reinterpret_cast<const float2*>(from + ROWS * D + 2 * r);
+      v[j] = *reinterpret_cast<const float4*>(from + r * D + d);
+      if (k0 + j * step >= parts) stat[j] = make_float2(-kInf, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, stat[j].x);
+    const float base = top == -kInf ? 0.f : top, old = ex2(m - base);
+    m = top;
+    l *= old;
+    sum.x *= old, sum.y *= old, sum.z *= old, sum.w *= old;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (k0 + j * step >= parts) break;
+      add(stat[j], v[j], base);
+    }
+  }
+  __device__ __forceinline__ void add(float2 stat, float4 v, float base) {
+    const float f = ex2(stat.x - base);
+    l = fmaf(stat.y, f, l);
+    sum.x = fmaf(v.x, f, sum.x);
+    sum.y = fmaf(v.y, f, sum.y);
+    sum.z = fmaf(v.z, f, sum.z);
+    sum.w = fmaf(v.w, f, sum.w);
+  }
+};
+
 template <int D>
 __device__ __forceinline__ int item_tiles(const Span& s) {
   constexpr int T = Decode<D>::kTile;
   if (s.count == 0) return 0;
   const int n = (s.length + T - 1) / T - s.begin / T;
-  return n > 0 ? n : 1;  // an item without keys still writes its rows
+  // An item without keys still writes its rows. One more: finding an item,
+  // loading its queries and writing its rows take about as long as a tile.
+  return (n > 0 ? n : 1) + 1;
 }
 
 template <int FORMAT, typename T, int D>
@@ -133,20 +185,25 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   }
   __syncthreads();
   const long long total = prefix[z.users];
-  const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
-  const int ctas = wanted < z.grid ? (int)wanted : z.grid;
-  Partial* partials = reinterpret_cast<Partial*>(a.workspace);
+  // Neighbouring shares lie in one CTA (of at least 6, for the join at its end).
+  const Shares shares(total, z);
+  const int per = min(max((shares.count + z.grid - 1) / z.grid, 6), K::kWarps);
+  const int worker = (int)blockIdx.x * per + warp;
+  const bool busy = warp < per && worker < shares.count;
+  Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
   Partial& mine = partials[blockIdx.x];
+  constexpr int kSize = K::kRows * (D + 2);
+  // Partial results of the CTAs, then of the warps, two each.
+  float* const cta_parts = reinterpret_cast<float*>(partials + z.grid) + (long long)blockIdx.x * 2 * kSize;
+  float* const warp_parts = reinterpret_cast<float*>(partials + z.grid) +
+                            ((long long)z.grid + (long long)blockIdx.x * K::kWarps) * 2 * kSize;
+  Piece* const pieces = reinterpret_cast<Piece*>(smem + K::kPieces);  // [warp][2]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) mine.parts = 0;
-  if ((int)blockIdx.x >= ctas) {
-    clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
-    return;
-  }
-  const Shares shares(total, ctas);
-  const long long lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
-  float* scratch = reinterpret_cast<float*>(partials + z.grid) +
-                   (long long)blockIdx.x * 2 * K::kRows * (D + 2);
+  if (lane < 2) pieces[2 * warp + lane].state = 0;
+  __syncwarp();
+  const long long lo = busy ? shares.begin(worker) : 0, hi = busy ? shares.begin(worker + 1) : 0;
+  float* const scratch = warp_parts + (long long)warp * 2 * kSize;
 
   // The item of a tile, found from the last one.
   auto seek = [&](Cursor& p) {
@@ -189,7 +246,8 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   auto look_up = [&](Cursor& p) -> int {
     if (p.tile >= hi) return -2;
     seek(p);
-    const int at = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile +
+    if (p.tile == p.item_begin && ++p.tile >= hi) return -2;  // (an item's first is no tile)
+    const int at = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin) - 1) * K::kTile +
                    (lane / 2 << piece_bits);
     if (lane >= copies || at >= p.span.length || at + (1 << piece_bits) <= p.span.begin) return -2;
     return __ldg(c.table + p.user * c.table_stride + (at >> page_bits));
@@ -198,7 +256,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   // copy's page and part) and which copies there are.
   auto fetch = [&](const Cursor& p, int stage, int id, unsigned* there) -> float {
     if (p.tile >= hi) return 1.f;
-    const int key0 = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin)) * K::kTile;
+    const int key0 = (p.span.begin / K::kTile + (int)(p.tile - p.item_begin) - 1) * K::kTile;
     const bool mine = id >= 0 && id < c.pages;
     if (!mine && id != -2) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
     *there = __ballot_sync(0xffffffffu, mine);
@@ -212,384 +270,356 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
     return __ldg(c.scales + cell);
   };
 
-  // The first item is found, and its queries asked for, before the copies:
-  // loads issued after them wait until they have arrived.
-  Cursor item{lo, -1, -1, 0, 0, 0, {}};
-  seek(item);
-  // A thread's 8 channels of one of the item's rows.
-  constexpr int kLanes = D / 8;  // of a row
-  auto load_queries = [&]() {
-    const int row = item.row0 + threadIdx.x / kLanes;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x >= K::kRows * kLanes || row >= item.span.count * z.group) return x;
-    const T* from = (const T*)a.query + 8 * (threadIdx.x % kLanes) +
-                    (long long)(item.span.first + row / z.group) * a.q_token_stride +
-                    (long long)(item.kv_head * z.group + row % z.group) * a.q_head_stride;
-    if (((uintptr_t)from & 15) == 0) return *reinterpret_cast<const uint4*>(from);
-    alignas(16) T in[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) in[e] = from[e];
-    return *reinterpret_cast<const uint4*>(in);
-  };
-  uint4 raw = load_queries();
-  Cursor ahead = item;
-  ahead.tile = lo + warp;
-  long long here = lo + warp;  // the next tile this warp takes
-  int taken = 0;                // tiles taken so far: stage taken % 2
-  unsigned next_there = 0;      // of the tile that is coming
-  int ahead_id = look_up(ahead);
-  float next_scale = fetch(ahead, 0, ahead_id, &next_there);
-  ahead.tile += K::kWarps;
-  ahead_id = look_up(ahead);
-  // Where this lane reads: its 16 channels of a key, its D / 8 of V.
-  const int k_at = key_of_column(g) * D + 16 * t;
-  const int v_at0 = t * D + D / 8 * g, v_at1 = (4 + (t ^ 1)) * D + D / 8 * g;
-  bool lost = false;  // a copy did not come
+  if (busy) {
+    Cursor item{lo, -1, -1, 0, 0, 0, {}};
+    seek(item);
+    Cursor ahead = item;
+    long long here = lo;          // the next tile
+    int taken = 0;                // tiles taken so far: stage taken % 2
+    unsigned next_there = 0;      // of the tile that is coming
+    int ahead_id = look_up(ahead);
+    float next_scale = fetch(ahead, 0, ahead_id, &next_there);
+    ++ahead.tile;
+    ahead_id = look_up(ahead);
+    // Where this lane reads: its 16 channels of a key, its D / 8 of V.
+    const int k_at = key_of_column(g) * D + 16 * t;
+    const int v_at0 = t * D + D / 8 * g, v_at1 = (4 + (t ^ 1)) * D + D / 8 * g;
+    bool lost = false;  // a copy did not come
 
-  float o[D / 8][4], m0, m1, l0, l1;  // rows g and g + 8
-  while (true) {
-    const long long item_hi = item.item_end < hi ? item.item_end : hi;
-    const Span& s = item.span;
-    const int rows = s.count * z.group;
-    const int first_tile = s.begin / K::kTile;
-    // The rows' queries, scaled by a power of two per row (and the scale's
-    // sign), as fp16 in shared memory: 8 channels a thread. (The last item's
-    // join ended with a barrier: nobody reads the last ones any more.)
-    __half* const queries = reinterpret_cast<__half*>(smem + K::kQuery);
-    float* const backs = reinterpret_cast<float*>(smem + K::kBack);
-    if (threadIdx.x < K::kRows * kLanes) {
-      const int r = threadIdx.x / kLanes, i = threadIdx.x % kLanes;
-      alignas(16) T in[8];
-      *reinterpret_cast<uint4*>(in) = raw;
-      float v[8];
+    float o[D / 8][4], m0, m1, l0, l1;  // rows g and g + 8
+    while (true) {
+      const long long item_hi = item.item_end < hi ? item.item_end : hi;
+      const Span& s = item.span;
+      const int rows = s.count * z.group;
+      const int first_tile = s.begin / K::kTile;
+      // This lane's rows g and g + 8: what they see, and their queries as
+      // operands (its 16 channels of each 64 are four steps' operand elements),
+      // scaled by a power of two (and the scale's sign).
+      uint32_t q[D / 16][4];
+      float back0, back1;
+      int2 see0 = make_int2(0, 0), see1 = make_int2(0, 0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = to_float(in[e]);
-      float top = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (fabsf(v[e]) < kInf) top = fmaxf(top, fabsf(v[e]));
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-      if (e < -100) e = -100;
-      if (top == 0.f) e = 14;
-      float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-      if (a.scale < 0.f) up = -up;
-      if (a.scale == 0.f) up = 0.f;  // every score is 0
-      if (i == 0) backs[r] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-      *reinterpret_cast<uint4*>(queries + r * D + 8 * i) =
-          make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
-                     pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
-    }
-    __syncthreads();
-    // This lane's rows g and g + 8: what they see, and their operands (its 16
-    // channels of each 64 are four steps' operand elements).
-    int2 see0 = make_int2(0, 0), see1 = make_int2(0, 0);
-    if (item.row0 + g < rows) see0 = row_range(a, s, (item.row0 + g) / z.group);
-    if (item.row0 + g + 8 < rows) see1 = row_range(a, s, (item.row0 + g + 8) / z.group);
-    const float back0 = backs[g], back1 = backs[g + 8];
-    uint32_t q[D / 16][4];
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 x = *reinterpret_cast<const uint4*>(queries + g * D + 64 * j + 16 * t + 8 * h);
-        const uint4 y =
-            *reinterpret_cast<const uint4*>(queries + (g + 8) * D + 64 * j + 16 * t + 8 * h);
-        q[4 * j + 2 * h][0] = x.x, q[4 * j + 2 * h][2] = x.y;
-        q[4 * j + 2 * h + 1][0] = x.z, q[4 * j + 2 * h + 1][2] = x.w;
-        q[4 * j + 2 * h][1] = y.x, q[4 * j + 2 * h][3] = y.y;
-        q[4 * j + 2 * h + 1][1] = y.z, q[4 * j + 2 * h + 1][3] = y.w;
-      }
-    const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    m0 = m1 = -kInf;
-    l0 = l1 = 0.f;
-    // All rows of the tile see the keys [all.x, all.y).
-    int2 all = make_int2(max(see0.x, see1.x), min(see0.y, see1.y));
-    if (item.row0 + g >= rows) all = make_int2(0, s.length);
-    else if (item.row0 + g + 8 >= rows) all = see0;
-    all.x = __reduce_max_sync(0xffffffffu, all.x);
-    all.y = __reduce_min_sync(0xffffffffu, all.y);
-
-    int latest = -1;  // the stage this warp took last (free until the next fetch)
-#pragma unroll 1
-    for (; here < item_hi; here += K::kWarps) {
-      // The stage taken in the previous round is free: the next tile's copies.
-      __syncwarp();
-      const float scale = next_scale;
-      const unsigned there = next_there;
-      next_scale = fetch(ahead, (taken + 1) % 2, ahead_id, &next_there);
-      ahead.tile += K::kWarps;
-      ahead_id = look_up(ahead);
-      if (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1)) {
-        const long long since = clock64();
-        while (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1) && !lost)
-          lost = clock64() - since > kSpinLimit;
-        if (lost) report(c.error, CXS_DEVICE_ERR_COPY_TIMEOUT);
-      }
-      latest = taken % 2;
-      ++taken;
-      uint8_t* const ks = stages + latest * K::kStage;
-      uint8_t* const vs = ks + K::kPart;
-      const int key0 = (first_tile + (int)(here - item.item_begin)) * K::kTile;
-      const bool partial = there != (1u << copies) - 1 || key0 + K::kTile > s.length;
-      if (partial) {
-        // V of keys without a token becomes 0: a probability of 0 times
-        // whatever the bytes hold could be NaN.
-#pragma unroll 1
-        for (int r = lane; r < K::kTile; r += 32) {
-          if (key0 + r < s.length && there >> (r >> piece_bits) * 2 & 1) continue;
-#pragma unroll 1
-          for (int i = 0; i < D; i += 16)
-            *reinterpret_cast<uint4*>(vs + r * D + i) = make_uint4(0, 0, 0, 0);
+      for (int half = 0; half < 2; ++half) {
+        const int row = item.row0 + g + 8 * half;
+        const bool live = row < rows;
+        const T* from = (const T*)a.query;
+        if (live) {
+          const int token = row / z.group;
+          from += (long long)(s.first + token) * a.q_token_stride +
+                  (long long)(item.kv_head * z.group + row - token * z.group) * a.q_head_stride;
+          const int2 see = row_range(a, s, token);
+          if (half) see1 = see; else see0 = see;
         }
-        cxs::fence_proxy_async_shared();
-        __syncwarp();
-      }
-
-      float x[K::kTile / 8][4];
+        alignas(16) T in[D / 4];
+        const bool wide = ((uintptr_t)from & 15) == 0;
 #pragma unroll
-      for (int n = 0; n < K::kTile / 8; ++n) {
-        x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(ks + 8 * n * D + k_at + 64 * j);
-          mma16816(x[n], q[4 * j + 0], half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1));
-          mma16816(x[n], q[4 * j + 1], half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
-          mma16816(x[n], q[4 * j + 2], half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1));
-          mma16816(x[n], q[4 * j + 3], half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
-        }
-      }
-      // -infinity where a row does not see the key.
-      if (partial || key0 < all.x || key0 + K::kTile > all.y) {
-#pragma unroll
-        for (int n = 0; n < K::kTile / 8; ++n) {
-          const int ka = key0 + 8 * n + t, kb = key0 + 8 * n + 4 + (t ^ 1);
-          const bool gone = !(there >> (8 * n >> piece_bits) * 2 & 1);
-          if (gone || ka < see0.x || ka >= see0.y) x[n][0] = -kInf;
-          if (gone || kb < see0.x || kb >= see0.y) x[n][1] = -kInf;
-          if (gone || ka < see1.x || ka >= see1.y) x[n][2] = -kInf;
-          if (gone || kb < see1.x || kb >= see1.y) x[n][3] = -kInf;
-        }
-      }
-      // A score is x f + lift: f = scale log2(e) s_k (and the row's power of
-      // two), lift = log2 s_v, per = 1 / s_v.
-      float f0[K::kGroups], f1[K::kGroups], lift[K::kGroups], per[K::kGroups];
-      float t0 = -kInf, t1 = -kInf;
-      // (Each copy's lane works out its part of them.)
-      const float my_scale = usable_scale(scale), my_f = my_scale * unit;
-      const float my_lift = __log2f(my_scale), my_per = ex2(-my_lift);
-#pragma unroll
-      for (int u = 0; u < K::kGroups; ++u) {
-        const int from = (16 * u >> piece_bits) * 2;
-        const float sk = __shfl_sync(0xffffffffu, my_f, from);
-        lift[u] = __shfl_sync(0xffffffffu, my_lift, from + 1);
-        per[u] = __shfl_sync(0xffffffffu, my_per, from + 1);
-        // Never 0, which times a hidden score would be NaN; NaN stays NaN.
-        f0[u] = sk * back0 < 1.2e-38f ? 1.2e-38f : sk * back0;
-        f1[u] = sk * back1 < 1.2e-38f ? 1.2e-38f : sk * back1;
-        const float(&ya)[4] = x[2 * u];
-        const float(&yb)[4] = x[2 * u + 1];
-        t0 = fmaxf(t0, fmaf(fmaxf(fmaxf(ya[0], ya[1]), fmaxf(yb[0], yb[1])), f0[u], lift[u]));
-        t1 = fmaxf(t1, fmaf(fmaxf(fmaxf(ya[2], ya[3]), fmaxf(yb[2], yb[3])), f1[u], lift[u]));
-      }
-      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
-      t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
-      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
-      t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-      // M moves when a score passes it by 2^8: p stays below 2^8, well inside
-      // fp16's range, and most tiles leave O as it is.
-      const bool g0 = t0 > m0 + 8.f, g1 = t1 > m1 + 8.f;
-      if (__any_sync(0xffffffffu, g0 || g1)) {
-        const float c0 = !g0 ? 1.f : m0 == -kInf ? 0.f : ex2(m0 - t0);
-        const float c1 = !g1 ? 1.f : m1 == -kInf ? 0.f : ex2(m1 - t1);
-        if (g0) m0 = t0;
-        if (g1) m1 = t1;
-        l0 *= c0;
-        l1 *= c1;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= c0;
-          o[i][1] *= c0;
-          o[i][2] *= c1;
-          o[i][3] *= c1;
-        }
-      }
-      const float b0 = m0 == -kInf ? 0.f : m0, b1 = m1 == -kInf ? 0.f : m1;
-#pragma unroll
-      for (int u = 0; u < K::kGroups; ++u) {
-        float(&ya)[4] = x[2 * u];
-        float(&yb)[4] = x[2 * u + 1];
-        const float s0 = lift[u] - b0, s1 = lift[u] - b1;
-        const float2 pa0 = exp2_pair(ya[0], ya[1], f0[u], s0), pb0 = exp2_pair(yb[0], yb[1], f0[u], s0);
-        const float2 pa1 = exp2_pair(ya[2], ya[3], f1[u], s1), pb1 = exp2_pair(yb[2], yb[3], f1[u], s1);
-        const float2 sum0 = __fadd2_rn(pa0, pb0), sum1 = __fadd2_rn(pa1, pb1);
-        l0 = fmaf(sum0.x + sum0.y, per[u], l0);
-        l1 = fmaf(sum1.x + sum1.y, per[u], l1);
-        const uint32_t p[4] = {pack_half2(pa0.x, pa0.y), pack_half2(pa1.x, pa1.y),
-                               pack_half2(pb0.x, pb0.y), pack_half2(pb1.x, pb1.y)};
-        // Keys of this lane's four operand rows; D / 8 of their channels each.
-        constexpr int kWords = D / 32;
-        uint32_t w[4][kWords];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* from = vs + (16 * u + 8 * (i / 2)) * D + (i % 2 ? v_at1 : v_at0);
-          if (D == 64) {
-            const uint2 v = *reinterpret_cast<const uint2*>(from);
-            w[i][0] = v.x;
-            w[i][1] = v.y;
+        for (int j = 0; j < D / 32; ++j) {  // 8 of the lane's channels
+          const T* const part = from + 64 * (j / 2) + 16 * t + 8 * (j % 2);
+          if (wide) {
+            *reinterpret_cast<uint4*>(in + 8 * j) = *reinterpret_cast<const uint4*>(part);
           } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(from);
-            w[i][0] = v.x;
-            w[i][1] = v.y;
-            w[i][kWords - 2] = v.z;
-            w[i][kWords - 1] = v.w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) in[8 * j + e] = part[e];
           }
         }
+        float top = 0.f;
 #pragma unroll
-        for (int n = 0; n < kWords; ++n) {
-          const uint32_t a01 = __byte_perm(w[0][n], w[1][n], 0x5140);
-          const uint32_t a23 = __byte_perm(w[0][n], w[1][n], 0x7362);
-          const uint32_t b01 = __byte_perm(w[2][n], w[3][n], 0x5140);
-          const uint32_t b23 = __byte_perm(w[2][n], w[3][n], 0x7362);
-          mma16816(o[4 * n + 0], p, half2_of<FORMAT>(a01, 0), half2_of<FORMAT>(b01, 0));
-          mma16816(o[4 * n + 1], p, half2_of<FORMAT>(a01, 1), half2_of<FORMAT>(b01, 1));
-          mma16816(o[4 * n + 2], p, half2_of<FORMAT>(a23, 0), half2_of<FORMAT>(b23, 0));
-          mma16816(o[4 * n + 3], p, half2_of<FORMAT>(a23, 1), half2_of<FORMAT>(b23, 1));
+        for (int e = 0; e < D / 4; ++e) {
+          const float x = fabsf(to_float(in[e]));
+          if (x < kInf) top = fmaxf(top, x);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+        if (e < -100) e = -100;
+        if (top == 0.f) e = 14;
+        float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        if (a.scale < 0.f) up = -up;
+        if (a.scale == 0.f) up = 0.f;  // every score is 0
+        const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+        if (half) back1 = down; else back0 = down;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float lo_half = live ? to_float(in[2 * i]) * up : 0.f;
+          const float hi_half = live ? to_float(in[2 * i + 1]) * up : 0.f;
+          q[i / 2][half + 2 * (i % 2)] = pack_half2(lo_half, hi_half);
         }
       }
-    }
+      const float unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+      m0 = m1 = -kInf;
+      l0 = l1 = 0.f;
+      // All rows of the tile see the keys [all.x, all.y).
+      int2 all = make_int2(max(see0.x, see1.x), min(see0.y, see1.y));
+      if (item.row0 + g >= rows) all = make_int2(0, s.length);
+      else if (item.row0 + g + 8 >= rows) all = see0;
+      all.x = __reduce_max_sync(0xffffffffu, all.x);
+      all.y = __reduce_min_sync(0xffffffffu, all.y);
 
-    // Join the warps. Each writes O into the stage it consumed last (nothing
-    // is in flight there), rows of D fp32, and its rows' M and l.
-    float2* const stats = reinterpret_cast<float2*>(smem + K::kStats);  // [row][warp]
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    int* const where = reinterpret_cast<int*>(warp_sum);  // place of each warp's O, -1: none
-    __syncwarp();
-    if (lane == 0) where[warp] = latest < 0 ? -1 : (warp * K::kStages + latest) * K::kStage;
-    if (t == 0) {
-      stats[g * K::kWarps + warp] = make_float2(m0, l0);
-      stats[(g + 8) * K::kWarps + warp] = make_float2(m1, l1);
-    }
-    if (latest >= 0) {
-      float* dst = reinterpret_cast<float*>(stages + latest * K::kStage);
+      if (here == item.item_begin) ++here;
+#pragma unroll 1
+      for (; here < item_hi; ++here) {
+        // The stage taken in the previous round is free: the next tile's copies.
+        __syncwarp();
+        const float scale = next_scale;
+        const unsigned there = next_there;
+        next_scale = fetch(ahead, (taken + 1) % 2, ahead_id, &next_there);
+        ++ahead.tile;
+        ahead_id = look_up(ahead);
+        if (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1)) {
+          const long long since = clock64();
+          while (!cxs::mbar_try_wait(bars + taken % 2, taken / 2 & 1) && !lost)
+            lost = clock64() - since > kSpinLimit;
+          if (lost) report(c.error, CXS_DEVICE_ERR_COPY_TIMEOUT);
+        }
+        uint8_t* const ks = stages + taken % 2 * K::kStage;
+        ++taken;
+        uint8_t* const vs = ks + K::kPart;
+        const int key0 = (first_tile + (int)(here - item.item_begin) - 1) * K::kTile;
+        const bool partial = there != (1u << copies) - 1 || key0 + K::kTile > s.length;
+        if (partial) {
+          // V of keys without a token becomes 0: a probability of 0 times
+          // whatever the bytes hold could be NaN.
+#pragma unroll 1
+          for (int r = lane; r < K::kTile; r += 32) {
+            if (key0 + r < s.length && there >> (r >> piece_bits) * 2 & 1) continue;
+#pragma unroll 1
+            for (int i = 0; i < D; i += 16)
+              *reinterpret_cast<uint4*>(vs + r * D + i) = make_uint4(0, 0, 0, 0);
+          }
+          cxs::fence_proxy_async_shared();
+          __syncwarp();
+        }
+
+        float x[K::kTile / 8][4];
+#pragma unroll
+        for (int n = 0; n < K::kTile / 8; ++n) {
+          x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) {
+            const uint4 w = *reinterpret_cast<const uint4*>(ks + 8 * n * D + k_at + 64 * j);
+            mma16816(x[n], q[4 * j + 0], half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1));
+            mma16816(x[n], q[4 * j + 1], half2_of<FORMAT>(w.y, 0), half2_of<FORMAT>(w.y, 1));
+            mma16816(x[n], q[4 * j + 2], half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1));
+            mma16816(x[n], q[4 * j + 3], half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
+          }
+        }
+        // -infinity where a row does not see the key.
+        if (partial || key0 < all.x || key0 + K::kTile > all.y) {
+#pragma unroll
+          for (int n = 0; n < K::kTile / 8; ++n) {
+            const int ka = key0 + 8 * n + t, kb = key0 + 8 * n + 4 + (t ^ 1);
+            const bool gone = !(there >> (8 * n >> piece_bits) * 2 & 1);
+            if (gone || ka < see0.x || ka >= see0.y) x[n][0] = -kInf;
+            if (gone || kb < see0.x || kb >= see0.y) x[n][1] = -kInf;
+            if (gone || ka < see1.x || ka >= see1.y) x[n][2] = -kInf;
+            if (gone || kb < see1.x || kb >= see1.y) x[n][3] = -kInf;
+          }
+        }
+        // A score is x f + lift: f = scale log2(e) s_k (and the row's power of
+        // two), lift = log2 s_v, per = 1 / s_v.
+        float f0[K::kGroups], f1[K::kGroups], lift[K::kGroups], per[K::kGroups];
+        float t0 = -kInf, t1 = -kInf;
+        // (Each copy's lane works out its part of them.)
+        const float my_scale = usable_scale(scale), my_f = my_scale * unit;
+        const float my_lift = __log2f(my_scale), my_per = ex2(-my_lift);
+#pragma unroll
+        for (int u = 0; u < K::kGroups; ++u) {
+          const int from = (16 * u >> piece_bits) * 2;
+          const float sk = __shfl_sync(0xffffffffu, my_f, from);
+          lift[u] = __shfl_sync(0xffffffffu, my_lift, from + 1);
+          per[u] = __shfl_sync(0xffffffffu, my_per, from + 1);
+          // Never 0, which times a hidden score would be NaN; NaN stays NaN.
+          f0[u] = sk * back0 < 1.2e-38f ? 1.2e-38f : sk * back0;
+          f1[u] = sk * back1 < 1.2e-38f ? 1.2e-38f : sk * back1;
+          const float(&ya)[4] = x[2 * u];
+          const float(&yb)[4] = x[2 * u + 1];
+          t0 = fmaxf(t0, fmaf(fmaxf(fmaxf(ya[0], ya[1]), fmaxf(yb[0], yb[1])), f0[u], lift[u]));
+          t1 = fmaxf(t1, fmaf(fmaxf(fmaxf(ya[2], ya[3]), fmaxf(yb[2], yb[3])), f1[u], lift[u]));
+        }
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
+        // M moves when a score passes it by 2^8: p stays below 2^8, well inside
+        // fp16's range, and most tiles leave O as it is.
+        const bool g0 = t0 > m0 + 8.f, g1 = t1 > m1 + 8.f;
+        if (__any_sync(0xffffffffu, g0 || g1)) {
+          const float c0 = !g0 ? 1.f : m0 == -kInf ? 0.f : ex2(m0 - t0);
+          const float c1 = !g1 ? 1.f : m1 == -kInf ? 0.f : ex2(m1 - t1);
+          if (g0) m0 = t0;
+          if (g1) m1 = t1;
+          l0 *= c0;
+          l1 *= c1;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][0] *= c0;
+            o[i][1] *= c0;
+            o[i][2] *= c1;
+            o[i][3] *= c1;
+          }
+        }
+        const float b0 = m0 == -kInf ? 0.f : m0, b1 = m1 == -kInf ? 0.f : m1;
+#pragma unroll
+        for (int u = 0; u < K::kGroups; ++u) {
+          float(&ya)[4] = x[2 * u];
+          float(&yb)[4] = x[2 * u + 1];
+          const float s0 = lift[u] - b0, s1 = lift[u] - b1;
+          const float2 pa0 = exp2_pair(ya[0], ya[1], f0[u], s0), pb0 = exp2_pair(yb[0], yb[1], f0[u], s0);
+          const float2 pa1 = exp2_pair(ya[2], ya[3], f1[u], s1), pb1 = exp2_pair(yb[2], yb[3], f1[u], s1);
+          const float2 sum0 = __fadd2_rn(pa0, pb0), sum1 = __fadd2_rn(pa1, pb1);
+          l0 = fmaf(sum0.x + sum0.y, per[u], l0);
+          l1 = fmaf(sum1.x + sum1.y, per[u], l1);
+          const uint32_t p[4] = {pack_half2(pa0.x, pa0.y), pack_half2(pa1.x, pa1.y),
+                                 pack_half2(pb0.x, pb0.y), pack_half2(pb1.x, pb1.y)};
+          // Keys of this lane's four operand rows; D / 8 of their channels each.
+          constexpr int kWords = D / 32;
+          uint32_t w[4][kWords];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* from = vs + (16 * u + 8 * (i / 2)) * D + (i % 2 ? v_at1 : v_at0);
+            if (D == 64) {
+              const uint2 v = *reinterpret_cast<const uint2*>(from);
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(from);
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+              w[i][kWords - 2] = v.z;
+              w[i][kWords - 1] = v.w;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < kWords; ++n) {
+            const uint32_t a01 = __byte_perm(w[0][n], w[1][n], 0x5140);
+            const uint32_t a23 = __byte_perm(w[0][n], w[1][n], 0x7362);
+            const uint32_t b01 = __byte_perm(w[2][n], w[3][n], 0x5140);
+            const uint32_t b23 = __byte_perm(w[2][n], w[3][n], 0x7362);
+            mma16816(o[4 * n + 0], p, half2_of<FORMAT>(a01, 0), half2_of<FORMAT>(b01, 0));
+            mma16816(o[4 * n + 1], p, half2_of<FORMAT>(a01, 1), half2_of<FORMAT>(b01, 1));
+            mma16816(o[4 * n + 2], p, half2_of<FORMAT>(a23, 0), half2_of<FORMAT>(b23, 0));
+            mma16816(o[4 * n + 3], p, half2_of<FORMAT>(a23, 1), half2_of<FORMAT>(b23, 1));
+          }
+        }
+      }
+
+      // The item's result, or this share's part of it: slot 0 for an item that
+      // began in an earlier share, slot 1 for one that goes on into the next.
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      const bool begins = item.tile == item.item_begin, whole = begins && item_hi == item.item_end;
+      float* const part = scratch + (begins ? K::kRows * (D + 2) : 0);
       // Accumulator i, columns 2t, 2t + 1: channels (D / 8) column + i.
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        const int r = g + 4 * (e & 2), row = item.row0 + r;
+        if (row >= rows) continue;
+        const float m = e < 2 ? m0 : m1, l = e < 2 ? l0 : l1;
+        const int d = D / 8 * (2 * t + (e & 1));
 #pragma unroll
-        for (int i = 0; i < D / 8; i += 4)
-          *reinterpret_cast<float4*>(dst + (g + 4 * (e & 2)) * D + (D / 8) * (2 * t + (e & 1)) + i) =
-              make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
-      cxs::fence_proxy_async_shared();  // before the copies that come here next
-    }
-    __syncthreads();
-    const bool whole = item.tile == item.item_begin && item_hi == item.item_end;
-    // An item that began in an earlier share leaves its partial in slot 0,
-    // one that begins here and goes on in slot 1.
-    float* const part = scratch + (item.tile == item.item_begin ? K::kRows * (D + 2) : 0);
-    // A thread for each four channels of a row.
-    for (int i = threadIdx.x; i < K::kRows * D / 4; i += K::kThreads) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      const int row = item.row0 + r;
-      if (row >= rows) continue;
-      const float2* const its = stats + r * K::kWarps;
-      float m = -kInf, l = 0.f;
-#pragma unroll 4
-      for (int w = 0; w < K::kWarps; ++w) m = fmaxf(m, its[w].x);
-      const float base = m == -kInf ? 0.f : m;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int w = 0; w < K::kWarps; ++w) {
-        if (where[w] < 0) continue;
-        const float f = ex2(its[w].x - base);
-        l = fmaf(its[w].y, f, l);
-        const float4 v = *reinterpret_cast<const float4*>(smem + where[w] + (r * D + d) * 4);
-        sum.x = fmaf(v.x, f, sum.x);
-        sum.y = fmaf(v.y, f, sum.y);
-        sum.z = fmaf(v.z, f, sum.z);
-        sum.w = fmaf(v.w, f, sum.w);
-      }
-      if (whole) {
-        write_row<T>(a, z, s.first, item.kv_head, row, D, d, sum, m, l);
-      } else {
-        *reinterpret_cast<float4*>(part + r * D + d) = sum;
-        if (d == 0)
+        for (int i = 0; i < D / 8; i += 4) {
+          const float4 sum = make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
+          if (whole)
+            write_row<T>(a, z, s.first, item.kv_head, row, D, d + i, sum, m, l);
+          else
+            *reinterpret_cast<float4*>(part + r * D + d + i) = sum;
+        }
+        if (!whole && d == 0)
           *reinterpret_cast<float2*>(part + K::kRows * D + 2 * r) = make_float2(m, l);
       }
+      if (!whole && lane == 0)
+        pieces[2 * warp + begins] =
+            Piece{item_hi == item.item_end ? 1 : 2, s.first, rows, item.row0, item.kv_head, item.item_end};
+      item.tile = item_hi;
+      if (item_hi >= hi) break;
+      seek(item);
     }
-    if (!whole && item.tile == item.item_begin && threadIdx.x == 0) {
-      // The last share that holds a tile of the item.
-      const int last = shares.of(item.item_end - 1);
-      mine.first = s.first;
-      mine.rows = rows;
-      mine.row0 = item.row0;
-      mine.kv_head = item.kv_head;
-      mine.parts = last - (int)blockIdx.x + 1;
-    }
-    item.tile = item_hi;
-    if (item_hi >= hi) break;
-    seek(item);
-    raw = load_queries();
-    __syncthreads();  // the stages are free again
   }
-  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
+  __syncthreads();
+
+  // Each item that the CTA holds in parts, in the order of the shares: one that
+  // comes in with the first warp, then those that begin in a warp and go on.
+  for (int start = -1; start < per; ++start) {
+    const bool before = start < 0;  // it began in an earlier CTA
+    const int first = before ? 0 : start;
+    const Piece piece = pieces[2 * first + !before];
+    if (!piece.state) continue;
+    bool on = piece.state == 2;
+    int last = first;
+    while (on && last + 1 < per) on = pieces[2 * ++last].state == 2;
+    const int parts = last - first + 1;
+    float* const to = cta_parts + (before ? 0 : kSize);
+    for (int i = threadIdx.x; i < K::kRows * D / 4; i += K::kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4, row = piece.row0 + r;
+      if (row >= piece.rows) continue;
+      Join join;
+      for (int k0 = 0; k0 < parts; k0 += 4)
+        join.add4<D, K::kRows>([&](int k) {
+          return warp_parts + (2 * (first + k) + (k == 0 && !before)) * kSize;
+        }, k0, 1, parts, r, d);
+      if (!before && !on) {
+        write_row<T>(a, z, piece.first, piece.kv_head, row, D, d, join.sum, join.m, join.l);
+      } else {
+        *reinterpret_cast<float4*>(to + r * D + d) = join.sum;
+        if (d == 0)
+          *reinterpret_cast<float2*>(to + K::kRows * D + 2 * r) = make_float2(join.m, join.l);
+      }
+    }
+    if (!before && on && threadIdx.x == 0) {
+      mine.first = piece.first;
+      mine.rows = piece.rows;
+      mine.row0 = piece.row0;
+      mine.kv_head = piece.kv_head;
+      mine.parts = shares.of(piece.end - 1) / per - (int)blockIdx.x + 1;
+    }
+  }
+  clear_rows<T, D>(a, z, blockIdx.x, z.grid, threadIdx.x, K::kThreads);
 }
 
-// Joins the partial results of the item (of ROWS rows) that starts in share
-// blockIdx.x and goes on into later ones: 16 rows a CTA, one thread per four
-// channels of a row, in the order of the shares.
-template <typename T, int D, int ROWS>
-__global__ void combine_kernel(const cxs_cache_attend_call a, const Shape z) {
-  constexpr int kRows = ROWS, kSize = kRows * (D + 2);
+// Joins the partial results of the item (of ROWS rows) that starts in CTA
+// blockIdx.x and goes on into later ones: 16 rows, a thread for four channels
+// of a row and every GROUPS-th CTA's part. Latency-bound: in each of the groups
+// four parts' loads are in flight at a time.
+template <typename T, int D, int ROWS, int GROUPS>
+__global__ void __launch_bounds__(GROUPS * 4 * D)
+    combine_kernel(const cxs_cache_attend_call a, const Shape z) {
+  constexpr int kSize = ROWS * (D + 2), kLanes = 4 * D;  // threads of a group
+  __shared__ float4 sums[GROUPS > 1 ? GROUPS * kLanes : 1];
+  __shared__ float2 stats[GROUPS > 1 ? GROUPS * 16 : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Partial* partials = reinterpret_cast<const Partial*>(a.workspace);
-  const Partial item = partials[blockIdx.x];
-  if (item.parts == 0) return;
-  const float* scratch =
+  const float* const own =
       reinterpret_cast<const float*>(partials + z.grid) + (long long)blockIdx.x * 2 * kSize;
-  const int r = 16 * blockIdx.y + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const Partial item = partials[blockIdx.x];
+  if (item.parts == 0 || item.row0 + 16 * (int)blockIdx.y >= item.rows) return;
+  const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int in_block = lane / (D / 4), r = 16 * blockIdx.y + in_block, d = lane % (D / 4) * 4;
   const int row = item.row0 + r;
-  if (row >= item.rows) return;
-  auto part = [&](int i) { return scratch + (i == 0 ? kSize : 2 * i * kSize); };
-  // Four shares at a time, all their loads in flight.
-  float m = -kInf, l = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < item.parts; i0 += 4) {
-    float2 stat[4];
-    float4 v[4];
-    float top = m;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float* from = part(min(i0 + j, item.parts - 1));
-      stat[j] = *reinterpret_cast<const float2*>(from + kRows * D + 2 * r);
-      v[j] = *reinterpret_cast<const float4*>(from + r * D + d);
-      if (i0 + j >= item.parts) stat[j] = make_float2(-kInf, 0.f);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = fmaxf(top, stat[j].x);
-    const float base = top == -kInf ? 0.f : top, old = ex2(m - base);
-    m = top;
-    l *= old;
-    sum.x *= old, sum.y *= old, sum.z *= old, sum.w *= old;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i0 + j >= item.parts) break;
-      const float f = ex2(stat[j].x - base);
-      l = fmaf(stat[j].y, f, l);
-      sum.x = fmaf(v[j].x, f, sum.x);
-      sum.y = fmaf(v[j].y, f, sum.y);
-      sum.z = fmaf(v[j].z, f, sum.z);
-      sum.w = fmaf(v[j].w, f, sum.w);
-    }
+  Join join;
+  if (row < item.rows)  // (the parts hold nothing of other rows)
+    for (int k0 = group; k0 < item.parts; k0 += 4 * GROUPS)
+      join.add4<D, ROWS>([&](int k) { return own + (k == 0 ? kSize : 2 * k * kSize); }, k0, GROUPS,
+                         item.parts, r, d);
+  if (GROUPS > 1) {
+    sums[threadIdx.x] = join.sum;
+    if (d == 0) stats[group * 16 + in_block] = make_float2(join.m, join.l);
+    __syncthreads();
+    if (group > 0) return;
+    float m = -kInf;
+    for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, stats[i * 16 + in_block].x);
+    join = Join();
+    join.m = m;
+    for (int i = 0; i < GROUPS; ++i)
+      join.add(stats[i * 16 + in_block], sums[i * kLanes + lane], m == -kInf ? 0.f : m);
   }
-  write_row<T>(a, z, item.first, item.kv_head, row, D, d, sum, m, l);
+  if (row < item.rows)
+    write_row<T>(a, z, item.first, item.kv_head, row, D, d, join.sum, join.m, join.l);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -635,8 +665,12 @@ bool few_rows(const cxs_cache_attend_call& a) {
 }
 
 long long workspace_bytes(const cxs_cache_attend_call& a) {
-  const long long rows = few_rows(a) ? 16 : kTileRows;
-  return kMostCtas * (sizeof(Partial) + 2 * rows * (a.cache.dim + 2) * (long long)sizeof(float));
+  // Two partial results for each CTA and, of few rows, each warp.
+  const bool few = few_rows(a);
+  const long long slots = 2 * kMostCtas * (few ? 1 + kDecodeWarps : 1);
+  const long long rows = few ? 16 : kTileRows;
+  return kMostCtas * sizeof(Partial) +
+         slots * rows * (a.cache.dim + 2) * (long long)sizeof(float);
 }
 
 template <int FORMAT, typename T, int D>
@@ -659,8 +693,9 @@ int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cud
   // Its CTAs may start while the last CTAs before finish; they wait for them
   // on the device.
   cudaLaunchConfig_t config = {};
+  constexpr int kGroups = 256 / D;  // for few rows: 1024 threads
   config.gridDim = dim3(z.grid, few ? 1 : kTileRows / 16);
-  config.blockDim = dim3(16 * D / 4);
+  config.blockDim = dim3(few ? kGroups * 4 * D : 4 * D);
   config.stream = stream;
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -668,9 +703,9 @@ int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cud
   config.attrs = &early;
   config.numAttrs = 1;
   if (few)
-    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, 16>, a, z));
+    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, 16, kGroups>, a, z));
   else
-    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, kTileRows>, a, z));
+    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, kTileRows, 1>, a, z));
   CXS_LAUNCH_CHECK("cache attend join");
   return CXS_OK;
 }
@@ -708,7 +743,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
     cxs_cache_attend_call a = *call;
     const int left = c.users - user0;
     const Shape z{call->heads / c.kv_heads, user0, left < kSlice ? left : kSlice, left <= kSlice,
-                  grid, !few ? 2 : c.dim == 64 ? Decode<64>::kWarps : Decode<128>::kWarps};
+                  grid, few ? grid * kDecodeWarps : grid, 2};
     a.cache.table += user0 * c.table_stride;
     a.cache.lengths += user0;
     if (a.cache.offsets) a.cache.offsets += user0;

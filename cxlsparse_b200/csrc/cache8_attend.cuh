@@ -62,9 +62,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // An item is one user's tile of query rows (a row is a new token and one of
 // the KV head's query heads: row r is token r / group, head r % group) with
 // one KV head. Its work is a run of key tiles. All items' tiles, in order,
-// are cut into equal shares, one for each CTA, whatever the users' lengths;
-// an item whose tiles fall into several shares leaves a partial result (O, M,
-// l) in each, which combine_kernel joins in the order of the keys.
+// are cut into equal shares, one for each worker (a warp of the kernel for few
+// rows, a CTA of the other), whatever the users' lengths; an item whose tiles
+// fall into several shares leaves a partial result (O, M, l) in each. They are
+// joined in the order of the keys: those of a CTA's warps at its end, those of
+// CTAs by combine_kernel.
 
 constexpr int kSlice = 2048;  // users of one launch (their tile counts sit in shared memory)
 
@@ -73,8 +75,9 @@ struct Shape {
   int user0;      // first user of this launch (table, lengths and offsets point at it)
   int users;
   int last;       // the launch holds the last user
-  int grid;       // most CTAs
-  int min_tiles;  // fewest tiles worth a CTA
+  int grid;       // CTAs
+  int workers;    // most shares: warps or CTAs of the grid
+  int min_tiles;  // fewest tiles worth a share
 };
 
 // One user's positions. Visible to some row: [begin, end).
@@ -122,33 +125,40 @@ __device__ __forceinline__ long long divide(long long a, int b) {
   return a / b;
 }
 
-// The tiles cut into shares, one a CTA: of `each` tiles, the first `more` of
-// them of one more.
+// The tiles cut into `count` shares: of `each` tiles, the first `more` of them
+// of one more.
 struct Shares {
+  int count;
   long long each;
   int more;
-  __device__ __forceinline__ Shares(long long total, int ctas)
-      : each(divide(total, ctas)), more((int)(total - each * ctas)) {}
-  __device__ __forceinline__ long long begin(int cta) const { return each * cta + min(cta, more); }
-  __device__ __forceinline__ int of(long long tile) const {  // the CTA that has it
+  __device__ __forceinline__ Shares(long long total, const Shape& z) {
+    const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
+    count = wanted < z.workers ? (int)wanted : z.workers;
+    each = count > 0 ? divide(total, count) : 0;
+    more = (int)(total - each * count);
+  }
+  __device__ __forceinline__ long long begin(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int of(long long tile) const {  // the share that has it
     const long long wide = (each + 1) * more;
     if (tile < wide || each == 0) return (int)(each + 1 > INT_MAX ? tile / (each + 1) : divide(tile, (int)each + 1));
     return more + (int)(each > INT_MAX ? (tile - wide) / each : divide(tile - wide, (int)each));
   }
 };
 
-struct alignas(16) Partial {  // the item that starts in a CTA's share and goes on past it
-  int parts;      // CTAs it falls into; 0: none
+struct alignas(16) Partial {  // the item that starts in a share and goes on past it
+  int parts;      // shares it falls into; 0: none
   int first, rows, row0, kv_head;  // the item's packed first row, user's rows, first row, head
 };
 
 // Rows of no user (before the first offset, past the last, or more than
-// max_tokens of one user): zero, and nothing in the sum.
+// max_tokens of one user): zero, and nothing in the sum. Shared out among the
+// workers, each of `threads` threads.
 template <typename T, int D>
-__device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int cta, int ctas) {
+__device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int worker, int workers,
+                           int thread, int threads) {
   const cxs_cache_call& c = a.cache;
   if (!c.offsets) return;
-  for (int b = cta - 1; b <= z.users; b += ctas) {
+  for (int b = worker - 1; b <= z.users; b += workers) {
     long long low, high;
     if (b < 0) {
       low = z.user0 == 0 ? 0 : 1;
@@ -166,10 +176,10 @@ __device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int c
     if (low < 0) low = 0;
     if (high > c.tokens) high = c.tokens;
     if (low >= high) continue;
-    for (long long i = low * a.heads * D + threadIdx.x; i < high * a.heads * D; i += blockDim.x)
+    for (long long i = low * a.heads * D + thread; i < high * a.heads * D; i += threads)
       ((T*)a.out)[i] = from_float<T>(0.f);
     if (a.lse)
-      for (long long i = low * a.heads + threadIdx.x; i < high * a.heads; i += blockDim.x)
+      for (long long i = low * a.heads + thread; i < high * a.heads; i += threads)
         a.lse[i] = -kInf;
   }
 }

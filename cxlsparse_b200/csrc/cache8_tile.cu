@@ -291,14 +291,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
   const long long total = prefix[z.users];
-  const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
-  const int ctas = wanted < z.grid ? (int)wanted : z.grid;
+  const Shares shares(total, z);
   Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
   Partial& mine = partials[blockIdx.x];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) mine.parts = 0;
-  const bool busy = (int)blockIdx.x < ctas;
-  const Shares shares(total, ctas > 0 ? ctas : 1);
+  const bool busy = (int)blockIdx.x < shares.count;
   const long long lo = busy ? shares.begin(blockIdx.x) : 0;
   const long long hi = busy ? shares.begin(blockIdx.x + 1) : 0;
   float* const scratch = reinterpret_cast<float*>(partials + z.grid) +
@@ -848,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 done:
   __syncwarp();
-  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x);
+  clear_rows<T, D>(a, z, blockIdx.x, gridDim.x, threadIdx.x, kThreads);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
