@@ -32,6 +32,7 @@ constexpr int kConvertWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
 constexpr int kPanel = 128 * 128;       // bytes: 128 rows (queries or keys) of 64 channels, swizzled
 constexpr int kRuns = kKeys / 16;       // runs of 16 keys: each within one page
 constexpr int kRing = 8;                // tiles whose Tile is kept: more than are ever in work
+constexpr int kItemCost = 4;            // tiles that an item's queries and results cost
 constexpr int kTmem = 512;              // columns: S/P of two groups (128 each), O of two groups
 
 // Registers a thread by role: twice the softmax's, the conversion's and the
@@ -75,7 +76,8 @@ struct Layout {
   static constexpr int kTiles = kRaw + kRawStages * 2 * kRawPart;  // [kRing]
   static constexpr int kBars = kTiles + kRing * (int)sizeof(Tile);
   static constexpr int kPrefix = kBars + 256;
-  static constexpr int kBytes = kPrefix + (kSlice + 1) * 8 + 1024;  // and the 1024-byte alignment
+  static constexpr int kCounts = kPrefix + (kSlice + 1) * 8;
+  static constexpr int kBytes = kCounts + (kSlice + 1) * 4 + 1024;  // and the 1024-byte alignment
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -198,6 +200,7 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
 struct Item {
   int user, tile_row, kv_head;   // rows kTileRows * tile_row ..
   long long begin, end;
+  long long index;               // among all items
   Span span;
   int rows;                      // of the user with this KV head
   int first;                     // its first tile of keys
@@ -225,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Bars* const bars = (Bars*)(smem + L::kBars);
   Tile* const ring = (Tile*)(smem + L::kTiles);
   long long* const prefix = (long long*)(smem + L::kPrefix);
+  int* const counts = (int*)(smem + L::kCounts);
   // (Broadcast: uniform across the warp also for the compiler.)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
@@ -255,35 +259,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                  "r"(kTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // Tiles before each user: a warp adds up a user's row tiles, one warp scans.
+  // Costs (tiles, and kItemCost for each item) and items before each user: a
+  // warp adds up a user's row tiles, one warp scans.
   for (int b = warp; b < z.users; b += kThreads / 32) {
     int bad = 0;
     const Span s = user_span(a, z, b, &bad);
-    const int rows = s.count * z.group;
+    const int rows = s.count * z.group, row_tiles = (rows + kTileRows - 1) / kTileRows;
     long long n = 0;
-    for (int r = lane; r * kTileRows < rows; r += 32) {
+    for (int r = lane; r < row_tiles; r += 32) {
       int first;
-      n += key_tiles(a, z, s, rows, r, &first);
+      n += key_tiles(a, z, s, rows, r, &first) + kItemCost;
     }
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     if (lane == 0) {
       prefix[b + 1] = n * c.kv_heads;
+      counts[b + 1] = row_tiles * c.kv_heads;
       if (bad && blockIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
     }
   }
   __syncthreads();
   if (warp == 0) {
     long long base = 0;
-    if (lane == 0) prefix[0] = 0;
+    int items = 0;
+    if (lane == 0) prefix[0] = 0, counts[0] = 0;
     for (int b0 = 0; b0 < z.users; b0 += 32) {
       const int b = b0 + lane;
       long long sum = b < z.users ? prefix[b + 1] : 0;
+      int count = b < z.users ? counts[b + 1] : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
+        const int more = __shfl_up_sync(0xffffffffu, count, o);
+        if (lane >= o) sum += up, count += more;
       }
-      if (b < z.users) prefix[b + 1] = base + sum;
+      if (b < z.users) prefix[b + 1] = base + sum, counts[b + 1] = items + count;
       base += __shfl_sync(0xffffffffu, sum, 31);
+      items += __shfl_sync(0xffffffffu, count, 31);
     }
   }
   tc::fence_before();
@@ -296,54 +306,61 @@ __global__ void __launch_bounds__(kThreads, 1)
   Partial& mine = partials[blockIdx.x];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) mine.parts = 0;
-  const bool busy = (int)blockIdx.x < shares.count;
-  const long long lo = busy ? shares.begin(blockIdx.x) : 0;
-  const long long hi = busy ? shares.begin(blockIdx.x + 1) : 0;
   float* const scratch = reinterpret_cast<float*>(partials + z.grid) +
                          (long long)blockIdx.x * 2 * kTileRows * (D + 2);
 
-  // The item that holds the share's first tile; every warp finds it.
-  Item item = {};
-  if (lo < hi) {
+  // The item that place `at` among all costs falls into; returns the tile there
+  // (the item's first one, if `at` is in the item's own cost). Every warp
+  // looks for itself.
+  auto locate = [&](long long at, Item& p) -> long long {
     int l = 0, h = z.users - 1;
     while (l < h) {
       const int m = (l + h) / 2;
-      if (prefix[m + 1] > lo) h = m; else l = m + 1;
+      if (prefix[m + 1] > at) h = m; else l = m + 1;
     }
     int bad = 0;
-    item.user = l;
-    item.span = user_span(a, z, l, &bad);
-    item.rows = item.span.count * z.group;
-    long long before = prefix[l];  // tiles before row tile r0
+    p.user = l;
+    p.span = user_span(a, z, l, &bad);
+    p.rows = p.span.count * z.group;
+    long long before = prefix[l];  // cost before row tile r0
     for (int r0 = 0;; r0 += 32) {
       const int r = r0 + lane;
-      int first = 0;
-      const int n = r * kTileRows < item.rows ? key_tiles(a, z, item.span, item.rows, r, &first) : 0;
+      int first = 0, n = 0;
+      if ((long long)r * kTileRows < p.rows) n = key_tiles(a, z, p.span, p.rows, r, &first) + kItemCost;
       long long sum = (long long)n * c.kv_heads;
       for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, before + sum > lo);
-      if (past || (r0 + 32) * (long long)kTileRows >= item.rows) {
-        const int at = past ? __ffs(past) - 1 : 31;
-        const int tiles = __shfl_sync(0xffffffffu, n, at);
-        const long long start = before + __shfl_sync(0xffffffffu, sum, at) -
-                                (long long)tiles * c.kv_heads;
-        item.tile_row = r0 + at;
-        item.first = __shfl_sync(0xffffffffu, first, at);
-        item.kv_head = (int)divide(lo - start, tiles);
-        item.begin = start + (long long)item.kv_head * tiles;
-        item.end = item.begin + tiles;
-        break;
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > at);
+      if (past) {
+        const int in = __ffs(past) - 1, cost = __shfl_sync(0xffffffffu, n, in);
+        const long long start = before + __shfl_sync(0xffffffffu, sum, in) - (long long)cost * c.kv_heads;
+        p.tile_row = r0 + in;
+        p.first = __shfl_sync(0xffffffffu, first, in);
+        p.kv_head = (int)divide(at - start, cost);
+        p.index = counts[l] + (long long)p.tile_row * c.kv_heads + p.kv_head;
+        const long long begin = start + (long long)p.kv_head * cost;
+        p.begin = begin - kItemCost * p.index;
+        p.end = p.begin + cost - kItemCost;
+        return p.begin + max(at - begin - kItemCost, 0ll);
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
+      if ((r0 + 32) * (long long)kTileRows >= p.rows) return 0;  // (not reached)
     }
+  };
+  long long lo = 0, hi = 0;
+  Item item = {};
+  if ((int)blockIdx.x < shares.count) {
+    hi = (int)blockIdx.x + 1 < shares.count ? locate(shares.begin(blockIdx.x + 1), item)
+                                            : total - (long long)kItemCost * counts[z.users];
+    lo = locate(shares.begin(blockIdx.x), item);
   }
   // The item after `p` (there is one: its tiles end before the share does).
   auto next = [&](Item& p) {
     const long long n = p.end - p.begin;
     p.begin = p.end;
+    ++p.index;
     if (++p.kv_head < c.kv_heads) {
       p.end = p.begin + n;
       return;
@@ -352,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ++p.tile_row;
     if ((long long)p.tile_row * kTileRows >= p.rows) {
       do ++p.user;
-      while (prefix[p.user + 1] <= p.begin);
+      while (counts[p.user + 1] == counts[p.user]);
       int bad = 0;
       p.span = user_span(a, z, p.user, &bad);
       p.rows = p.span.count * z.group;
@@ -386,51 +403,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (until < hi) next(item);
       }
       if (tile < hi) {
-        // The row's query, scaled by a power of two (and the scale's sign),
-        // into the group's Q panels, before the last item's O is written: S
-        // of this item may start meanwhile. Twice: once for the largest
-        // element, once (from L1) for the values.
-        const int row = item.tile_row * kTileRows + 128 * g + r;
-        const bool live = row < item.rows;
-        const T* from = (const T*)a.query;
-        if (live)
-          from += (long long)(item.span.first + row / z.group) * a.q_token_stride +
-                  (long long)(item.kv_head * z.group + row % z.group) * a.q_head_stride;
-        const bool wide = ((uintptr_t)from & 15) == 0;
-        auto eight = [&](float (&v)[8], int i) {  // channels 8 i ..
-          alignas(16) T x[8];
-          if (wide) {
-            *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(from)[i];
-          } else {
+        // The warp's 32 rows of queries, scaled by a power of two each (and the
+        // scale's sign), into the group's Q panels, before the last item's O
+        // is written: S of this item may start meanwhile. D / 8 lanes read a
+        // row together (a lane for each row would touch 32 lines at once).
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kBatch = 8;  // rows
+        int row = item.tile_row * kTileRows + 32 * (warp % 8) + lane / kLanes;
+        int token = row / z.group, head = row - token * z.group;
+#pragma unroll 1
+        for (int b0 = 0; b0 < 32; b0 += kAtOnce * kBatch) {
+          uint4 in[kBatch];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = from[8 * i + j];
+          for (int j = 0; j < kBatch; ++j) {
+            in[j] = make_uint4(0, 0, 0, 0);
+            if (row < item.rows) {
+              const T* const from =
+                  (const T*)a.query + (long long)(item.span.first + token) * a.q_token_stride +
+                  (long long)(item.kv_head * z.group + head) * a.q_head_stride + 8 * (lane % kLanes);
+              if (((uintptr_t)from & 15) == 0) {
+                in[j] = *reinterpret_cast<const uint4*>(from);
+              } else {
+                alignas(16) T x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = from[e];
+                in[j] = *reinterpret_cast<const uint4*>(x);
+              }
+            }
+            row += kAtOnce;
+            for (head += kAtOnce; head >= z.group; head -= z.group) ++token;
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = live ? to_float(x[j]) : 0.f;
-        };
-        float top = 0.f;
+          for (int j = 0; j < kBatch; ++j) {
+            const int r32 = b0 + j * kAtOnce + lane / kLanes, r128 = 32 * (warp % 4) + r32;
+            alignas(16) T x[8];
+            *reinterpret_cast<uint4*>(x) = in[j];
+            float v[8], top = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {  // all loads in flight
-          float v[8];
-          eight(v, i);
+            for (int e = 0; e < 8; ++e) {
+              v[e] = to_float(x[e]);
+              if (fabsf(v[e]) < kInf) top = fmaxf(top, fabsf(v[e]));
+            }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (fabsf(v[j]) < kInf) top = fmaxf(top, fabsf(v[j]));
-        }
-        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-        if (e < -100) e = -100;
-        if (top == 0.f) e = 14;
-        float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        if (a.scale < 0.f) up = -up;
-        if (a.scale == 0.f) up = 0.f;  // every score is 0
-        back = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-#pragma unroll 2
-        for (int i = 0; i < D / 8; ++i) {
-          float v[8];
-          eight(v, i);
-          *reinterpret_cast<uint4*>(q_panels + i / 8 * kPanel + tc::sw128_chunk(r, i % 8)) =
-              make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
-                         pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
+            for (int o = 1; o < kLanes; o <<= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+            if (e < -100) e = -100;
+            if (top == 0.f) e = 14;
+            float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+            if (a.scale < 0.f) up = -up;
+            if (a.scale == 0.f) up = 0.f;  // every score is 0
+            const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+            // The inverse goes to the row's own lane.
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+              const float its = __shfl_sync(0xffffffffu, down, k * kLanes);
+              if (lane == b0 + j * kAtOnce + k) back = its;
+            }
+            const int chunk = lane % kLanes;
+            *reinterpret_cast<uint4*>(q_panels + chunk / 8 * kPanel +
+                                      tc::sw128_chunk(r128, chunk % 8)) =
+                make_uint4(pack_half2(v[0] * up, v[1] * up), pack_half2(v[2] * up, v[3] * up),
+                           pack_half2(v[4] * up, v[5] * up), pack_half2(v[6] * up, v[7] * up));
+          }
         }
         cxs::fence_proxy_async_shared();
         warp_arrive(&bars->q_full[g], lane);
@@ -476,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
         }
         if (!complete && started == ended.begin && g == 0 && r == 0) {
-          const int last = shares.of(ended.end - 1);
+          const int last = shares.of(ended.end - 1 + kItemCost * (ended.index + 1));
           mine.first = ended.span.first;
           mine.rows = ended.rows;
           mine.row0 = ended.tile_row * kTileRows;
