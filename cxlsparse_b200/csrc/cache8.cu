@@ -66,27 +66,29 @@ __device__ __forceinline__ void load16(float (&x)[16], const T* from, bool wide)
 // several CTAs share an SM, so one's reduction hides under the others' loads.
 // Older codes are touched only where the page's scale grows.
 template <int FORMAT, typename T>
-__global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
+__global__ void __launch_bounds__(512, 4) append_kernel(const cxs_cache_call c, const T* __restrict__ k,
                               long long k_token, long long k_head, const T* __restrict__ v,
-                              long long v_token, long long v_head, int reach) {
+                              long long v_token, long long v_head, int page_bits) {
   using C = Code<FORMAT>;
-  const int user = blockIdx.x / reach, step = blockIdx.x % reach;
-  const int head = blockIdx.y, part = blockIdx.z;
+  const int step = blockIdx.x, head = blockIdx.y >> 1, part = blockIdx.y & 1, user = blockIdx.z;
   int bad = 0;
   const Rows rows = user_rows(c, user, &bad);
-  const long long start = (long long)c.lengths[user] - rows.count;
-  const long long end = start + rows.count;
-  const long long most = (long long)c.width * c.page_size;
-  if (start < 0 || end > most) bad = 1;
-  if (bad && step == 0 && head == 0 && part == 0 && threadIdx.x == 0)
+  const int most = c.width << page_bits;
+  const int length = c.lengths[user];
+  const long long start = (long long)length - rows.count;  // of the new tokens
+  if (start < 0 || length > most) bad = 1;
+  if (bad && step == 0 && blockIdx.y == 0 && threadIdx.x == 0)
     report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
-  const long long from = start > 0 ? start : 0, to = end < most ? end : most;
-  const long long low = (from / c.page_size + step) * c.page_size;  // position of slot 0
-  if (from >= to || low >= to) return;
-  const int fill = from > low ? (int)(from - low) : 0;  // slots of older tokens
-  const int stop = to - low < c.page_size ? (int)(to - low) : c.page_size;
-  const int chunks = c.dim / 16, slot = threadIdx.x / chunks, channel = threadIdx.x % chunks * 16;
+  const int from = start > 0 ? (int)start : 0, to = min(length, most);
+  const int block = (from >> page_bits) + step, low = block << page_bits;  // position of slot 0
+  if (rows.count == 0 || from >= to || low >= to) return;
+  const int fill = max(from - low, 0);                 // slots of older tokens
+  const int stop = min(to - low, 1 << page_bits);
+  const int chunk_bits = c.dim == 64 ? 2 : 3;
+  const int slot = threadIdx.x >> chunk_bits;
+  const int channel = (threadIdx.x & ((1 << chunk_bits) - 1)) * 16;
   const bool fresh = slot >= fill && slot < stop, old = slot < fill;
+  const int page = c.table[user * c.table_stride + block];
 
   float x[16];
   float size = 0.f;
@@ -95,24 +97,32 @@ __global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
     row += (rows.first + (low - start) + slot) * (part ? v_token : k_token) + channel;
     load16(x, row, ((uintptr_t)row & 15) == 0);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float a = fabsf(x[e]);
-      if (a < INFINITY) size = fmaxf(size, a);  // neither infinity nor NaN
-    }
+    for (int e = 0; e < 16; ++e) size = fmaxf(size, fabsf(x[e]));  // (passes over NaN)
   }
-  const int page = c.table[user * c.table_stride + low / c.page_size];
   if (page < 0 || page >= c.pages) {
-    if (head == 0 && part == 0 && threadIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
+    if (blockIdx.y == 0 && threadIdx.x == 0) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
     return;
   }
   const long long cell = ((long long)page * c.kv_heads + head) * 2 + part;
   uint4* codes = (uint4*)((uint8_t*)c.codes + cell * c.page_size * c.dim) + threadIdx.x;
   const float before = fill ? c.scales[cell] : 0.f;
-  __shared__ float partial[16];
-  for (int o = 16; o; o >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
-  if (threadIdx.x % 32 == 0) partial[threadIdx.x / 32] = size;
-  __syncthreads();  // and every thread has read the older scale
-  for (int w = 0; w < blockDim.x / 32; ++w) size = fmaxf(size, partial[w]);
+  __shared__ float partial[2][16];
+  auto largest = [&](float mine, float* slots) {
+    for (int o = 16; o; o >>= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if (threadIdx.x % 32 == 0) slots[threadIdx.x / 32] = mine;
+    __syncthreads();
+    for (int w = 0; w < blockDim.x / 32; ++w) mine = fmaxf(mine, slots[w]);
+    return mine;
+  };
+  size = largest(size, partial[0]);  // (and every thread has read the older scale)
+  if (size == INFINITY) {            // rare: the largest finite magnitude
+    size = 0.f;
+    if (fresh)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (fabsf(x[e]) < INFINITY) size = fmaxf(size, fabsf(x[e]));
+    size = largest(size, partial[1]);
+  }
   const float scale = fmaxf(fmaxf(size * C::kInverseTop, kLeastScale), before);
   if (threadIdx.x == 0) c.scales[cell] = scale;
   float factor;
@@ -142,27 +152,26 @@ __global__ void append_kernel(const cxs_cache_call c, const T* __restrict__ k,
   *codes = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// One page and head per CTA: K and V of a page are one run of bytes, read 16
-// a thread with kUnroll reads in flight, multiplied, rounded and written to
-// the two outputs. Memory-bound: 1 byte in, 2 or 4 out.
-constexpr int kReadThreads = 128, kUnroll = 4;
+// One page and head per CTA: K and V of a page are one run of bytes. A thread
+// reads as many codes as make 16 bytes of the result (a warp's stores are then
+// whole lines), kUnroll times at once. Memory-bound: 1 byte in, 2 or 4 out.
+constexpr int kReadThreads = 128, kUnroll = 8;
 
 template <int FORMAT, typename T>
 __global__ void __launch_bounds__(kReadThreads)
-    read_kernel(const cxs_cache_call c, T* __restrict__ k, T* __restrict__ v, int reach) {
+    read_kernel(const cxs_cache_call c, T* __restrict__ k, T* __restrict__ v, int page_bits) {
   using C = Code<FORMAT>;
-  const int user = blockIdx.x / reach, step = blockIdx.x % reach, head = blockIdx.y;
+  const int step = blockIdx.x, head = blockIdx.y, user = blockIdx.z;
   int bad = 0;
   const Rows rows = user_rows(c, user, &bad);
-  const long long start = c.lengths[user], end = start + rows.count;
-  const long long most = (long long)c.width * c.page_size;
+  const int start = c.lengths[user], most = c.width << page_bits;
+  const long long end = (long long)start + rows.count;
   if (start < 0 || end > most) bad = 1;
   if (bad && step == 0 && head == 0 && threadIdx.x == 0)
     report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
   // Pages are counted from the one (possibly before the first) that holds `start`.
-  const long long block = (start >= 0 ? start / c.page_size
-                                      : -((-start + c.page_size - 1) / c.page_size)) + step;
-  const long long low = block * c.page_size;
+  const int block = (start >> page_bits) + step;
+  const long long low = (long long)block << page_bits;
   if (low >= end) return;
   const int fill = start > low ? (int)(start - low) : 0;
   const int stop = end - low < c.page_size ? (int)(end - low) : c.page_size;
@@ -177,37 +186,48 @@ __global__ void __launch_bounds__(kReadThreads)
   const long long cell = ((long long)(page < 0 ? 0 : page) * c.kv_heads + head) * 2;
   const float scale_k = page < 0 ? 0.f : c.scales[cell];
   const float scale_v = page < 0 ? 0.f : c.scales[cell + 1];
-  const uint4* codes = (const uint4*)((const uint8_t*)c.codes + cell * c.page_size * c.dim);
-  const int chunks = c.dim / 16, half = c.page_size * chunks;
+  const uint8_t* codes = (const uint8_t*)c.codes + cell * c.page_size * c.dim;
+  constexpr int kCodes = 16 / sizeof(T), kCodeBits = kCodes == 8 ? 3 : 2;  // of a unit
+  const int unit_bits = (c.dim == 64 ? 6 : 7) - kCodeBits;               // units of a row
+  const int half = 1 << (page_bits + unit_bits);
   const long long row0 = rows.first + (low - start);
   for (int base = threadIdx.x; base < 2 * half; base += kReadThreads * kUnroll) {
-    uint4 w[kUnroll];
+    uint32_t w[kUnroll][kCodes / 4];
     bool live[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int n = base + i * kReadThreads, slot = n % half / chunks;
+      const int n = base + i * kReadThreads, slot = (n & (half - 1)) >> unit_bits;
       live[i] = n < 2 * half && slot >= fill && slot < stop;
-      w[i] = live[i] && page >= 0 ? __ldcs(codes + n) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < kCodes / 4; ++j) w[i][j] = 0;
+      if (live[i] && page >= 0) {
+        if constexpr (kCodes == 8) {
+          const uint2 in = __ldcs(reinterpret_cast<const uint2*>(codes) + n);
+          w[i][0] = in.x;
+          w[i][1] = in.y;
+        } else {
+          w[i][0] = __ldcs(reinterpret_cast<const uint32_t*>(codes) + n);
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       if (!live[i]) continue;
       const int n = base + i * kReadThreads;
       const bool second = n >= half;
-      const int slot = n % half / chunks, channel = n % chunks * 16;
+      const int slot = (n & (half - 1)) >> unit_bits;
+      const int channel = (n & ((1 << unit_bits) - 1)) << kCodeBits;
       const float scale = second ? scale_v : scale_k;
-      alignas(16) T out[16];
-      const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      alignas(16) T out[kCodes];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kCodes / 4; ++j) {
         float x[4];
-        C::decode4(in[j], x);
+        C::decode4(w[i][j], x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[4 * j + e] = from_float<T>(x[e] * scale);
       }
-      uint4* to = (uint4*)((second ? v : k) + ((row0 + slot) * c.kv_heads + head) * c.dim + channel);
-#pragma unroll
-      for (int j = 0; j < (int)sizeof(T); ++j) to[j] = reinterpret_cast<const uint4*>(out)[j];
+      *(uint4*)((second ? v : k) + ((row0 + slot) * c.kv_heads + head) * c.dim + channel) =
+          *reinterpret_cast<const uint4*>(out);
     }
   }
 }
@@ -224,15 +244,14 @@ extern "C" int cxs_cache_append(const cxs_cache_call* call, const void* k, int64
   if (status != CXS_OK) return status;
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache append: null keys or values");
   const int reach = (call->max_tokens + call->page_size - 2) / call->page_size + 1;
-  if ((long long)call->users * reach > 0x7fffffffll)
-    return set_error(CXS_ERR_CAPACITY, "cache append: too many pages in one call");
-  const dim3 grid(call->users * reach, call->kv_heads, 2);
+  const dim3 grid(reach, call->kv_heads * 2, call->users);
+  const int page_bits = call->page_size == 16 ? 4 : call->page_size == 32 ? 5 : 6;
   const int threads = call->page_size * call->dim / 16;
   CXS_CACHE_FORMAT(call->format, F,
                    CXS_CACHE_TYPE(call->type, T,
                                   (append_kernel<F, T><<<grid, threads, 0, (cudaStream_t)stream>>>(
                                       *call, (const T*)k, k_token_stride, k_head_stride,
-                                      (const T*)v, v_token_stride, v_head_stride, reach))));
+                                      (const T*)v, v_token_stride, v_head_stride, page_bits))));
   CXS_LAUNCH_CHECK("cache append");
   return CXS_OK;
 }
@@ -247,14 +266,13 @@ extern "C" int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void
   if ((uintptr_t)k % 16 || (uintptr_t)v % 16)
     return set_error(CXS_ERR_INVALID, "cache read: outputs must be 16-byte aligned");
   const int reach = (call->max_tokens + call->page_size - 2) / call->page_size + 1;
-  if ((long long)call->users * reach > 0x7fffffffll)
-    return set_error(CXS_ERR_CAPACITY, "cache read: too many pages in one call");
-  const dim3 grid(call->users * reach, call->kv_heads);
+  const dim3 grid(reach, call->kv_heads, call->users);
+  const int page_bits = call->page_size == 16 ? 4 : call->page_size == 32 ? 5 : 6;
   CXS_CACHE_FORMAT(
       call->format, F,
       CXS_CACHE_TYPE(call->type, T,
                      (read_kernel<F, T><<<grid, kReadThreads, 0, (cudaStream_t)stream>>>(
-                         *call, (T*)k, (T*)v, reach))));
+                         *call, (T*)k, (T*)v, page_bits))));
   CXS_LAUNCH_CHECK("cache read");
   return CXS_OK;
 }

@@ -28,8 +28,11 @@ struct Code<CXS_FORMAT_E4M3> {
   }
   // Nearest codes, ties to even, saturated; NaN stays NaN.
   static __device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    uint32_t lo, hi;
+    asm("{.reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; cvt.u32.u16 %0, h;}"
+        : "=r"(lo) : "f"(x[0]), "f"(x[1]));
+    asm("{.reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, %2, %1; cvt.u32.u16 %0, h;}"
+        : "=r"(hi) : "f"(x[2]), "f"(x[3]));
     return lo | hi << 16;
   }
 };

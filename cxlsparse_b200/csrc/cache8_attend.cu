@@ -657,11 +657,13 @@ int sm_count(int* sms) {
 // workspace's size does not depend on the device.
 constexpr int kMostCtas = 148;
 
-// Most rows of a user and KV head for which the mma.sync kernel runs.
-constexpr int kFewRows = 64;
-
+// Most rows of a user and KV head for which the mma.sync kernel runs: it takes
+// 16 rows at a time and reads the keys again for the next 16, the tcgen05
+// kernel takes up to 256 at about the same cost. Measured (us, mma.sync /
+// tcgen05), D = 64, 8 users of 8K tokens, 2 KV heads: 64 rows 27 / 31, 128 rows
+// 38 / 32; D = 128, 8 users of 8K, 8 KV heads: 32 rows 86 / 92, 64 rows 138 / 95.
 bool few_rows(const cxs_cache_attend_call& a) {
-  return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= kFewRows;
+  return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= (a.cache.dim == 64 ? 64 : 32);
 }
 
 long long workspace_bytes(const cxs_cache_attend_call& a) {
