@@ -406,6 +406,58 @@ def test_attend_skips_pages_out_of_range(cuda, new):
     assert torch.equal(out[:new], whole)
 
 
+@pytest.mark.parametrize("new", [1, 300])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_any_scale_on_the_scores(cuda, new, scale, dim):
+    lengths = [700, 301]
+    codes, scales, table = paged(lengths, kv_heads=2, dim=dim, page_size=32, format="int8")
+    q = 0.2 * torch.randn(2 * new, 8, dim, device="cuda").bfloat16()
+    out, lse = QuantizedCache(codes=codes, scales=scales).attend(
+        q, table, ints(lengths), offsets_of([new, new]), max_tokens=new, scale=scale,
+        return_lse=True)
+    want, want_lse, tol, tol_lse = attend(q, codes, scales, table, lengths, [new, new],
+                                          causal=True, window=0, scale=scale)
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - want_lse).abs() <= tol_lse).all()
+
+
+@pytest.mark.parametrize("dim,new", [(64, 1), (128, 1), (64, 9), (128, 33)])
+def test_attend_one_long_user_is_split_over_the_gpu(cuda, dim, new):
+    """100,001 tokens of one user: every SM holds a part of the same item."""
+    check_attend([100001], [new], heads=8, kv_heads=1, dim=dim, page=64, format="e4m3",
+                 dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_attend_more_users_than_one_launch_holds(cuda, new):
+    """4,500 users of 0 to 40 tokens: three launches of at most 2048 users, many
+    items for every worker."""
+    lengths = [(i * 37) % 41 for i in range(4500)]
+    counts = [new if i % 3 else 0 for i in range(4500)]
+    check_attend(lengths, counts, heads=8, kv_heads=1, dim=64, page=16, format="int8",
+                 dtype=torch.float16)
+    if new == 1:
+        codes, scales, table = paged(lengths, kv_heads=1, dim=64, page_size=16, format="int8")
+        q = torch.randn(4500, 8, 64, device="cuda").half()
+        cache = QuantizedCache(codes=codes, scales=scales)
+        packed = cache.attend(q, table, ints(lengths), offsets_of([1] * 4500), max_tokens=1)
+        assert torch.equal(cache.attend(q, table, ints(lengths)), packed)
+
+
+def test_append_unaligned_rows(cuda):
+    """Rows that start 2 bytes past a 16-byte boundary, of uneven strides."""
+    rows = torch.randn(70, 2 * 2 * 64 + 9, device="cuda").bfloat16()
+    k, v = (rows[:, 1 + 128 * i:129 + 128 * i].view(70, 2, 64) for i in range(2))
+    table = ints([[1, 0, 2, 3, 4]])
+    first, second = (QuantizedCache(5, 2, 64, page_size=16, format="e4m3") for _ in range(2))
+    first.append(k, v, table, ints([70]), ints([0, 70]))
+    second.append(k.contiguous(), v.contiguous(), table, ints([70]), ints([0, 70]))
+    first.check()
+    assert torch.equal(raw(first.codes), raw(second.codes))
+    assert torch.equal(first.scales, second.scales)
+
+
 def test_attend_of_nothing(cuda):
     cache = QuantizedCache(2, 1, 64)
     q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda")
