@@ -771,13 +771,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         return true;
       };
-      // Whatever is ready, P V first: a group's softmax waits for it longest.
+      // Whatever is ready, a group's P V and then its next S: the groups then
+      // run half a tile apart, and one's softmax hides the other's MMAs.
       bool fine = true;
       long long since = clock64();
       while (o_next[0] < count || o_next[1] < count) {
         bool some = try_o(0);
-        some |= try_o(1);
         some |= try_s(0);
+        some |= try_o(1);
         some |= try_s(1);
         if (some) {
           since = clock64();
