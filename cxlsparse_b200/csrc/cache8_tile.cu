@@ -701,6 +701,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dv = tc::desc_sw128(base + L::kV, kPanel, 1024);
       const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, D, 1);
       const int count = (int)(hi - lo);
+      // Tiles whose K and V have come: seen in order, since a group that has no
+      // rows for some tiles may ask for one long after the next has taken its
+      // stage (the barrier's parity then says nothing).
+      int k_ready = 0, v_ready = 0;
       // Next tile and uses of the barriers so far, by group.
       int s_next[2] = {0, 0}, s_items[2] = {0, 0}, s_tiles[2] = {0, 0};
       int o_next[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
@@ -711,8 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // queries, and its columns (read, or with P over S: their P V issued).
       auto try_s = [&](int g) -> bool {
         const int n = s_next[g], stage = stage_of<L::kKStages>(n);
-        if (n >= count || (!L::kApart && n > o_next[g])) return false;
-        if (!ready(&bars->k_full[stage], phase_of<L::kKStages>(n))) return false;
+        if (n >= k_ready || (!L::kApart && n > o_next[g])) return false;
         const int flags = ring[n % kRing].flags;
         if (g == 1 && !(flags & kTwo)) {  // not for this group
           ++s_next[1];
@@ -751,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return true;
         }
         if (!ready(&bars->p_full[g], o_tiles[g])) return false;
-        if (!ready(&bars->v_full[n & 1], n >> 1)) return false;
+        if (n >= v_ready) return false;
         if ((flags & kFirst) && o_items[g] > 0 && !ready(&bars->o_free[g], o_items[g] - 1))
           return false;
         o_items[g] += flags & kFirst ? 1 : 0;
@@ -776,6 +779,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool fine = true;
       long long since = clock64();
       while (o_next[0] < count || o_next[1] < count) {
+        if (k_ready < count && ready(&bars->k_full[stage_of<L::kKStages>(k_ready)],
+                                     phase_of<L::kKStages>(k_ready)))
+          ++k_ready;
+        if (v_ready < count && ready(&bars->v_full[v_ready & 1], v_ready >> 1)) ++v_ready;
         bool some = try_o(0);
         some |= try_s(0);
         some |= try_o(1);

@@ -70,13 +70,16 @@ class QuantizedCache:
     # -- checks ------------------------------------------------------------
     def check(self):
         """Wait for the device and raise if a call met a page or length out of
-        range since the last check (such tokens are skipped, never followed)."""
+        range since the last check (such tokens are skipped, never followed),
+        or gave up a wait."""
         bits = int(self.error.item())
         if bits:
             self.error.zero_()
             what = [text for bit, text in (
                 (_lib.DEVICE_ERR_BAD_BLOCK, "a page id outside the cache"),
-                (_lib.DEVICE_ERR_BAD_LENGTH, "lengths or offsets out of range")) if bits & bit]
+                (_lib.DEVICE_ERR_BAD_LENGTH, "lengths or offsets out of range"),
+                (_lib.DEVICE_ERR_COPY_TIMEOUT, "a wait inside the kernel that ran out (its "
+                 "result is not valid)")) if bits & bit]
             raise _lib.CxsError(_lib.ERR_INVALID, "cache call met " + " and ".join(what))
 
     def _call(self, table, lengths, offsets, tokens, max_tokens, type_):

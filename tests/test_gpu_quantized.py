@@ -406,6 +406,22 @@ def test_attend_skips_pages_out_of_range(cuda, new):
     assert torch.equal(out[:new], whole)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_full_and_half_items_in_turn(cuda, dim):
+    """Items whose second 128 rows are there, partly there and missing, one after
+    the other and in every order, over few and many key tiles: the groups of
+    rows pass each other's tiles."""
+    g = torch.Generator().manual_seed(0)
+    for trial in range(6):
+        users = 24
+        lengths = torch.randint(1, 1500, (users,), generator=g).tolist()
+        new = [int(torch.randint(1, 130, (1,), generator=g)) if i % 2 == trial % 2
+               else (1, 30, 64, 65, 127, 128)[i // 2 % 6] for i in range(users)]
+        for _ in range(3):
+            check_attend(lengths, new, heads=4, kv_heads=2, dim=dim, page=32, format="e4m3",
+                         dtype=torch.float16, seed=trial)
+
+
 @pytest.mark.parametrize("new", [1, 300])
 @pytest.mark.parametrize("scale", [-0.125, 0.0, 1.0])
 @pytest.mark.parametrize("dim", [64, 128])
