@@ -705,17 +705,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       // rows for some tiles may ask for one long after the next has taken its
       // stage (the barrier's parity then says nothing).
       int k_ready = 0, v_ready = 0;
-      // Next tile and uses of the barriers so far, by group.
-      int s_next[2] = {0, 0}, s_items[2] = {0, 0}, s_tiles[2] = {0, 0};
-      int o_next[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
       auto ready = [&](uint64_t* bar, int phase) {
         return __all_sync(0xffffffffu, test_wait(bar, phase & 1));
       };
+      auto have_k = [&](int n) {
+        if (n == k_ready && ready(&bars->k_full[stage_of<L::kKStages>(n)], phase_of<L::kKStages>(n)))
+          ++k_ready;
+        return n < k_ready;
+      };
+      auto have_v = [&](int n) {
+        if (n == v_ready && ready(&bars->v_full[n & 1], n >> 1)) ++v_ready;
+        return n < v_ready;
+      };
+      // Next tile and uses of the barriers so far, by group.
+      int s_next[2] = {0, 0}, s_items[2] = {0, 0}, s_tiles[2] = {0, 0};
+      int o_next[2] = {0, 0}, o_items[2] = {0, 0}, o_tiles[2] = {0, 0};
       // S of group g's next tile, if what it needs is there: K, the item's
       // queries, and its columns (read, or with P over S: their P V issued).
       auto try_s = [&](int g) -> bool {
         const int n = s_next[g], stage = stage_of<L::kKStages>(n);
-        if (n >= k_ready || (!L::kApart && n > o_next[g])) return false;
+        if (n >= count || (!L::kApart && n > o_next[g]) || !have_k(n)) return false;
         const int flags = ring[n % kRing].flags;
         if (g == 1 && !(flags & kTwo)) {  // not for this group
           ++s_next[1];
@@ -754,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return true;
         }
         if (!ready(&bars->p_full[g], o_tiles[g])) return false;
-        if (n >= v_ready) return false;
+        if (!have_v(n)) return false;
         if ((flags & kFirst) && o_items[g] > 0 && !ready(&bars->o_free[g], o_items[g] - 1))
           return false;
         o_items[g] += flags & kFirst ? 1 : 0;
@@ -779,10 +788,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool fine = true;
       long long since = clock64();
       while (o_next[0] < count || o_next[1] < count) {
-        if (k_ready < count && ready(&bars->k_full[stage_of<L::kKStages>(k_ready)],
-                                     phase_of<L::kKStages>(k_ready)))
-          ++k_ready;
-        if (v_ready < count && ready(&bars->v_full[v_ready & 1], v_ready >> 1)) ++v_ready;
         bool some = try_o(0);
         some |= try_s(0);
         some |= try_o(1);
