@@ -64,11 +64,14 @@ __device__ __forceinline__ void load16(float (&x)[16], const T* from, bool wide)
 // magnitude, then written as codes, 16 bytes a thread. Memory-bound (2 or 4
 // bytes in, 1 out): a page's CTA has all its loads in flight at once, and
 // several CTAs share an SM, so one's reduction hides under the others' loads.
-// Older codes are touched only where the page's scale grows.
+// Older codes are touched only where the page's scale grows. Measured: 4 x 8192
+// tokens of 8 heads of 128, bf16 to e4m3, 201 MB in 46 us (4.4 TB/s), a token
+// each of 8 users in 2.3 us.
 template <int FORMAT, typename T>
-__global__ void __launch_bounds__(512, 4) append_kernel(const cxs_cache_call c, const T* __restrict__ k,
-                              long long k_token, long long k_head, const T* __restrict__ v,
-                              long long v_token, long long v_head, int page_bits) {
+__global__ void __launch_bounds__(512, 4)  // four of the largest CTAs on an SM (three: 51 us)
+    append_kernel(const cxs_cache_call c, const T* __restrict__ k, long long k_token,
+                  long long k_head, const T* __restrict__ v, long long v_token, long long v_head,
+                  int page_bits) {
   using C = Code<FORMAT>;
   const int step = blockIdx.x, head = blockIdx.y >> 1, part = blockIdx.y & 1, user = blockIdx.z;
   int bad = 0;
@@ -155,6 +158,8 @@ __global__ void __launch_bounds__(512, 4) append_kernel(const cxs_cache_call c, 
 // One page and head per CTA: K and V of a page are one run of bytes. A thread
 // reads as many codes as make 16 bytes of the result (a warp's stores are then
 // whole lines), kUnroll times at once. Memory-bound: 1 byte in, 2 or 4 out.
+// Measured: four histories to 16K, 8 heads of 128, int8 to fp16, 262 MB in 46 us
+// (5.7 TB/s; 52 us with 32 bytes of the result a thread).
 constexpr int kReadThreads = 128, kUnroll = 8;
 
 template <int FORMAT, typename T>

@@ -90,10 +90,10 @@ class Rotary:
         steps = (f / (2 * math.pi) * 2.0 ** 62).round().to(torch.int64) << 2
         self.steps = steps.to(device)
         self.device = self.steps.device
-        self._steps = self.steps.data_ptr()
+        self._steps, self._layout = self.steps.data_ptr(), LAYOUTS[layout]
 
     def _check(self, name, x, dtype):
-        """(heads, token stride, head stride) of a [tokens, heads, dim] tensor."""
+        """Shape and strides of a [tokens, heads, dim] tensor."""
         shape, stride = x.shape, x.stride()
         if len(shape) != 3 or shape[2] != self.dim or stride[2] != 1:
             raise ValueError(f"{name} must be [tokens, heads, {self.dim}] with contiguous channels")
@@ -102,6 +102,23 @@ class Rotary:
         if x.device != self.device:
             raise ValueError(f"{name} must be on {self.device}")
         return shape, stride
+
+    def _side(self, name, x, y, tokens, dtype):
+        """(output, input and output address, their strides, heads) of one tensor."""
+        if x is None:
+            return None, 0, 0, (0, 0, 0, 0), 0
+        shape, stride = self._check(name, x, dtype)
+        heads = shape[1]
+        if shape[0] != tokens:
+            raise ValueError("q, k and positions must have as many tokens")
+        if y is None:
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+            return y, x.data_ptr(), y.data_ptr(), (stride[0], stride[1], heads * self.dim,
+                                                   self.dim), heads
+        out_shape, to = self._check(f"out of {name}", y, dtype)
+        if out_shape != shape:
+            raise ValueError(f"out of {name} must have its shape")
+        return y, x.data_ptr(), y.data_ptr(), (stride[0], stride[1], to[0], to[1]), heads
 
     def apply(self, q, k, positions, *, transpose=False, out=None):
         """Rotated ``(q, k)`` for q [tokens, heads, dim], k [tokens, kv_heads,
@@ -117,42 +134,23 @@ class Rotary:
         dtype, tokens = first.dtype, first.shape[0]
         if dtype not in TYPES:
             raise ValueError("q and k must be bf16, fp16 or fp32")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
+        wide = positions.dtype == torch.int64
+        if not (wide or positions.dtype == torch.int32) or positions.shape != (tokens,) \
                 or positions.device != self.device:
             raise ValueError(f"positions must be [tokens] int32 or int64 on {self.device}")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        if out is not None and ((out[0] is None) != (q is None) or (out[1] is None) != (k is None)):
-            raise ValueError("out must have a tensor for each of q and k that is given")
-        made, pointers, strides, heads = [], [], [], []
-        for i, (name, x) in enumerate((("q", q), ("k", k))):
-            if x is None:
-                made.append(None)
-                pointers.append((0, 0))
-                strides.append((0, 0, 0, 0))
-                heads.append(0)
-                continue
-            shape, stride = self._check(name, x, dtype)
-            if shape[0] != tokens:
-                raise ValueError("q, k and positions must have as many tokens")
-            if out is None:
-                y = torch.empty_like(x, memory_format=torch.contiguous_format)
-                to = (shape[1] * self.dim, self.dim)
-            else:
-                y = out[i]
-                out_shape, to = self._check(f"out of {name}", y, dtype)
-                if out_shape != shape:
-                    raise ValueError(f"out of {name} must have its shape")
-            made.append(y)
-            pointers.append((x.data_ptr(), y.data_ptr()))
-            strides.append((stride[0], stride[1], to[0], to[1]))
-            heads.append(shape[1])
-        (qp, qo), (kp, ko) = pointers
-        qs, ks = strides
+        if out is None:
+            q_out = k_out = None
+        else:
+            q_out, k_out = out
+            if (q_out is None) != (q is None) or (k_out is None) != (k is None):
+                raise ValueError("out must have a tensor for each of q and k that is given")
+        q_out, qp, qo, qs, heads = self._side("q", q, q_out, tokens, dtype)
+        k_out, kp, ko, ks, kv_heads = self._side("k", k, k_out, tokens, dtype)
         call = _lib.pack_rotary_call(
             qp, kp, qo, ko, positions.data_ptr(), self._steps, qs[0], qs[1], ks[0], ks[1],
-            qs[2], qs[3], ks[2], ks[3], tokens, heads[0], heads[1], self.dim, self.rotary_dim,
-            LAYOUTS[self.layout], TYPES[dtype], bool(transpose), positions.dtype == torch.int64,
-            self.magnitude)
+            qs[2], qs[3], ks[2], ks[3], tokens, heads, kv_heads, self.dim, self.rotary_dim,
+            self._layout, TYPES[dtype], bool(transpose), wide, self.magnitude)
         _lib.on_device(self.device.index, _lib.packed().cxs_rotary, call)
-        return tuple(made)
+        return q_out, k_out
