@@ -189,9 +189,12 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
   }
   __syncthreads();
   const long long total = prefix[z.users];
-  // Neighbouring shares lie in one CTA (of at least 6, for the join at its end).
+  // Neighbouring shares lie in one CTA, at least 3, for the join at its end.
+  // (Few tiles: shares of one, 3 a CTA, take 9.2 us for 100 keys and 12.9 for 4K,
+  // shares of two, 6 a CTA, 12.8 and 14.5; with more tiles than that, shares of
+  // two: 8 users of 8K, 17.5 us against 20.4.)
   const Shares shares(total, z);
-  const int per = min(max((shares.count + z.grid - 1) / z.grid, 6), K::kWarps);
+  const int per = min(max((shares.count + z.grid - 1) / z.grid, 3), K::kWarps);
   const int worker = (int)blockIdx.x * per + warp;
   const bool busy = warp < per && worker < shares.count;
   Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
@@ -756,7 +759,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
     cxs_cache_attend_call a = *call;
     const int left = c.users - user0;
     const Shape z{call->heads / c.kv_heads, user0, left < kSlice ? left : kSlice, left <= kSlice,
-                  grid, few ? grid * kDecodeWarps : grid, 2};
+                  grid, few ? grid * kDecodeWarps : grid, 2, few ? 3 * grid : 0};
     a.cache.table += user0 * c.table_stride;
     a.cache.lengths += user0;
     if (a.cache.offsets) a.cache.offsets += user0;

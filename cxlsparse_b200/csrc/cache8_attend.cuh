@@ -77,7 +77,8 @@ struct Shape {
   int last;       // the launch holds the last user
   int grid;       // CTAs
   int workers;    // most shares: warps or CTAs of the grid
-  int min_tiles;  // fewest tiles worth a share
+  int min_tiles;  // fewest tiles worth a share,
+  int few_tiles;  // but of no more tiles in all than this, each is one
 };
 
 // One user's positions. Visible to some row: [begin, end).
@@ -132,7 +133,8 @@ struct Shares {
   long long each;
   int more;
   __device__ __forceinline__ Shares(long long total, const Shape& z) {
-    const long long wanted = divide(total + z.min_tiles - 1, z.min_tiles);
+    const long long wanted =
+        total <= z.few_tiles ? total : divide(total + z.min_tiles - 1, z.min_tiles);
     count = wanted < z.workers ? (int)wanted : z.workers;
     each = count > 0 ? divide(total, count) : 0;
     more = (int)(total - each * count);
