@@ -59,6 +59,13 @@ __device__ __forceinline__ void load16(float (&x)[16], const T* from, bool wide)
   for (int e = 0; e < 16; ++e) x[e] = to_float(in[e]);
 }
 
+// Pages that a user's new tokens reach at most, wherever they start: a user has
+// no more rows than there are, whatever max_tokens says.
+int most_pages(const cxs_cache_call& c) {
+  const long long most = c.max_tokens < c.tokens ? c.max_tokens : c.tokens;
+  return (int)((most + c.page_size - 2) / c.page_size) + 1;
+}
+
 // One page, head and part (K or V) per CTA, 16 channels of a slot per thread:
 // the values are read once, kept in registers while the CTA finds the largest
 // magnitude, then written as codes, 16 bytes a thread. Memory-bound (2 or 4
@@ -83,8 +90,9 @@ __global__ void __launch_bounds__(512, 4)  // four of the largest CTAs on an SM 
   if (bad && step == 0 && blockIdx.y == 0 && threadIdx.x == 0)
     report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
   const int from = start > 0 ? (int)start : 0, to = min(length, most);
-  const int block = (from >> page_bits) + step, low = block << page_bits;  // position of slot 0
-  if (rows.count == 0 || from >= to || low >= to) return;
+  const int block = (from >> page_bits) + step;
+  if (rows.count == 0 || from >= to || block > (to - 1) >> page_bits) return;
+  const int low = block << page_bits;                  // position of slot 0
   const int fill = max(from - low, 0);                 // slots of older tokens
   const int stop = min(to - low, 1 << page_bits);
   const int chunk_bits = c.dim == 64 ? 2 : 3;
@@ -248,8 +256,7 @@ extern "C" int cxs_cache_append(const cxs_cache_call* call, const void* k, int64
   status = cxs_host::check_cache_pointers(call, "cache append");
   if (status != CXS_OK) return status;
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache append: null keys or values");
-  const int reach = (call->max_tokens + call->page_size - 2) / call->page_size + 1;
-  const dim3 grid(reach, call->kv_heads * 2, call->users);
+  const dim3 grid(most_pages(*call), call->kv_heads * 2, call->users);
   const int page_bits = call->page_size == 16 ? 4 : call->page_size == 32 ? 5 : 6;
   const int threads = call->page_size * call->dim / 16;
   CXS_CACHE_FORMAT(call->format, F,
@@ -270,8 +277,7 @@ extern "C" int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache read: null output");
   if ((uintptr_t)k % 16 || (uintptr_t)v % 16)
     return set_error(CXS_ERR_INVALID, "cache read: outputs must be 16-byte aligned");
-  const int reach = (call->max_tokens + call->page_size - 2) / call->page_size + 1;
-  const dim3 grid(reach, call->kv_heads, call->users);
+  const dim3 grid(most_pages(*call), call->kv_heads, call->users);
   const int page_bits = call->page_size == 16 ? 4 : call->page_size == 32 ? 5 : 6;
   CXS_CACHE_FORMAT(
       call->format, F,
