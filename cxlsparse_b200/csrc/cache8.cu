@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(512, 4)  // four of the largest CTAs on an SM 
 // reads as many codes as make 16 bytes of the result (a warp's stores are then
 // whole lines), kUnroll times at once. Memory-bound: 1 byte in, 2 or 4 out.
 // Measured: four histories to 16K, 8 heads of 128, int8 to fp16, 262 MB in 46 us
-// (5.7 TB/s; 52 us with 32 bytes of the result a thread).
+// (5.7 TB/s; 52 us with 32 bytes of the result a thread). Rows of no user are
+// cleared by the CTAs of a user beside them.
 constexpr int kReadThreads = 128, kUnroll = 8;
 
 template <int FORMAT, typename T>
@@ -182,6 +183,19 @@ __global__ void __launch_bounds__(kReadThreads)
   if (start < 0 || end > most) bad = 1;
   if (bad && step == 0 && head == 0 && threadIdx.x == 0)
     report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
+  constexpr int kCodes = 16 / sizeof(T), kCodeBits = kCodes == 8 ? 3 : 2;  // of a unit
+  const int unit_bits = (c.dim == 64 ? 6 : 7) - kCodeBits;               // units of a row
+  const auto clear = [&](const Gap& gap) {  // every gridDim.x-th row of it
+    for (long long row = gap.low + step; row < gap.high; row += gridDim.x)
+      for (int n = threadIdx.x; n < 2 << unit_bits; n += kReadThreads) {
+        const int channel = (n & ((1 << unit_bits) - 1)) << kCodeBits;
+        T* const to = (n >> unit_bits ? v : k) + (row * c.kv_heads + head) * c.dim + channel;
+        *(uint4*)to = make_uint4(0, 0, 0, 0);
+      }
+  };
+  if (user == 0) clear(row_gap(c, -1, c.users));
+  if (bad) clear(row_gap(c, user, c.users));
+  if (user == c.users - 1) clear(row_gap(c, c.users, c.users));
   // Pages are counted from the one (possibly before the first) that holds `start`.
   const int block = (start >> page_bits) + step;
   const long long low = (long long)block << page_bits;
@@ -200,8 +214,6 @@ __global__ void __launch_bounds__(kReadThreads)
   const float scale_k = page < 0 ? 0.f : c.scales[cell];
   const float scale_v = page < 0 ? 0.f : c.scales[cell + 1];
   const uint8_t* codes = (const uint8_t*)c.codes + cell * c.page_size * c.dim;
-  constexpr int kCodes = 16 / sizeof(T), kCodeBits = kCodes == 8 ? 3 : 2;  // of a unit
-  const int unit_bits = (c.dim == 64 ? 6 : 7) - kCodeBits;               // units of a row
   const int half = 1 << (page_bits + unit_bits);
   const long long row0 = rows.first + (low - start);
   for (int base = threadIdx.x; base < 2 * half; base += kReadThreads * kUnroll) {
@@ -271,12 +283,19 @@ extern "C" int cxs_cache_append(const cxs_cache_call* call, const void* k, int64
 extern "C" int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream) {
   int status = cxs_host::check_cache(call, "cache read");
   if (status != CXS_OK) return status;
-  if (call->users == 0 || call->tokens == 0 || call->max_tokens == 0) return CXS_OK;
-  status = cxs_host::check_cache_pointers(call, "cache read");
-  if (status != CXS_OK) return status;
+  if (call->tokens == 0) return CXS_OK;
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache read: null output");
   if ((uintptr_t)k % 16 || (uintptr_t)v % 16)
     return set_error(CXS_ERR_INVALID, "cache read: outputs must be 16-byte aligned");
+  if (call->users == 0) {  // rows of no user
+    const size_t bytes = (size_t)call->tokens * call->kv_heads * call->dim *
+                         (call->type == CXS_TYPE_F32 ? 4 : 2);
+    CXS_CUDA(cudaMemsetAsync(k, 0, bytes, (cudaStream_t)stream));
+    CXS_CUDA(cudaMemsetAsync(v, 0, bytes, (cudaStream_t)stream));
+    return CXS_OK;
+  }
+  status = cxs_host::check_cache_pointers(call, "cache read");
+  if (status != CXS_OK) return status;
   const dim3 grid(most_pages(*call), call->kv_heads, call->users);
   const int page_bits = call->page_size == 16 ? 4 : call->page_size == 32 ? 5 : 6;
   CXS_CACHE_FORMAT(

@@ -103,6 +103,29 @@ __device__ __forceinline__ Rows user_rows(const cxs_cache_call& c, int user, int
   return {static_cast<int>(lo), static_cast<int>(hi - lo)};
 }
 
+// Packed rows of no user: before the first user's (b = -1), past the last
+// user's (b = users), and those past what the call lets user b have.
+struct Gap {
+  long long low, high;
+};
+__device__ __forceinline__ Gap row_gap(const cxs_cache_call& c, int b, int users) {
+  if (!c.offsets) return {0, 0};
+  Gap g;
+  if (b < 0) {
+    g = {0, c.offsets[0]};
+  } else if (b == users) {
+    g = {c.offsets[users], c.tokens};
+  } else {
+    int bad = 0;
+    const Rows rows = user_rows(c, b, &bad);
+    if (!bad) return {0, 0};
+    g = {(long long)rows.first + rows.count, c.offsets[b + 1]};
+  }
+  if (g.low < 0) g.low = 0;
+  if (g.high > c.tokens) g.high = c.tokens;
+  return g;
+}
+
 }  // namespace cache8
 }  // namespace cxs
 

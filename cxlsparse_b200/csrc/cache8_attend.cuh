@@ -161,27 +161,12 @@ __device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int w
   const cxs_cache_call& c = a.cache;
   if (!c.offsets) return;
   for (int b = worker - 1; b <= z.users; b += workers) {
-    long long low, high;
-    if (b < 0) {
-      low = z.user0 == 0 ? 0 : 1;
-      high = z.user0 == 0 ? c.offsets[0] : 0;
-    } else if (b < z.users) {
-      int bad = 0;
-      const Rows rows = user_rows(c, b, &bad);
-      if (!bad) continue;
-      low = (long long)rows.first + rows.count;
-      high = c.offsets[b + 1];
-    } else {
-      low = z.last ? c.offsets[z.users] : 1;
-      high = z.last ? c.tokens : 0;
-    }
-    if (low < 0) low = 0;
-    if (high > c.tokens) high = c.tokens;
-    if (low >= high) continue;
-    for (long long i = low * a.heads * D + thread; i < high * a.heads * D; i += threads)
+    if ((b < 0 && z.user0 > 0) || (b == z.users && !z.last)) continue;  // (another launch's)
+    const Gap gap = row_gap(c, b, z.users);
+    for (long long i = gap.low * a.heads * D + thread; i < gap.high * a.heads * D; i += threads)
       ((T*)a.out)[i] = from_float<T>(0.f);
     if (a.lse)
-      for (long long i = low * a.heads + thread; i < high * a.heads; i += threads)
+      for (long long i = gap.low * a.heads + thread; i < gap.high * a.heads; i += threads)
         a.lse[i] = -kInf;
   }
 }

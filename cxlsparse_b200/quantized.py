@@ -147,7 +147,8 @@ class QuantizedCache:
 
     def read(self, table, starts, offsets, *, total, max_tokens=None, dtype=torch.bfloat16):
         """``(k, v)`` [total, kv_heads, dim] of consecutive tokens: row
-        offsets[b] + i is user b's token starts[b] + i."""
+        offsets[b] + i is user b's token starts[b] + i, and rows that no user
+        has are 0."""
         if dtype not in TYPES:
             raise ValueError("dtype must be bf16, fp16 or fp32")
         call = _lib.pack_cache_call(

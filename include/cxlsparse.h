@@ -539,8 +539,9 @@ int cxs_cache_append(const cxs_cache_call* call, const void* k, int64_t k_token_
 
 /* Values code * scale of consecutive tokens of each user, rounded once to
  * `type`, into k and v [tokens, kv_heads, dim] (contiguous, 16-byte aligned): row offsets[b] + i
- * is position lengths[b] + i (lengths holds the first position here). Tokens
- * of a page that is not there come back as 0, with the error bit. */
+ * is position lengths[b] + i (lengths holds the first position here). Every row
+ * is written: tokens of a page that is not there come back as 0, with the error
+ * bit, and so do (without it) rows that no user has. */
 int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream);
 
 /* Attention of the new tokens' queries [tokens, heads, dim] (bf16 or fp16,
