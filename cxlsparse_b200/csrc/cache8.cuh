@@ -83,7 +83,9 @@ __device__ __forceinline__ void report(int* error, int bits) {
 // A scale as the kernels use it: at least 2^-64, NaN kept.
 __device__ __forceinline__ float usable_scale(float s) { return s < kLeastScale ? kLeastScale : s; }
 
-// The packed rows of one user, cut to what the call says they can be.
+// The packed rows of one user. A user whose rows are not what the call says
+// they can be (outside the packed ones, backwards, more than max_tokens) has
+// none: rows taken from either end would stand for other positions.
 struct Rows {
   int first;  // first packed row
   int count;  // rows
@@ -96,15 +98,13 @@ __device__ __forceinline__ Rows user_rows(const cxs_cache_call& c, int user, int
   }
   if (lo < 0 || hi < lo || hi > c.tokens || hi - lo > c.max_tokens) {
     *bad = 1;
-    if (hi > c.tokens) hi = c.tokens;
-    if (lo < 0 || hi < lo) return {kInt32Max, 0};
-    if (hi - lo > c.max_tokens) hi = lo + c.max_tokens;
+    return {0, 0};
   }
   return {static_cast<int>(lo), static_cast<int>(hi - lo)};
 }
 
 // Packed rows of no user: before the first user's (b = -1), past the last
-// user's (b = users), and those past what the call lets user b have.
+// user's (b = users), and user b's where user_rows lets it have none.
 struct Gap {
   long long low, high;
 };
@@ -117,9 +117,9 @@ __device__ __forceinline__ Gap row_gap(const cxs_cache_call& c, int b, int users
     g = {c.offsets[users], c.tokens};
   } else {
     int bad = 0;
-    const Rows rows = user_rows(c, b, &bad);
+    user_rows(c, b, &bad);
     if (!bad) return {0, 0};
-    g = {(long long)rows.first + rows.count, c.offsets[b + 1]};
+    g = {c.offsets[b], c.offsets[b + 1]};
   }
   if (g.low < 0) g.low = 0;
   if (g.high > c.tokens) g.high = c.tokens;

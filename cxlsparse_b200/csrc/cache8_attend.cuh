@@ -152,8 +152,7 @@ struct alignas(16) Partial {  // the item that starts in a share and goes on pas
   int first, rows, row0, kv_head;  // the item's packed first row, user's rows, first row, head
 };
 
-// Rows of no user (before the first offset, past the last, or more than
-// max_tokens of one user): zero, and nothing in the sum. Shared out among the
+// Rows of no user (see row_gap): zero, and nothing in the sum. Shared out among the
 // workers, each of `threads` threads.
 template <typename T, int D>
 __device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int worker, int workers,

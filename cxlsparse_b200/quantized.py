@@ -133,7 +133,8 @@ class QuantizedCache:
     def append(self, k, v, table, lengths, offsets=None, *, max_tokens=None):
         """Quantise the new tokens' keys and values [tokens, kv_heads, dim]
         (bf16, fp16 or fp32) into their pages. ``max_tokens``: most new tokens
-        of one user, if known on the host (it bounds the launch)."""
+        of one user, if known on the host (it bounds the launch; a user with
+        more is left as it was, with an error that ``check`` raises)."""
         (shape, ks), (v_shape, vs) = self._rows("k", k), self._rows("v", v)
         if shape[1] != self.kv_heads or v_shape != shape:
             raise ValueError(f"k and v must both be [tokens, {self.kv_heads}, {self.dim}]")

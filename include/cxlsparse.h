@@ -493,7 +493,9 @@ int cxs_silu_mul(const void* gate_up, int32_t rows, int32_t ffn, void* out, void
  * What the device finds wrong is reported in `error` (bits, never cleared by
  * the calls) and skipped: CXS_DEVICE_ERR_BAD_BLOCK for a page id outside
  * [0, pages), CXS_DEVICE_ERR_BAD_LENGTH for lengths or offsets that reach
- * past the table, the packed rows or max_tokens.
+ * past the table, the packed rows or max_tokens. Positions past the table are
+ * left out one by one; a user whose rows lie outside the packed ones, or are
+ * more than max_tokens, has no rows in that call.
  */
 #define CXS_DEVICE_ERR_BAD_LENGTH 8
 

@@ -1,15 +1,18 @@
-"""Which packed rows a cache call takes: rows of no user."""
+"""Which packed rows a cache call takes: rows of no user, rows that do not fit."""
 
 import math
 
 import pytest
 import torch
 
-from cache8_case import paged
+from cache8_case import attend, paged
+from cxlsparse_b200 import CxsError
 from cxlsparse_b200.quantized import QuantizedCache
 
 pytestmark = pytest.mark.gpu
 
+# Offsets of three users in ten packed rows, max_tokens, the user that does not fit.
+MISFITS = [([0, 2, 8, 10], 4, 1), ([0, 2, 4, 14], None, 2), ([-2, 2, 4, 10], None, 0)]
 LENGTHS = [20, 31, 17]
 
 
@@ -17,8 +20,86 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+def raw(t):
+    return t.view(torch.uint8)
+
+
+def scaled(offsets, most, by):
+    lengths = [n * by for n in LENGTHS]
+    return [o * by for o in offsets], None if most is None else most * by, lengths
+
+
 def case(by, format, heads=2, dim=64, page=16):
     return paged([n * by for n in LENGTHS], kv_heads=heads, dim=dim, page_size=page, format=format)
+
+
+@pytest.mark.parametrize("by", [1, 40])
+@pytest.mark.parametrize("format", ["e4m3", "int8"])
+@pytest.mark.parametrize("offsets,most,misfit", MISFITS)
+def test_append_leaves_a_user_whose_rows_do_not_fit(cuda, offsets, most, misfit, format, by):
+    """Its pages stay as they were, with the error bit; the others are written."""
+    offsets, most, lengths = scaled(offsets, most, by)
+    codes, scales, table = case(by, format)
+    k, v = (torch.randn(10 * by, 2, 64, device="cuda") for _ in range(2))
+    cache = QuantizedCache(codes=codes.clone(), scales=scales.clone())
+    cache.append(k, v, table, ints(lengths), ints(offsets), max_tokens=most)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    alone = QuantizedCache(codes=codes.clone(), scales=scales.clone())
+    for b in range(3):
+        if b != misfit:
+            rows = slice(offsets[b], offsets[b + 1])
+            alone.append(k[rows], v[rows], table[b:b + 1], ints(lengths[b:b + 1]),
+                         ints([0, offsets[b + 1] - offsets[b]]))
+    alone.check()
+    assert torch.equal(raw(cache.codes), raw(alone.codes))
+    torch.testing.assert_close(cache.scales, alone.scales, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("by", [1, 40])
+@pytest.mark.parametrize("offsets,most,misfit", MISFITS)
+def test_attend_gives_nothing_to_rows_that_do_not_fit(cuda, offsets, most, misfit, by):
+    offsets, most, lengths = scaled(offsets, most, by)
+    codes, scales, table = case(by, "int8")
+    q = torch.randn(10 * by, 4, 64, device="cuda").half()
+    nothing = torch.full((10 * by, 4, 64), math.nan, device="cuda").half()
+    del nothing                                    # its memory is what the call finds
+    cache = QuantizedCache(codes=codes, scales=scales)
+    out, lse = cache.attend(q, table, ints(lengths), ints(offsets), max_tokens=most,
+                            return_lse=True)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    for b in range(3):
+        low, high = max(offsets[b], 0), min(offsets[b + 1], 10 * by)
+        if b == misfit:
+            assert (out[low:high] == 0).all() and (lse[low:high] == -math.inf).all()
+            continue
+        want, want_lse, tol, tol_lse = attend(q[low:high], codes, scales, table[b:b + 1],
+                                              lengths[b:b + 1], [high - low], causal=True,
+                                              window=0, scale=0.125)
+        assert ((out[low:high].double() - want).abs() <= tol).all()
+        assert ((lse[low:high].double() - want_lse).abs() <= tol_lse).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offsets,most,misfit", MISFITS)
+def test_read_gives_zeros_to_rows_that_do_not_fit(cuda, offsets, most, misfit, dtype):
+    codes, scales, table = case(1, "int8")
+    cache = QuantizedCache(codes=codes, scales=scales)
+    garbage = [torch.full((10, 2, 64), math.nan, dtype=dtype, device="cuda") for _ in range(2)]
+    del garbage                                    # its memory is what the call finds
+    k, v = cache.read(table, ints([0, 1, 2]), ints(offsets), total=10, max_tokens=most,
+                      dtype=dtype)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    for b in range(3):
+        rows = slice(max(offsets[b], 0), min(offsets[b + 1], 10))
+        if b == misfit:
+            assert (k[rows] == 0).all() and (v[rows] == 0).all()
+            continue
+        n = rows.stop - rows.start
+        want = cache.read(table[b:b + 1], ints([b]), ints([0, n]), total=n, dtype=dtype)
+        assert torch.equal(k[rows], want[0]) and torch.equal(v[rows], want[1])
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
