@@ -26,6 +26,8 @@ int check_cache(const cxs_cache_call* c, const char* what) {
     return set_error(CXS_ERR_CAPACITY, "%s: at most 65535 users and 32767 heads", what);
   if (!c->offsets && c->tokens != c->users)
     return set_error(CXS_ERR_INVALID, "%s: without offsets every user has one token", what);
+  if (!c->offsets && c->tokens > 0 && c->max_tokens < 1)
+    return set_error(CXS_ERR_INVALID, "%s: without offsets max_tokens must not be 0", what);
   return CXS_OK;
 }
 
@@ -264,7 +266,7 @@ extern "C" int cxs_cache_append(const cxs_cache_call* call, const void* k, int64
                                 int64_t v_head_stride, void* stream) {
   int status = cxs_host::check_cache(call, "cache append");
   if (status != CXS_OK) return status;
-  if (call->users == 0 || call->tokens == 0 || call->max_tokens == 0) return CXS_OK;
+  if (call->users == 0 || call->tokens == 0) return CXS_OK;
   status = cxs_host::check_cache_pointers(call, "cache append");
   if (status != CXS_OK) return status;
   if (!k || !v) return set_error(CXS_ERR_INVALID, "cache append: null keys or values");

@@ -133,3 +133,34 @@ def test_read_of_no_users_is_zero(cuda):
     none = torch.zeros(0, 1, dtype=torch.int32, device="cuda")
     k, v = cache.read(none, ints([]), ints([0]), total=40, dtype=torch.float32)
     assert (k == 0).all() and (v == 0).all()
+
+
+def test_rows_without_room_for_any_are_reported(cuda):
+    """max_tokens = 0 for a user that has rows: an error, not silence; no error
+    where no user has any (packed rows may be padding)."""
+    codes, scales, table = case(1, "int8")
+    k = torch.randn(3, 2, 64, device="cuda")
+    q = torch.randn(3, 4, 64, device="cuda").half()
+    cache = QuantizedCache(codes=codes.clone(), scales=scales.clone())
+    one = ints([0, 1, 2, 3])
+    cache.append(k, k, table, ints(LENGTHS), one, max_tokens=0)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    out, lse = cache.attend(q, table, ints(LENGTHS), one, max_tokens=0, return_lse=True)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    assert (out == 0).all() and (lse == -math.inf).all()
+    got, _ = cache.read(table, ints([0, 0, 0]), one, total=3, max_tokens=0)
+    with pytest.raises(CxsError, match="lengths or offsets"):
+        cache.check()
+    assert (got == 0).all()
+    # Without offsets every user has a row: refused before the launch.
+    for call in (lambda: cache.append(k, k, table, ints(LENGTHS), max_tokens=0),
+                 lambda: cache.attend(q, table, ints(LENGTHS), max_tokens=0),
+                 lambda: cache.read(table, ints([0, 0, 0]), None, total=3, max_tokens=0)):
+        with pytest.raises(ValueError, match="max_tokens"):
+            call()
+    cache.append(k, k, table, ints(LENGTHS), ints([0, 0, 0, 0]), max_tokens=0)
+    cache.read(table, ints([0, 0, 0]), ints([0, 0, 0, 0]), total=3, max_tokens=0)
+    cache.check()
+    assert torch.equal(raw(cache.codes), raw(codes))
