@@ -452,9 +452,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-        // M moves when a score passes it by 2^8: p stays below 2^8, well inside
-        // fp16's range, and most tiles leave O as it is.
-        const bool g0 = t0 > m0 + 8.f, g1 = t1 > m1 + 8.f;
+        const bool g0 = t0 > m0 + kLag, g1 = t1 > m1 + kLag;
         if (__any_sync(0xffffffffu, g0 || g1)) {
           const float c0 = !g0 ? 1.f : m0 == -kInf ? 0.f : ex2(m0 - t0);
           const float c1 = !g1 ? 1.f : m1 == -kInf ? 0.f : ex2(m1 - t1);
@@ -470,7 +468,7 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
             o[i][3] *= c1;
           }
         }
-        const float b0 = m0 == -kInf ? 0.f : m0, b1 = m1 == -kInf ? 0.f : m1;
+        const float b0 = m0 == -kInf ? 0.f : m0 - kHead, b1 = m1 == -kInf ? 0.f : m1 - kHead;
 #pragma unroll
         for (int u = 0; u < K::kGroups; ++u) {
           float(&ya)[4] = x[2 * u];
@@ -521,6 +519,8 @@ __global__ void __launch_bounds__(Decode<D>::kThreads, 1)
       l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
       l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      m0 -= kHead;  // what O and l are relative to
+      m1 -= kHead;
       const bool begins = item.tile == item.item_begin, whole = begins && item_hi == item.item_end;
       float* const part = scratch + (begins ? K::kRows * (D + 2) : 0);
       // Accumulator i, columns 2t, 2t + 1: channels (D / 8) column + i.

@@ -3,11 +3,17 @@
 // Mathematics. With codes c and scales s_k, s_v constant over a page, a score
 // in base-2 units is x = scale log2(e) s_k (q . c_k), and
 //   out = sum 2^x s_v c_v / sum 2^x = sum p c_v / sum p / s_v,
-//   p = 2^(x + log2 s_v - M),  M = running max of x + log2 s_v.
-// Folding s_v into the exponent keeps p <= 1 whatever the pages' scales, so p
-// is rounded to fp16 (11 bits) and multiplied with the codes themselves, which
-// fp16 holds exactly (e4m3 and integers to 128); the denominator divides each
-// page's sum of p by its s_v in fp32. Queries are scaled by a power of two per
+//   p = 2^(x + log2 s_v - M + 13),  M = running max of x + log2 s_v, moved when
+//   a score passes it by 2: p <= 2^15.
+// p is rounded to fp16 and multiplied with the codes themselves, which fp16
+// holds exactly (e4m3 and integers to 128); the denominator divides each page's
+// sum of p by its s_v in fp32. fp16 keeps 11 bits down to 2^-14: of every key
+// whose 2^x s_v is within 2^-27 of the row's largest, and of smaller ones what
+// is left above 2^-38 of it. The top of fp16's range is used because keys far
+// below the largest are not always negligible: its V may be 0 (a first token
+// that takes 0.999 of the softmax before 64K others, each 2^-26 of it; a page
+// whose scale a hidden outlier has set). With M at the largest p itself such
+// rows were off by a half. Queries are scaled by a power of two per
 // row so that fp16 holds them: exact for fp16 inputs, and for bf16 (8 bits of
 // mantissa) but for parts 2^-28 below the row's largest element, which lose
 // less than 2^-39 of it.
@@ -23,6 +29,12 @@ namespace cache8 {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = INFINITY;
+// M moves when a score passes it by kLag, and a score of M weighs 2^kHead:
+// most tiles leave O as it is, and fp16 has the room above and below. Measured
+// for lags of 8 / 4 / 2 / 1 (weights to 2^15 in each): prefill chunk 603 / 606 /
+// 609 / 611 us, suffixes and decode steps the same; beside a dominant key of
+// V = 0 over 64K tokens the error of out is 2e-2, 2.3e-3, below 1e-3, below 1e-3.
+constexpr float kLag = 2.f, kHead = 13.f;
 constexpr long long kSpinLimit = 1ll << 32;  // clock cycles before a wait gives up
 
 __device__ __forceinline__ float ex2(float x) {

@@ -4,8 +4,8 @@
 // An item is 256 query rows (two groups of 128) of one user and KV head; its
 // keys come in tiles of 128. One CTA per SM, 16 warps:
 //   warps 0-3, 4-7  softmax of group 0 and 1, one row a thread: reads S from
-//                   TMEM, writes p = 2^(x - M) as fp16 (for D = 128 over S),
-//                   rescales O when M grows by more than 2^8
+//                   TMEM, writes p as fp16 (for D = 128 over S), rescales O when
+//                   M moves
 //   warps 8-11      conversion of K and V codes to fp16 operand tiles in shared
 //                   memory, which both groups use
 //   warp 12         one thread issues every MMA: S = Q K^T (Q, K in shared
@@ -514,9 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
         warp_arrive(&bars->o_free[g], lane);
         if (live && complete) {
-          if (a.lse) a.lse[head] = some ? (m + log2f(l)) * kLn2 : -kInf;
+          if (a.lse) a.lse[head] = some ? (m - kHead + log2f(l)) * kLn2 : -kInf;
         } else if (live) {
-          part[kTileRows * D + 2 * (128 * g + r)] = m;
+          part[kTileRows * D + 2 * (128 * g + r)] = m - kHead;  // what O and l are relative to
           part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
         }
         if (!complete && started == ended.begin && g == 0 && r == 0) {
@@ -584,9 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           top = fmaxf(top, fmaf(fmaxf(t0, t1), factor_of(run.x), run.y));
         }
-        // M moves when a score passes it by 2^8: p stays below 2^8, well inside
-        // fp16's range, and most tiles leave O as it is.
-        const bool grows = top > m + 8.f;
+        const bool grows = top > m + kLag;
         // The last tile's P V is done: O may be rescaled and P overwritten.
         // (With P over S, S of this tile came after it.)
         if (L::kApart && mine_s > 0) {
@@ -608,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float base = m == -kInf ? 0.f : m;
+        const float base = m == -kInf ? 0.f : m - kHead;
 #pragma unroll
         for (int q = 0; q < kKeys / 32; ++q) {
           uint32_t p[16];
