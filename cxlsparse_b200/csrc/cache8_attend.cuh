@@ -182,6 +182,58 @@ __device__ void clear_rows(const cxs_cache_attend_call& a, const Shape& z, int w
   }
 }
 
+// A probability of 0 times a NaN would be NaN, so V of a tile with keys that
+// some row does not see has its NaN codes (e4m3 only) replaced by 0 before the
+// product. The rows that do see such a key get their NaN once the item's result
+// is written, from the codes themselves: few tiles can have any, and hardly one
+// does, so this stays out of the loops (in them it cost 4 %).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0x80 in each NaN byte's place
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t w, uint32_t* found) {
+  const uint32_t n = nan_codes(w);
+  *found |= n;
+  return w & ~(n | (n - (n >> 7)));
+}
+__device__ __forceinline__ uint4 without_nan(uint4 w, uint32_t* found) {
+  return make_uint4(without_nan(w.x, found), without_nan(w.y, found), without_nan(w.z, found),
+                    without_nan(w.w, found));
+}
+// The keys [lo, hi) that all rows of an item see; tiles beyond are hidden in part.
+__device__ __forceinline__ int2 seen_by_all(const cxs_cache_attend_call& a, const Shape& z,
+                                            const Span& s, int row0, int row1) {
+  return make_int2(row_range(a, s, row1 / z.group).x, row_range(a, s, row0 / z.group).y);
+}
+// Makes NaN the channels d .. d + count - 1 of a row's result (out, or its part
+// where that is not null) in which V of some key of [lo, hi), but for the keys
+// [skip.x, skip.y), is NaN. `codes` are the KV head's V of page 0, pages
+// page_bytes apart, `table` the user's.
+template <typename T, int D>
+__device__ __noinline__ void mark_nans(const uint8_t* codes, long long page_bytes, int pages,
+                                       const int* table, int page_size, int lo, int hi, int2 skip,
+                                       T* out, float* part, int d, int count) {
+  for (int w = d; w < d + count; w += 4) {
+    uint32_t nans = 0;
+    for (int t = lo; t < hi; ++t) {
+      if (t >= skip.x && t < skip.y) {
+        t = skip.y - 1;
+        continue;
+      }
+      const int page = table[t / page_size];
+      if (page < 0 || page >= pages) continue;
+      nans |= nan_codes(*reinterpret_cast<const uint32_t*>(codes + page * page_bytes +
+                                                           t % page_size * D + w));
+    }
+    for (int e = 0; e < 4; ++e) {
+      if (!(nans >> (8 * e + 7) & 1)) continue;
+      if (part)
+        part[w + e] = __uint_as_float(0x7fffffffu);
+      else
+        out[w + e] = from_float<T>(__uint_as_float(0x7fffffffu));
+    }
+  }
+}
+
 constexpr int kTileRows = 256;  // query rows of an item of the tile kernel
 
 // One launch of the tile kernel over z.users users (cache8_tile.cu).

@@ -58,7 +58,8 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-constexpr int kFirst = 1, kLast = 2, kTwo = 4;  // of its item here; rows for group 1
+// First and last of its item here; rows for group 1; keys that some row does not see.
+constexpr int kFirst = 1, kLast = 2, kTwo = 4, kHidden = 8;
 
 struct Tile {                // what the roles need of a tile of keys
   float4 runs[kRuns];        // of 16 keys: |scale| log2(e) s_k, log2 s_v, 1 / s_v, unused
@@ -97,6 +98,7 @@ struct Bars {
   uint64_t s_full[2], s_free[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
   uint64_t drain;
   int abort;
+  int nans;  // V had NaN codes where keys are hidden
   uint32_t tmem;
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
@@ -261,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cxs::mbar_init(&bars->drain, 1);
     bars->abort = 0;
+    bars->nans = 0;
     cxs::fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -519,6 +522,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           part[kTileRows * D + 2 * (128 * g + r)] = m - kHead;  // what O and l are relative to
           part[kTileRows * D + 2 * (128 * g + r) + 1] = l;
         }
+        // (Set before the last of these V was ready, or by an earlier item.)
+        if (FORMAT == CXS_FORMAT_E4M3 && *(volatile int*)&bars->nans && live) {
+          const int2 see = row_range(a, ended.span, row / z.group);
+          const int2 all = seen_by_all(a, z, ended.span, ended.tile_row * kTileRows,
+                                       min(ended.rows, (ended.tile_row + 1) * kTileRows) - 1);
+          const int key = (ended.first + (int)(started - ended.begin)) * kKeys;
+          const long long half_page = (long long)c.page_size * D;
+          // (Tiles that every row sees whole went as they are.)
+          mark_nans<T, D>((const uint8_t*)c.codes + (2 * ended.kv_head + 1) * half_page,
+                          2 * c.kv_heads * half_page, c.pages,
+                          c.table + ended.user * c.table_stride, c.page_size, max(see.x, key),
+                          min(see.y, key + (int)(until - started) * kKeys),
+                          make_int2((all.x + kKeys - 1) / kKeys * kKeys, all.y / kKeys * kKeys),
+                          (T*)a.out + head * D, complete ? nullptr : part + (128 * g + r) * D, 0, D);
+        }
         if (!complete && started == ended.begin && g == 0 && r == 0) {
           const int last = shares.of(ended.end - 1 + kItemCost * (ended.index + 1));
           mine.first = ended.span.first;
@@ -654,9 +672,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int to1 = panel * kPanel + tc::sw128_chunk(key, 2 * chunk + 1);
     // Codes -> fp16 in the operand's layout; keys without a token become 0 (a
     // probability of 0 times whatever their bytes hold could be NaN).
-    auto convert = [&](const uint8_t* raw, uint8_t* panels, const Tile& tile) {
+    // So do NaN codes of V in a tile that hides keys from some row.
+    auto convert = [&](const uint8_t* raw, uint8_t* panels, const Tile& tile, int part) {
       const unsigned missing = tile.missing;
       const int left = tile.left;
+      const bool hidden = FORMAT == CXS_FORMAT_E4M3 && part && tile.flags & kHidden;
       auto pass = [&](int at, uint4 w) {
         *reinterpret_cast<uint4*>(panels + to0 + at * 128) =
             make_uint4(half2_of<FORMAT>(w.x, 0), half2_of<FORMAT>(w.x, 1),
@@ -665,17 +685,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_uint4(half2_of<FORMAT>(w.z, 0), half2_of<FORMAT>(w.z, 1),
                        half2_of<FORMAT>(w.w, 0), half2_of<FORMAT>(w.w, 1));
       };
-      if (left >= kKeys && missing == 0) {
+      if (left >= kKeys && missing == 0 && !hidden) {
 #pragma unroll 4
         for (int at = 0; at < kKeys; at += kStep)
           pass(at, *reinterpret_cast<const uint4*>(raw + from + at * D));
       } else {
+        uint32_t found = 0;
 #pragma unroll 1
         for (int at = 0; at < kKeys; at += kStep) {
           const bool here = key + at < left && !(missing >> ((key + at) / 16) & 1);
-          pass(at, here ? *reinterpret_cast<const uint4*>(raw + from + at * D)
-                        : make_uint4(0, 0, 0, 0));
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (here) w = *reinterpret_cast<const uint4*>(raw + from + at * D);
+          if (hidden) w = without_nan(w, &found);
+          pass(at, w);
         }
+        if (found) *(volatile int*)&bars->nans = 1;
       }
     };
     const int n = (int)(hi - lo);
@@ -689,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!warp_wait(&bars->raw_full[raw][part], phase_of<L::kRawStages>(t), bars, c.error)) goto done;
         if (!warp_wait(part ? &bars->v_free[to] : &bars->k_free[to], use + 1, bars, c.error)) goto done;
         convert(smem + L::kRaw + (2 * raw + part) * L::kRawPart,
-                smem + (part ? L::kV : L::kK) + to * L::kPanels * kPanel, ring[t % kRing]);
+                smem + (part ? L::kV : L::kK) + to * L::kPanels * kPanel, ring[t % kRing], part);
         cxs::fence_proxy_async_shared();
         warp_arrive(part ? &bars->v_full[to] : &bars->k_full[to], lane);
         if (lane == 0) cxs::mbar_arrive(&bars->raw_free[raw][part]);
@@ -833,6 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return needed ? __ldg(c.table + item.user * c.table_stride + (at >> page_bits)) : -2;
       };
       int id = n > 0 ? look_up() : -2;
+      int2 all = make_int2(0, 0);  // keys that every row of the item sees
 #pragma unroll 1
       for (int t = 0; t < n; ++t) {
         if (id != -2 && (id < 0 || id >= c.pages)) report(c.error, CXS_DEVICE_ERR_BAD_BLOCK);
@@ -850,8 +875,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const unsigned missing = __ballot_sync(0xffffffffu, lane < kRuns && !here);
         const bool first = tile == item.begin || t == 0, last = tile + 1 == item.end || t + 1 == n;
-        const int flags = (first ? kFirst : 0) | (last ? kLast : 0) | (active(item, 1) ? kTwo : 0);
-        const int left = item.span.length - (item.first + (int)(tile - item.begin)) * kKeys;
+        const int key0 = (item.first + (int)(tile - item.begin)) * kKeys;
+        const int left = item.span.length - key0;
+        if (FORMAT == CXS_FORMAT_E4M3 && first)
+          all = seen_by_all(a, z, item.span, item.tile_row * kTileRows,
+                            min(item.rows, (item.tile_row + 1) * kTileRows) - 1);
+        const bool hidden = FORMAT == CXS_FORMAT_E4M3 &&
+                            (key0 < all.x || key0 + min(left, kKeys) > all.y);
+        const int flags = (first ? kFirst : 0) | (last ? kLast : 0) | (active(item, 1) ? kTwo : 0) |
+                          (hidden ? kHidden : 0);
         const uint8_t* from = (const uint8_t*)c.codes + cell * page_bytes;
         ++tile;
         if (t + 1 < n) {
