@@ -22,7 +22,7 @@ def frequencies(rotary_dim, theta=10000.0, scaling=None):
     factor on the rotated values. ``scaling``:
 
     - None: theta ** (-2 i / rotary_dim);
-    - ``dict(type="linear", factor=s)``: positions divided by s;
+    - ``dict(type="linear", factor=s)``: positions divided by s (any s > 0);
     - ``dict(type="ntk", factor=s)``: theta raised so that the slowest pair is
       stretched s times and the fastest is kept;
     - ``dict(type="yarn", factor=s, original=n, fast=32, slow=1)`` (Peng et al.
@@ -85,9 +85,13 @@ class Rotary:
             raise ValueError(f"unknown rotary layout {layout!r}")
         self.dim, self.rotary_dim, self.layout = dim, rotary_dim, layout
         f, self.magnitude = frequencies(rotary_dim, theta, scaling)
-        # Fractions of 2^62 doubled twice: a full turn per position stays in
-        # range, and the product with a position wraps modulo one turn.
-        steps = (f / (2 * math.pi) * 2.0 ** 62).round().to(torch.int64) << 2
+        if not (f.isfinite().all() and math.isfinite(self.magnitude)):
+            raise ValueError("the scaling's frequencies or magnitude are not finite")
+        # Whole turns per position do not matter: at most half a turn is left,
+        # whose 2^62-fold fits 64 bits. Doubled twice it wraps modulo one turn,
+        # as its product with a position does.
+        turns = f / (2 * math.pi)
+        steps = ((turns - turns.round()) * 2.0 ** 62).round().to(torch.int64) << 2
         self.steps = steps.to(device)
         self.device = self.steps.device
         self._steps, self._layout = self.steps.data_ptr(), LAYOUTS[layout]
