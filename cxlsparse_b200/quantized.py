@@ -17,6 +17,7 @@ reference.
 """
 
 import math
+import threading
 
 import torch
 
@@ -63,18 +64,26 @@ class QuantizedCache:
         self.format = CODE_TYPES[codes.dtype]
         self.device = codes.device
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._first = torch.zeros(1, dtype=torch.int64, device=self.device)
+        self._lock = threading.Lock()
         self._codes, self._scales, self._error = (
             t.data_ptr() for t in (codes, scales, self.error))
         self._workspace = {}
 
     # -- checks ------------------------------------------------------------
     def check(self):
-        """Wait for the device and raise if a call met a page or length out of
-        range since the last check (such tokens are skipped, never followed),
-        or gave up a wait."""
-        bits = int(self.error.item())
+        """Wait for the device, the calls on all its streams, and raise if one
+        met a page or length out of range since the last check (such tokens are
+        skipped, never followed), or gave up a wait."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        with self._lock:
+            bits = int(self.error.item())
+            if bits:
+                # Taken off by an atomic addition: bits that a call of another
+                # thread sets meanwhile stay for the next check.
+                self.error.index_add_(0, self._first, torch.full_like(self.error, -bits))
         if bits:
-            self.error.zero_()
             what = [text for bit, text in (
                 (_lib.DEVICE_ERR_BAD_BLOCK, "a page id outside the cache"),
                 (_lib.DEVICE_ERR_BAD_LENGTH, "lengths or offsets out of range"),
