@@ -68,6 +68,26 @@ def frequencies(rotary_dim, theta=10000.0, scaling=None):
     return f, 1.0
 
 
+class _Turn(torch.autograd.Function):
+    """``Rotary.apply`` under autograd: the gradient is the transposed rotation
+    of the outputs' gradients (of those that there are)."""
+
+    @staticmethod
+    def forward(ctx, rotary, positions, transpose, q, k):
+        ctx.rotary, ctx.transpose = rotary, transpose
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        return rotary.apply(q, k, positions, transpose=transpose)
+
+    @staticmethod
+    def backward(ctx, q, k):
+        # (Gradients of sums are broadcast along the channels.)
+        q, k = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (q, k))
+        if q is not None or k is not None:
+            q, k = ctx.rotary.apply(q, k, *ctx.saved_tensors, transpose=not ctx.transpose)
+        return None, None, None, q, k
+
+
 class Rotary:
     """The rotation of one head geometry: ``apply(q, k, positions)``.
 
@@ -129,9 +149,10 @@ class Rotary:
         dim] (either may be None) and positions [tokens] int32 or int64, in one
         launch on the current stream. ``transpose`` turns the other way: given
         the gradients of the outputs it returns those of the inputs (and, for
-        magnitude 1, undoes the rotation). ``out=(q_out, k_out)`` receives the
-        result; each may be its input itself, and must not overlap an input in
-        another way."""
+        magnitude 1, undoes the rotation); autograd does so by itself.
+        ``out=(q_out, k_out)`` receives the result; each may be its input
+        itself, and must not overlap an input in another way. ``out`` has no
+        gradient: it is refused for tensors that need one."""
         first = q if q is not None else k
         if first is None:
             raise ValueError("q or k is needed")
@@ -144,6 +165,11 @@ class Rotary:
             raise ValueError(f"positions must be [tokens] int32 or int64 on {self.device}")
         if not positions.is_contiguous():
             positions = positions.contiguous()
+        if torch.is_grad_enabled() and any(
+                t is not None and t.requires_grad for t in (q, k, *(out or ()))):
+            if out is not None:
+                raise ValueError("out cannot receive a result that needs a gradient")
+            return _Turn.apply(self, positions, bool(transpose), q, k)
         if out is None:
             q_out = k_out = None
         else:
@@ -157,4 +183,6 @@ class Rotary:
             qs[2], qs[3], ks[2], ks[3], tokens, heads, kv_heads, self.dim, self.rotary_dim,
             self._layout, TYPES[dtype], bool(transpose), wide, self.magnitude)
         _lib.on_device(self.device.index, _lib.packed().cxs_rotary, call)
+        if out is not None:
+            torch.autograd.graph.increment_version([t for t in out if t is not None])
         return q_out, k_out
