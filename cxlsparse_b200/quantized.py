@@ -12,8 +12,8 @@ channel, in pages with a scale for each page, KV head and part (K or V):
 The three take the same description of a step: ``table [users, width]`` int32
 page ids (shared by all layers of a model), ``lengths [users]`` int32 tokens
 with the new ones counted, and ``offsets [users + 1]`` int32, the packed rows
-of each user (None: one new token for every user). No counterpart in the
-reference.
+of each user (None: one new token for every user). No gradient passes through
+them. No counterpart in the reference.
 """
 
 import math
@@ -145,6 +145,8 @@ class QuantizedCache:
         of one user, if known on the host (it bounds the launch; a user with
         more is left as it was, with an error that ``check`` raises)."""
         (shape, ks), (v_shape, vs) = self._rows("k", k), self._rows("v", v)
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            raise ValueError("the cache has no gradient: append detached k and v")
         if shape[1] != self.kv_heads or v_shape != shape:
             raise ValueError(f"k and v must both be [tokens, {self.kv_heads}, {self.dim}]")
         dtype = k.dtype
@@ -178,6 +180,8 @@ class QuantizedCache:
         [tokens, heads, dim], with ``return_lse`` also the softmax's log-sum
         [tokens, heads] fp32 (for joining with attention over other keys)."""
         shape, stride = self._rows("q", q)
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the cache has no gradient: attend with a detached q")
         dtype = q.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("q must be bf16 or fp16")
