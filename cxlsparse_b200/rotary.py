@@ -165,15 +165,16 @@ class Rotary:
             raise ValueError(f"positions must be [tokens] int32 or int64 on {self.device}")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        if torch.is_grad_enabled() and any(
-                t is not None and t.requires_grad for t in (q, k, *(out or ()))):
-            if out is not None:
-                raise ValueError("out cannot receive a result that needs a gradient")
-            return _Turn.apply(self, positions, bool(transpose), q, k)
+        needs = first.requires_grad or (k is not None and k.requires_grad)
         if out is None:
+            if needs and torch.is_grad_enabled():
+                return _Turn.apply(self, positions, bool(transpose), q, k)
             q_out = k_out = None
         else:
             q_out, k_out = out
+            if torch.is_grad_enabled() and (needs or any(
+                    t is not None and t.requires_grad for t in out)):
+                raise ValueError("out cannot receive a result that needs a gradient")
             if (q_out is None) != (q is None) or (k_out is None) != (k is None):
                 raise ValueError("out must have a tensor for each of q and k that is given")
         q_out, qp, qo, qs, heads = self._side("q", q, q_out, tokens, dtype)
