@@ -92,9 +92,10 @@ __global__ void __launch_bounds__(512, 4)  // four of the largest CTAs on an SM 
   if (bad && step == 0 && blockIdx.y == 0 && threadIdx.x == 0)
     report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
   const int from = start > 0 ? (int)start : 0, to = min(length, most);
+  // Position of slot 0; unsigned, as a page past the last may lie past 2^31.
   const int block = (from >> page_bits) + step;
-  if (rows.count == 0 || from >= to || block > (to - 1) >> page_bits) return;
-  const int low = block << page_bits;                  // position of slot 0
+  if (rows.count == 0 || from >= to || (unsigned)block << page_bits >= (unsigned)to) return;
+  const int low = block << page_bits;
   const int fill = max(from - low, 0);                 // slots of older tokens
   const int stop = min(to - low, 1 << page_bits);
   const int chunk_bits = c.dim == 64 ? 2 : 3;

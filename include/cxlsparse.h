@@ -554,8 +554,8 @@ int cxs_cache_read(const cxs_cache_call* call, void* k, void* v, void* stream);
  * The row at position p sees positions <= p (causal) or < lengths[b], and with
  * window > 0 only positions > p - window. A row that sees nothing gets out = 0
  * and lse = -infinity. Bytes of slots past lengths[b], and pages not in the
- * table's used part, are never part of a result, whatever they hold, and a key
- * or value that is NaN reaches the rows that see its token and no other. Scales
+ * table's used part, are never part of a result, whatever they hold, and a code
+ * that is NaN reaches the rows that see its token and no other. Scales
  * below 2^-64 count as 2^-64. Scores, sums and out are accumulated in fp32; a
  * key's weight (its probability times its page's V scale) is rounded to 11 bits,
  * to fewer where it is below 2^-27 of the row's largest, to nothing below 2^-38. */
