@@ -39,9 +39,12 @@ __device__ __forceinline__ float2 exp2_pair(float x, float y, float f, float shi
 // lane's V bytes of four keys pair up by byte permutes. No transposition
 // passes through shared memory.
 // Measured: 64 users of 0 to 16K tokens, 32 / 2 heads of 64, 137 MB of codes in
-// 43 us (3.2 TB/s); 32 users of 8K, 32 / 8 heads of 128, 537 MB in 131 us
-// with the join (4.1 TB/s). Bound by instruction issue: converting codes, and an exponential
-// and about three more instructions for each of a key's 16 scores.
+// 43 us (3.2 TB/s); 32 users of 8K, 32 / 8 heads of 128, 537 MB in 135 us
+// with the join (4.0 TB/s). No unit is full (40 % of the issue slots, ALU 36 %,
+// tensor core 22 %): converting codes, and an exponential and about three more
+// instructions for each of a key's 16 scores, follow one another in a warp, and
+// three warps a scheduler do not cover that. At D = 128 registers are short too
+// (254 bytes spilled a thread).
 constexpr int kDecodeWarps = 12;
 
 template <int D>
@@ -723,8 +726,11 @@ constexpr int kMostCtas = 148;
 // Most rows of a user and KV head for which the mma.sync kernel runs: it takes
 // 16 rows at a time and reads the keys again for the next 16, the tcgen05
 // kernel takes up to 256 at about the same cost. Measured (us, mma.sync /
-// tcgen05), D = 64, 8 users of 8K tokens, 2 KV heads: 64 rows 27 / 31, 128 rows
-// 38 / 32; D = 128, 8 users of 8K, 8 KV heads: 32 rows 86 / 92, 64 rows 138 / 95.
+// tcgen05, e4m3; 1 user of 16K tokens, 8 of 8K, 64 of 4K):
+//   D = 64, 2 KV heads    64 rows   23 / 41    32 / 33    65 / 80
+//                        128 rows   28 / 42    43 / 35   110 / 82
+//   D = 128, 8 KV heads   32 rows   47 / 43    89 / 97   260 / 334
+//                         64 rows   60 / 45   142 / 100  480 / 340
 bool few_rows(const cxs_cache_attend_call& a) {
   return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= (a.cache.dim == 64 ? 64 : 32);
 }

@@ -13,8 +13,10 @@
 // below the largest are not always negligible: its V may be 0 (a first token
 // that takes 0.999 of the softmax before 64K others, each 2^-26 of it; a page
 // whose scale a hidden outlier has set). With M at the largest p itself such
-// rows were off by a half. Queries are scaled by a power of two per
-// row so that fp16 holds them: exact for fp16 inputs, and for bf16 (8 bits of
+// rows were off by a half. 2^ and log2 are
+// the approximate instructions (2^-22 of the result, 2 units of the last place):
+// far below the rounding of p. Queries are scaled by a power of two per row so
+// that fp16 holds them: exact for fp16 inputs, and for bf16 (8 bits of
 // mantissa) but for parts 2^-28 below the row's largest element, which lose
 // less than 2^-39 of it.
 #pragma once

@@ -21,11 +21,12 @@
 // Waits are bounded: a wait that runs out sets the error word and an abort
 // flag that ends every role.
 // Measured: 256 tokens of 32 query and 2 KV heads of 64 over 16K keys (e4m3) in
-// 79 us, 440 TFLOP/s; 3 users' prefill chunks, 32 / 8 heads of 128 (int8), in
-// 588 us, 805 TFLOP/s of the 1650 that cuBLAS reaches in bf16. Bound by the
-// softmax (one exponential a score, at 16 a clock and SM, about half of the
-// time in use) and, at 128 channels, by S and P V that wait for it: TMEM holds
-// only one S of each group there.
+// 79 us, 438 TFLOP/s; 3 users' prefill chunks, 32 / 8 heads of 128 (int8), in
+// 595 us, 796 TFLOP/s of the 1650 that cuBLAS reaches in bf16. No unit is full
+// (special functions 41 and 38 % of the time, tensor core 20 and 38 %): a row's
+// softmax is a chain (read S, maximum, exponentials) that two warps a scheduler
+// do not cover, S and P V wait for it at 128 channels, where TMEM holds only one
+// S of each group, and registers are short (188 to 396 bytes spilled a thread).
 #include "cache8_attend.cuh"
 #include "tile_tc.cuh"
 
