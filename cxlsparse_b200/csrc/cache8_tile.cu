@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           make_int2((all.x + kKeys - 1) / kKeys * kKeys, all.y / kKeys * kKeys),
                           (T*)a.out + head * D, complete ? nullptr : part + (128 * g + r) * D, 0, D);
         }
+        __syncwarp();
         if (!complete && started == ended.begin && g == 0 && r == 0) {
           const int last = shares.of(ended.end - 1 + kItemCost * (ended.index + 1));
           mine.first = ended.span.first;
