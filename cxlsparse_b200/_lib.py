@@ -19,6 +19,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_CAPACITY, ERR_REGISTRATION, ERR_UNSUPPORTED = ran
 # Device error word bits.
 DEVICE_ERR_READY_TIMEOUT, DEVICE_ERR_COPY_TIMEOUT, DEVICE_ERR_BAD_BLOCK = 1, 2, 4
 DEVICE_ERR_BAD_LENGTH = 8
+DEVICE_ERR_NO_PAGES, DEVICE_ERR_BAD_SEQUENCE, DEVICE_ERR_SHARED_PAGE = 16, 32, 64
 ORDER_PHYSICAL, ORDER_DEPTH, ORDER_DEPTH_SHARED = 0, 1, 2
 READ_ORDERS = {
     "physical": ORDER_PHYSICAL,
@@ -119,6 +120,13 @@ class RotaryCall(ctypes.Structure):
                 "transpose", "wide_positions")] + [("magnitude", ctypes.c_float)]
 
 
+class PagesCall(ctypes.Structure):
+    _fields_ = [(name, c_vp) for name in (
+        "layer_buffers", "table", "lengths", "references", "lowest", "error", "workspace")] + [
+        ("workspace_bytes", c_i64)] + [(name, c_i32) for name in (
+            "layers", "pages", "kv_heads", "dim", "page_size", "sequences", "width")]
+
+
 def _packer(cls):
     """Packs the fields of a ctypes structure (nested ones flattened, null
     pointers as 0) into bytes with the C layout, at a fraction of the cost of
@@ -134,8 +142,8 @@ def _packer(cls):
     return packer.pack
 
 
-pack_cache_call, pack_cache_attend_call, pack_rotary_call = map(
-    _packer, (CacheCall, CacheAttendCall, RotaryCall))
+pack_cache_call, pack_cache_attend_call, pack_rotary_call, pack_pages_call = map(
+    _packer, (CacheCall, CacheAttendCall, RotaryCall, PagesCall))
 
 _lib = None
 _packed = None
@@ -214,6 +222,13 @@ def lib():
             "cxs_cache_attend_workspace": (c_i32, [ctypes.POINTER(CacheAttendCall),
                                                    ctypes.POINTER(c_i64)]),
             "cxs_rotary": (c_i32, [ctypes.POINTER(RotaryCall), c_vp]),
+            "cxs_pages_workspace": (c_i32, [ctypes.POINTER(PagesCall), ctypes.POINTER(c_i64)]),
+            "cxs_pages_extend": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_vp]),
+            "cxs_pages_fork": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_vp, c_i32, c_vp]),
+            "cxs_pages_free": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_i32, c_vp]),
+            "cxs_pages_adopt": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_i64, c_i32, c_vp,
+                                        c_vp]),
+            "cxs_pages_compact": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_vp]),
         }
         for name, (restype, argtypes) in sigs.items():
             fn = getattr(handle, name)
@@ -233,7 +248,13 @@ class _Packed:
                 ("cxs_cache_read", [c_vp, c_vp, c_vp, c_vp]),
                 ("cxs_cache_attend", [c_vp, c_vp]),
                 ("cxs_cache_attend_workspace", [c_vp, ctypes.POINTER(c_i64)]),
-                ("cxs_rotary", [c_vp, c_vp])):
+                ("cxs_rotary", [c_vp, c_vp]),
+                ("cxs_pages_workspace", [c_vp, ctypes.POINTER(c_i64)]),
+                ("cxs_pages_extend", [c_vp, c_vp, c_vp]),
+                ("cxs_pages_fork", [c_vp, c_vp, c_vp, c_i32, c_vp]),
+                ("cxs_pages_free", [c_vp, c_vp, c_i32, c_vp]),
+                ("cxs_pages_adopt", [c_vp, c_vp, c_i64, c_i32, c_vp, c_vp]),
+                ("cxs_pages_compact", [c_vp, c_vp, c_vp])):
             fn = handle[name]  # a function object of its own
             fn.restype, fn.argtypes = c_i32, argtypes
             setattr(self, name, fn)
@@ -291,4 +312,6 @@ def exported_symbols():
             "cxs_device_alloc",
             "cxs_device_free", "cxs_ipc_get_handle", "cxs_ipc_open_handle", "cxs_ipc_close",
             "cxs_exchange_barrier", "cxs_cache_append", "cxs_cache_read", "cxs_cache_attend",
-            "cxs_cache_attend_workspace", "cxs_rotary")
+            "cxs_cache_attend_workspace", "cxs_rotary", "cxs_pages_workspace",
+            "cxs_pages_extend", "cxs_pages_fork", "cxs_pages_free", "cxs_pages_adopt",
+            "cxs_pages_compact")

@@ -604,6 +604,58 @@ typedef struct cxs_rotary_call {
 } cxs_rotary_call;
 int cxs_rotary(const cxs_rotary_call* call, void* stream);
 
+/* -------------------------------------- sequences over the cache's pages ---
+ * Page tables kept on the device: extending, forking, freeing and compacting
+ * sequences without the host, so that a decode step with all of it can be
+ * captured. State: table [sequences, width] (page ids, -1 where there is none),
+ * lengths [sequences], references [pages] (table entries that name the page; 0:
+ * free) and lowest [1] (no page below it is free; 0 will do to begin with).
+ * Page ids are those of every layer. Pages are handed out lowest id first, in
+ * the order of the sequences or children.
+ *
+ * What the device finds wrong is reported in `error` (bits, never cleared by
+ * the calls): CXS_DEVICE_ERR_NO_PAGES where too few pages are free,
+ * _BAD_SEQUENCE for an id out of range, a child that holds tokens or is there
+ * twice, _SHARED_PAGE for tokens that would go on in a page with other
+ * references, _BAD_LENGTH for lengths outside the row, _BAD_BLOCK for a page
+ * id outside the pool. extend and fork then change nothing at all; free and
+ * adopt leave out what is wrong. Calls on one state must follow one another. */
+#define CXS_DEVICE_ERR_NO_PAGES 16
+#define CXS_DEVICE_ERR_BAD_SEQUENCE 32
+#define CXS_DEVICE_ERR_SHARED_PAGE 64
+
+typedef struct cxs_pages_call {
+  void* const* layer_buffers; /* device array [layers][2]: a layer's codes (16-byte aligned)
+                                 and scales, as in cxs_cache_call */
+  int32_t* table;
+  int32_t* lengths;
+  int32_t* references;
+  int32_t* lowest;
+  int32_t* error;             /* or NULL */
+  void* workspace;            /* cxs_pages_workspace bytes; nothing is kept in it */
+  int64_t workspace_bytes;
+  int32_t layers, pages, kv_heads, dim, page_size, sequences, width;
+} cxs_pages_call;
+int cxs_pages_workspace(const cxs_pages_call* call, int64_t* bytes);
+/* Room for counts[b] more tokens of every sequence (NULL: one each): lengths
+ * grow by them, rows get the pages they need. */
+int cxs_pages_extend(const cxs_pages_call* call, const int32_t* counts, void* stream);
+/* children[i], empty before, becomes a copy of parents[i]: the parent's full
+ * pages are shared (references + 1), of a partly filled last page the child gets
+ * a fresh page with the filled slots and the scales, in every layer. */
+int cxs_pages_fork(const cxs_pages_call* call, const int32_t* parents, const int32_t* children,
+                   int32_t count, void* stream);
+/* The sequences hold nothing any more; pages that no other names are free. */
+int cxs_pages_free(const cxs_pages_call* call, const int32_t* sequences, int32_t count,
+                   void* stream);
+/* Takes over a table [sequences, width] (rows table_stride apart) and lengths
+ * that the caller kept, and counts the references. */
+int cxs_pages_adopt(const cxs_pages_call* call, const int32_t* table, int64_t table_stride,
+                    int32_t width, const int32_t* lengths, void* stream);
+/* Moves pages, in every layer, until the n pages in use are ids 0 .. n - 1: the
+ * k-th used page from n on goes to the k-th free one below n. live (or NULL): n. */
+int cxs_pages_compact(const cxs_pages_call* call, int32_t* live, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
