@@ -127,6 +127,15 @@ class PagesCall(ctypes.Structure):
             "layers", "pages", "kv_heads", "dim", "page_size", "sequences", "width")]
 
 
+class SampleCall(ctypes.Structure):
+    _fields_ = [(name, c_vp) for name in (
+        "logits", "uniforms", "tokens", "logprobs", "temperature", "top_k", "top_p", "min_p")] + [
+        ("row_stride", c_i64)] + [(name, c_i32) for name in (
+            "rows", "vocab", "draws", "type", "wide_uniforms")] + [
+        ("temperature_all", ctypes.c_float), ("top_k_all", c_i32),
+        ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float)]
+
+
 def _packer(cls):
     """Packs the fields of a ctypes structure (nested ones flattened, null
     pointers as 0) into bytes with the C layout, at a fraction of the cost of
@@ -142,8 +151,8 @@ def _packer(cls):
     return packer.pack
 
 
-pack_cache_call, pack_cache_attend_call, pack_rotary_call, pack_pages_call = map(
-    _packer, (CacheCall, CacheAttendCall, RotaryCall, PagesCall))
+pack_cache_call, pack_cache_attend_call, pack_rotary_call, pack_pages_call, pack_sample_call = map(
+    _packer, (CacheCall, CacheAttendCall, RotaryCall, PagesCall, SampleCall))
 
 _lib = None
 _packed = None
@@ -229,6 +238,7 @@ def lib():
             "cxs_pages_adopt": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_i64, c_i32, c_vp,
                                         c_vp]),
             "cxs_pages_compact": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_vp]),
+            "cxs_sample": (c_i32, [ctypes.POINTER(SampleCall), c_vp]),
         }
         for name, (restype, argtypes) in sigs.items():
             fn = getattr(handle, name)
@@ -254,7 +264,8 @@ class _Packed:
                 ("cxs_pages_fork", [c_vp, c_vp, c_vp, c_i32, c_vp]),
                 ("cxs_pages_free", [c_vp, c_vp, c_i32, c_vp]),
                 ("cxs_pages_adopt", [c_vp, c_vp, c_i64, c_i32, c_vp, c_vp]),
-                ("cxs_pages_compact", [c_vp, c_vp, c_vp])):
+                ("cxs_pages_compact", [c_vp, c_vp, c_vp]),
+                ("cxs_sample", [c_vp, c_vp])):
             fn = handle[name]  # a function object of its own
             fn.restype, fn.argtypes = c_i32, argtypes
             setattr(self, name, fn)
@@ -314,4 +325,4 @@ def exported_symbols():
             "cxs_exchange_barrier", "cxs_cache_append", "cxs_cache_read", "cxs_cache_attend",
             "cxs_cache_attend_workspace", "cxs_rotary", "cxs_pages_workspace",
             "cxs_pages_extend", "cxs_pages_fork", "cxs_pages_free", "cxs_pages_adopt",
-            "cxs_pages_compact")
+            "cxs_pages_compact", "cxs_sample")

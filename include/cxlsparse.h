@@ -656,6 +656,42 @@ int cxs_pages_adopt(const cxs_pages_call* call, const int32_t* table, int64_t ta
  * k-th used page from n on goes to the k-th free one below n. live (or NULL): n. */
 int cxs_pages_compact(const cxs_pages_call* call, int32_t* live, void* stream);
 
+/* ------------------------------------------------------------- sampling ---
+ * Tokens drawn from logits [rows, vocab] (values contiguous, rows row_stride
+ * apart) with uniforms [rows, draws] in [0, 1) (contiguous) given by the caller.
+ * Tokens are ordered by logit, larger first, equal ones by index. With M the
+ * row's largest logit and w_i = exp((x_i - M) / temperature), kept are the first
+ * tokens of that order: at most top_k (0: all), with w_i >= min_p, and of these
+ * the ones before which less than top_p of their mass lies (the first always).
+ * The token is the first index whose kept mass so far is above u times all kept
+ * mass; temperature 0 and top_k 1 give the first token of the order. Weights
+ * are integers in units of at most 2^-38 (2^-45 to 2^17 tokens) of the largest,
+ * so results do not depend on the order of sums. u below 0 or NaN counts as 0, u of
+ * 1 or more as the largest below 1.
+ * Logits that are NaN or -infinity are never drawn; beside +infinity nothing
+ * else is. A row without any other logit, or with a setting out of range
+ * (temperature negative or not finite, top_k or top_p negative, min_p outside
+ * 0 .. 1), gets tokens -1 and logprobs -infinity.
+ * logprobs: log softmax(x) at the token (no temperature, nothing cut). */
+typedef struct cxs_sample_call {
+  const void* logits;
+  const void* uniforms;      /* fp32, or fp64 when wide_uniforms */
+  int64_t* tokens;           /* [rows, draws] */
+  float* logprobs;           /* [rows, draws], or NULL */
+  const float* temperature;  /* [rows] each, or NULL: the value for all rows */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t row_stride;
+  int32_t rows, vocab, draws;
+  int32_t type;              /* CXS_TYPE_* */
+  int32_t wide_uniforms;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+} cxs_sample_call;
+int cxs_sample(const cxs_sample_call* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
