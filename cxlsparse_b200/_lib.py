@@ -110,6 +110,11 @@ class CacheAttendCall(ctypes.Structure):
         (name, c_i32) for name in ("heads", "causal", "window")] + [("scale", ctypes.c_float)]
 
 
+class CacheSharedCall(ctypes.Structure):
+    _fields_ = [("attend", CacheAttendCall)] + [(name, c_vp) for name in ("groups", "shared")] + [
+        ("group_count", c_i32)]
+
+
 class RotaryCall(ctypes.Structure):
     _fields_ = [(name, c_vp) for name in (
         "q", "k", "q_out", "k_out", "positions", "steps")] + [(name, c_i64) for name in (
@@ -151,8 +156,9 @@ def _packer(cls):
     return packer.pack
 
 
-pack_cache_call, pack_cache_attend_call, pack_rotary_call, pack_pages_call, pack_sample_call = map(
-    _packer, (CacheCall, CacheAttendCall, RotaryCall, PagesCall, SampleCall))
+pack_cache_call, pack_cache_attend_call, pack_rotary_call, pack_pages_call, pack_sample_call, \
+    pack_cache_shared_call = map(_packer, (CacheCall, CacheAttendCall, RotaryCall, PagesCall,
+                                           SampleCall, CacheSharedCall))
 
 _lib = None
 _packed = None
@@ -230,6 +236,9 @@ def lib():
             "cxs_cache_attend": (c_i32, [ctypes.POINTER(CacheAttendCall), c_vp]),
             "cxs_cache_attend_workspace": (c_i32, [ctypes.POINTER(CacheAttendCall),
                                                    ctypes.POINTER(c_i64)]),
+            "cxs_cache_attend_shared": (c_i32, [ctypes.POINTER(CacheSharedCall), c_vp]),
+            "cxs_cache_attend_shared_workspace": (c_i32, [ctypes.POINTER(CacheSharedCall),
+                                                          ctypes.POINTER(c_i64)]),
             "cxs_rotary": (c_i32, [ctypes.POINTER(RotaryCall), c_vp]),
             "cxs_pages_workspace": (c_i32, [ctypes.POINTER(PagesCall), ctypes.POINTER(c_i64)]),
             "cxs_pages_extend": (c_i32, [ctypes.POINTER(PagesCall), c_vp, c_vp]),
@@ -258,6 +267,8 @@ class _Packed:
                 ("cxs_cache_read", [c_vp, c_vp, c_vp, c_vp]),
                 ("cxs_cache_attend", [c_vp, c_vp]),
                 ("cxs_cache_attend_workspace", [c_vp, ctypes.POINTER(c_i64)]),
+                ("cxs_cache_attend_shared", [c_vp, c_vp]),
+                ("cxs_cache_attend_shared_workspace", [c_vp, ctypes.POINTER(c_i64)]),
                 ("cxs_rotary", [c_vp, c_vp]),
                 ("cxs_pages_workspace", [c_vp, ctypes.POINTER(c_i64)]),
                 ("cxs_pages_extend", [c_vp, c_vp, c_vp]),
@@ -325,4 +336,5 @@ def exported_symbols():
             "cxs_exchange_barrier", "cxs_cache_append", "cxs_cache_read", "cxs_cache_attend",
             "cxs_cache_attend_workspace", "cxs_rotary", "cxs_pages_workspace",
             "cxs_pages_extend", "cxs_pages_fork", "cxs_pages_free", "cxs_pages_adopt",
-            "cxs_pages_compact", "cxs_sample")
+            "cxs_pages_compact", "cxs_sample", "cxs_cache_attend_shared",
+            "cxs_cache_attend_shared_workspace")

@@ -690,60 +690,6 @@ __global__ void __launch_bounds__(GROUPS * 4 * D)
 
 // ------------------------------------------------------------------ host ---
 
-int check_attend(const cxs_cache_attend_call* a) {
-  if (!a) return set_error(CXS_ERR_INVALID, "cache attend: null call");
-  const int status = cxs_host::check_cache(&a->cache, "cache attend");
-  if (status != CXS_OK) return status;
-  if (a->cache.type == CXS_TYPE_F32)
-    return set_error(CXS_ERR_INVALID, "cache attend: queries must be bf16 or fp16");
-  if (a->heads < 1 || a->heads % a->cache.kv_heads)
-    return set_error(CXS_ERR_INVALID, "cache attend: heads must be a multiple of kv_heads");
-  if (a->window < 0) return set_error(CXS_ERR_INVALID, "cache attend: negative window");
-  if ((long long)a->cache.max_tokens * a->heads > 0x40000000ll)
-    return set_error(CXS_ERR_CAPACITY, "cache attend: more than 2^30 rows of one user");
-  return CXS_OK;
-}
-
-// SMs of the current device (looked up once).
-int sm_count(int* sms) {
-  static int known;
-  static cxs_host::OncePerDevice looked;
-  const int status = looked.run([] {
-    int device = 0, n = 0;
-    CXS_CUDA(cudaGetDevice(&device));
-    CXS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
-    __atomic_store_n(&known, n, __ATOMIC_RELAXED);
-    return (int)CXS_OK;
-  });
-  *sms = __atomic_load_n(&known, __ATOMIC_RELAXED);
-  return status;
-}
-
-// Largest grid a call uses: one CTA per SM of a B200. A constant, so that the
-// workspace's size does not depend on the device.
-constexpr int kMostCtas = 148;
-
-// Most rows of a user and KV head for which the mma.sync kernel runs: it takes
-// 16 rows at a time and reads the keys again for the next 16, the tcgen05
-// kernel takes up to 256 at about the same cost. Measured (us, mma.sync /
-// tcgen05, e4m3; 1 user of 16K tokens, 8 of 8K, 64 of 4K):
-//   D = 64, 2 KV heads    64 rows   23 / 41    32 / 33    65 / 80
-//                        128 rows   28 / 42    43 / 35   110 / 82
-//   D = 128, 8 KV heads   32 rows   47 / 43    89 / 97   260 / 334
-//                         64 rows   60 / 45   142 / 100  480 / 340
-bool few_rows(const cxs_cache_attend_call& a) {
-  return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= (a.cache.dim == 64 ? 64 : 32);
-}
-
-long long workspace_bytes(const cxs_cache_attend_call& a) {
-  // Two partial results for each CTA and, of few rows, each warp.
-  const bool few = few_rows(a);
-  const long long slots = 2 * kMostCtas * (few ? 1 + kDecodeWarps : 1);
-  const long long rows = few ? 16 : kTileRows;
-  return kMostCtas * sizeof(Partial) +
-         slots * rows * (a.cache.dim + 2) * (long long)sizeof(float);
-}
-
 template <int FORMAT, typename T, int D, bool HIDES>
 int launch_decode_as(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream) {
   using K = Decode<D>;
@@ -791,32 +737,96 @@ int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cud
 
 }  // namespace
 
+int cxs::cache8::check_attend(const cxs_cache_attend_call* a, const char* what) {
+  if (!a) return set_error(CXS_ERR_INVALID, "%s: null call", what);
+  const int status = cxs_host::check_cache(&a->cache, what);
+  if (status != CXS_OK) return status;
+  if (a->cache.type == CXS_TYPE_F32)
+    return set_error(CXS_ERR_INVALID, "%s: queries must be bf16 or fp16", what);
+  if (a->heads < 1 || a->heads % a->cache.kv_heads)
+    return set_error(CXS_ERR_INVALID, "%s: heads must be a multiple of kv_heads", what);
+  if (a->window < 0) return set_error(CXS_ERR_INVALID, "%s: negative window", what);
+  if ((long long)a->cache.max_tokens * a->heads > 0x40000000ll)
+    return set_error(CXS_ERR_CAPACITY, "%s: more than 2^30 rows of one user", what);
+  return CXS_OK;
+}
+
+int cxs::cache8::check_attend_pointers(const cxs_cache_attend_call* a, long long workspace,
+                                       const char* what) {
+  const int status = cxs_host::check_cache_pointers(&a->cache, what);
+  if (status != CXS_OK) return status;
+  if (!a->query || !a->out) return set_error(CXS_ERR_INVALID, "%s: null query or out", what);
+  if ((uintptr_t)a->out % 16) return set_error(CXS_ERR_INVALID, "%s: out must be 16-byte aligned", what);
+  if (!a->workspace || (uintptr_t)a->workspace % 16 || a->workspace_bytes < workspace)
+    return set_error(CXS_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
+  return CXS_OK;
+}
+
+// SMs of the current device (looked up once).
+int cxs::cache8::sm_count(int* sms) {
+  static int known;
+  static cxs_host::OncePerDevice looked;
+  const int status = looked.run([] {
+    int device = 0, n = 0;
+    CXS_CUDA(cudaGetDevice(&device));
+    CXS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+    __atomic_store_n(&known, n, __ATOMIC_RELAXED);
+    return (int)CXS_OK;
+  });
+  *sms = __atomic_load_n(&known, __ATOMIC_RELAXED);
+  return status;
+}
+
+// Most rows of a user and KV head for which the mma.sync kernel runs: it takes
+// 16 rows at a time and reads the keys again for the next 16, the tcgen05
+// kernel takes up to 256 at about the same cost. Measured (us, mma.sync /
+// tcgen05, e4m3; 1 user of 16K tokens, 8 of 8K, 64 of 4K):
+//   D = 64, 2 KV heads    64 rows   23 / 41    32 / 33    65 / 80
+//                        128 rows   28 / 42    43 / 35   110 / 82
+//   D = 128, 8 KV heads   32 rows   47 / 43    89 / 97   260 / 334
+//                         64 rows   60 / 45   142 / 100  480 / 340
+bool cxs::cache8::few_rows(const cxs_cache_attend_call& a) {
+  return (long long)a.cache.max_tokens * (a.heads / a.cache.kv_heads) <= (a.cache.dim == 64 ? 64 : 32);
+}
+
+long long cxs::cache8::partial_bytes(const cxs_cache_attend_call& a, bool few) {
+  // Two partial results for each CTA and, of few rows, each warp.
+  const long long slots = 2 * kMostCtas * (few ? 1 + kDecodeWarps : 1);
+  const long long rows = few ? 16 : kTileRows;
+  return kMostCtas * sizeof(Partial) +
+         slots * rows * (a.cache.dim + 2) * (long long)sizeof(float);
+}
+
+int cxs::cache8::launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few,
+                             cudaStream_t s) {
+  if (a.cache.type == CXS_TYPE_BF16)
+    return a.cache.dim == 64 ? launch_combine<__nv_bfloat16, 64>(a, z, few, s)
+                             : launch_combine<__nv_bfloat16, 128>(a, z, few, s);
+  return a.cache.dim == 64 ? launch_combine<__half, 64>(a, z, few, s)
+                           : launch_combine<__half, 128>(a, z, few, s);
+}
+
 extern "C" int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes) {
-  const int status = check_attend(call);
+  const int status = check_attend(call, "cache attend");
   if (status != CXS_OK) return status;
   if (!bytes) return set_error(CXS_ERR_INVALID, "cache attend: null result");
-  *bytes = workspace_bytes(*call);
+  *bytes = partial_bytes(*call, few_rows(*call));
   return CXS_OK;
 }
 
 extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream) {
-  int status = check_attend(call);
+  int status = check_attend(call, "cache attend");
   if (status != CXS_OK) return status;
   const cxs_cache_call& c = call->cache;
   if (c.tokens == 0) return CXS_OK;
   if (c.users == 0) return set_error(CXS_ERR_INVALID, "cache attend: rows without users");
-  status = cxs_host::check_cache_pointers(&c, "cache attend");
+  const bool few = few_rows(*call);
+  status = check_attend_pointers(call, partial_bytes(*call, few), "cache attend");
   if (status != CXS_OK) return status;
-  if (!call->query || !call->out) return set_error(CXS_ERR_INVALID, "cache attend: null query or out");
-  if ((uintptr_t)call->out % 16) return set_error(CXS_ERR_INVALID, "cache attend: out must be 16-byte aligned");
-  if (!call->workspace || (uintptr_t)call->workspace % 16 ||
-      call->workspace_bytes < workspace_bytes(*call))
-    return set_error(CXS_ERR_INVALID, "cache attend: workspace missing, unaligned or too small");
   int sms = 0;
   status = sm_count(&sms);
   if (status != CXS_OK) return status;
   const int grid = sms < kMostCtas ? sms : kMostCtas;
-  const bool few = few_rows(*call);
   cudaStream_t s = (cudaStream_t)stream;
   for (int user0 = 0; user0 < c.users; user0 += kSlice) {
     cxs_cache_attend_call a = *call;
@@ -839,12 +849,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
       status = launch_tile(a, z, s);
     }
     if (status != CXS_OK) return status;
-    if (c.type == CXS_TYPE_BF16)
-      status = c.dim == 64 ? launch_combine<__nv_bfloat16, 64>(a, z, few, s)
-                           : launch_combine<__nv_bfloat16, 128>(a, z, few, s);
-    else
-      status = c.dim == 64 ? launch_combine<__half, 64>(a, z, few, s)
-                           : launch_combine<__half, 128>(a, z, few, s);
+    status = launch_join(a, z, few, s);
     if (status != CXS_OK) return status;
   }
   return CXS_OK;

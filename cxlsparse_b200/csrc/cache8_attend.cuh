@@ -238,8 +238,48 @@ __device__ __noinline__ void mark_nans(const uint8_t* codes, long long page_byte
 
 constexpr int kTileRows = 256;  // query rows of an item of the tile kernel
 
+// What attention over shared tokens works out beforehand (cache8_shared.cu).
+struct GroupPlan {
+  int first, count;   // packed rows
+  int shared;         // common tokens that all rows see
+  int user0;          // whose pages they are in
+};
+struct ItemPlan {     // kTileRows query rows of a group, for every KV head
+  long long before;   // cost of the items before it
+  int group, tile_row;
+  int tiles, common_tiles;
+  int user_a, user_b; // its rows' users
+};
+struct SharePlan {    // a CTA's tiles and the item they begin in
+  long long low, high;
+  int item, kv_head;
+};
+struct PlanHead {
+  long long total;    // cost of all items
+  int items, gaps;
+};
+struct SharedPlan {
+  PlanHead* head;
+  GroupPlan* groups;
+  ItemPlan* items;
+  SharePlan* shares;
+  long long* runs;    // [users + groups]: runs of 16 own keys of the group's users
+                      // before user u of group g at [u + g], of all of them after the last
+  Gap* gaps;          // packed rows of no group
+};
+
 // One launch of the tile kernel over z.users users (cache8_tile.cu).
 int launch_tile(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream);
+// The launch that joins what was left in parts (cache8_attend.cu).
+int launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few, cudaStream_t stream);
+int check_attend(const cxs_cache_attend_call* a, const char* what);
+int check_attend_pointers(const cxs_cache_attend_call* a, long long workspace, const char* what);
+int sm_count(int* sms);
+bool few_rows(const cxs_cache_attend_call& a);
+// Bytes that the kernels of few or many rows leave their partial results in.
+long long partial_bytes(const cxs_cache_attend_call& a, bool few);
+constexpr int kMostCtas = 148;  // largest grid of a call: one CTA per SM of a B200. (A
+                                // constant: the workspace does not depend on the device.)
 
 }  // namespace cache8
 }  // namespace cxs

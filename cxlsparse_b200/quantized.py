@@ -128,14 +128,27 @@ class QuantizedCache:
             raise ValueError(f"{name} must be on {self.device}")
         return shape, stride
 
-    def _workspace_bytes(self, common, heads):
-        """Scratch of an attend call, kept by (heads, most rows of one user)."""
+    def _queries(self, q, scale):
+        """(tokens, heads, strides, scale) of an attend call's queries."""
+        shape, stride = self._rows("q", q)
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the cache has no gradient: attend with a detached q")
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("q must be bf16 or fp16")
+        if shape[1] < 1 or shape[1] % self.kv_heads:
+            raise ValueError("heads must be a multiple of kv_heads")
+        scale = self.dim ** -0.5 if scale is None else float(scale)
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
+        return shape[0], shape[1], stride, scale
+
+    def _workspace_size(self, known, fn, call):
+        """Scratch of an attend call, kept by what it depends on."""
         size = _lib.c_i64(0)
-        _lib.check(_lib.packed().cxs_cache_attend_workspace(
-            _lib.pack_cache_attend_call(*common, 0, 0, 0, 0, 0, 0, 0, heads, 1, 0, 1.0), size))
+        _lib.check(fn(call, size))
         if len(self._workspace) >= 4096:
             self._workspace.clear()
-        self._workspace[heads, common[15]] = size.value
+        self._workspace[known] = size.value
         return size.value
 
     # -- operators ---------------------------------------------------------
@@ -179,24 +192,15 @@ class QuantizedCache:
         row also sees only the last ``window`` positions up to its own. Returns
         [tokens, heads, dim], with ``return_lse`` also the softmax's log-sum
         [tokens, heads] fp32 (for joining with attention over other keys)."""
-        shape, stride = self._rows("q", q)
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("the cache has no gradient: attend with a detached q")
-        dtype = q.dtype
-        if dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError("q must be bf16 or fp16")
-        tokens, heads = shape[0], shape[1]
-        if heads < 1 or heads % self.kv_heads:
-            raise ValueError("heads must be a multiple of kv_heads")
-        scale = self.dim ** -0.5 if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError("scale must be finite")
+        tokens, heads, stride, scale = self._queries(q, scale)
         if window < 0:
             raise ValueError("window must not be negative")
-        common = self._call(table, lengths, offsets, tokens, max_tokens, TYPES[dtype])
+        common = self._call(table, lengths, offsets, tokens, max_tokens, TYPES[q.dtype])
         size = self._workspace.get((heads, common[15]))
         if size is None:
-            size = self._workspace_bytes(common, heads)
+            size = self._workspace_size(
+                (heads, common[15]), _lib.packed().cxs_cache_attend_workspace,
+                _lib.pack_cache_attend_call(*common, 0, 0, 0, 0, 0, 0, 0, heads, 1, 0, 1.0))
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) \
             if return_lse else None
@@ -205,4 +209,41 @@ class QuantizedCache:
             *common, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
             workspace.data_ptr(), size, stride[0], stride[1], heads, bool(causal), window, scale)
         _lib.on_device(self.device.index, _lib.packed().cxs_cache_attend, call)
+        return (out, lse) if return_lse else out
+
+    def attend_shared(self, q, table, lengths, offsets, groups, shared, *, max_tokens=None,
+                      causal=True, scale=None, return_lse=False):
+        """``attend`` for users that have their first tokens in common, such as
+        the candidates of one history (``PageTable.fork``): the common tokens are
+        read once for all of them. Users groups[g] .. groups[g + 1] - 1 (``groups
+        [count + 1]`` int32, ascending from 0 to all users) are group g; their
+        first shared[g] tokens (``shared [count]`` int32) are the same, codes and
+        scales, in whichever pages. A user alone is a group of its own, with 0
+        shared tokens if need be."""
+        tokens, heads, stride, scale = self._queries(q, scale)
+        common = self._call(table, lengths, offsets, tokens, max_tokens, TYPES[q.dtype])
+        users, count = common[12], shared.shape[0] if shared.ndim == 1 else -1
+        for name, x, n in (("shared", shared, count), ("groups", groups, count + 1)):
+            if x.shape != (n,) or x.dtype != torch.int32 or not x.is_contiguous() \
+                    or x.device != self.device:
+                raise ValueError("shared must be [groups] and groups [groups + 1] int32, "
+                                 f"contiguous, on {self.device}")
+        if count > users or (tokens and not count):
+            raise ValueError("every group must have a user, every row a group")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) \
+            if return_lse else None
+        known = heads, common[15], tokens, users, count
+        size = self._workspace.get(known)
+        if size is None:
+            size = self._workspace_size(
+                known, _lib.packed().cxs_cache_attend_shared_workspace,
+                _lib.pack_cache_shared_call(*common, 0, 0, 0, 0, 0, 0, 0, heads, 1, 0, 1.0, 0, 0,
+                                            count))
+        workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        call = _lib.pack_cache_shared_call(
+            *common, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            workspace.data_ptr(), size, stride[0], stride[1], heads, bool(causal), 0, scale,
+            groups.data_ptr(), shared.data_ptr(), count)
+        _lib.on_device(self.device.index, _lib.packed().cxs_cache_attend_shared, call)
         return (out, lse) if return_lse else out

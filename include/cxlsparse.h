@@ -578,6 +578,26 @@ int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream);
  * may overlap need their own. */
 int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes);
 
+/* Attention (cxs_cache_attend, without a window) of users that have their first
+ * tokens in common, such as the candidates of one history. Users groups[g] ..
+ * groups[g + 1] - 1 (groups [group_count + 1] ascends from 0 to users) are group
+ * g, and their first shared[g] tokens are the same, code by code and scale by
+ * scale; they are read once for the rows of all of them, from the first user's
+ * pages. (Of them only those count as common that every row of the group sees.)
+ * Where groups or offsets do not ascend no row is computed, and none of a group
+ * with a user of more than max_tokens rows, with CXS_DEVICE_ERR_BAD_LENGTH; rows
+ * of no group have out = 0 and lse = -infinity. (Groups of few rows, 64 a KV head
+ * on average, 32 for dim 128, are computed user by user: rows then depend on
+ * nothing but their user.) */
+typedef struct cxs_cache_shared_call {
+  cxs_cache_attend_call attend;
+  const int32_t* groups;   /* [group_count + 1] */
+  const int32_t* shared;   /* [group_count] */
+  int32_t group_count;
+} cxs_cache_shared_call;
+int cxs_cache_attend_shared(const cxs_cache_shared_call* call, void* stream);
+int cxs_cache_attend_shared_workspace(const cxs_cache_shared_call* call, int64_t* bytes);
+
 /* Rotary positions of queries and keys in one launch. Pair i of a head at
  * position p turns by the angle p * f_i:
  *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin),
