@@ -13,11 +13,15 @@
 // large as the sum over the vocabulary allows (45 bits for 2^17 tokens). Sums of
 // integers do not depend on their order, so neither does a result.
 //
-// A row is worked on by a cluster of CTAs, each with a run of the vocabulary and
-// in it a run for each warp. The border token of a cut is found in a histogram of
-// 2048 bins of log2 w (counts for top-k, masses for top-p), then among the
-// tokens of one bin: by rank if they are few, by histograms of their order's
-// key (logit and index, 64 bits) until they are.
+// A row is worked on by a cluster of CTAs, each with a run of the vocabulary (kept
+// in shared memory) and in it a run for each warp.
+// - top_k up to kMostListed: the k-th largest of the threads' own maxima bounds
+//   the k-th logit from below. What is at or above it, little more than k tokens,
+//   is gathered in one CTA, sorted, and cut and drawn from there.
+// - otherwise the border token of a cut is found in a histogram of 2048 bins of
+//   log2 w (counts for top-k, masses for top-p), then among the tokens of one
+//   bin: by rank if they are few, by histograms of their order's key (logit and
+//   index, 64 bits) until they are.
 #include <cooperative_groups.h>
 #include <limits.h>
 
@@ -30,10 +34,14 @@ namespace {
 using cxs::cache8::to_float;
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kBinsPerOctave = 32;   // of the weight: 64 octaves in all
 constexpr int kFew = 512;            // tokens whose ranks are counted one by one
+constexpr int kList = 2048;          // tokens that are gathered for a small top_k
+constexpr int kMostListed = 1024;    // largest such top_k
+constexpr int kMostCtas = 16;        // of a cluster
+constexpr int kSliceBytes = 72 << 10;  // of a CTA's run in shared memory: two CTAs fit an SM
 constexpr float kInf = INFINITY;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -43,11 +51,12 @@ __device__ __forceinline__ uint64_t key_of(float x, int index) {
   const uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
   return (uint64_t)k << 32 | (0xffffffffu - (uint32_t)index);
 }
-// Its logit.
+// Its logit and index.
 __device__ __forceinline__ float logit_of(uint64_t key) {
   const uint32_t k = (uint32_t)(key >> 32);
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
 // 2^-t, t in [0, 64), times 2^bits as an integer: Taylor's polynomial of 2^-f
 // for |f| <= 1/2 (the next term is below 2^-42), rounded at the last place.
@@ -78,16 +87,21 @@ struct Settings {  // of a row
 
 struct Shared {
   uint32_t counts[kBins];
-  unsigned long long masses[kBins];
+  union {
+    unsigned long long masses[kBins];
+    uint64_t gathered[kList];
+  };
   uint64_t list[kFew];                         // this CTA's
   uint64_t all[kFew];                          // the cluster's
   unsigned long long weights[kFew];
   unsigned long long sums[kWarps];             // of a scan
   unsigned long long spans[kWarps];            // kept mass before each warp's tokens
-  uint64_t exchanged;                          // read by the cluster: largest key,
+  float top;                                   // read by the cluster: largest logit,
+  uint64_t bounds[2];                          // keys of a bin,
   unsigned long long mass;                     // kept mass of this CTA,
   float total;                                 // its sum of exp(x - M),
-  int listed;                                  // and what it has listed
+  int listed;                                  // and what it has listed;
+  int wanted;                                  // (first CTA's) how many it was sent
   int bin, count;
   unsigned long long before;
   uint64_t cut;
@@ -107,60 +121,108 @@ __device__ __forceinline__ unsigned long long block_scan(Shared& s, unsigned lon
   __syncthreads();
   if (lane == 31) s.sums[warp] = sum;
   __syncthreads();
-  unsigned long long all = s.sums[lane];
+  unsigned long long all = lane < kWarps ? s.sums[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < kWarps; o <<= 1) {
     const unsigned long long up = __shfl_up_sync(0xffffffffu, all, o);
     if (lane >= o) all += up;
   }
-  *total = __shfl_sync(0xffffffffu, all, 31);
+  *total = __shfl_sync(0xffffffffu, all, kWarps - 1);
   const unsigned long long before = __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0);
   return sum - v + (warp > 0 ? before : 0);
 }
+__device__ __forceinline__ float block_sum(Shared& s, float v) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) s.warp_totals[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int w = 0; w < kWarps; ++w) v += s.warp_totals[w];
+  return v;
+}
 
+// This CTA's part of a row, in 16-byte vectors (those of the row's memory: a row
+// may begin inside one).
 template <typename T>
 struct Row {
   static constexpr int kVector = 16 / sizeof(T);
-  const T* base;       // the 16-byte vector that the row begins in
-  int skip;            // values of it before the row
+  const T* base;       // vector 0, or (kept) where vector `first` is in shared memory
+  bool kept;
+  int skip;            // values of vector 0 before the row
   int vocab;
-  int first, last;     // vectors of this warp
-  // f(logit, index, there) for this warp's tokens, vector by vector: all lanes call it.
-  // NaN counts as -infinity.
+  int first, count;    // the CTA's vectors
+  int each;            // of them, a warp's
+
+  __device__ __forceinline__ Row(const T* values, int vocab_, int rank, int ctas) {
+    vocab = vocab_;
+    kept = false;
+    skip = (int)((uintptr_t)values % 16 / sizeof(T));
+    base = values - skip;
+    const int vectors = (int)(((long long)vocab + skip + kVector - 1) / kVector);
+    const int part = (vectors + ctas - 1) / ctas;
+    first = min(part * rank, vectors);
+    count = min(part, vectors - first);
+    each = (count + kWarps - 1) / kWarps;
+  }
+  __device__ __forceinline__ int begin(int warp) const { return min(each * warp, count); }
+  __device__ __forceinline__ int index(int v, int e) const { return (first + v) * kVector + e - skip; }
+  // Vector v of the CTA's; values that are not the row's: -infinity.
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (kept) return *reinterpret_cast<const uint4*>(base + v * kVector);
+    const int i = index(v, 0);
+    const T* const from = base + (long long)(first + v) * kVector;
+    if (i >= 0 && i + kVector <= vocab) return *reinterpret_cast<const uint4*>(from);
+    alignas(16) T x[kVector];
+#pragma unroll
+    for (int e = 0; e < kVector; ++e)
+      x[e] = i + e >= 0 && i + e < vocab ? from[e] : cxs::cache8::from_float<T>(-kInf);
+    return *reinterpret_cast<const uint4*>(x);
+  }
+  // Its values, NaN as -infinity.
+  static __device__ __forceinline__ void unpack(uint4 w, float (&x)[kVector]) {
+    alignas(16) T y[kVector];
+    *reinterpret_cast<uint4*>(y) = w;
+#pragma unroll
+    for (int e = 0; e < kVector; ++e) x[e] = fmaxf(to_float(y[e]), -kInf);
+  }
+  // f(logits, index of the first) for the vectors of this warp.
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    const int lane = threadIdx.x % 32;
+  __device__ __forceinline__ void each_vector(F f) const {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     constexpr int kAtOnce = 4;
-    for (int v0 = first; v0 < last; v0 += 32 * kAtOnce) {
-      alignas(16) T x[kAtOnce][kVector];
+    const int stop = begin(warp + 1);
+    for (int v0 = begin(warp) + lane; v0 < stop; v0 += 32 * kAtOnce) {
+      uint4 w[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (v0 + 32 * j < stop) w[j] = load(v0 + 32 * j);
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
-        const int v = v0 + 32 * j + lane;
-        if (v < last) load(v, x[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        if (v0 + 32 * j >= last) break;
-        const int v = v0 + 32 * j + lane;
-#pragma unroll
-        for (int e = 0; e < kVector; ++e) {
-          const int i = v * kVector + e - skip;
-          const bool there = v < last && i >= 0 && i < vocab;
-          const float y = there ? to_float(x[j][e]) : -kInf;
-          f(y == y ? y : -kInf, i, there);
-        }
+        if (v0 + 32 * j >= stop) break;
+        float x[kVector];
+        unpack(w[j], x);
+        f(x, index(v0 + 32 * j, 0));
       }
     }
   }
-  __device__ __forceinline__ void load(int v, T (&x)[kVector]) const {
-    const int i = v * kVector - skip;
-    if (i >= 0 && i + kVector <= vocab) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(base + (long long)v * kVector);
-    } else {
+  template <typename F>
+  __device__ __forceinline__ void each_value(F f) const {
+    each_vector([&](const float (&x)[kVector], int i) {
 #pragma unroll
-      for (int e = 0; e < kVector; ++e)
-        if (i + e >= 0 && i + e < vocab) x[e] = base[(long long)v * kVector + e];
-    }
+      for (int e = 0; e < kVector; ++e) f(x[e], i + e);
+    });
+  }
+};
+
+// Kept tokens: those up to this one in the order.
+struct Cut {
+  float x;
+  int index;
+  // (A key without an index: all tokens of its logit. Key 0: every token.)
+  __device__ __forceinline__ Cut(uint64_t key)
+      : x(key ? logit_of(key) : -kInf), index((uint32_t)key ? index_of(key) : INT_MAX) {}
+  __device__ __forceinline__ bool keeps(float y, int i) const {
+    return y > -kInf && (y > x || (y == x && i <= index));
   }
 };
 
@@ -181,59 +243,93 @@ struct Weigh {
     if (!(octaves(x) < 60.f)) return 0;
     return fixed_exp2(x == top ? 0.0 : ((double)top - (double)x) * rate, bits);
   }
+  __device__ __forceinline__ float odds(float x) const {  // exp(x - M)
+    return x == top ? 1.f : exp2f((x - top) * (float)kLog2e);
+  }
 };
 
+// The first bin at which the cluster's counts (MASS: masses), with `before`,
+// reach the target: into s.bin, with what is before it and its count. Returns
+// the sum of all. Every CTA finds the same.
+template <bool MASS>
+__device__ unsigned long long find_bin(cg::cluster_group& cluster, Shared& s,
+                                       unsigned long long before, unsigned long long target,
+                                       float share) {
+  constexpr int kEach = kBins / kThreads;
+  const int ctas = cluster.num_blocks();
+  uint32_t count[kEach] = {};
+  unsigned long long amount[kEach] = {}, sum = 0;
+#pragma unroll 4
+  for (int c = 0; c < ctas; ++c) {
+    const Shared* from = cluster.map_shared_rank(&s, c);
+    const uint4 n = *reinterpret_cast<const uint4*>(&from->counts[threadIdx.x * kEach]);
+    count[0] += n.x, count[1] += n.y, count[2] += n.z, count[3] += n.w;
+    if (MASS) {
+#pragma unroll
+      for (int e = 0; e < kEach; e += 2) {
+        const ulonglong2 m =
+            *reinterpret_cast<const ulonglong2*>(&from->masses[threadIdx.x * kEach + e]);
+        amount[e] += m.x;
+        amount[e + 1] += m.y;
+      }
+    }
+  }
+  static_assert(kEach == 4, "bins of a thread");
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (!MASS) amount[e] = count[e];
+    sum += amount[e];
+  }
+  unsigned long long all, at = before + block_scan(s, sum, &all);
+  if (MASS && share >= 0.f) {
+    const double part = ceil((double)share * (double)all);
+    target = part < 1.0 ? 1 : (unsigned long long)part;
+    if (target > all) target = all;
+  }
+  if (threadIdx.x == 0) s.bin = -1;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (at < target && at + amount[e] >= target) {
+      s.bin = threadIdx.x * kEach + e;
+      s.count = (int)count[e];
+      s.before = at;
+    }
+    at += amount[e];
+  }
+  __syncthreads();
+  return all;
+}
+
 // The key of the first token (in the order) at which what is counted, 1 or the
-// weight of every token with a key of at least `cut`, reaches `target` (at least
-// 1); 0 where all of it does not. MASS: target is the part `share` of the mass.
+// weight of every token that `cut` keeps, reaches `target` (at least 1); 0 where
+// all of it does not. MASS: target is the part `share` of the mass.
 template <bool MASS, typename T>
 __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& row,
-                           const Weigh& weigh, uint64_t cut, unsigned long long target,
+                           const Weigh& weigh, uint64_t cut_key, unsigned long long target,
                            float share) {
   const int lane = threadIdx.x % 32, ctas = cluster.num_blocks();
-  uint64_t low = 0, high = 0;          // keys still looked at, from the second round on
+  const Cut cut(cut_key);
+  uint64_t low = 0, high = ~0ull;      // keys still looked at, from the second round on
   int shift = 0, coarse_bin = -1;
   unsigned long long before = 0;       // of the tokens ahead of them
   for (int round = 0;; ++round) {
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0, s.masses[i] = 0;
-    if (threadIdx.x == 0) s.listed = 0;
+    if (threadIdx.x == 0) s.listed = 0, s.bounds[0] = ~0ull, s.bounds[1] = 0;
     __syncthreads();
-    row.each([&](float x, int i, bool there) {
-      const uint64_t key = key_of(x, i);
-      int bin = -1;
-      if (there && x > -kInf && key >= cut) {
-        if (round == 0)
-          bin = weigh.bin(x);
-        else if (key >= low && key <= high && weigh.bin(x) == coarse_bin)
-          bin = (int)((high - key) >> shift);
+    row.each_value([&](float x, int i) {
+      if (!cut.keeps(x, i)) return;
+      int bin = weigh.bin(x);
+      if (round > 0) {
+        const uint64_t key = key_of(x, i);
+        if (bin != coarse_bin || key < low || key > high) return;
+        bin = (int)((high - key) >> shift);
       }
-      if (!__any_sync(0xffffffffu, bin >= 0)) return;
-      unsigned long long w = 0;
-      if (MASS && bin >= 0) w = weigh.weight(x);
-      if (bin >= 0) {
-        atomicAdd(&s.counts[bin], 1u);
-        if (MASS) atomicAdd(&s.masses[bin], w);
-      }
+      atomicAdd(&s.counts[bin], 1u);
+      if (MASS) atomicAdd(&s.masses[bin], weigh.weight(x));
     });
     cluster.sync();
-    // The cluster's bins: two to a thread.
-    constexpr int kEach = kBins / kThreads;
-    uint32_t count[kEach] = {};
-    unsigned long long amount[kEach] = {}, sum = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const Shared* from = cluster.map_shared_rank(&s, c);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        count[e] += from->counts[threadIdx.x * kEach + e];
-        if (MASS) amount[e] += from->masses[threadIdx.x * kEach + e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (!MASS) amount[e] = count[e];
-      sum += amount[e];
-    }
-    unsigned long long all, at = before + block_scan(s, sum, &all);
+    const unsigned long long all = find_bin<MASS>(cluster, s, before, target, round == 0 ? share : -1.f);
     if (MASS && round == 0) {
       const double part = ceil((double)share * (double)all);
       target = part < 1.0 ? 1 : (unsigned long long)part;
@@ -243,24 +339,10 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
       cluster.sync();  // (the bins have been read)
       return 0;
     }
-    if (threadIdx.x == 0) s.bin = -1;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (at < target && at + amount[e] >= target) {
-        s.bin = threadIdx.x * kEach + e;
-        s.count = (int)count[e];
-        s.before = at;
-      }
-      at += amount[e];
-    }
-    __syncthreads();
     const int bin = s.bin, found = s.count;
     before = s.before;
     if (round == 0) {
       coarse_bin = bin;
-      low = cut;
-      high = ~0ull;
     } else {
       high -= (uint64_t)bin << shift;
       const uint64_t width = (1ull << shift) - 1;
@@ -270,31 +352,29 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
     if (round == 0) {
       // Keys of the bin: the bounds of what is there.
       uint64_t least = ~0ull, most = 0;
-      row.each([&](float x, int i, bool there) {
+      row.each_value([&](float x, int i) {
+        if (!cut.keeps(x, i) || weigh.bin(x) != coarse_bin) return;
         const uint64_t key = key_of(x, i);
-        if (there && x > -kInf && key >= cut && weigh.bin(x) == coarse_bin) {
-          least = key < least ? key : least;
-          most = key > most ? key : most;
-        }
+        least = key < least ? key : least;
+        most = key > most ? key : most;
       });
+      __syncwarp();
       for (int o = 16; o; o >>= 1) {
         const uint64_t a = __shfl_xor_sync(0xffffffffu, least, o);
         const uint64_t b = __shfl_xor_sync(0xffffffffu, most, o);
         least = a < least ? a : least;
         most = b > most ? b : most;
       }
-      if (threadIdx.x == 0) s.list[0] = ~0ull, s.list[1] = 0;
-      __syncthreads();
       if (lane == 0) {
-        atomicMin((unsigned long long*)&s.list[0], (unsigned long long)least);
-        atomicMax((unsigned long long*)&s.list[1], (unsigned long long)most);
+        atomicMin((unsigned long long*)&s.bounds[0], (unsigned long long)least);
+        atomicMax((unsigned long long*)&s.bounds[1], (unsigned long long)most);
       }
       cluster.sync();
       low = ~0ull, high = 0;
       for (int c = 0; c < ctas; ++c) {
         const Shared* from = cluster.map_shared_rank(&s, c);
-        low = from->list[0] < low ? from->list[0] : low;
-        high = from->list[1] > high ? from->list[1] : high;
+        low = from->bounds[0] < low ? from->bounds[0] : low;
+        high = from->bounds[1] > high ? from->bounds[1] : high;
       }
     }
     shift = 0;
@@ -302,10 +382,10 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
     cluster.sync();  // (the bins and bounds have been read)
   }
   // Few enough: a list of them all, the rank of each.
-  row.each([&](float x, int i, bool there) {
+  row.each_value([&](float x, int i) {
+    if (!cut.keeps(x, i) || weigh.bin(x) != coarse_bin) return;
     const uint64_t key = key_of(x, i);
-    if (there && x > -kInf && key >= low && key <= high && weigh.bin(x) == coarse_bin)
-      s.list[atomicAdd(&s.listed, 1)] = key;
+    if (key >= low && key <= high) s.list[atomicAdd(&s.listed, 1)] = key;
   });
   cluster.sync();
   int n = 0;
@@ -330,51 +410,168 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
   return s.cut;
 }
 
+// Where u falls in `mass`.
+__device__ __forceinline__ unsigned long long place_of(const cxs_sample_call& a, long long draw,
+                                                       unsigned long long mass) {
+  double u = a.wide_uniforms ? ((const double*)a.uniforms)[draw]
+                             : (double)((const float*)a.uniforms)[draw];
+  u = u > 0.0 ? u : 0.0;  // (NaN, too)
+  const double part = u * (double)mass;
+  const unsigned long long at = part < (double)mass ? (unsigned long long)part : mass - 1;
+  return at < mass ? at : mass - 1;
+}
+
+// Descending, of `n` (a power of two) in shared memory.
+__device__ void sort_down(uint64_t* x, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size / 2; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const uint64_t p = x[a], q = x[b];
+        if ((p < q) == ((a & size) == 0)) x[a] = q, x[b] = p;
+      }
+    }
+  __syncthreads();
+}
+
+// Draws from the `n` gathered tokens (all that may be kept, and perhaps some
+// more): one CTA. log_total: of the sum of exp(x - M).
+__device__ void draw_listed(const cxs_sample_call& a, Shared& s, const Weigh& weigh,
+                            const Settings& set, int n, long long draws, float log_total) {
+  constexpr int kEach = kList / kThreads;
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) s.gathered[i] = 0;
+  sort_down(s.gathered, size);
+  // The kept ones are the first: at most top_k, with w >= min_p, and then top_p.
+  int most = min(n, set.top_k);
+  const double least = set.min_p > 0.f
+      ? (double)weigh.top + (double)set.temperature * log((double)set.min_p) : -INFINITY;
+  unsigned long long w[kEach], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x * kEach + e;
+    w[e] = 0;
+    if (i < most) {
+      const float x = logit_of(s.gathered[i]);
+      if (x == weigh.top || (double)x >= least) w[e] = weigh.weight(x);
+    }
+    sum += w[e];
+  }
+  unsigned long long mass, before = block_scan(s, sum, &mass);
+  const double part = set.top_p < 1.f ? (double)set.top_p * (double)mass : INFINITY;
+  // By index: the same keys with index (larger first) and place.
+  unsigned long long kept = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x * kEach + e;
+    if (i > 0 && !((double)before < part)) w[e] = 0;
+    before += w[e];
+    kept += w[e];
+  }
+  block_scan(s, kept, &mass);
+  uint64_t mine[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x * kEach + e;
+    mine[e] = i < n ? s.gathered[i] : 0;
+  }
+  __syncthreads();
+  // (Tokens of no weight cannot be drawn and need no place.)
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x * kEach + e;
+    if (i < size)
+      s.gathered[i] = w[e] ? (uint64_t)(uint32_t)mine[e] << 32 | (uint32_t)(mine[e] >> 32) : 0;
+  }
+  sort_down(s.gathered, size);
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x * kEach + e;
+    mine[e] = i < size ? s.gathered[i] : 0;
+    mine[e] = mine[e] << 32 | mine[e] >> 32;
+    w[e] = mine[e] ? weigh.weight(logit_of(mine[e])) : 0;
+    sum += w[e];
+  }
+  unsigned long long all;
+  before = block_scan(s, sum, &all);
+  for (int d = 0; d < a.draws; ++d) {
+    const unsigned long long at = place_of(a, draws + d, mass);
+    if (at < before || at >= before + sum) continue;
+    unsigned long long left = at - before;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (left < w[e]) {
+        const float x = logit_of(mine[e]);
+        a.tokens[draws + d] = index_of(mine[e]);
+        if (a.logprobs)
+          a.logprobs[draws + d] = (x == weigh.top ? 0.f : x - weigh.top) - log_total;
+        break;
+      }
+      left -= w[e];
+    }
+  }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const cxs_sample_call a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_call a, int slice) {
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ Shared s;
+  extern __shared__ __align__(16) uint8_t slice_memory[];
+  __shared__ __align__(16) Shared s;
   const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int r = blockIdx.x / ctas, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const T* const values = (const T*)a.logits + r * a.row_stride;
-  Row<T> row;
-  row.vocab = a.vocab;
-  row.skip = (int)((uintptr_t)values % 16 / sizeof(T));
-  row.base = values - row.skip;
-  {
-    const int vectors = (int)(((long long)a.vocab + row.skip + row.kVector - 1) / row.kVector);
-    const int each = (vectors + ctas - 1) / ctas, first = min(each * rank, vectors);
-    const int here = min(each, vectors - first), mine = (here + kWarps - 1) / kWarps;
-    row.first = first + min(mine * warp, here);
-    row.last = first + min(mine * (warp + 1), here);
-  }
+  Row<T> row((const T*)a.logits + r * a.row_stride, a.vocab, rank, ctas);
+  constexpr int kVector = Row<T>::kVector;
   Settings set{a.temperature ? a.temperature[r] : a.temperature_all,
                a.top_p ? a.top_p[r] : a.top_p_all, a.min_p ? a.min_p[r] : a.min_p_all,
                a.top_k ? a.top_k[r] : a.top_k_all};
   const bool wrong = !(set.temperature >= 0.f && set.temperature < kInf) || !(set.top_p >= 0.f) ||
                      !(set.min_p >= 0.f && set.min_p <= 1.f) || set.top_k < 0;
+  const bool greedy = set.temperature == 0.f || set.top_k == 1;
+  const bool listed = greedy || (set.top_k > 0 && set.top_k <= kMostListed &&
+                                 set.top_k <= ctas * kThreads / 2);
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0;
+  if (threadIdx.x == 0) s.wanted = 0;
 
-  // The largest logit.
-  uint64_t key = 0;
-  row.each([&](float x, int i, bool there) {
-    const uint64_t k = key_of(x, i);
-    if (there && x > -kInf && k > key) key = k;
-  });
-  for (int o = 16; o; o >>= 1) {
-    const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
-    key = other > key ? other : key;
+  // The largest logit, of the thread and of the row; the run into shared memory.
+  float mine = -kInf;
+  {
+    T* const keep = slice ? reinterpret_cast<T*>(slice_memory) : nullptr;
+    constexpr int kAtOnce = 8;
+    const int stop = row.begin(warp + 1);
+    for (int v0 = row.begin(warp) + lane; v0 < stop; v0 += 32 * kAtOnce) {
+      uint4 w[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (v0 + 32 * j < stop) w[j] = row.load(v0 + 32 * j);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (v0 + 32 * j >= stop) break;
+        if (keep) *reinterpret_cast<uint4*>(keep + (v0 + 32 * j) * kVector) = w[j];
+        float x[kVector];
+        Row<T>::unpack(w[j], x);
+#pragma unroll
+        for (int e = 0; e < kVector; ++e) mine = fmaxf(mine, x[e]);
+      }
+    }
+    if (keep) row.base = keep, row.kept = true;
   }
-  if (threadIdx.x == 0) s.exchanged = 0;
-  __syncthreads();
-  if (lane == 0) atomicMax((unsigned long long*)&s.exchanged, (unsigned long long)key);
+  {
+    float top = mine;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) s.warp_totals[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s.warp_totals[w]);
+    if (threadIdx.x == 0) s.top = top;
+  }
   cluster.sync();
-  key = 0;
-  for (int c = 0; c < ctas; ++c) {
-    const uint64_t other = cluster.map_shared_rank(&s, c)->exchanged;
-    key = other > key ? other : key;
-  }
+  Weigh weigh;
+  weigh.top = -kInf;
+  for (int c = 0; c < ctas; ++c) weigh.top = fmaxf(weigh.top, cluster.map_shared_rank(&s, c)->top);
   const long long draws = (long long)r * a.draws;
-  if (wrong || key == 0) {  // no answer
+  if (wrong || weigh.top == -kInf) {  // no answer
     if (rank == 0)
       for (int d = threadIdx.x; d < a.draws; d += kThreads) {
         a.tokens[draws + d] = -1;
@@ -383,51 +580,78 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const cxs_sample_ca
     cluster.sync();
     return;
   }
-
-  Weigh weigh;
-  weigh.top = logit_of(key);
-  const bool greedy = set.temperature == 0.f || set.top_k == 1;
   weigh.rate = greedy ? 0.0 : kLog2e / set.temperature;
   weigh.rate32 = fminf((float)weigh.rate, 1e30f);
   weigh.bits = min(51, 62 - (32 - __clz(a.vocab)));
+  const bool want = a.logprobs != nullptr;
+
+  if (listed) {
+    // The bin that top_k of the threads' maxima reach: so many tokens at least lie
+    // in it and before it.
+    int last = 0;
+    if (greedy) {
+      set.top_k = 1;
+    } else {
+      if (mine > -kInf) atomicAdd(&s.counts[weigh.bin(mine)], 1u);
+      cluster.sync();
+      find_bin<false>(cluster, s, 0, set.top_k, -1.f);
+      last = s.bin < 0 ? kBins - 1 : s.bin;
+    }
+    Shared* const first = cluster.map_shared_rank(&s, 0);
+    float total = 0.f;
+    row.each_value([&](float x, int i) {
+      if (greedy ? x == weigh.top : x > -kInf && weigh.bin(x) <= last) {
+        const int at = atomicAdd(&first->wanted, 1);
+        if (at < kList) first->gathered[at] = key_of(x, i);
+      }
+      if (want) total += weigh.odds(x);
+    });
+    if (want) {
+      total = block_sum(s, total);
+      if (threadIdx.x == 0) s.total = total;
+    }
+    cluster.sync();
+    const int n = first->wanted;
+    if (n <= kList) {
+      total = 0.f;
+      if (rank == 0 && want)
+        for (int c = 0; c < ctas; ++c) total += cluster.map_shared_rank(&s, c)->total;
+      cluster.sync();  // (what is read of other CTAs has been)
+      if (rank == 0) draw_listed(a, s, weigh, set, n, draws, logf(total));
+      return;
+    }
+    cluster.sync();  // (`wanted` and the list are free)
+  }
+
   uint64_t cut = 0;  // keys of kept tokens are at least this
-  if (greedy) {
-    cut = key;
-  } else {
-    if (set.top_k > 0 && set.top_k < a.vocab)
-      cut = border<false>(cluster, s, row, weigh, 0, set.top_k, 0.f);
-    if (set.min_p > 0.f) {
-      const float least =
-          __double2float_ru((double)weigh.top + (double)set.temperature * log((double)set.min_p));
-      const uint64_t other = key_of(fminf(least, weigh.top), INT_MAX) & ~0xffffffffull;
-      cut = other > cut ? other : cut;
-    }
-    if (set.top_p < 1.f) {
-      const uint64_t other = border<true>(cluster, s, row, weigh, cut, 0, set.top_p);
-      cut = other > cut ? other : cut;
-    }
+  if (set.top_k > 0 && set.top_k < a.vocab)
+    cut = border<false>(cluster, s, row, weigh, 0, set.top_k, 0.f);
+  if (set.min_p > 0.f && !greedy) {
+    const float least =
+        __double2float_ru((double)weigh.top + (double)set.temperature * log((double)set.min_p));
+    const uint64_t other = key_of(fminf(least, weigh.top), INT_MAX) & ~0xffffffffull;
+    cut = other > cut ? other : cut;
+  }
+  if (set.top_p < 1.f && !greedy) {
+    const uint64_t other = border<true>(cluster, s, row, weigh, cut, 0, set.top_p);
+    cut = other > cut ? other : cut;
   }
 
   // Kept mass of every warp's run, and the sum of exp(x - M) over all tokens.
+  const Cut keep(cut);
   unsigned long long mass = 0;
   float total = 0.f;
-  const bool want = a.logprobs != nullptr;
-  row.each([&](float x, int i, bool there) {
-    const bool kept = there && x > -kInf && key_of(x, i) >= cut;
-    if (__any_sync(0xffffffffu, kept) && kept) mass += weigh.weight(x);
-    if (want) total += x == weigh.top ? 1.f : exp2f((x - weigh.top) * (float)kLog2e);
+  row.each_value([&](float x, int i) {
+    if (keep.keeps(x, i)) mass += weigh.weight(x);
+    if (want) total += weigh.odds(x);
   });
-  for (int o = 16; o; o >>= 1) {
-    mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  if (lane == 0) s.warp_totals[warp] = total;
+  __syncwarp();
+  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  total = want ? block_sum(s, total) : 1.f;
   unsigned long long all;
   const unsigned long long ahead = block_scan(s, lane == 0 ? mass : 0, &all);
   if (lane == 0) s.spans[warp] = ahead;
   if (threadIdx.x == 0) {
-    total = 0.f;
-    for (int w = 0; w < kWarps; ++w) total += s.warp_totals[w];
     s.total = total;
     s.mass = all;
   }
@@ -440,43 +664,28 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const cxs_sample_ca
     kept_mass += from->mass;
     total += from->total;
   }
+  cluster.sync();  // (the sums have been read)
   const float log_total = logf(total);
 
   // A warp for each draw that falls into this CTA.
   for (int d = warp; d < a.draws; d += kWarps) {
-    double u = a.wide_uniforms ? ((const double*)a.uniforms)[draws + d]
-                               : (double)((const float*)a.uniforms)[draws + d];
-    u = u > 0.0 ? u : 0.0;  // (NaN, too)
-    const double part = u * (double)kept_mass;
-    unsigned long long at = part < (double)kept_mass ? (unsigned long long)part : kept_mass - 1;
-    if (at >= kept_mass) at = kept_mass - 1;
+    unsigned long long at = place_of(a, draws + d, kept_mass);
     if (at < before || at >= before + all) continue;
     at -= before;
     // The run it falls into: the last that begins at or before it and has any.
-    const unsigned run =
-        __ballot_sync(0xffffffffu, s.spans[lane] <= at &&
-                                       at < (lane + 1 < kWarps ? s.spans[lane + 1] : all));
-    const int w = __ffs(run) - 1;
+    const bool in = lane < kWarps && s.spans[min(lane, kWarps - 1)] <= at &&
+                    at < (lane + 1 < kWarps ? s.spans[lane + 1] : all);
+    const int w = __ffs(__ballot_sync(0xffffffffu, in)) - 1;
     at -= s.spans[w];
-    Row<T> its = row;
-    {
-      const int vectors = (int)(((long long)a.vocab + row.skip + row.kVector - 1) / row.kVector);
-      const int each = (vectors + ctas - 1) / ctas, first = min(each * rank, vectors);
-      const int here = min(each, vectors - first), mine = (here + kWarps - 1) / kWarps;
-      its.first = first + min(mine * w, here);
-      its.last = first + min(mine * (w + 1), here);
-    }
-    for (int v0 = its.first; v0 < its.last; v0 += 32) {
+    const int stop = row.begin(w + 1);
+    for (int v0 = row.begin(w); v0 < stop; v0 += 32) {
       const int v = v0 + lane;
-      T x[Row<T>::kVector];
-      if (v < its.last) its.load(v, x);
-      unsigned long long weights[Row<T>::kVector], sum = 0;
+      float x[kVector];
+      unsigned long long weights[kVector], sum = 0;
+      if (v < stop) Row<T>::unpack(row.load(v), x);
 #pragma unroll
-      for (int e = 0; e < Row<T>::kVector; ++e) {
-        const int i = v * Row<T>::kVector + e - its.skip;
-        const bool there = v < its.last && i >= 0 && i < a.vocab;
-        const float y = there ? to_float(x[e]) : -kInf;
-        weights[e] = there && y > -kInf && key_of(y, i) >= cut ? weigh.weight(y) : 0;
+      for (int e = 0; e < kVector; ++e) {
+        weights[e] = v < stop && keep.keeps(x[e], row.index(v, e)) ? weigh.weight(x[e]) : 0;
         sum += weights[e];
       }
       unsigned long long to = sum;
@@ -492,11 +701,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const cxs_sample_ca
       if (at < to && at >= to - sum) {
         unsigned long long left = at - (to - sum);
 #pragma unroll
-        for (int e = 0; e < Row<T>::kVector; ++e) {
+        for (int e = 0; e < kVector; ++e) {
           if (left < weights[e]) {
-            const float y = to_float(x[e]);
-            a.tokens[draws + d] = v * Row<T>::kVector + e - its.skip;
-            if (want) a.logprobs[draws + d] = (y == weigh.top ? 0.f : y - weigh.top) - log_total;
+            a.tokens[draws + d] = row.index(v, e);
+            if (want)
+              a.logprobs[draws + d] = (x[e] == weigh.top ? 0.f : x[e] - weigh.top) - log_total;
             break;
           }
           left -= weights[e];
@@ -505,14 +714,38 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const cxs_sample_ca
       break;
     }
   }
-  cluster.sync();  // (the sums have been read)
+}
+
+// CTAs of a row's cluster: as many as still run at once (two to an SM) and have
+// kLeast values each, and so many that the row fits into their shared memory.
+int ctas_of(const cxs_sample_call& a, int size) {
+  constexpr int kAtOnce = 296, kLeast = 2048;
+  int ctas = 1;
+  while (ctas < kMostCtas && ((long long)a.rows * ctas * 2 <= kAtOnce && a.vocab >= 2 * kLeast * ctas ||
+                              (long long)a.vocab * size > (long long)ctas * (kSliceBytes - 64)))
+    ctas *= 2;
+  return ctas;
 }
 
 template <typename T>
-int launch(const cxs_sample_call& a, int ctas, cudaStream_t stream) {
+int launch(const cxs_sample_call& a, cudaStream_t stream) {
+  static cxs_host::OncePerDevice ready;
+  const int status = ready.run([] {
+    CXS_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  kSliceBytes));
+    CXS_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    return (int)CXS_OK;
+  });
+  if (status != CXS_OK) return status;
+  const int ctas = ctas_of(a, sizeof(T));
+  // (A row may begin inside a vector, and vectors are shared out whole.)
+  const long long vectors = ((long long)a.vocab * sizeof(T) + 15) / 16 + 1;
+  const long long bytes = (vectors + ctas - 1) / ctas * 16;
+  const int slice = bytes <= kSliceBytes ? (int)bytes : 0;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(a.rows * ctas);
   config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = slice;
   config.stream = stream;
   cudaLaunchAttribute cluster = {};
   cluster.id = cudaLaunchAttributeClusterDimension;
@@ -520,7 +753,7 @@ int launch(const cxs_sample_call& a, int ctas, cudaStream_t stream) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  CXS_CUDA(cudaLaunchKernelEx(&config, sample_kernel<T>, a));
+  CXS_CUDA(cudaLaunchKernelEx(&config, sample_kernel<T>, a, slice));
   CXS_LAUNCH_CHECK("sample");
   return CXS_OK;
 }
@@ -547,7 +780,5 @@ extern "C" int cxs_sample(const cxs_sample_call* call, void* stream) {
     return set_error(CXS_ERR_INVALID, "sample: null logits, uniforms or tokens");
   const int size = a.type == CXS_TYPE_F32 ? 4 : 2;
   if ((uintptr_t)a.logits % size) return set_error(CXS_ERR_INVALID, "sample: unaligned logits");
-  const int ctas = 1;
-  cudaStream_t s = (cudaStream_t)stream;
-  CXS_CACHE_TYPE(a.type, T, return launch<T>(a, ctas, s));
+  CXS_CACHE_TYPE(a.type, T, return launch<T>(a, (cudaStream_t)stream));
 }
