@@ -9,9 +9,11 @@
 //
 // Whether a token is kept, and which one u falls on, are decisions next to a
 // border: with 2^17 tokens fp32 sums would miss one in about a hundred. So a
-// weight is a 64-bit integer, 2^-t in fp64 (to 2^-42 of itself) times 2^S with S as
-// large as the sum over the vocabulary allows (45 bits for 2^17 tokens). Sums of
-// integers do not depend on their order, so neither does a result.
+// weight is a 64-bit integer, 2^-t (to 2^-30 of itself, see Weigh) times 2^S with S
+// as large as the sum over the vocabulary allows (45 bits for 2^17 tokens): errors
+// of single tokens' weights next to a border matter, not those of the sum, whose
+// parts' errors average out. Sums of integers do not depend on their order, so
+// neither does a result.
 //
 // A row is worked on by a cluster of CTAs, each with a run of the vocabulary (kept
 // in shared memory) and in it a run for each warp.
@@ -23,6 +25,7 @@
 //   bin: by rank if they are few, by histograms of their order's key (logit and
 //   index, 64 bits) until they are.
 #include <cooperative_groups.h>
+#include <float.h>
 #include <limits.h>
 
 #include "cache8.cuh"
@@ -41,6 +44,7 @@ constexpr int kFew = 512;            // tokens whose ranks are counted one by on
 constexpr int kList = 2048;          // tokens that are gathered for a small top_k
 constexpr int kMostListed = 1024;    // largest such top_k
 constexpr int kMostCtas = 16;        // of a cluster
+constexpr int kBlocks = 128;         // parts of a warp's run whose kept mass is kept
 constexpr int kSliceBytes = 72 << 10;  // of a CTA's run in shared memory: two CTAs fit an SM
 constexpr float kInf = INFINITY;
 constexpr double kLog2e = 1.4426950408889634;
@@ -58,26 +62,14 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-// 2^-t, t in [0, 64), times 2^bits as an integer: Taylor's polynomial of 2^-f
-// for |f| <= 1/2 (the next term is below 2^-42), rounded at the last place.
-__device__ __forceinline__ uint64_t fixed_exp2(double t, int bits) {
-  const double shift = 6755399441055744.0;  // 1.5 * 2^52: t rounded in the low bits
-  const double n = t + shift;
-  const double g = (t - (n - shift)) * -0.6931471805599453;
-  double p = 1.0 / 3628800;
-  p = fma(p, g, 1.0 / 362880);
-  p = fma(p, g, 1.0 / 40320);
-  p = fma(p, g, 1.0 / 5040);
-  p = fma(p, g, 1.0 / 720);
-  p = fma(p, g, 1.0 / 120);
-  p = fma(p, g, 1.0 / 24);
-  p = fma(p, g, 1.0 / 6);
-  p = fma(p, g, 0.5);
-  p = fma(p, g, 1.0);
-  p = fma(p, g, 1.0);
-  const int e = bits - __double2loint(n);
-  p = __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
-  return (uint64_t)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;
+// 2^(32 - i / 256), rounded (below 2^32 for i = 0), by Taylor's polynomial: the
+// exponent is at most ln 2, the next term below 2^-48.
+__device__ __forceinline__ uint32_t power_of(int i) {
+  const double g = i * (-0.6931471805599453 / 256);
+  double p = 1.0;
+#pragma unroll
+  for (int k = 13; k > 0; --k) p = fma(p, g * (1.0 / k), 1.0);
+  return (uint32_t)fmin(p * 4294967296.0 + 0.5, 4294967295.0);
 }
 
 struct Settings {  // of a row
@@ -85,27 +77,62 @@ struct Settings {  // of a row
   int top_k;
 };
 
+// A sum of 64 bits in two words of shared memory (an atomic addition of 64 bits
+// there is a loop).
+struct Wide {
+  uint32_t* low;
+  uint32_t* high;
+  __device__ __forceinline__ void add(int i, unsigned long long v) const {
+    const uint32_t lo = (uint32_t)v, old = atomicAdd(low + i, lo);
+    const uint32_t hi = (uint32_t)(v >> 32) + (old + lo < lo);
+    if (hi) atomicAdd(high + i, hi);
+  }
+  __device__ __forceinline__ unsigned long long get(int i) const {
+    return (unsigned long long)high[i] << 32 | low[i];
+  }
+};
+
+struct Found {  // a bin: its count, what is before it, the sum of all bins
+  int bin, count;
+  unsigned long long before, all;
+};
+
 struct Shared {
-  uint32_t counts[kBins];
   union {
-    unsigned long long masses[kBins];
-    uint64_t gathered[kList];
+    struct {
+      uint32_t counts[kBins];
+      union {
+        uint32_t masses[2][kBins];             // low and high words
+        uint64_t gathered[kList];
+      };
+    };
+    unsigned long long blocks[kWarps][kBlocks];  // kept mass of parts of a warp's run
   };
-  uint64_t list[kFew];                         // this CTA's
-  uint64_t all[kFew];                          // the cluster's
-  unsigned long long weights[kFew];
+  union {
+    struct {
+      uint64_t list[kFew];                     // this CTA's few
+      uint64_t all[kFew];                      // the cluster's
+      unsigned long long weights[kFew];
+    };
+    struct {                                   // (of several CTAs) the cluster's bins,
+      uint32_t part_masses[2][kBins / 2];      // this CTA's part of them
+      uint32_t part_counts[kBins / 2];
+    };
+  };
   unsigned long long sums[kWarps];             // of a scan
   unsigned long long spans[kWarps];            // kept mass before each warp's tokens
-  float top;                                   // read by the cluster: largest logit,
+  float top, bound;                            // read by the cluster: largest logit, a bound
+                                               // below which the CTA has no first top_k,
   uint64_t bounds[2];                          // keys of a bin,
   unsigned long long mass;                     // kept mass of this CTA,
   float total;                                 // its sum of exp(x - M),
   int listed;                                  // and what it has listed;
   int wanted;                                  // (first CTA's) how many it was sent
-  int bin, count;
-  unsigned long long before;
+  unsigned long long part;                     // sum of this CTA's part of the bins
+  Found found;
   uint64_t cut;
   float warp_totals[kWarps];
+  uint32_t powers[256];                        // 2^(32 - i / 256)
 };
 
 // Sum of v over the threads before this one; *total: over all.
@@ -185,32 +212,23 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < kVector; ++e) x[e] = fmaxf(to_float(y[e]), -kInf);
   }
-  // f(logits, index of the first) for the vectors of this warp.
-  template <typename F>
-  __device__ __forceinline__ void each_vector(F f) const {
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    constexpr int kAtOnce = 4;
-    const int stop = begin(warp + 1);
-    for (int v0 = begin(warp) + lane; v0 < stop; v0 += 32 * kAtOnce) {
-      uint4 w[kAtOnce];
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-        if (v0 + 32 * j < stop) w[j] = load(v0 + 32 * j);
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        if (v0 + 32 * j >= stop) break;
-        float x[kVector];
-        unpack(w[j], x);
-        f(x, index(v0 + 32 * j, 0));
-      }
-    }
-  }
+  // f(logit, index) for this warp's tokens; the next vector is on its way meanwhile.
   template <typename F>
   __device__ __forceinline__ void each_value(F f) const {
-    each_vector([&](const float (&x)[kVector], int i) {
+    const int warp = threadIdx.x / 32, stop = begin(warp + 1);
+    int v = begin(warp) + threadIdx.x % 32;
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (v < stop) next = load(v);
+#pragma unroll 1
+    for (; v < stop; v += 32) {
+      const uint4 w = next;
+      if (v + 32 < stop) next = load(v + 32);
+      float x[kVector];
+      unpack(w, x);
+      const int i = index(v, 0);
 #pragma unroll
       for (int e = 0; e < kVector; ++e) f(x[e], i + e);
-    });
+    }
   }
 };
 
@@ -226,12 +244,25 @@ struct Cut {
   }
 };
 
-// What a row's tokens are weighed by.
+// What a row's tokens are weighed by. 2^-t with t = n + i / 256 + r, r < 2^-8:
+// t comes from fp64 as a fixed-point number (exact to 2^-33), 2^-(i / 256) from a
+// table of 32 bits, and 1 - 2^-r, at most 2^-8.5, from its Taylor polynomial in
+// fp32, whose rounding errors are then 2^-32 of the weight. A third of the
+// instructions of a polynomial in fp64.
 struct Weigh {
   float top;       // largest logit
+  float least;     // below it a weight is nothing
   float rate32;    // log2(e) / T, and in fp64
   double rate;
   int bits;
+  const uint32_t* powers;
+  __device__ __forceinline__ Weigh(const uint32_t* powers_, float top_, double rate_, int vocab)
+      : top(top_), rate(rate_), powers(powers_) {
+    rate32 = fminf((float)rate, 1e30f);
+    bits = min(51, 62 - (32 - __clz(vocab)));
+    const float to = __double2float_rd((double)top - (bits + 2) / rate);
+    least = to > -FLT_MAX ? to : -FLT_MAX;  // (never -infinity)
+  }
   __device__ __forceinline__ float octaves(float x) const {
     return x == top ? 0.f : (top - x) * rate32;
   }
@@ -239,66 +270,127 @@ struct Weigh {
     const float t = octaves(x) * kBinsPerOctave;
     return t < kBins - 1 ? (int)t : kBins - 1;  // (what is not a number, too)
   }
+  // The weight added to `sum`, top being finite: what is far below it, -infinity
+  // and NaN come out with so large an n that nothing is left.
+  __device__ __forceinline__ unsigned long long add(unsigned long long sum, float x) const {
+    // 1.5 * 2^20 + t: the low word is t's fraction in 2^-32.
+    const double t = fma((double)top - (double)x, rate, 1572864.0);
+    const uint32_t fraction = (uint32_t)__double2loint(t);
+    const int n = __double2hiint(t) - 0x41380000;
+    // r in units of 2^-31, 1 - 2^-r in the low 23 bits of `less`.
+    const float r = __uint_as_float(0x4b000000u | (fraction >> 1 & 0x7fffffu)) - 8388608.f;
+    const float kLn2 = 0.693147181f, kUnit = 4.65661287e-10f;  // 2^-31
+    float less = fmaf(r, kLn2 * kLn2 * kLn2 / 6 * kUnit * kUnit, -kLn2 * kLn2 / 2 * kUnit);
+    less = fmaf(r, less, kLn2);
+    less = fmaf(r, less, 8388608.f);
+    const uint32_t power = powers[fraction >> 24];
+    const uint32_t w = power - __umulhi(power, __float_as_uint(less) << 1 & 0xffffffu);
+    // w 2^(bits - 32 - n): shifted down in 32 bits or up by a product.
+    const int up = bits - 32 - n;
+    const uint32_t down = up >= 0 ? w : up > -32 ? w >> -up : 0;
+    return sum + (unsigned long long)down * (1u << max(up, 0));
+  }
   __device__ __forceinline__ unsigned long long weight(float x) const {
-    if (!(octaves(x) < 60.f)) return 0;
-    return fixed_exp2(x == top ? 0.0 : ((double)top - (double)x) * rate, bits);
+    if (top == kInf) return x == top ? 1ull << bits : 0;
+    return x >= least ? add(0, x) : 0;
   }
   __device__ __forceinline__ float odds(float x) const {  // exp(x - M)
-    return x == top ? 1.f : exp2f((x - top) * (float)kLog2e);
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - top) * (float)kLog2e));
+    return x == top ? 1.f : y;
   }
 };
 
-// The first bin at which the cluster's counts (MASS: masses), with `before`,
-// reach the target: into s.bin, with what is before it and its count. Returns
-// the sum of all. Every CTA finds the same.
-template <bool MASS>
-__device__ unsigned long long find_bin(cg::cluster_group& cluster, Shared& s,
-                                       unsigned long long before, unsigned long long target,
-                                       float share) {
-  constexpr int kEach = kBins / kThreads;
-  const int ctas = cluster.num_blocks();
-  uint32_t count[kEach] = {};
-  unsigned long long amount[kEach] = {}, sum = 0;
-#pragma unroll 4
-  for (int c = 0; c < ctas; ++c) {
-    const Shared* from = cluster.map_shared_rank(&s, c);
-    const uint4 n = *reinterpret_cast<const uint4*>(&from->counts[threadIdx.x * kEach]);
-    count[0] += n.x, count[1] += n.y, count[2] += n.z, count[3] += n.w;
-    if (MASS) {
+// What lane c of a warp's first `ctas` lanes reads from CTA c (others: 0), summed
+// over the lanes before, and over all.
+template <typename V>
+__device__ __forceinline__ V lanes_before(V v, V* all) {
+  const int lane = threadIdx.x % 32;
+  V sum = v;
 #pragma unroll
-      for (int e = 0; e < kEach; e += 2) {
-        const ulonglong2 m =
-            *reinterpret_cast<const ulonglong2*>(&from->masses[threadIdx.x * kEach + e]);
-        amount[e] += m.x;
-        amount[e + 1] += m.y;
-      }
-    }
+  for (int o = 1; o < kMostCtas; o <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
   }
-  static_assert(kEach == 4, "bins of a thread");
+  *all = __shfl_sync(0xffffffffu, sum, kMostCtas - 1);
+  return sum - v;
+}
+
+// The first bin at which the cluster's counts (MASS: masses), with `before`,
+// reach the target: into s.found of every CTA, with what is before it, its count and the
+// sum of all; bin -1 where they do not. Each CTA adds up its part of the bins, a
+// thread four of them from one CTA: were every CTA to read all of them, 16 CTAs'
+// reads of 24 KB each from 16 others took 50 us. With share >= 0 the target is
+// that part of the sum, at least 1.
+template <bool MASS>
+__device__ void find_bin(cg::cluster_group& cluster, Shared& s, unsigned long long before,
+                         unsigned long long target, float share) {
+  static_assert(kBins == 4 * kThreads, "four bins of one CTA a thread");
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int bins = kBins / ctas, quads = bins / 4;  // of this CTA
+  uint32_t* const counts = ctas > 1 ? s.part_counts : s.counts;
+  const Wide masses = ctas > 1 ? Wide{s.part_masses[0], s.part_masses[1]}
+                               : Wide{s.masses[0], s.masses[1]};
+  if (ctas > 1) {
+    for (int i = threadIdx.x; i < bins; i += kThreads)
+      counts[i] = masses.low[i] = masses.high[i] = 0;
+    __syncthreads();
+    // (The CTAs begin with different ones.)
+    const int c = (threadIdx.x / quads + rank) % ctas, q = threadIdx.x % quads;
+    const Shared* from = cluster.map_shared_rank(&s, c);
+    const uint4 n = *reinterpret_cast<const uint4*>(&from->counts[rank * bins + 4 * q]);
+    const uint32_t count[4] = {n.x, n.y, n.z, n.w};
+    if (MASS) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(&from->masses[0][rank * bins + 4 * q]);
+      const uint4 hi = *reinterpret_cast<const uint4*>(&from->masses[1][rank * bins + 4 * q]);
+      const unsigned long long mass[4] = {
+          (unsigned long long)hi.x << 32 | lo.x, (unsigned long long)hi.y << 32 | lo.y,
+          (unsigned long long)hi.z << 32 | lo.z, (unsigned long long)hi.w << 32 | lo.w};
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    if (!MASS) amount[e] = count[e];
+      for (int e = 0; e < 4; ++e)
+        if (mass[e]) masses.add(4 * q + e, mass[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (count[e]) atomicAdd(&counts[4 * q + e], count[e]);
+    __syncthreads();
+  }
+  const int each = (bins + kThreads - 1) / kThreads;  // 1 to 4
+  unsigned long long amount[4], sum = 0, mine;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int i = threadIdx.x * each + e;
+    amount[e] = e < each && i < bins ? MASS ? masses.get(i) : counts[i] : 0;
     sum += amount[e];
   }
-  unsigned long long all, at = before + block_scan(s, sum, &all);
+  unsigned long long at = block_scan(s, sum, &mine), all;
+  if (threadIdx.x == 0) s.part = mine;
+  cluster.sync();
+  const unsigned long long other =
+      lane < ctas ? cluster.map_shared_rank(&s, lane)->part : 0;
+  const unsigned long long ahead = lanes_before(other, &all);
+  at += before + __shfl_sync(0xffffffffu, ahead, rank);
   if (MASS && share >= 0.f) {
     const double part = ceil((double)share * (double)all);
     target = part < 1.0 ? 1 : (unsigned long long)part;
     if (target > all) target = all;
   }
-  if (threadIdx.x == 0) s.bin = -1;
-  __syncthreads();
+  if (before + all < target) {  // the same everywhere
+    if (threadIdx.x == 0) s.found = Found{-1, 0, 0, all};
+  } else {
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    if (at < target && at + amount[e] >= target) {
-      s.bin = threadIdx.x * kEach + e;
-      s.count = (int)count[e];
-      s.before = at;
+    for (int e = 0; e < 4; ++e) {
+      const int i = threadIdx.x * each + e;
+      if (at < target && at + amount[e] >= target) {
+        const Found found{rank * bins + i, (int)counts[i], at, all};
+        for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&s, c)->found = found;
+      }
+      at += amount[e];
     }
-    at += amount[e];
   }
-  __syncthreads();
-  return all;
+  (void)warp;
+  cluster.sync();
 }
 
 // The key of the first token (in the order) at which what is counted, 1 or the
@@ -314,7 +406,9 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
   int shift = 0, coarse_bin = -1;
   unsigned long long before = 0;       // of the tokens ahead of them
   for (int round = 0;; ++round) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0, s.masses[i] = 0;
+    const Wide masses{s.masses[0], s.masses[1]};
+    for (int i = threadIdx.x; i < kBins; i += kThreads)
+      s.counts[i] = masses.low[i] = masses.high[i] = 0;
     if (threadIdx.x == 0) s.listed = 0, s.bounds[0] = ~0ull, s.bounds[1] = 0;
     __syncthreads();
     row.each_value([&](float x, int i) {
@@ -326,21 +420,19 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
         bin = (int)((high - key) >> shift);
       }
       atomicAdd(&s.counts[bin], 1u);
-      if (MASS) atomicAdd(&s.masses[bin], weigh.weight(x));
+      if (MASS) masses.add(bin, weigh.weight(x));
     });
     cluster.sync();
-    const unsigned long long all = find_bin<MASS>(cluster, s, before, target, round == 0 ? share : -1.f);
+    find_bin<MASS>(cluster, s, before, target, round == 0 ? share : -1.f);
+    const Found its = s.found;
+    if (its.bin < 0) return 0;
     if (MASS && round == 0) {
-      const double part = ceil((double)share * (double)all);
+      const double part = ceil((double)share * (double)its.all);
       target = part < 1.0 ? 1 : (unsigned long long)part;
-      if (target > all) target = all;
+      if (target > its.all) target = its.all;
     }
-    if (before + all < target) {
-      cluster.sync();  // (the bins have been read)
-      return 0;
-    }
-    const int bin = s.bin, found = s.count;
-    before = s.before;
+    const int bin = its.bin, found = its.count;
+    before = its.before;
     if (round == 0) {
       coarse_bin = bin;
     } else {
@@ -371,11 +463,19 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
       }
       cluster.sync();
       low = ~0ull, high = 0;
-      for (int c = 0; c < ctas; ++c) {
-        const Shared* from = cluster.map_shared_rank(&s, c);
-        low = from->bounds[0] < low ? from->bounds[0] : low;
-        high = from->bounds[1] > high ? from->bounds[1] : high;
+      if (lane < ctas) {
+        const Shared* from = cluster.map_shared_rank(&s, lane);
+        low = from->bounds[0];
+        high = from->bounds[1];
       }
+      for (int o = kMostCtas / 2; o; o >>= 1) {
+        const uint64_t a = __shfl_xor_sync(0xffffffffu, low, o);
+        const uint64_t b = __shfl_xor_sync(0xffffffffu, high, o);
+        low = a < low ? a : low;
+        high = b > high ? b : high;
+      }
+      low = __shfl_sync(0xffffffffu, low, 0);
+      high = __shfl_sync(0xffffffffu, high, 0);
     }
     shift = 0;
     while ((high - low) >> shift >= kBins) ++shift;
@@ -388,16 +488,21 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
     if (key >= low && key <= high) s.list[atomicAdd(&s.listed, 1)] = key;
   });
   cluster.sync();
-  int n = 0;
-  for (int c = 0; c < ctas; ++c) {
-    const Shared* from = cluster.map_shared_rank(&s, c);
-    const int some = from->listed;
-    for (int i = threadIdx.x; i < some; i += kThreads) {
-      const uint64_t key = from->list[i];
-      s.all[n + i] = key;
-      s.weights[n + i] = MASS ? weigh.weight(logit_of(key)) : 1;
+  // (A warp for each CTA's list.)
+  static_assert(kWarps >= kMostCtas, "warps for lists");
+  int n;
+  {
+    const int listed = lane < ctas ? cluster.map_shared_rank(&s, lane)->listed : 0;
+    const int ahead = lanes_before(listed, &n), warp = threadIdx.x / 32;
+    const int from0 = __shfl_sync(0xffffffffu, ahead, warp), some = __shfl_sync(0xffffffffu, listed, warp);
+    if (warp < ctas) {
+      const Shared* from = cluster.map_shared_rank(&s, warp);
+      for (int i = lane; i < some; i += 32) {
+        const uint64_t key = from->list[i];
+        s.all[from0 + i] = key;
+        s.weights[from0 + i] = MASS ? weigh.weight(logit_of(key)) : 1;
+      }
     }
-    n += some;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -421,17 +526,40 @@ __device__ __forceinline__ unsigned long long place_of(const cxs_sample_call& a,
   return at < mass ? at : mass - 1;
 }
 
-// Descending, of `n` (a power of two) in shared memory.
+// Descending, of `n` (a power of two) in shared memory. Up to one a thread: in
+// registers, between the lanes of a warp without a barrier (7 times as fast).
 __device__ void sort_down(uint64_t* x, int n) {
+  __syncthreads();
+  if (n > kThreads) {
+    for (int size = 2; size <= n; size <<= 1)
+      for (int step = size / 2; step > 0; step >>= 1) {
+        for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+          const int a = 2 * i - (i & (step - 1)), b = a + step;
+          const uint64_t p = x[a], q = x[b];
+          if ((p < q) == ((a & size) == 0)) x[a] = q, x[b] = p;
+        }
+        __syncthreads();
+      }
+    return;
+  }
+  const int i = threadIdx.x;
+  uint64_t mine = i < n ? x[i] : 0;
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size / 2; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int a = 2 * i - (i & (step - 1)), b = a + step;
-        const uint64_t p = x[a], q = x[b];
-        if ((p < q) == ((a & size) == 0)) x[a] = q, x[b] = p;
+      uint64_t other;
+      if (step >= 32) {
+        __syncthreads();
+        if (i < n) x[i] = mine;
+        __syncthreads();
+        other = i < n ? x[i ^ step] : 0;
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, mine, step);
       }
+      const bool larger = ((i & size) == 0) == ((i & step) == 0);
+      mine = (mine > other) == larger ? mine : other;
     }
+  __syncthreads();
+  if (i < n) x[i] = mine;
   __syncthreads();
 }
 
@@ -533,6 +661,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   const bool listed = greedy || (set.top_k > 0 && set.top_k <= kMostListed &&
                                  set.top_k <= ctas * kThreads / 2);
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0;
+  if (threadIdx.x < 256) s.powers[threadIdx.x] = power_of(threadIdx.x);
   if (threadIdx.x == 0) s.wanted = 0;
 
   // The largest logit, of the thread and of the row; the run into shared memory.
@@ -564,14 +693,43 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     if (lane == 0) s.warp_totals[warp] = top;
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s.warp_totals[w]);
-    if (threadIdx.x == 0) s.top = top;
+    if (threadIdx.x == 0) s.top = top, s.bound = -kInf;
+    if (listed && !greedy && top > -kInf && !wrong) {
+      // At least 1 / ctas of top_k tokens of this CTA lie in the bins that as many
+      // of its threads' maxima reach; the least of these maxima bounds them.
+      const Weigh local(s.powers, top, kLog2e / set.temperature, a.vocab);
+      const int bin = mine > -kInf ? local.bin(mine) : kBins;
+      if (bin < kBins) atomicAdd(&s.counts[bin], 1u);
+      __syncthreads();
+      const uint4 n = *reinterpret_cast<const uint4*>(&s.counts[4 * threadIdx.x]);
+      const unsigned wanted = (set.top_k + ctas - 1) / ctas;
+      unsigned long long all;
+      const unsigned sum = n.x + n.y + n.z + n.w, at = (unsigned)block_scan(s, sum, &all);
+      if (at < wanted && at + sum >= wanted)
+        s.found.bin = 4 * threadIdx.x + (at + n.x < wanted) + (at + n.x + n.y < wanted) +
+                      (at + n.x + n.y + n.z < wanted);
+      __syncthreads();
+      float least = all >= wanted && bin <= s.found.bin ? mine : kInf;
+      for (int o = 16; o; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+      if (lane == 0) s.warp_totals[warp] = least;
+      __syncthreads();
+      if (threadIdx.x == 0 && all >= wanted) {
+        for (int w = 0; w < kWarps; ++w) least = fminf(least, s.warp_totals[w]);
+        s.bound = least;
+      }
+    }
   }
   cluster.sync();
-  Weigh weigh;
-  weigh.top = -kInf;
-  for (int c = 0; c < ctas; ++c) weigh.top = fmaxf(weigh.top, cluster.map_shared_rank(&s, c)->top);
+  float top = lane < ctas ? cluster.map_shared_rank(&s, lane)->top : -kInf;
+  float bound = lane < ctas ? cluster.map_shared_rank(&s, lane)->bound : kInf;
+  for (int o = kMostCtas / 2; o; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bound = fminf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+  }
+  top = __shfl_sync(0xffffffffu, top, 0);
+  bound = __shfl_sync(0xffffffffu, bound, 0);
   const long long draws = (long long)r * a.draws;
-  if (wrong || weigh.top == -kInf) {  // no answer
+  if (wrong || top == -kInf) {  // no answer
     if (rank == 0)
       for (int d = threadIdx.x; d < a.draws; d += kThreads) {
         a.tokens[draws + d] = -1;
@@ -580,27 +738,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     cluster.sync();
     return;
   }
-  weigh.rate = greedy ? 0.0 : kLog2e / set.temperature;
-  weigh.rate32 = fminf((float)weigh.rate, 1e30f);
-  weigh.bits = min(51, 62 - (32 - __clz(a.vocab)));
+  const Weigh weigh(s.powers, top, greedy ? 0.0 : kLog2e / set.temperature, a.vocab);
   const bool want = a.logprobs != nullptr;
 
   if (listed) {
-    // The bin that top_k of the threads' maxima reach: so many tokens at least lie
-    // in it and before it.
-    int last = 0;
-    if (greedy) {
-      set.top_k = 1;
-    } else {
-      if (mine > -kInf) atomicAdd(&s.counts[weigh.bin(mine)], 1u);
-      cluster.sync();
-      find_bin<false>(cluster, s, 0, set.top_k, -1.f);
-      last = s.bin < 0 ? kBins - 1 : s.bin;
-    }
+    if (greedy) set.top_k = 1, bound = top;
     Shared* const first = cluster.map_shared_rank(&s, 0);
     float total = 0.f;
     row.each_value([&](float x, int i) {
-      if (greedy ? x == weigh.top : x > -kInf && weigh.bin(x) <= last) {
+      if (x >= bound && x > -kInf) {
         const int at = atomicAdd(&first->wanted, 1);
         if (at < kList) first->gathered[at] = key_of(x, i);
       }
@@ -613,9 +759,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     cluster.sync();
     const int n = first->wanted;
     if (n <= kList) {
-      total = 0.f;
-      if (rank == 0 && want)
-        for (int c = 0; c < ctas; ++c) total += cluster.map_shared_rank(&s, c)->total;
+      lanes_before(rank == 0 && want && lane < ctas ? cluster.map_shared_rank(&s, lane)->total : 0.f,
+                   &total);
       cluster.sync();  // (what is read of other CTAs has been)
       if (rank == 0) draw_listed(a, s, weigh, set, n, draws, logf(total));
       return;
@@ -637,16 +782,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     cut = other > cut ? other : cut;
   }
 
-  // Kept mass of every warp's run, and the sum of exp(x - M) over all tokens.
+  // Kept mass of every warp's run and of its parts, and the sum of exp(x - M) over
+  // all tokens.
   const Cut keep(cut);
+  const int begin = row.begin(warp), stop = row.begin(warp + 1);
+  const int rounds = ((row.each + 31) / 32 + kBlocks - 1) / kBlocks;  // of a part
   unsigned long long mass = 0;
   float total = 0.f;
-  row.each_value([&](float x, int i) {
-    if (keep.keeps(x, i)) mass += weigh.weight(x);
-    if (want) total += weigh.odds(x);
-  });
+  auto weigh_all = [&](auto add) {
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (begin + lane < stop) next = row.load(begin + lane);
+    for (int v0 = begin, part = 0; v0 < stop; ++part) {
+      unsigned long long sum = 0;
+#pragma unroll 1
+      for (int k = 0; k < rounds && v0 < stop; ++k, v0 += 32) {
+        const uint4 w = next;
+        const int v = v0 + lane;
+        if (v + 32 < stop) next = row.load(v + 32);
+        if (v >= stop) continue;
+        float x[kVector];
+        Row<T>::unpack(w, x);
+#pragma unroll
+        for (int e = 0; e < kVector; ++e) {
+          sum = add(sum, x[e], row.index(v, e));
+          if (want) total += weigh.odds(x[e]);
+        }
+      }
+      __syncwarp();
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s.blocks[warp][part] = sum;
+      mass += sum;
+    }
+  };
+  if (cut == 0 && weigh.top < kInf)
+    weigh_all([&](unsigned long long sum, float x, int) { return weigh.add(sum, x); });
+  else
+    weigh_all([&](unsigned long long sum, float x, int i) {
+      return keep.keeps(x, i) ? sum + weigh.weight(x) : sum;
+    });
   __syncwarp();
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
   total = want ? block_sum(s, total) : 1.f;
   unsigned long long all;
   const unsigned long long ahead = block_scan(s, lane == 0 ? mass : 0, &all);
@@ -656,14 +830,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     s.mass = all;
   }
   cluster.sync();
-  unsigned long long before = 0, kept_mass = 0;
-  total = 0.f;
-  for (int c = 0; c < ctas; ++c) {
-    const Shared* from = cluster.map_shared_rank(&s, c);
-    if (c == rank) before = kept_mass;
-    kept_mass += from->mass;
-    total += from->total;
-  }
+  const Shared* const other = cluster.map_shared_rank(&s, min(lane, ctas - 1));
+  unsigned long long kept_mass;
+  unsigned long long before = lanes_before(lane < ctas ? other->mass : 0, &kept_mass);
+  before = __shfl_sync(0xffffffffu, before, rank);
+  lanes_before(lane < ctas ? other->total : 0.f, &total);
   cluster.sync();  // (the sums have been read)
   const float log_total = logf(total);
 
@@ -677,15 +848,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
                     at < (lane + 1 < kWarps ? s.spans[lane + 1] : all);
     const int w = __ffs(__ballot_sync(0xffffffffu, in)) - 1;
     at -= s.spans[w];
-    const int stop = row.begin(w + 1);
-    for (int v0 = row.begin(w); v0 < stop; v0 += 32) {
+    // The part of the run: four a lane.
+    static_assert(kBlocks == 4 * 32, "four parts a lane");
+    const int its_begin = row.begin(w), its_stop = row.begin(w + 1);
+    const int parts = (its_stop - its_begin + 32 * rounds - 1) / (32 * rounds);
+    unsigned long long four[4], sum4 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      four[e] = 4 * lane + e < parts ? s.blocks[w][4 * lane + e] : 0;
+      sum4 += four[e];
+    }
+    unsigned long long to4 = sum4;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, to4, o);
+      if (lane >= o) to4 += up;
+    }
+    int part = 0;
+    unsigned long long rest = at - (to4 - sum4);
+    const unsigned holds = __ballot_sync(0xffffffffu, at < to4 && at >= to4 - sum4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (part == e && rest >= four[e]) rest -= four[e], ++part;
+    }
+    const int owner = __ffs(holds) - 1;
+    at = __shfl_sync(0xffffffffu, rest, owner);
+    const int its_part = 4 * owner + __shfl_sync(0xffffffffu, part, owner);
+    const int from = its_begin + its_part * 32 * rounds, to_v = min(its_stop, from + 32 * rounds);
+    for (int v0 = from; v0 < to_v; v0 += 32) {
       const int v = v0 + lane;
       float x[kVector];
       unsigned long long weights[kVector], sum = 0;
-      if (v < stop) Row<T>::unpack(row.load(v), x);
+      if (v < to_v) Row<T>::unpack(row.load(v), x);
 #pragma unroll
       for (int e = 0; e < kVector; ++e) {
-        weights[e] = v < stop && keep.keeps(x[e], row.index(v, e)) ? weigh.weight(x[e]) : 0;
+        weights[e] = v < to_v && keep.keeps(x[e], row.index(v, e)) ? weigh.weight(x[e]) : 0;
         sum += weights[e];
       }
       unsigned long long to = sum;
@@ -717,12 +913,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
 }
 
 // CTAs of a row's cluster: as many as still run at once (two to an SM) and have
-// kLeast values each, and so many that the row fits into their shared memory.
-int ctas_of(const cxs_sample_call& a, int size) {
+// kLeast values each.
+int ctas_of(const cxs_sample_call& a) {
   constexpr int kAtOnce = 296, kLeast = 2048;
   int ctas = 1;
-  while (ctas < kMostCtas && ((long long)a.rows * ctas * 2 <= kAtOnce && a.vocab >= 2 * kLeast * ctas ||
-                              (long long)a.vocab * size > (long long)ctas * (kSliceBytes - 64)))
+  while (ctas < kMostCtas && (long long)a.rows * ctas * 2 <= kAtOnce && a.vocab >= 2 * kLeast * ctas)
     ctas *= 2;
   return ctas;
 }
@@ -737,7 +932,7 @@ int launch(const cxs_sample_call& a, cudaStream_t stream) {
     return (int)CXS_OK;
   });
   if (status != CXS_OK) return status;
-  const int ctas = ctas_of(a, sizeof(T));
+  const int ctas = ctas_of(a);
   // (A row may begin inside a vector, and vectors are shared out whole.)
   const long long vectors = ((long long)a.vocab * sizeof(T) + 15) / 16 + 1;
   const long long bytes = (vectors + ctas - 1) / ctas * 16;
