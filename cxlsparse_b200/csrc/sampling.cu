@@ -41,8 +41,8 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kBinsPerOctave = 32;   // of the weight: 64 octaves in all
 constexpr int kFew = 512;            // tokens whose ranks are counted one by one
-constexpr int kList = 2048;          // tokens that are gathered for a small top_k
-constexpr int kMostListed = 1024;    // largest such top_k
+constexpr int kList = kThreads;      // tokens that are gathered for a small top_k
+constexpr int kMostListed = 384;     // largest such top_k
 constexpr int kMostCtas = 16;        // of a cluster
 constexpr int kBlocks = 128;         // parts of a warp's run whose kept mass is kept
 constexpr int kSliceBytes = 72 << 10;  // of a CTA's run in shared memory: two CTAs fit an SM
@@ -213,21 +213,28 @@ struct Row {
     for (int e = 0; e < kVector; ++e) x[e] = fmaxf(to_float(y[e]), -kInf);
   }
   // f(logit, index) for this warp's tokens; the next vector is on its way meanwhile.
+  // Only four bytes' copies of f: what runs once in a launch runs from a cold
+  // instruction cache, where its length counts.
   template <typename F>
   __device__ __forceinline__ void each_value(F f) const {
+    constexpr int kPair = 4 / sizeof(T);
     const int warp = threadIdx.x / 32, stop = begin(warp + 1);
     int v = begin(warp) + threadIdx.x % 32;
     uint4 next = make_uint4(0, 0, 0, 0);
     if (v < stop) next = load(v);
 #pragma unroll 1
     for (; v < stop; v += 32) {
-      const uint4 w = next;
+      uint4 w = next;
       if (v + 32 < stop) next = load(v + 32);
-      float x[kVector];
-      unpack(w, x);
-      const int i = index(v, 0);
+      int i = index(v, 0);
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        alignas(4) T y[kPair];
+        *reinterpret_cast<uint32_t*>(y) = w.x;
+        w.x = w.y, w.y = w.z, w.z = w.w;
 #pragma unroll
-      for (int e = 0; e < kVector; ++e) f(x[e], i + e);
+        for (int e = 0; e < kPair; ++e, ++i) f(fmaxf(to_float(y[e]), -kInf), i);
+      }
     }
   }
 };
@@ -526,120 +533,47 @@ __device__ __forceinline__ unsigned long long place_of(const cxs_sample_call& a,
   return at < mass ? at : mass - 1;
 }
 
-// Descending, of `n` (a power of two) in shared memory. Up to one a thread: in
-// registers, between the lanes of a warp without a barrier (7 times as fast).
-__device__ void sort_down(uint64_t* x, int n) {
-  __syncthreads();
-  if (n > kThreads) {
-    for (int size = 2; size <= n; size <<= 1)
-      for (int step = size / 2; step > 0; step >>= 1) {
-        for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-          const int a = 2 * i - (i & (step - 1)), b = a + step;
-          const uint64_t p = x[a], q = x[b];
-          if ((p < q) == ((a & size) == 0)) x[a] = q, x[b] = p;
-        }
-        __syncthreads();
-      }
-    return;
-  }
-  const int i = threadIdx.x;
-  uint64_t mine = i < n ? x[i] : 0;
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size / 2; step > 0; step >>= 1) {
-      uint64_t other;
-      if (step >= 32) {
-        __syncthreads();
-        if (i < n) x[i] = mine;
-        __syncthreads();
-        other = i < n ? x[i ^ step] : 0;
-      } else {
-        other = __shfl_xor_sync(0xffffffffu, mine, step);
-      }
-      const bool larger = ((i & size) == 0) == ((i & step) == 0);
-      mine = (mine > other) == larger ? mine : other;
-    }
-  __syncthreads();
-  if (i < n) x[i] = mine;
-  __syncthreads();
-}
-
 // Draws from the `n` gathered tokens (all that may be kept, and perhaps some
-// more): one CTA. log_total: of the sum of exp(x - M).
-__device__ void draw_listed(const cxs_sample_call& a, Shared& s, const Weigh& weigh,
-                            const Settings& set, int n, long long draws, float log_total) {
-  constexpr int kEach = kList / kThreads;
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) s.gathered[i] = 0;
-  sort_down(s.gathered, size);
-  // The kept ones are the first: at most top_k, with w >= min_p, and then top_p.
-  int most = min(n, set.top_k);
-  const double least = set.min_p > 0.f
-      ? (double)weigh.top + (double)set.temperature * log((double)set.min_p) : -INFINITY;
-  unsigned long long w[kEach], sum = 0;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    w[e] = 0;
-    if (i < most) {
-      const float x = logit_of(s.gathered[i]);
-      if (x == weigh.top || (double)x >= least) w[e] = weigh.weight(x);
-    }
-    sum += w[e];
-  }
-  unsigned long long mass, before = block_scan(s, sum, &mass);
-  const double part = set.top_p < 1.f ? (double)set.top_p * (double)mass : INFINITY;
-  // By index: the same keys with index (larger first) and place.
-  unsigned long long kept = 0;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    if (i > 0 && !((double)before < part)) w[e] = 0;
-    before += w[e];
-    kept += w[e];
-  }
-  block_scan(s, kept, &mass);
-  uint64_t mine[kEach];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    mine[e] = i < n ? s.gathered[i] : 0;
-  }
+// more): one CTA. Their places in the order and by index are counted, each
+// token's by as many lanes of a warp as there are for it: two bitonic sorts took
+// 4 us each for 200 tokens. log_total: of the sum of exp(x - M).
+__device__ __forceinline__ void draw_listed(const cxs_sample_call& a, Shared& s, const Weigh& weigh,
+                                            const Settings& set, int n, long long draws,
+                                            float log_total) {
+  int lanes = 1;
+  while (lanes < 32 && 2 * lanes * n <= kThreads) lanes *= 2;
+  const int mine = threadIdx.x / lanes, from = threadIdx.x % lanes;
+  uint64_t key = mine < n ? s.gathered[mine] : 0;
+  int place = 0;
+  for (int j = from; j < n; j += lanes) place += s.gathered[j] > key;
+  for (int o = lanes / 2; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+  if (from == 0 && mine < n) s.all[place] = key;
   __syncthreads();
-  // (Tokens of no weight cannot be drawn and need no place.)
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    if (i < size)
-      s.gathered[i] = w[e] ? (uint64_t)(uint32_t)mine[e] << 32 | (uint32_t)(mine[e] >> 32) : 0;
-  }
-  sort_down(s.gathered, size);
-  sum = 0;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    mine[e] = i < size ? s.gathered[i] : 0;
-    mine[e] = mine[e] << 32 | mine[e] >> 32;
-    w[e] = mine[e] ? weigh.weight(logit_of(mine[e])) : 0;
-    sum += w[e];
-  }
-  unsigned long long all;
-  before = block_scan(s, sum, &all);
-  for (int d = 0; d < a.draws; ++d) {
+  // The kept ones are the first: at most top_k, with w >= min_p, and then top_p.
+  key = threadIdx.x < n ? s.all[threadIdx.x] : 0;
+  float x = key ? logit_of(key) : -kInf;
+  const bool kept = threadIdx.x < min(n, set.top_k) && (set.min_p == 0.f || x == weigh.top ||
+      (double)x >= (double)weigh.top + (double)set.temperature * log((double)set.min_p));
+  unsigned long long w = kept ? weigh.weight(x) : 0, mass;
+  unsigned long long before = block_scan(s, w, &mass);
+  if (threadIdx.x > 0 && set.top_p < 1.f && !((double)before < (double)set.top_p * (double)mass))
+    w = 0;
+  s.weights[threadIdx.x] = w;
+  const int count = __syncthreads_count(w > 0);
+  // (Tokens without weight lie behind those that have some.)
+  block_scan(s, w, &mass);
+  key = mine < count ? s.all[mine] : 0;
+  w = mine < count ? s.weights[mine] : 0;
+  before = 0;
+  for (int j = from; j < count; j += lanes)
+    before += (uint32_t)s.all[j] > (uint32_t)key ? s.weights[j] : 0;
+  for (int o = lanes / 2; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  x = logit_of(key);
+  for (int d = from; d < a.draws; d += lanes) {
     const unsigned long long at = place_of(a, draws + d, mass);
-    if (at < before || at >= before + sum) continue;
-    unsigned long long left = at - before;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (left < w[e]) {
-        const float x = logit_of(mine[e]);
-        a.tokens[draws + d] = index_of(mine[e]);
-        if (a.logprobs)
-          a.logprobs[draws + d] = (x == weigh.top ? 0.f : x - weigh.top) - log_total;
-        break;
-      }
-      left -= w[e];
-    }
+    if (at < before || at >= before + w) continue;
+    a.tokens[draws + d] = index_of(key);
+    if (a.logprobs) a.logprobs[draws + d] = (x == weigh.top ? 0.f : x - weigh.top) - log_total;
   }
 }
 
@@ -874,14 +808,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     at = __shfl_sync(0xffffffffu, rest, owner);
     const int its_part = 4 * owner + __shfl_sync(0xffffffffu, part, owner);
     const int from = its_begin + its_part * 32 * rounds, to_v = min(its_stop, from + 32 * rounds);
-    for (int v0 = from; v0 < to_v; v0 += 32) {
-      const int v = v0 + lane;
-      float x[kVector];
-      unsigned long long weights[kVector], sum = 0;
-      if (v < to_v) Row<T>::unpack(row.load(v), x);
+    // Four bytes a lane at a time.
+    constexpr int kPair = 4 / sizeof(T);
+#pragma unroll 1
+    for (int u0 = 4 * from; u0 < 4 * to_v; u0 += 32) {
+      const int u = u0 + lane;
+      const uint4 vector = row.load(min(u / 4, to_v - 1));
+      alignas(4) T y[kPair];
+      *reinterpret_cast<uint32_t*>(y) = u % 4 == 0 ? vector.x : u % 4 == 1 ? vector.y
+                                      : u % 4 == 2 ? vector.z : vector.w;
+      unsigned long long weights[kPair], sum = 0;
+      float x[kPair];
 #pragma unroll
-      for (int e = 0; e < kVector; ++e) {
-        weights[e] = v < to_v && keep.keeps(x[e], row.index(v, e)) ? weigh.weight(x[e]) : 0;
+      for (int e = 0; e < kPair; ++e) {
+        x[e] = fmaxf(to_float(y[e]), -kInf);
+        const bool in = u < 4 * to_v && keep.keeps(x[e], row.index(0, u * kPair + e));
+        weights[e] = in ? weigh.weight(x[e]) : 0;
         sum += weights[e];
       }
       unsigned long long to = sum;
@@ -897,9 +839,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       if (at < to && at >= to - sum) {
         unsigned long long left = at - (to - sum);
 #pragma unroll
-        for (int e = 0; e < kVector; ++e) {
+        for (int e = 0; e < kPair; ++e) {
           if (left < weights[e]) {
-            a.tokens[draws + d] = row.index(v, e);
+            a.tokens[draws + d] = row.index(0, u * kPair + e);
             if (want)
               a.logprobs[draws + d] = (x[e] == weigh.top ? 0.f : x[e] - weigh.top) - log_total;
             break;
