@@ -28,6 +28,8 @@
 #include <float.h>
 #include <limits.h>
 
+#include <type_traits>
+
 #include "cache8.cuh"
 
 using cxs_host::set_error;
@@ -40,6 +42,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kBinsPerOctave = 32;   // of the weight: 64 octaves in all
+constexpr int kPowers = 512;         // of two, in a table
 constexpr int kFew = 512;            // tokens whose ranks are counted one by one
 constexpr int kList = kThreads;      // tokens that are gathered for a small top_k
 constexpr int kMostListed = 384;     // largest such top_k
@@ -62,10 +65,10 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-// 2^(32 - i / 256), rounded (below 2^32 for i = 0), by Taylor's polynomial: the
+// 2^(32 - i / kPowers), rounded (below 2^32 for i = 0), by Taylor's polynomial: the
 // exponent is at most ln 2, the next term below 2^-48.
 __device__ __forceinline__ uint32_t power_of(int i) {
-  const double g = i * (-0.6931471805599453 / 256);
+  const double g = i * (-0.6931471805599453 / kPowers);
   double p = 1.0;
 #pragma unroll
   for (int k = 13; k > 0; --k) p = fma(p, g * (1.0 / k), 1.0);
@@ -132,7 +135,7 @@ struct Shared {
   Found found;
   uint64_t cut;
   float warp_totals[kWarps];
-  uint32_t powers[256];                        // 2^(32 - i / 256)
+  uint32_t powers[kPowers];                    // 2^(32 - i / kPowers)
 };
 
 // Sum of v over the threads before this one; *total: over all.
@@ -205,12 +208,35 @@ struct Row {
       x[e] = i + e >= 0 && i + e < vocab ? from[e] : cxs::cache8::from_float<T>(-kInf);
     return *reinterpret_cast<const uint4*>(x);
   }
-  // Its values, NaN as -infinity.
+  // NaN as -infinity, in all values of a vector.
+  static __device__ __forceinline__ uint4 without_nan(uint4 w) {
+    auto two = [](uint32_t x) {
+      if constexpr (sizeof(T) == 4) return __float_as_uint(fmaxf(__uint_as_float(x), -kInf));
+      else return bits_of(larger(pair_of(x), pair_of(lowest())));
+    };
+    return make_uint4(two(w.x), two(w.y), two(w.z), two(w.w));
+  }
+  // The larger ones of two vectors' values, NaN counting as nothing.
+  static __device__ __forceinline__ uint4 larger_of(uint4 a, uint4 b) {
+    auto two = [](uint32_t x, uint32_t y) {
+      if constexpr (sizeof(T) == 4)
+        return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+      else return bits_of(larger(pair_of(x), pair_of(y)));
+    };
+    return make_uint4(two(a.x, b.x), two(a.y, b.y), two(a.z, b.z), two(a.w, b.w));
+  }
+  static __device__ __forceinline__ uint32_t lowest() {  // -infinity, one or two
+    return sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  }
+  using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  static __device__ __forceinline__ Pair pair_of(uint32_t x) { return *reinterpret_cast<Pair*>(&x); }
+  static __device__ __forceinline__ uint32_t bits_of(Pair x) { return *reinterpret_cast<uint32_t*>(&x); }
+  static __device__ __forceinline__ Pair larger(Pair a, Pair b) { return __hmax2(a, b); }
   static __device__ __forceinline__ void unpack(uint4 w, float (&x)[kVector]) {
     alignas(16) T y[kVector];
     *reinterpret_cast<uint4*>(y) = w;
 #pragma unroll
-    for (int e = 0; e < kVector; ++e) x[e] = fmaxf(to_float(y[e]), -kInf);
+    for (int e = 0; e < kVector; ++e) x[e] = to_float(y[e]);
   }
   // f(logit, index) for this warp's tokens; the next vector is on its way meanwhile.
   // Only four bytes' copies of f: what runs once in a launch runs from a cold
@@ -224,7 +250,7 @@ struct Row {
     if (v < stop) next = load(v);
 #pragma unroll 1
     for (; v < stop; v += 32) {
-      uint4 w = next;
+      uint4 w = without_nan(next);
       if (v + 32 < stop) next = load(v + 32);
       int i = index(v, 0);
 #pragma unroll 1
@@ -233,7 +259,7 @@ struct Row {
         *reinterpret_cast<uint32_t*>(y) = w.x;
         w.x = w.y, w.y = w.z, w.z = w.w;
 #pragma unroll
-        for (int e = 0; e < kPair; ++e, ++i) f(fmaxf(to_float(y[e]), -kInf), i);
+        for (int e = 0; e < kPair; ++e, ++i) f(to_float(y[e]), i);
       }
     }
   }
@@ -251,11 +277,13 @@ struct Cut {
   }
 };
 
-// What a row's tokens are weighed by. 2^-t with t = n + i / 256 + r, r < 2^-8:
-// t comes from fp64 as a fixed-point number (exact to 2^-33), 2^-(i / 256) from a
-// table of 32 bits, and 1 - 2^-r, at most 2^-8.5, from its Taylor polynomial in
-// fp32, whose rounding errors are then 2^-32 of the weight. A third of the
-// instructions of a polynomial in fp64.
+// What a row's tokens are weighed by. 2^-t with t = n + i / 512 + r, r < 2^-9:
+// t comes from fp64 as a fixed-point number (exact to 2^-33), 2^-(i / 512) from a
+// table of 32 bits, and 1 - 2^-r, at most 2^-9.5, from its Taylor polynomial in
+// fp32, whose rounding errors are then 2^-33 of the weight. Integer instructions
+// bound the pass over all tokens, so there are few of them: 58 instructions a
+// token, 24 for the integer unit, became 35 and 12, and 256 rows of 128000 tokens
+// %LARGE%.
 struct Weigh {
   float top;       // largest logit
   float least;     // below it a weight is nothing
@@ -284,27 +312,34 @@ struct Weigh {
     const double t = fma((double)top - (double)x, rate, 1572864.0);
     const uint32_t fraction = (uint32_t)__double2loint(t);
     const int n = __double2hiint(t) - 0x41380000;
-    // r in units of 2^-31, 1 - 2^-r in the low 23 bits of `less`.
-    const float r = __uint_as_float(0x4b000000u | (fraction >> 1 & 0x7fffffu)) - 8388608.f;
-    const float kLn2 = 0.693147181f, kUnit = 4.65661287e-10f;  // 2^-31
+    // r and 1 - 2^-r in units of 2^-32, in the low 23 bits of floats from 2^23 on.
+    const float r = __uint_as_float(0x4b000000u | (fraction & 0x7fffffu)) - 8388608.f;
+    const float kLn2 = 0.693147181f, kUnit = 2.32830644e-10f;  // 2^-32
     float less = fmaf(r, kLn2 * kLn2 * kLn2 / 6 * kUnit * kUnit, -kLn2 * kLn2 / 2 * kUnit);
     less = fmaf(r, less, kLn2);
     less = fmaf(r, less, 8388608.f);
-    const uint32_t power = powers[fraction >> 24];
-    const uint32_t w = power - __umulhi(power, __float_as_uint(less) << 1 & 0xffffffu);
-    // w 2^(bits - 32 - n): shifted down in 32 bits or up by a product.
-    const int up = bits - 32 - n;
-    const uint32_t down = up >= 0 ? w : up > -32 ? w >> -up : 0;
-    return sum + (unsigned long long)down * (1u << max(up, 0));
+    const uint32_t power = powers[fraction >> 23];
+    const uint32_t w = power - __umulhi(power, __float_as_uint(less) - 0x4b000000u);
+    // w 2^(bits - 32 - n): up by a product or down by a shift. (Shifts by more than
+    // 31, or fewer than none, leave nothing: one of the two is 0.)
+    uint32_t up, down;
+    asm("shl.b32 %0, 2, %1;" : "=r"(up) : "r"(bits - 33 - n));
+    asm("shr.u32 %0, %1, %2;" : "=r"(down) : "r"(w), "r"(n + 32 - bits));
+    asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(sum) : "r"(w), "r"(up));
+    asm("mad.wide.u32 %0, %1, 1, %0;" : "+l"(sum) : "r"(down));
+    return sum;
   }
   __device__ __forceinline__ unsigned long long weight(float x) const {
     if (top == kInf) return x == top ? 1ull << bits : 0;
     return x >= least ? add(0, x) : 0;
   }
   __device__ __forceinline__ float odds(float x) const {  // exp(x - M)
+    return x == top ? 1.f : finite_odds(x);
+  }
+  __device__ __forceinline__ float finite_odds(float x) const {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - top) * (float)kLog2e));
-    return x == top ? 1.f : y;
+    return y;
   }
 };
 
@@ -595,12 +630,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   const bool listed = greedy || (set.top_k > 0 && set.top_k <= kMostListed &&
                                  set.top_k <= ctas * kThreads / 2);
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0;
-  if (threadIdx.x < 256) s.powers[threadIdx.x] = power_of(threadIdx.x);
+  static_assert(kPowers == kThreads, "a power a thread");
+  s.powers[threadIdx.x] = power_of(threadIdx.x);
   if (threadIdx.x == 0) s.wanted = 0;
 
   // The largest logit, of the thread and of the row; the run into shared memory.
   float mine = -kInf;
   {
+    uint4 largest = make_uint4(Row<T>::lowest(), Row<T>::lowest(), Row<T>::lowest(), Row<T>::lowest());
     T* const keep = slice ? reinterpret_cast<T*>(slice_memory) : nullptr;
     constexpr int kAtOnce = 8;
     const int stop = row.begin(warp + 1);
@@ -613,12 +650,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       for (int j = 0; j < kAtOnce; ++j) {
         if (v0 + 32 * j >= stop) break;
         if (keep) *reinterpret_cast<uint4*>(keep + (v0 + 32 * j) * kVector) = w[j];
-        float x[kVector];
-        Row<T>::unpack(w[j], x);
-#pragma unroll
-        for (int e = 0; e < kVector; ++e) mine = fmaxf(mine, x[e]);
+        largest = Row<T>::larger_of(largest, w[j]);
       }
     }
+    float x[kVector];
+    Row<T>::unpack(largest, x);
+#pragma unroll
+    for (int e = 0; e < kVector; ++e) mine = fmaxf(mine, x[e]);
     if (keep) row.base = keep, row.kept = true;
   }
   {
@@ -730,17 +768,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       unsigned long long sum = 0;
 #pragma unroll 1
       for (int k = 0; k < rounds && v0 < stop; ++k, v0 += 32) {
-        const uint4 w = next;
+        const uint4 w = Row<T>::without_nan(next);
         const int v = v0 + lane;
         if (v + 32 < stop) next = row.load(v + 32);
         if (v >= stop) continue;
         float x[kVector];
         Row<T>::unpack(w, x);
+        const int i = row.index(v, 0);
 #pragma unroll
-        for (int e = 0; e < kVector; ++e) {
-          sum = add(sum, x[e], row.index(v, e));
-          if (want) total += weigh.odds(x[e]);
-        }
+        for (int e = 0; e < kVector; ++e) add(sum, total, x[e], i + e);
       }
       __syncwarp();
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -749,10 +785,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     }
   };
   if (cut == 0 && weigh.top < kInf)
-    weigh_all([&](unsigned long long sum, float x, int) { return weigh.add(sum, x); });
+    weigh_all([&](unsigned long long& sum, float& odds, float x, int) {
+      sum = weigh.add(sum, x);
+      if (want) odds += weigh.finite_odds(x);
+    });
   else
-    weigh_all([&](unsigned long long sum, float x, int i) {
-      return keep.keeps(x, i) ? sum + weigh.weight(x) : sum;
+    weigh_all([&](unsigned long long& sum, float& odds, float x, int i) {
+      if (keep.keeps(x, i)) sum += weigh.weight(x);
+      if (want) odds += weigh.odds(x);
     });
   __syncwarp();
   total = want ? block_sum(s, total) : 1.f;
@@ -813,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
 #pragma unroll 1
     for (int u0 = 4 * from; u0 < 4 * to_v; u0 += 32) {
       const int u = u0 + lane;
-      const uint4 vector = row.load(min(u / 4, to_v - 1));
+      const uint4 vector = Row<T>::without_nan(row.load(min(u / 4, to_v - 1)));
       alignas(4) T y[kPair];
       *reinterpret_cast<uint32_t*>(y) = u % 4 == 0 ? vector.x : u % 4 == 1 ? vector.y
                                       : u % 4 == 2 ? vector.z : vector.w;
@@ -821,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       float x[kPair];
 #pragma unroll
       for (int e = 0; e < kPair; ++e) {
-        x[e] = fmaxf(to_float(y[e]), -kInf);
+        x[e] = to_float(y[e]);
         const bool in = u < 4 * to_v && keep.keeps(x[e], row.index(0, u * kPair + e));
         weights[e] = in ? weigh.weight(x[e]) : 0;
         sum += weights[e];
