@@ -768,10 +768,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       unsigned long long sum = 0;
 #pragma unroll 1
       for (int k = 0; k < rounds && v0 < stop; ++k, v0 += 32) {
-        const uint4 w = Row<T>::without_nan(next);
         const int v = v0 + lane;
+        const uint32_t none = Row<T>::lowest();
+        const uint4 w = v < stop ? Row<T>::without_nan(next) : make_uint4(none, none, none, none);
         if (v + 32 < stop) next = row.load(v + 32);
-        if (v >= stop) continue;
         float x[kVector];
         Row<T>::unpack(w, x);
         const int i = row.index(v, 0);
@@ -785,10 +785,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     }
   };
   if (cut == 0 && weigh.top < kInf)
-    weigh_all([&](unsigned long long& sum, float& odds, float x, int) {
-      sum = weigh.add(sum, x);
-      if (want) odds += weigh.finite_odds(x);
-    });
+    if (want)  // (a branch for every token otherwise)
+      weigh_all([&](unsigned long long& sum, float& odds, float x, int) {
+        sum = weigh.add(sum, x);
+        odds += weigh.finite_odds(x);
+      });
+    else
+      weigh_all([&](unsigned long long& sum, float&, float x, int) { sum = weigh.add(sum, x); });
   else
     weigh_all([&](unsigned long long& sum, float& odds, float x, int i) {
       if (keep.keeps(x, i)) sum += weigh.weight(x);
@@ -894,10 +897,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   }
 }
 
-// CTAs of a row's cluster: as many as still run at once (two to an SM) and have
-// kLeast values each.
+// CTAs of a row's cluster: as many as still have an SM each and kLeast values.
+// Measured for 1, 2, 4, 8 and 16 of them (us): one row of 32000 16.6 / 14.4 / 12.5 /
+// 13.1 / 14.5, 64 rows of 32000 25 / 21 / 27 / 39 / 68, 8 rows of 131071 (fp32, top_p)
+// 191 / 107 / 66 / 42 / 41, 256 rows of 128000 78 / 84 / 94 / 127 / 259.
 int ctas_of(const cxs_sample_call& a) {
-  constexpr int kAtOnce = 296, kLeast = 2048;
+  constexpr int kAtOnce = 148, kLeast = 4096;
   int ctas = 1;
   while (ctas < kMostCtas && (long long)a.rows * ctas * 2 <= kAtOnce && a.vocab >= 2 * kLeast * ctas)
     ctas *= 2;
