@@ -714,13 +714,14 @@ int launch_decode(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t s
 }
 
 template <typename T, int D>
-int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cudaStream_t stream) {
+int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, bool spread,
+                   cudaStream_t stream) {
   // Its CTAs may start while the last CTAs before finish; they wait for them
   // on the device.
   cudaLaunchConfig_t config = {};
-  constexpr int kGroups = 256 / D;  // for few rows: 1024 threads
+  constexpr int kGroups = 256 / D;  // for few rows, or many parts: 1024 threads
   config.gridDim = dim3(z.grid, few ? 1 : kTileRows / 16);
-  config.blockDim = dim3(few ? kGroups * 4 * D : 4 * D);
+  config.blockDim = dim3(few || spread ? kGroups * 4 * D : 4 * D);
   config.stream = stream;
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -729,6 +730,8 @@ int launch_combine(const cxs_cache_attend_call& a, const Shape& z, bool few, cud
   config.numAttrs = 1;
   if (few)
     CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, 16, kGroups>, a, z));
+  else if (spread)
+    CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, kTileRows, kGroups>, a, z));
   else
     CXS_CUDA(cudaLaunchKernelEx(&config, combine_kernel<T, D, kTileRows, 1>, a, z));
   CXS_LAUNCH_CHECK("cache attend join");
@@ -797,13 +800,13 @@ long long cxs::cache8::partial_bytes(const cxs_cache_attend_call& a, bool few) {
          slots * rows * (a.cache.dim + 2) * (long long)sizeof(float);
 }
 
-int cxs::cache8::launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few,
+int cxs::cache8::launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few, bool spread,
                              cudaStream_t s) {
   if (a.cache.type == CXS_TYPE_BF16)
-    return a.cache.dim == 64 ? launch_combine<__nv_bfloat16, 64>(a, z, few, s)
-                             : launch_combine<__nv_bfloat16, 128>(a, z, few, s);
-  return a.cache.dim == 64 ? launch_combine<__half, 64>(a, z, few, s)
-                           : launch_combine<__half, 128>(a, z, few, s);
+    return a.cache.dim == 64 ? launch_combine<__nv_bfloat16, 64>(a, z, few, spread, s)
+                             : launch_combine<__nv_bfloat16, 128>(a, z, few, spread, s);
+  return a.cache.dim == 64 ? launch_combine<__half, 64>(a, z, few, spread, s)
+                           : launch_combine<__half, 128>(a, z, few, spread, s);
 }
 
 extern "C" int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes) {
@@ -849,7 +852,7 @@ extern "C" int cxs_cache_attend(const cxs_cache_attend_call* call, void* stream)
       status = launch_tile(a, z, s);
     }
     if (status != CXS_OK) return status;
-    status = launch_join(a, z, few, s);
+    status = launch_join(a, z, few, false, s);
     if (status != CXS_OK) return status;
   }
   return CXS_OK;

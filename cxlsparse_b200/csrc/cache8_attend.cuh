@@ -249,14 +249,16 @@ struct ItemPlan {     // kTileRows query rows of a group, for every KV head
   int group, tile_row;
   int tiles, common_tiles;
   int user_a, user_b; // its rows' users
+  GroupPlan of;
 };
-struct SharePlan {    // a CTA's tiles and the item they begin in
-  long long low, high;
-  int item, kv_head;
+struct SharePlan {    // a CTA's tiles and the item they begin in (all in one place: a CTA
+  long long low, high;    // begins with reading it)
+  long long total;    // cost of all items
+  int id, kv_head;
+  ItemPlan item;
 };
 struct PlanHead {
-  long long total;    // cost of all items
-  int items, gaps;
+  int gaps;
 };
 struct SharedPlan {
   PlanHead* head;
@@ -271,7 +273,9 @@ struct SharedPlan {
 // One launch of the tile kernel over z.users users (cache8_tile.cu).
 int launch_tile(const cxs_cache_attend_call& a, const Shape& z, cudaStream_t stream);
 // The launch that joins what was left in parts (cache8_attend.cu).
-int launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few, cudaStream_t stream);
+// `spread`: items fall into many parts, read by several groups of threads.
+int launch_join(const cxs_cache_attend_call& a, const Shape& z, bool few, bool spread,
+                cudaStream_t stream);
 int check_attend(const cxs_cache_attend_call* a, const char* what);
 int check_attend_pointers(const cxs_cache_attend_call* a, long long workspace, const char* what);
 int sm_count(int* sms);

@@ -67,9 +67,10 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (__syncthreads_or(broken)) {
     if (threadIdx.x == 0) {
       report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
-      *plan.head = PlanHead{0, 0, 1};
+      *plan.head = PlanHead{1};
       plan.gaps[0] = Gap{0, c.tokens};
     }
+    for (int i = threadIdx.x; i < z.grid; i += kPlanThreads) plan.shares[i].total = 0;
     return;
   }
   // A warp for each group: the tokens that all its rows see, its users' own runs.
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads)
       const GroupPlan group = plan.groups[l];
       const int end = call.groups[l + 1] - 1;
       item.group = l;
+      item.of = group;
       item.tile_row = i - first_item[l];
       const int row0 = item.tile_row * kTileRows;
       const int row1 = min(group.count * z.group, row0 + kTileRows) - 1;
@@ -165,12 +167,11 @@ __global__ void __launch_bounds__(kPlanThreads)
     total += all;
   }
   __syncthreads();
-  if (threadIdx.x == 0) *plan.head = PlanHead{total, (int)items, gaps + 2};
+  if (threadIdx.x == 0) *plan.head = PlanHead{gaps + 2};
   // Where each share begins: among all tiles, without the items' own costs.
   const Shares shares(total, z);
-  for (int i = threadIdx.x; i <= shares.count; i += kPlanThreads) {
-    if (shares.count == 0) break;
-    SharePlan share = {};
+  for (int i = threadIdx.x; i < z.grid; i += kPlanThreads) plan.shares[i].total = total;
+  for (int i = threadIdx.x; shares.count > 0 && i <= shares.count; i += kPlanThreads) {
     long long at = total - (long long)kItemCost * items * c.kv_heads;
     if (i < shares.count) {
       const long long place = shares.begin(i);
@@ -179,16 +180,15 @@ __global__ void __launch_bounds__(kPlanThreads)
         const int m = (l + h + 1) / 2;
         if (plan.items[m].before <= place) l = m; else h = m - 1;
       }
-      const ItemPlan& item = plan.items[l];
-      const int cost = item.tiles + kItemCost;
-      share.item = l;
-      share.kv_head = (int)divide(place - item.before, cost);
-      const long long begin = item.before + (long long)share.kv_head * cost;
-      at = begin - kItemCost * ((long long)l * c.kv_heads + share.kv_head) +
+      const ItemPlan item = plan.items[l];
+      const int cost = item.tiles + kItemCost, kv_head = (int)divide(place - item.before, cost);
+      const long long begin = item.before + (long long)kv_head * cost;
+      at = begin - kItemCost * ((long long)l * c.kv_heads + kv_head) +
            max(place - begin - kItemCost, 0ll);
       plan.shares[i].low = at;
-      plan.shares[i].item = share.item;
-      plan.shares[i].kv_head = share.kv_head;
+      plan.shares[i].id = l;
+      plan.shares[i].kv_head = kv_head;
+      plan.shares[i].item = item;
     }
     if (i > 0) plan.shares[i - 1].high = at;
   }
@@ -281,5 +281,5 @@ extern "C" int cxs_cache_attend_shared(const cxs_cache_shared_call* call, void* 
   CXS_LAUNCH_CHECK("cache attend shared plan");
   status = launch_of<true>(call->attend, z, plan, s);
   if (status != CXS_OK) return status;
-  return launch_join(call->attend, z, false, s);
+  return launch_join(call->attend, z, false, false, s);
 }

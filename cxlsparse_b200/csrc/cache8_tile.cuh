@@ -96,7 +96,7 @@ struct Layout {
   static constexpr int kRaw = kV + kVStages * kPanels * kPanel;  // [stages][K, V]
   static constexpr int kTiles = kRaw + kRawStages * 2 * kRawPart;  // [kRing]
   static constexpr int kBars = kTiles + kRing * (int)sizeof(Tile);
-  static constexpr int kPrefix = kBars + 256;
+  static constexpr int kPrefix = kBars + 320;
   static constexpr int kCounts = kPrefix + (kSlice + 1) * 8;
   static constexpr int kBytes = kCounts + (kSlice + 1) * 4 + 1024;  // and the 1024-byte alignment
   static_assert(kBytes <= 232448, "shared memory of one CTA");
@@ -106,12 +106,13 @@ struct Bars {
   uint64_t raw_full[2][2], raw_free[2][2];          // by raw stage and part
   uint64_t k_full[2], v_full[2], k_free[2], v_free[2];  // by operand stage
   uint64_t s_full[2], s_free[2], p_full[2], q_full[2], o_done[2], o_free[2];  // by group
-  uint64_t drain;
+  uint64_t turn[2][4];  // (SHARED) of a group's warps to take their exponentials
+  uint64_t drain[2];
   int abort;
   int nans;  // V had NaN codes where keys are hidden
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+static_assert(sizeof(Bars) <= 320, "barrier block");
 
 // Stage of use n of a ring of N and the parity of its n-th phase.
 template <int N>
@@ -209,6 +210,30 @@ __device__ __forceinline__ void ld64(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
+// 32 of them.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;"
+      : "=f"(d)
+      : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
+}
+
 // (No memory clobber: loads of what a tile's next columns need move ahead.)
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
@@ -245,10 +270,8 @@ __device__ __forceinline__ int key_tiles(const cxs_cache_attend_call& a, const S
 
 // The item of plan `id` and KV head, its tiles and its group's span: `length`
 // common tokens, the packed rows of the group.
-__device__ __forceinline__ void plan_item(const SharedPlan& plan, const Shape& z, int id,
+__device__ __forceinline__ void plan_item(const ItemPlan& item, const Shape& z, int id,
                                           int kv_head, int kv_heads, Item& p) {
-  const ItemPlan item = plan.items[id];
-  const GroupPlan group = plan.groups[item.group];
   p.id = id;
   p.group = item.group;
   p.tile_row = item.tile_row;
@@ -259,10 +282,10 @@ __device__ __forceinline__ void plan_item(const SharedPlan& plan, const Shape& z
   p.common_tiles = item.common_tiles;
   p.user_a = item.user_a;
   p.user_b = item.user_b;
-  p.user = group.user0;
-  p.rows = group.count * z.group;
+  p.user = item.of.user0;
+  p.rows = item.of.count * z.group;
   p.first = 0;
-  p.span = Span{group.first, group.count, 0, group.shared, 0};
+  p.span = Span{item.of.first, item.of.count, 0, item.of.shared, 0};
 }
 
 // The last of users [lo, hi] whose packed rows begin at or before `row`.
@@ -350,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       cxs::mbar_init(&bars->k_full[i], 4);
       cxs::mbar_init(&bars->v_full[i], 4);
-      cxs::mbar_init(&bars->k_free[i], 1);
-      cxs::mbar_init(&bars->v_free[i], 1);
+      cxs::mbar_init(&bars->k_free[i], SHARED ? 2 : 1);  // (by the last group, or each)
+      cxs::mbar_init(&bars->v_free[i], SHARED ? 2 : 1);
       cxs::mbar_init(&bars->s_full[i], 1);
       cxs::mbar_init(&bars->s_free[i], 4);
       cxs::mbar_init(&bars->p_full[i], 4);
@@ -359,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       cxs::mbar_init(&bars->o_done[i], 1);
       cxs::mbar_init(&bars->o_free[i], 4);
     }
-    cxs::mbar_init(&bars->drain, 1);
+    for (int w = 0; w < 8; ++w) cxs::mbar_init(&bars->turn[w / 4][w % 4], 1);
+    for (int i = 0; i < 2; ++i) cxs::mbar_init(&bars->drain[i], 1);
     bars->abort = 0;
     bars->nans = 0;
     cxs::fence_mbar_init();
@@ -412,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
-  const long long total = SHARED ? plan.head->total : prefix[z.users];
+  const long long total = SHARED ? plan.shares[blockIdx.x].total : prefix[z.users];
   const Shares shares(total, z);
   Partial* const partials = reinterpret_cast<Partial*>(a.workspace);
   Partial& mine = partials[blockIdx.x];
@@ -464,11 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   long long lo = 0, hi = 0;
   Item item = {};
   if constexpr (SHARED) {
+    const SharePlan share = plan.shares[blockIdx.x];
     if ((int)blockIdx.x < shares.count) {
-      const SharePlan mine_now = plan.shares[blockIdx.x];
-      lo = mine_now.low;
-      hi = mine_now.high;
-      plan_item(plan, z, mine_now.item, mine_now.kv_head, c.kv_heads, item);
+      lo = share.low;
+      hi = share.high;
+      plan_item(share.item, z, share.id, share.kv_head, c.kv_heads, item);
     }
   } else if ((int)blockIdx.x < shares.count) {
     hi = (int)blockIdx.x + 1 < shares.count ? locate(shares.begin(blockIdx.x + 1), item)
@@ -486,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     p.kv_head = 0;
     if constexpr (SHARED) {
-      plan_item(plan, z, p.id + 1, 0, c.kv_heads, p);
+      plan_item(plan.items[p.id + 1], z, p.id + 1, 0, c.kv_heads, p);
       return;
     }
     ++p.tile_row;
@@ -513,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* const q_panels = smem + L::kQ + g * L::kPanels * kPanel;
     int tiles = 0;    // of the share
     int mine_s = 0;   // tiles of this group
+    int turns = 0;    // tiles that both groups have had
     float m = -kInf, l = 0.f, back = 1.f;
     bool pending = false;  // an item whose O is still in TMEM:
     Item ended = {};
@@ -555,11 +580,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             row += kAtOnce;
             for (head += kAtOnce; head >= z.group; head -= z.group) ++token;
           }
-#pragma unroll
+          // (One copy of a long loop, from a cold instruction cache.)
+#pragma unroll 1
           for (int j = 0; j < kBatch; ++j) {
             const int r32 = b0 + j * kAtOnce + lane / kLanes, r128 = 32 * (warp % 4) + r32;
             alignas(16) T x[8];
-            *reinterpret_cast<uint4*>(x) = in[j];
+            *reinterpret_cast<uint4*>(x) = in[0];
+#pragma unroll
+            for (int k = 1; k < kBatch; ++k) in[k - 1] = in[k];
             float v[8], top = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -697,87 +725,192 @@ __global__ void __launch_bounds__(kThreads, 1)
         int from = see.x - key0, to = see.y - key0;  // visible columns
         if (SHARED && key0 >= item.common_tiles * kKeys) from = own.x - key0, to = own.y - key0;
         const unsigned missing = tile_info.missing;
-        uint32_t x[kKeys];
-        ld64(s_at, x);
-        ld64(s_at + 64, x + 64);
-        if (L::kApart) {  // S of the next tile may come
-          tc::fence_before();
-          warp_arrive(&bars->s_free[g], lane);
-        }
-        if (!__all_sync(0xffffffffu, from <= 0 && to >= kKeys && missing == 0)) {
-          // What the row does not see becomes -infinity.
-#pragma unroll
-          for (int q = 0; q < kKeys / 32; ++q) {
-            const int low = min(max(from - 32 * q, 0), 32), high = min(max(to - 32 * q, 0), 32);
-            unsigned seen =
-                (high == 32 ? ~0u : (1u << high) - 1) & ~(low == 32 ? ~0u : (1u << low) - 1);
-            if (missing >> (2 * q) & 1) seen &= 0xffff0000u;
-            if (missing >> (2 * q + 1) & 1) seen &= 0x0000ffffu;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[32 * q + e] = seen >> e & 1 ? x[32 * q + e] : 0xff800000u;
-          }
-        }
         // A run's factor; never 0, which times a hidden score would be NaN
         // (scores that small are 0 either way); NaN stays NaN.
         auto factor_of = [&](float run) {
           const float f = run * back;
           return f < 1.2e-38f ? 1.2e-38f : f;
         };
-        float top = -kInf;
+        if constexpr (SHARED) {
+          // Half of the columns in registers at a time: the second half first, for the
+          // maximum alone, then the first for both, then the second again. (With all
+          // of them there are no registers left to have loads and exponentials in
+          // flight: the suffix case 160 us against 155.)
+          uint32_t x[kKeys / 2];
+          const bool edge = !__all_sync(0xffffffffu, from <= 0 && to >= kKeys && missing == 0);
+          auto load = [&](int half) {
+            ld64(s_at + 64 * half, x);
+            if (!edge) return;
+            // What the row does not see becomes -infinity.
 #pragma unroll
-        for (int u = 0; u < kRuns; ++u) {
-          const float2 run = *reinterpret_cast<const float2*>(&tile_info.runs[u]);
-          float t0 = __uint_as_float(x[16 * u]), t1 = __uint_as_float(x[16 * u + 1]);
+            for (int h = 0; h < 2; ++h) {
+              const int q = 2 * half + h;
+              const int low = min(max(from - 32 * q, 0), 32), high = min(max(to - 32 * q, 0), 32);
+              unsigned seen =
+                  (high == 32 ? ~0u : (1u << high) - 1) & ~(low == 32 ? ~0u : (1u << low) - 1);
+              if (missing >> (2 * q) & 1) seen &= 0xffff0000u;
+              if (missing >> (2 * q + 1) & 1) seen &= 0x0000ffffu;
 #pragma unroll
-          for (int e = 2; e < 16; e += 2) {
-            t0 = fmaxf(t0, __uint_as_float(x[16 * u + e]));
-            t1 = fmaxf(t1, __uint_as_float(x[16 * u + e + 1]));
+              for (int e = 0; e < 32; ++e)
+                x[32 * h + e] = seen >> e & 1 ? x[32 * h + e] : 0xff800000u;
+            }
+          };
+          float top = -kInf, factor[kRuns], lift[kRuns];
+#pragma unroll
+          for (int half = 1; half >= 0; --half) {
+            load(half);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int u = 4 * half + h;
+              const float2 run = *reinterpret_cast<const float2*>(&tile_info.runs[u]);
+              factor[u] = factor_of(run.x);
+              lift[u] = run.y;
+              float t = max3(x[16 * h], x[16 * h + 1], x[16 * h + 2]);
+#pragma unroll
+              for (int e = 3; e < 15; e += 2) t = max3(__float_as_uint(t), x[16 * h + e], x[16 * h + e + 1]);
+              t = fmaxf(t, __uint_as_float(x[16 * h + 15]));
+              top = fmaxf(top, fmaf(t, factor[u], lift[u]));
+            }
           }
-          top = fmaxf(top, fmaf(fmaxf(t0, t1), factor_of(run.x), run.y));
-        }
-        const bool grows = top > m + kLag;
-        // The last tile's P V is done: O may be rescaled and P overwritten.
-        // (With P over S, S of this tile came after it.)
-        if (L::kApart && mine_s > 0) {
-          if (!warp_wait(&bars->o_done[g], mine_s - 1, bars, c.error)) goto done;
-          tc::fence_after();
-        }
-        if (__any_sync(0xffffffffu, grows)) {
-          const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
-          if (grows) m = top;
-          l *= f;
-          if (i > 0) {
+          const bool grows = top > m + kLag;
+          // The last tile's P V is done: O may be rescaled and P overwritten.
+          // (With P over S, S of this tile came after it.)
+          if (L::kApart && mine_s > 0) {
+            if (!warp_wait(&bars->o_done[g], mine_s - 1, bars, c.error)) goto done;
+            tc::fence_after();
+          }
+          if (__any_sync(0xffffffffu, grows)) {
+            const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
+            if (grows) m = top;
+            l *= f;
+            if (i > 0) {
 #pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
-              float o[16];
-              tc::ld16(o_at + d, o);
+              for (int d = 0; d < D; d += 16) {
+                float o[16];
+                tc::ld16(o_at + d, o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= f;
-              tc::st16(o_at + d, o);
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                tc::st16(o_at + d, o);
+              }
             }
           }
-        }
-        const float base = m == -kInf ? 0.f : m - kHead;
-#pragma unroll
-        for (int q = 0; q < kKeys / 32; ++q) {
-          uint32_t p[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 run = tile_info.runs[2 * q + h];
-            const float factor = factor_of(run.x), shift = run.y - base;
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const uint32_t* const s2 = x + 32 * q + 16 * h + e;
-              float2 y = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])),
-                                    make_float2(factor, factor), make_float2(shift, shift));
-              y = make_float2(ex2(y.x), ex2(y.y));
-              sum = __fadd2_rn(sum, y);
-              p[8 * h + e / 2] = pack_half2(y.x, y.y);
-            }
-            l = fmaf(sum.x + sum.y, run.z, l);
+          const float base = m == -kInf ? 0.f : m - kHead;
+          // The groups' exponentials in turn, half a tile apart: one's wait for S, its
+          // maximum and its stores then lie beside the other's: 139 us against 143.
+          const bool two = active(item, 1);
+          if (two && (g == 1 || turns > 0)) {
+            if (!warp_wait(&bars->turn[g][warp % 4], turns - (g == 0), bars, c.error)) goto done;
           }
-          st16(p_at + 16 * q, p);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (half == 1) {
+              load(1);
+              if (L::kApart) {  // S of the next tile may come
+                tc::fence_before();
+                warp_arrive(&bars->s_free[g], lane);
+              }
+              if (two) warp_arrive(&bars->turn[1 - g][warp % 4], lane);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t p[16];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int u = 4 * half + 2 * q + h;
+                const float shift = lift[u] - base;
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                  const uint32_t* const s2 = x + 32 * q + 16 * h + e;
+                  float2 y = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])),
+                                        make_float2(factor[u], factor[u]), make_float2(shift, shift));
+                  y = make_float2(ex2(y.x), ex2(y.y));
+                  sum = __fadd2_rn(sum, y);
+                  p[8 * h + e / 2] = pack_half2(y.x, y.y);
+                }
+                l = fmaf(sum.x + sum.y, tile_info.runs[u].z, l);
+              }
+              st16(p_at + 32 * half + 16 * q, p);
+            }
+          }
+          turns += two;
+        } else {
+          uint32_t x[kKeys];
+          ld64(s_at, x);
+          ld64(s_at + 64, x + 64);
+          if (L::kApart) {  // S of the next tile may come
+            tc::fence_before();
+            warp_arrive(&bars->s_free[g], lane);
+          }
+          if (!__all_sync(0xffffffffu, from <= 0 && to >= kKeys && missing == 0)) {
+            // What the row does not see becomes -infinity.
+#pragma unroll
+            for (int q = 0; q < kKeys / 32; ++q) {
+              const int low = min(max(from - 32 * q, 0), 32), high = min(max(to - 32 * q, 0), 32);
+              unsigned seen =
+                  (high == 32 ? ~0u : (1u << high) - 1) & ~(low == 32 ? ~0u : (1u << low) - 1);
+              if (missing >> (2 * q) & 1) seen &= 0xffff0000u;
+              if (missing >> (2 * q + 1) & 1) seen &= 0x0000ffffu;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[32 * q + e] = seen >> e & 1 ? x[32 * q + e] : 0xff800000u;
+            }
+          }
+          float top = -kInf;
+#pragma unroll
+          for (int u = 0; u < kRuns; ++u) {
+            const float2 run = *reinterpret_cast<const float2*>(&tile_info.runs[u]);
+            float t0 = __uint_as_float(x[16 * u]), t1 = __uint_as_float(x[16 * u + 1]);
+#pragma unroll
+            for (int e = 2; e < 16; e += 2) {
+              t0 = fmaxf(t0, __uint_as_float(x[16 * u + e]));
+              t1 = fmaxf(t1, __uint_as_float(x[16 * u + e + 1]));
+            }
+            top = fmaxf(top, fmaf(fmaxf(t0, t1), factor_of(run.x), run.y));
+          }
+          const bool grows = top > m + kLag;
+          // The last tile's P V is done: O may be rescaled and P overwritten.
+          // (With P over S, S of this tile came after it.)
+          if (L::kApart && mine_s > 0) {
+            if (!warp_wait(&bars->o_done[g], mine_s - 1, bars, c.error)) goto done;
+            tc::fence_after();
+          }
+          if (__any_sync(0xffffffffu, grows)) {
+            const float f = !grows ? 1.f : m == -kInf ? 0.f : ex2(m - top);
+            if (grows) m = top;
+            l *= f;
+            if (i > 0) {
+#pragma unroll 1
+              for (int d = 0; d < D; d += 16) {
+                float o[16];
+                tc::ld16(o_at + d, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                tc::st16(o_at + d, o);
+              }
+            }
+          }
+          const float base = m == -kInf ? 0.f : m - kHead;
+#pragma unroll
+          for (int q = 0; q < kKeys / 32; ++q) {
+            uint32_t p[16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 run = tile_info.runs[2 * q + h];
+              const float factor = factor_of(run.x), shift = run.y - base;
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const uint32_t* const s2 = x + 32 * q + 16 * h + e;
+                float2 y = __ffma2_rn(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])),
+                                      make_float2(factor, factor), make_float2(shift, shift));
+                y = make_float2(ex2(y.x), ex2(y.y));
+                sum = __fadd2_rn(sum, y);
+                p[8 * h + e / 2] = pack_half2(y.x, y.y);
+              }
+              l = fmaf(sum.x + sum.y, run.z, l);
+            }
+            st16(p_at + 16 * q, p);
+          }
         }
         tc::wait_st();
         tc::fence_before();
@@ -858,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fewer_registers<kOtherRegs>();
     // The whole warp walks the tiles, so that what the MMAs need stays in
     // uniform registers; one elected lane issues them.
-    if (warp == kMmaWarp && lo < hi) {
+    if (!SHARED && warp == kMmaWarp && lo < hi) {
       const uint32_t base = cxs::smem_addr(smem);
       constexpr uint32_t kPanel16 = kPanel / 16;  // descriptors count 16-byte units
       const uint64_t dq = tc::desc_sw128(base + L::kQ, 16, 1024);
@@ -969,10 +1102,96 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!fine) {  // let the MMAs in flight end before TMEM is freed
-        if (elect_one()) tc::commit(&bars->drain);
+        if (elect_one()) tc::commit(&bars->drain[0]);
         __syncwarp();
         const long long start = clock64();
-        while (!cxs::mbar_try_wait(&bars->drain, 0) && clock64() - start < kSpinLimit) {
+        while (!cxs::mbar_try_wait(&bars->drain[0], 0) && clock64() - start < kSpinLimit) {
+        }
+      }
+      // SHARED: a warp for each group, which sleeps on what must come next. (One that
+      // looks for whatever is ready in both groups notices a P late: a tile took
+      // 4200 cycles in the place of 3600. Without SHARED and for 128 channels it is
+      // the other way round, 613 us against 650: the groups then stay in turn.)
+    } else if (SHARED && (warp == kMmaWarp || warp == kMmaWarp + 2) && lo < hi) {
+      const int g = warp != kMmaWarp;
+      const uint32_t base = cxs::smem_addr(smem);
+      constexpr uint32_t kPanel16 = kPanel / 16;  // descriptors count 16-byte units
+      const uint64_t dq = tc::desc_sw128(base + L::kQ, 16, 1024) + g * L::kPanels * kPanel16;
+      const uint64_t dk = tc::desc_sw128(base + L::kK, 16, 1024);
+      // V is read channel-major: 64-channel panels kPanel apart, 8 keys 1024.
+      const uint64_t dv = tc::desc_sw128(base + L::kV, kPanel, 1024);
+      const uint32_t id_s = idesc_f16(128, 128, 0), id_o = idesc_f16(128, D, 1);
+      const int count = (int)(hi - lo);
+      int s_items = 0, s_tiles = 0, o_items = 0, o_tiles = 0;  // of this group, so far
+      // S of tile n: K, the item's queries and (read, or with P over S: their P V
+      // issued) its columns.
+      auto issue_s = [&](int n) -> bool {
+        const int stage = stage_of<L::kKStages>(n);
+        if (!warp_wait(&bars->k_full[stage], phase_of<L::kKStages>(n), bars, c.error)) return false;
+        const int flags = ring[n % kRing].flags;
+        if (g == 1 && !(flags & kTwo)) {  // not for this group
+          if (lane == 0) cxs::mbar_arrive(&bars->k_free[stage]);
+          return true;
+        }
+        if ((flags & kFirst) && !warp_wait(&bars->q_full[g], s_items++, bars, c.error)) return false;
+        if (L::kApart && s_tiles > 0 && !warp_wait(&bars->s_free[g], s_tiles - 1, bars, c.error))
+          return false;
+        ++s_tiles;
+        tc::fence_after();
+        const uint64_t k = dk + stage * L::kPanels * kPanel16;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            mma_ss(tmem + 128 * g, dq + i / 4 * kPanel16 + 2 * (i % 4),
+                   k + i / 4 * kPanel16 + 2 * (i % 4), id_s, i > 0);
+          tc::commit(&bars->s_full[g]);
+          tc::commit(&bars->k_free[stage]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // O of tile n: its P and V and, for an item's first tile, the last item's O
+      // read.
+      auto issue_o = [&](int n) -> bool {
+        if (!warp_wait(&bars->v_full[n & 1], n >> 1, bars, c.error)) return false;
+        const int flags = ring[n % kRing].flags;
+        if (g == 1 && !(flags & kTwo)) {
+          if (lane == 0) cxs::mbar_arrive(&bars->v_free[n & 1]);
+          return true;
+        }
+        if (!warp_wait(&bars->p_full[g], o_tiles++, bars, c.error)) return false;
+        if (flags & kFirst) {
+          if (o_items > 0 && !warp_wait(&bars->o_free[g], o_items - 1, bars, c.error)) return false;
+          ++o_items;
+        }
+        tc::fence_after();
+        const uint64_t v = dv + (n & 1) * L::kPanels * kPanel16;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tmem + L::kO + D * g, tmem + L::kP + L::kPStep * g + 8 * i, v + 128 * i, id_o,
+                   !(flags & kFirst) || i > 0);
+          tc::commit(&bars->o_done[g]);
+          tc::commit(&bars->v_free[n & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // Where P has its own columns S of the next tile goes before P V of this one,
+      // but at an item's end: the next item's queries come later.
+      bool fine = issue_s(0);
+#pragma unroll 1
+      for (int n = 0; fine && n < count; ++n) {
+        const bool o_first = !L::kApart || (ring[n % kRing].flags & kLast);
+        if (o_first) fine = issue_o(n);
+        if (fine && n + 1 < count) fine = issue_s(n + 1);
+        if (fine && !o_first) fine = issue_o(n);
+      }
+      if (!fine) {  // let the MMAs in flight end before TMEM is freed
+        if (elect_one()) tc::commit(&bars->drain[g]);
+        __syncwarp();
+        const long long start = clock64();
+        while (!cxs::mbar_try_wait(&bars->drain[g], 0) && clock64() - start < kSpinLimit) {
         }
       }
     } else if (warp == kLoadWarp) {
