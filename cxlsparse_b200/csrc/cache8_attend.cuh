@@ -255,6 +255,7 @@ struct SharePlan {    // a CTA's tiles and the item they begin in (all in one pl
   long long low, high;    // begins with reading it)
   long long total;    // cost of all items
   int id, kv_head;
+  int solo;           // no group has more than half of kTileRows rows
   ItemPlan item;
 };
 struct PlanHead {

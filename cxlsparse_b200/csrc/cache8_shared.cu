@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   const cxs_cache_attend_call& a = call.attend;
   const cxs_cache_call& c = a.cache;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, groups = call.group_count;
-  __shared__ int gaps;
+  __shared__ int gaps, many;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // Offsets and groups must ascend within the packed rows and the users.
   bool broken = false;
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     const int lo = call.groups[g], hi = call.groups[g + 1];
     broken |= lo < 0 || hi < lo || hi > c.users;
   }
-  if (threadIdx.x == 0) gaps = 0;
+  if (threadIdx.x == 0) gaps = many = 0;
   if (__syncthreads_or(broken)) {
     if (threadIdx.x == 0) {
       report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kPlanThreads)
       plan.runs[u1 + g] = runs;
       plan.groups[g] = GroupPlan{lo, none ? 0 : hi - lo, shared, u0};
       if (none) plan.gaps[atomicAdd(&gaps, 1)] = Gap{lo, hi};
+      else if ((hi - lo) * z.group > kTileRows / 2) many = 1;
     }
   }
   __syncthreads();
@@ -170,7 +171,10 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (threadIdx.x == 0) *plan.head = PlanHead{gaps + 2};
   // Where each share begins: among all tiles, without the items' own costs.
   const Shares shares(total, z);
-  for (int i = threadIdx.x; i < z.grid; i += kPlanThreads) plan.shares[i].total = total;
+  for (int i = threadIdx.x; i < z.grid; i += kPlanThreads) {
+    plan.shares[i].total = total;
+    plan.shares[i].solo = !many;
+  }
   for (int i = threadIdx.x; shares.count > 0 && i <= shares.count; i += kPlanThreads) {
     long long at = total - (long long)kItemCost * items * c.kv_heads;
     if (i < shares.count) {
