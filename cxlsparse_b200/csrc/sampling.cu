@@ -128,13 +128,14 @@ struct Shared {
                                                // below which the CTA has no first top_k,
   uint64_t bounds[2];                          // keys of a bin,
   unsigned long long mass;                     // kept mass of this CTA,
-  float total;                                 // its sum of exp(x - M),
+  float2 odds;                                 // its Odds,
   int listed;                                  // and what it has listed;
   int wanted;                                  // (first CTA's) how many it was sent
   unsigned long long part;                     // sum of this CTA's part of the bins
   Found found;
   uint64_t cut;
   float warp_totals[kWarps];
+  float2 warp_odds[kWarps];
   uint32_t powers[kPowers];                    // 2^(32 - i / kPowers)
 };
 
@@ -161,14 +162,24 @@ __device__ __forceinline__ unsigned long long block_scan(Shared& s, unsigned lon
   const unsigned long long before = __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0);
   return sum - v + (warp > 0 ? before : 0);
 }
-__device__ __forceinline__ float block_sum(Shared& s, float v) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+
+// The sum of exp(x - M): x how many tokens have M, y of the others. (Apart, so
+// that the log-probability of a token that takes nearly all of it keeps its bits.)
+using Odds = float2;
+__device__ __forceinline__ Odds block_sum(Shared& s, Odds v) {
+  for (int o = 16; o; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
   __syncthreads();
-  if (threadIdx.x % 32 == 0) s.warp_totals[threadIdx.x / 32] = v;
+  if (threadIdx.x % 32 == 0) s.warp_odds[threadIdx.x / 32] = v;
   __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < kWarps; ++w) v += s.warp_totals[w];
+  v = make_float2(0.f, 0.f);
+  for (int w = 0; w < kWarps; ++w) v.x += s.warp_odds[w].x, v.y += s.warp_odds[w].y;
   return v;
+}
+__device__ __forceinline__ float log_of(Odds v) {
+  return v.x == 1.f ? log1pf(v.y) : logf(v.x + v.y);
 }
 
 // This CTA's part of a row, in 16-byte vectors (those of the row's memory: a row
@@ -280,10 +291,9 @@ struct Cut {
 // What a row's tokens are weighed by. 2^-t with t = n + i / 512 + r, r < 2^-9:
 // t comes from fp64 as a fixed-point number (exact to 2^-33), 2^-(i / 512) from a
 // table of 32 bits, and 1 - 2^-r, at most 2^-9.5, from its Taylor polynomial in
-// fp32, whose rounding errors are then 2^-33 of the weight. Integer instructions
-// bound the pass over all tokens, so there are few of them: 58 instructions a
-// token, 24 for the integer unit, became 35 and 12, and 256 rows of 128000 tokens
-// %LARGE%.
+// fp32, whose rounding errors are then 2^-33 of the weight. Instructions bound the
+// pass over all tokens: 97 a token with a polynomial in fp64, 44 now (256 rows of
+// 128000 tokens 218 -> 76 us).
 struct Weigh {
   float top;       // largest logit
   float least;     // below it a weight is nothing
@@ -333,10 +343,10 @@ struct Weigh {
     if (top == kInf) return x == top ? 1ull << bits : 0;
     return x >= least ? add(0, x) : 0;
   }
-  __device__ __forceinline__ float odds(float x) const {  // exp(x - M)
-    return x == top ? 1.f : finite_odds(x);
+  __device__ __forceinline__ void add_odds(float x, Odds& sum) const {
+    if (x == top) sum.x += 1.f; else sum.y += odds(x);
   }
-  __device__ __forceinline__ float finite_odds(float x) const {
+  __device__ __forceinline__ float odds(float x) const {  // exp(x - M) for a finite M
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - top) * (float)kLog2e));
     return y;
@@ -356,6 +366,15 @@ __device__ __forceinline__ V lanes_before(V v, V* all) {
   }
   *all = __shfl_sync(0xffffffffu, sum, kMostCtas - 1);
   return sum - v;
+}
+
+__device__ __forceinline__ Odds cluster_odds(cg::cluster_group& cluster, Shared& s) {
+  const int lane = threadIdx.x % 32, ctas = cluster.num_blocks();
+  const Odds its = lane < ctas ? cluster.map_shared_rank(&s, lane)->odds : make_float2(0.f, 0.f);
+  Odds all;
+  lanes_before(its.x, &all.x);
+  lanes_before(its.y, &all.y);
+  return all;
 }
 
 // The first bin at which the cluster's counts (MASS: masses), with `before`,
@@ -716,25 +735,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   if (listed) {
     if (greedy) set.top_k = 1, bound = top;
     Shared* const first = cluster.map_shared_rank(&s, 0);
-    float total = 0.f;
+    Odds total = make_float2(0.f, 0.f);
     row.each_value([&](float x, int i) {
       if (x >= bound && x > -kInf) {
         const int at = atomicAdd(&first->wanted, 1);
         if (at < kList) first->gathered[at] = key_of(x, i);
       }
-      if (want) total += weigh.odds(x);
+      if (want) weigh.add_odds(x, total);
     });
     if (want) {
       total = block_sum(s, total);
-      if (threadIdx.x == 0) s.total = total;
+      if (threadIdx.x == 0) s.odds = total;
     }
     cluster.sync();
     const int n = first->wanted;
     if (n <= kList) {
-      lanes_before(rank == 0 && want && lane < ctas ? cluster.map_shared_rank(&s, lane)->total : 0.f,
-                   &total);
+      if (rank == 0 && want) total = cluster_odds(cluster, s);
       cluster.sync();  // (what is read of other CTAs has been)
-      if (rank == 0) draw_listed(a, s, weigh, set, n, draws, logf(total));
+      if (rank == 0) draw_listed(a, s, weigh, set, n, draws, log_of(total));
       return;
     }
     cluster.sync();  // (`wanted` and the list are free)
@@ -760,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   const int begin = row.begin(warp), stop = row.begin(warp + 1);
   const int rounds = ((row.each + 31) / 32 + kBlocks - 1) / kBlocks;  // of a part
   unsigned long long mass = 0;
-  float total = 0.f;
+  Odds total = make_float2(0.f, 0.f);
   auto weigh_all = [&](auto add) {
     uint4 next = make_uint4(0, 0, 0, 0);
     if (begin + lane < stop) next = row.load(begin + lane);
@@ -775,8 +793,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
         float x[kVector];
         Row<T>::unpack(w, x);
         const int i = row.index(v, 0);
-#pragma unroll
-        for (int e = 0; e < kVector; ++e) add(sum, total, x[e], i + e);
+        add(sum, x, i);
       }
       __syncwarp();
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -785,25 +802,35 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
     }
   };
   if (cut == 0 && weigh.top < kInf)
-    if (want)  // (a branch for every token otherwise)
-      weigh_all([&](unsigned long long& sum, float& odds, float x, int) {
-        sum = weigh.add(sum, x);
-        odds += weigh.finite_odds(x);
-      });
-    else
-      weigh_all([&](unsigned long long& sum, float&, float x, int) { sum = weigh.add(sum, x); });
+    weigh_all([&](unsigned long long& sum, const float (&x)[kVector], int) {
+#pragma unroll
+      for (int e = 0; e < kVector; ++e) sum = weigh.add(sum, x[e]);
+      if (!want) return;
+      float odds = 0.f;
+#pragma unroll
+      for (int e = 0; e < kVector; ++e) odds += weigh.odds(x[e]);
+      if (odds < 1.f) {  // (M is not among them)
+        total.y += odds;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVector; ++e) weigh.add_odds(x[e], total);
+      }
+    });
   else
-    weigh_all([&](unsigned long long& sum, float& odds, float x, int i) {
-      if (keep.keeps(x, i)) sum += weigh.weight(x);
-      if (want) odds += weigh.odds(x);
+    weigh_all([&](unsigned long long& sum, const float (&x)[kVector], int i) {
+#pragma unroll
+      for (int e = 0; e < kVector; ++e) {
+        if (keep.keeps(x[e], i + e)) sum += weigh.weight(x[e]);
+        if (want) weigh.add_odds(x[e], total);
+      }
     });
   __syncwarp();
-  total = want ? block_sum(s, total) : 1.f;
+  if (want) total = block_sum(s, total);
   unsigned long long all;
   const unsigned long long ahead = block_scan(s, lane == 0 ? mass : 0, &all);
   if (lane == 0) s.spans[warp] = ahead;
   if (threadIdx.x == 0) {
-    s.total = total;
+    s.odds = total;
     s.mass = all;
   }
   cluster.sync();
@@ -811,9 +838,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   unsigned long long kept_mass;
   unsigned long long before = lanes_before(lane < ctas ? other->mass : 0, &kept_mass);
   before = __shfl_sync(0xffffffffu, before, rank);
-  lanes_before(lane < ctas ? other->total : 0.f, &total);
+  if (want) total = cluster_odds(cluster, s);
   cluster.sync();  // (the sums have been read)
-  const float log_total = logf(total);
+  const float log_total = log_of(total);
 
   // A warp for each draw that falls into this CTA.
   for (int d = warp; d < a.draws; d += kWarps) {

@@ -35,7 +35,8 @@ def same(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         want, logs = draw(x[r], u[r], **each)
         assert got[r].tolist() == want.tolist(), (r, each)
         want = numpy.where(want < 0, -numpy.inf, logs[want])
-        off = numpy.where(prob[r] == want, 0.0, numpy.abs(prob[r] - want))
+        with numpy.errstate(invalid="ignore"):
+            off = numpy.where(prob[r] == want, 0.0, numpy.abs(prob[r] - want))
         assert (off <= 2.0 ** -18 + 2.0 ** -22 * numpy.abs(want)).all()
     return tokens
 
@@ -143,6 +144,23 @@ def test_masked_and_infinite_logits(cuda, dtype):
         assert (tokens[:2] == -1).all() and (tokens[2] == 3000).all() and (tokens[3] < 5).all()
         assert (tokens[4] == 100).all() and (tokens[5] // 100 == 2).all()
         assert (tokens[6] % 2 == 1).all() and (tokens[7] == 77).all()
+
+
+@pytest.mark.parametrize("vocab", [300, 40000])
+def test_log_probability_of_a_nearly_certain_token(cuda, vocab):
+    """log(1 + e) for a small e keeps its bits: e is a sum of positive terms in
+    fp32 (at most 2^-18 off), whatever is 1 beside it."""
+    x = torch.randn(4, vocab, generator=generator(8), device="cuda")
+    for r, high in enumerate((18.0, 24.0, 30.0, 40.0)):
+        x[r, 7 * r] = high
+    u = torch.full((4,), 0.5, device="cuda")
+    for settings in (dict(), dict(top_k=5), dict(top_p=0.9), dict(temperature=0.0)):
+        tokens, logprobs = sample(x, u, return_logprobs=True, **settings)
+        assert tokens.tolist() == [0, 7, 14, 21]
+        far = (x.double() - x.double().amax(-1, keepdim=True)).exp()
+        far[far == 1] = 0
+        want = -torch.log1p(far.sum(-1))
+        assert ((logprobs.double() - want).abs() <= 2.0 ** -17 * want.abs()).all()
 
 
 def test_empty_calls_and_repeated_rows(cuda):
