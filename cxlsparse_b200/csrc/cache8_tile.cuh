@@ -69,11 +69,12 @@ __device__ __forceinline__ void fewer_registers() {
 
 // First and last of its item here; rows for group 1; keys that some row does not see.
 constexpr int kFirst = 1, kLast = 2, kTwo = 4, kHidden = 8;
+constexpr unsigned kWild = 1u << kRuns;  // a scale of the tile is infinite or NaN
 
 struct Tile {                // what the roles need of a tile of keys
   float4 runs[kRuns];        // of 16 keys: |scale| log2(e) s_k, log2 s_v, 1 / s_v, and (SHARED)
                              // how many of a user's own keys hold tokens
-  unsigned missing;          // bit u: run u has no page, no row sees it
+  unsigned missing;          // bit u: run u has no page, no row sees it; (SHARED) kWild
   int left;                  // keys of the tile that hold tokens (may be negative or above kKeys)
   int flags;
   int unused;
@@ -787,6 +788,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               top = fmaxf(top, fmaf(t, factor[u], lift[u]));
             }
           }
+          // (Another user's runs count for nothing, whatever their scales are. The
+          // maximum passes over the NaN that comes of one times -infinity.)
+          if (missing & kWild) {
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u)
+              if (from >= 16 * u + 16 || to <= 16 * u) factor[u] = 1.f, lift[u] = 0.f;
+          }
           const bool grows = top > m + kLag;
           // The last tile's P V is done: O may be rescaled and P overwritten.
           // (With P over S, S of this tile came after it.)
@@ -1256,7 +1264,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           sk = __ldg(c.scales + its);
           sv = __ldg(c.scales + its + 1);
         }
-        const unsigned missing = __ballot_sync(0xffffffffu, lane < kRuns && !here);
+        unsigned missing = __ballot_sync(0xffffffffu, lane < kRuns && !here);
+        if constexpr (SHARED)
+          if (__any_sync(0xffffffffu, !(sk < kInf && sv < kInf))) missing |= kWild;
         const bool first = tile == item.begin || t == 0, last = tile + 1 == item.end || t + 1 == n;
         const int key0 = (item.first + (int)(tile - item.begin)) * kKeys;
         const int left = own ? kKeys : item.span.length - key0;
@@ -1300,7 +1310,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             Tile& about = ring[t % kRing];
             if (lane < kRuns)
               about.runs[lane] = make_float4(usable_scale(sk) * unit, __log2f(usable_scale(sv)),
-                                             __frcp_rn(usable_scale(sv)), keys_here);
+                                             !SHARED || sv == sv ? __frcp_rn(usable_scale(sv)) : 1.f,
+                                             keys_here);
             if (lane == 0) {
               about.missing = missing;
               about.left = left;

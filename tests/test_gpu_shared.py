@@ -142,6 +142,29 @@ def test_nan_reaches_the_rows_that_see_it(cuda, dim):
     assert lse.isfinite().all()
 
 
+@pytest.mark.parametrize("kv_heads,dim,format", [(2, 64, "e4m3"), (8, 128, "int8"),
+                                                 (2, 128, "e4m3")])
+def test_scales_that_are_no_numbers_stay_with_their_user(cuda, kv_heads, dim, format):
+    """Own pages whose scales are NaN or infinite: no other user's row sees them."""
+    case = family([(256, [(20 + n, 1) for n in range(40)])], kv_heads=kv_heads, dim=dim,
+                  page_size=32, format=format)
+    q = queries(40, 16, dim, torch.bfloat16)
+    want, want_lse, tol, tol_lse = attend(q, case["codes"], case["scales"], case["table"],
+                                          case["lengths"], case["new"], causal=True, window=0,
+                                          scale=0.1)
+    for user, value in ((3, math.nan), (17, math.inf), (18, -math.inf), (39, math.nan)):
+        for page in case["table"][user, 8:].tolist():
+            if page >= 0:
+                case["scales"][page] = value
+    cache = QuantizedCache(codes=case["codes"], scales=case["scales"])
+    out, lse = cache.attend_shared(q, *case["call"], scale=0.1, return_lse=True)
+    cache.check()
+    others = [n for n in range(40) if n not in (3, 17, 18, 39)]
+    close(out[others].double(), want[others], tol[others])
+    close(lse[others].double(), want_lse[others], tol_lse[others])
+    assert not lse[[3, 17, 39]].isfinite().any()
+
+
 def test_groups_that_do_not_fit(cuda):
     case = family([(100, [(n, 3) for n in range(9)]), (50, [(4, 8), (2, 30)]),
                    (80, [(1, 2)] * 12)], kv_heads=2, dim=64, page_size=16, format="e4m3")
