@@ -387,8 +387,7 @@ template <bool MASS>
 __device__ void find_bin(cg::cluster_group& cluster, Shared& s, unsigned long long before,
                          unsigned long long target, float share) {
   static_assert(kBins == 4 * kThreads, "four bins of one CTA a thread");
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), lane = threadIdx.x % 32;
   const int bins = kBins / ctas, quads = bins / 4;  // of this CTA
   uint32_t* const counts = ctas > 1 ? s.part_counts : s.counts;
   const Wide masses = ctas > 1 ? Wide{s.part_masses[0], s.part_masses[1]}
@@ -450,7 +449,6 @@ __device__ void find_bin(cg::cluster_group& cluster, Shared& s, unsigned long lo
       at += amount[e];
     }
   }
-  (void)warp;
   cluster.sync();
 }
 

@@ -586,9 +586,9 @@ int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes
  * pages. (Of them only those count as common that every row of the group sees.)
  * Where groups or offsets do not ascend no row is computed, and none of a group
  * with a user of more than max_tokens rows, with CXS_DEVICE_ERR_BAD_LENGTH; rows
- * of no group have out = 0 and lse = -infinity. (Groups of few rows, 64 a KV head
- * on average, 32 for dim 128, are computed user by user: rows then depend on
- * nothing but their user.) */
+ * of no group have out = 0 and lse = -infinity. Calls with few rows (64 of a group
+ * and KV head on average, 32 for dim 128) are computed user by user, as
+ * cxs_cache_attend does, without a look at groups and shared. */
 typedef struct cxs_cache_shared_call {
   cxs_cache_attend_call attend;
   const int32_t* groups;   /* [group_count + 1] */
