@@ -89,17 +89,19 @@ __global__ void __launch_bounds__(kPlanThreads)
   for (int g = warp; g < groups; g += kPlanWarps) {
     const int u0 = call.groups[g], u1 = call.groups[g + 1];
     const int lo = first_row(u0), hi = first_row(u1);
-    int seen = most, bad = 0, none = 0, longest = 0;
+    int seen = most, bad = 0, none = 0, longest = 0, holder = u1;
     for (int u = u0 + lane; u < u1; u += 32) {
       const int n = first_row(u + 1) - first_row(u), length = c.lengths[u];
       none |= n > c.max_tokens;
       bad |= length < 0 || length > most;
-      if (n == 0) continue;
+      if (n == 0) continue;  // (it may hold other tokens, or none)
+      holder = min(holder, u);
       seen = min(seen, max(a.causal ? min(length, length - n + 1) : length, 0));
       longest = max(longest, min(length, most));
     }
     seen = __reduce_min_sync(0xffffffffu, seen);
     longest = __reduce_max_sync(0xffffffffu, longest);
+    holder = __reduce_min_sync(0xffffffffu, holder);
     none = __any_sync(0xffffffffu, none);
     int shared = call.shared[g];
     bad |= shared < 0;
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (bad || none) report(c.error, CXS_DEVICE_ERR_BAD_LENGTH);
     if (lane == 0) {
       plan.runs[u1 + g] = runs_at[u1 + g] = runs;
-      groups_at[g] = GroupPlan{lo, none ? 0 : hi - lo, shared, u0};
+      groups_at[g] = GroupPlan{lo, none ? 0 : hi - lo, shared, holder};
       if (none) plan.gaps[atomicAdd(&gaps, 1)] = Gap{lo, hi};
       else if ((hi - lo) * z.group > kTileRows / 2) many = 1;
     }

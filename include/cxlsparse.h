@@ -582,10 +582,12 @@ int cxs_cache_attend_workspace(const cxs_cache_attend_call* call, int64_t* bytes
  * tokens in common, such as the candidates of one history. Users groups[g] ..
  * groups[g + 1] - 1 (groups [group_count + 1] ascends from 0 to users) are group
  * g, and their first shared[g] tokens are the same, code by code and scale by
- * scale; they are read once for the rows of all of them, from the first user's
- * pages. (Of them only those count as common that every row of the group sees.)
+ * scale; they are read once for the rows of all of them, from the pages of the
+ * first user that has rows. (Of them only those count as common that every row of
+ * the group sees. Users without rows may hold other tokens, or none.)
  * Where groups or offsets do not ascend no row is computed, and none of a group
- * with a user of more than max_tokens rows, with CXS_DEVICE_ERR_BAD_LENGTH; rows
+ * with a user of more than max_tokens rows, or whose longest user's own keys are
+ * more than 2^30 for 256 users (or all of fewer), with CXS_DEVICE_ERR_BAD_LENGTH; rows
  * of no group have out = 0 and lse = -infinity. Calls with few rows (64 of a group
  * and KV head on average, 32 for dim 128) are computed user by user, as
  * cxs_cache_attend does, without a look at groups and shared. */

@@ -212,6 +212,19 @@ def test_groups_that_do_not_fit(cuda):
     right(out, lse, slice(27, None))
 
 
+@pytest.mark.parametrize("gone", [[0], [0, 1, 2, 41, 79], list(range(39))])
+def test_users_that_have_ended(cuda, gone):
+    """Users without rows may hold nothing at all, the first of a group too."""
+    case = family([(200, [(n % 7, 2) for n in range(40)])] * 2, kv_heads=2, dim=64, page_size=32,
+                  format="int8")
+    for user in gone:
+        case["table"][user] = -1
+        case["lengths"][user] = case["new"][user] = 0
+    table, _, _, groups, shared = case["call"]
+    case["call"] = (table, ints(case["lengths"]), offsets_of(case["new"]), groups, shared)
+    agree(case, queries(sum(case["new"]), 32, 64, torch.bfloat16))
+
+
 def test_bad_pages_are_left_out(cuda):
     case = family([(200, [(20, 1)] * 70)], kv_heads=1, dim=64, page_size=16, format="e4m3")
     q = queries(70, 4, 64, torch.bfloat16)
