@@ -6,7 +6,10 @@ import torch
 
 from cxlsparse_b200.dense import DenseCacheModel
 from cxlsparse_b200.model import NSAConfig
+from cxlsparse_b200.pages import PageTable
+from cxlsparse_b200.quantized import QuantizedCache
 from cxlsparse_b200.sampling import sample
+from shared_case import family
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +100,54 @@ def test_generate_refuses(cuda):
             model.generate(*args)
     with pytest.raises(ValueError):
         made(2).generate(logits, u)
+
+
+def test_pages_behind_four_gigabytes(cuda):
+    """The same cache at the end of a pool of 2^32 bytes: forked, attended to,
+    compacted and attended to again, with results equal to the bit."""
+    case = family([(300, [(n, 2) for n in range(36)])], kv_heads=8, dim=64, page_size=64,
+                  format="e4m3")
+    table, lengths, offsets, groups, shared = case["call"]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(72, 64, 64, generator=g, device="cuda").bfloat16()
+    small = QuantizedCache(codes=case["codes"], scales=case["scales"])
+    want = small.attend_shared(q, *case["call"])
+    pages, count = 66000, case["codes"].shape[0]
+    large = QuantizedCache(pages, 8, 64, page_size=64, format="e4m3")
+    assert large.codes.numel() > 2 ** 32
+    at = pages - count
+    large.codes.view(torch.uint8)[at:] = case["codes"].view(torch.uint8)
+    large.scales[at:] = case["scales"]
+    pool = PageTable([large], 37, table.shape[1])
+    rows = torch.full((37, table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    rows[:36] = torch.where(table >= 0, table + at, table)
+    pool.adopt(rows, torch.cat((lengths, lengths.new_zeros(1))))
+    pool.fork(lengths.new_tensor([35]), lengths.new_tensor([36]))
+
+    def agree():
+        for last in (35, 36):
+            order = list(range(35)) + [last]
+            got = large.attend_shared(q, pool.table[order], pool.lengths[order], offsets, groups,
+                                      shared)
+            assert torch.equal(got, want)
+        large.check()
+        pool.check()
+
+    agree()
+    live = pool.compact().item()
+    assert live < count + 2 and pool.table.max().item() == live - 1
+    agree()
+
+
+def test_rows_behind_four_gigabytes(cuda):
+    vocab, stride = 50000, 2 ** 30 + 24
+    g = torch.Generator(device="cuda").manual_seed(4)
+    few = torch.randn(3, vocab, generator=g, device="cuda").bfloat16()
+    far = torch.empty(2 * stride + vocab, dtype=torch.bfloat16, device="cuda")
+    far = far.as_strided((3, vocab), (stride, 1))
+    far.copy_(few)
+    u = torch.rand(3, 40, generator=g, device="cuda")
+    for settings in ({}, SETTINGS, dict(top_p=0.5), dict(temperature=0.0)):
+        for got, want in zip(sample(far, u, return_logprobs=True, **settings),
+                             sample(few, u, return_logprobs=True, **settings)):
+            assert torch.equal(got, want)
