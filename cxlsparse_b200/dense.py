@@ -117,7 +117,7 @@ class DenseCacheModel:
     def generate(self, logits, uniforms, **settings):
         """Continuations of every user's history: tokens and their
         log-probabilities [users, candidates, steps], drawn (``sample``, with
-        its settings) from ``logits [users, vocab]`` after each history for the
+        its settings, numbers or one for each user) from ``logits [users, vocab]`` after each history for the
         first token, and from the model for the others, with ``uniforms
         [users, candidates, steps]``. The histories stay as they are."""
         users = len(self.lengths)
@@ -140,6 +140,8 @@ class DenseCacheModel:
         at = slice(users, users + total)
         u = uniforms.permute(2, 0, 1).contiguous()
         found = [sample(logits, u[0], return_logprobs=True, **settings)]
+        settings = {name: x.repeat_interleave(count) if torch.is_tensor(x) else x
+                    for name, x in settings.items()}
 
         def attend(cache, q):
             return cache.attend_shared(q, pages.table[at], pages.lengths[at], None, groups, shared,

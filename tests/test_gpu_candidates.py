@@ -89,6 +89,21 @@ def test_candidates_of_one_history_differ_and_repeat(cuda):
     model.check()
 
 
+def test_settings_of_each_user(cuda):
+    lengths = [70, 30, 100]
+    model = made(3, candidates=4, candidate_tokens=6)
+    logits = model.step(prompt(lengths), lengths)[last_rows(lengths)]
+    u = torch.rand(3, 4, 6, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    heat = torch.tensor([0.0, 1.0, 0.5], device="cuda")
+    most = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    tokens, _ = model.generate(logits, u, temperature=heat, top_k=most)
+    for n in range(3):
+        one, _ = model.generate(logits, u, temperature=heat[n].item(), top_k=most[n].item())
+        assert torch.equal(tokens[n], one[n])
+    assert (tokens[:2] == tokens[:2, :1]).all()
+    model.check()
+
+
 def test_generate_refuses(cuda):
     model = made(2, candidates=4, candidate_tokens=5)
     logits = model.step(prompt([9, 9]), [9, 9])[[8, 17]]
