@@ -8,6 +8,44 @@
 #include "cxs_common.cuh"
 
 namespace cxs {
+// Stands in a kernel that was launched with cxs_host::launch_early before its first
+// access to memory: nothing that the kernel before writes is there, and nothing that
+// it reads may be written, until it has ended.
+__device__ __forceinline__ void after_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// The next kernel, if it was launched so, may be set up from here on.
+__device__ __forceinline__ void next_may_come() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+}  // namespace cxs
+
+namespace cxs_host {
+// A launch whose CTAs may be set up while the kernel before on the stream still
+// runs; they wait for it on the device. `cluster`: CTAs of a cluster, 0 for none.
+template <typename... P, typename... A>
+int launch_early(const char* what, void (*kernel)(P...), dim3 grid, int block, int shared,
+                 int cluster, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(block);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster ? 2 : 1;
+  CXS_CUDA(cudaLaunchKernelEx(&config, kernel, args...));
+  CXS_LAUNCH_CHECK(what);
+  return CXS_OK;
+}
+}  // namespace cxs_host
+
+namespace cxs {
 namespace cache8 {
 
 constexpr float kLeastScale = 5.421010862427522e-20f;  // 2^-64

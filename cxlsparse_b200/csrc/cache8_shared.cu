@@ -60,7 +60,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   GroupPlan* const groups_at = here ? groups_here : plan.groups;
   if (here) first_item = first_here;
   const auto first_row = [&](int user) { return offsets ? offsets[user] : user; };
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cxs::after_earlier();
+  cxs::next_may_come();
   // Offsets and groups must ascend within the packed rows and the users.
   bool broken = false;
   for (int u = threadIdx.x; u <= c.users; u += kPlanThreads) {
@@ -294,8 +295,8 @@ extern "C" int cxs_cache_attend_shared(const cxs_cache_shared_call* call, void* 
   SharedPlan plan;
   int* first_item;
   lay_out(*call, (char*)call->attend.workspace, &plan, &first_item);
-  plan_kernel<<<1, kPlanThreads, 0, s>>>(*call, z, plan, first_item);
-  CXS_LAUNCH_CHECK("cache attend shared plan");
+  status = cxs_host::launch_early("cache attend shared plan", plan_kernel, 1, kPlanThreads, 0, 0, s,
+                                  *call, z, plan, first_item);
   status = launch_of<true>(call->attend, z, plan, s);
   if (status != CXS_OK) return status;
   return launch_join(call->attend, z, false, false, s);

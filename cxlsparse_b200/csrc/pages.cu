@@ -125,6 +125,8 @@ __device__ __forceinline__ int pages_for(long long tokens, int page_bits) {
 __global__ void __launch_bounds__(kPlanThreads)
     extend_kernel(const cxs_pages_call c, const int* counts, int page_bits) {
   const Work w = work_of(c);
+  cxs::after_earlier();
+  cxs::next_may_come();
   const long long most = (long long)c.width << page_bits;
   int total = 0, bad = 0;
   for (int b0 = 0; b0 < c.sequences; b0 += kPlanThreads) {
@@ -176,7 +178,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     fork_kernel(const cxs_pages_call c, const int* parents, const int* children, int n,
                 int page_bits) {
   const Work w = work_of(c);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cxs::after_earlier();
+  cxs::next_may_come();
   if (threadIdx.x == 0) w.copies[0] = w.copies[1] = 0;
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     const int child = children[i];
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 __global__ void __launch_bounds__(kPlanThreads)
     compact_kernel(const cxs_pages_call c, int* live_out) {
   const Work w = work_of(c);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  cxs::after_earlier();
+  cxs::next_may_come();
   const int live = find_pages(c.references, 0, c.pages, true, INT_MAX, [](int, int) {});
   const int moves = find_pages(c.references, 0, live, false, INT_MAX,
                                [&](int page, int rank) { w.target[rank] = page; });
@@ -270,7 +274,8 @@ __global__ void __launch_bounds__(kApplyThreads)
   const int lane = threadIdx.x % 32;
   const int warp = (blockIdx.x * kApplyThreads + threadIdx.x) / 32;
   const int warps = gridDim.x * (kApplyThreads / 32);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  cxs::after_earlier();
+  cxs::next_may_come();
   const int copies = w.copies[0], count = w.copies[1];
   const int parts = 2 * c.kv_heads;
   const long long part_bytes = (long long)c.page_size * c.dim;
@@ -323,6 +328,8 @@ __global__ void __launch_bounds__(kApplyThreads)
 // Each entry is taken out once, so a sequence that is there twice is freed once.
 __global__ void __launch_bounds__(kApplyThreads)
     free_kernel(const cxs_pages_call c, const int* sequences, int n) {
+  cxs::after_earlier();
+  cxs::next_may_come();
   const int chunks = (c.width + kApplyThreads - 1) / kApplyThreads;
   for (long long unit = blockIdx.x; unit < (long long)n * chunks; unit += gridDim.x) {
     const int i = (int)(unit / chunks), chunk = (int)(unit - (long long)i * chunks);
@@ -403,18 +410,9 @@ int blocks_for(long long units) {
 template <bool COMPACT>
 int launch_apply(const cxs_pages_call& c, const int* parents, const int* children, long long work,
                  cudaStream_t stream) {
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(blocks_for((work + kApplyThreads / 32 - 1) / (kApplyThreads / 32)));
-  config.blockDim = dim3(kApplyThreads);
-  config.stream = stream;
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  CXS_CUDA(cudaLaunchKernelEx(&config, apply_kernel<COMPACT>, c, parents, children, page_bits_of(c)));
-  CXS_LAUNCH_CHECK("pages apply");
-  return CXS_OK;
+  const int blocks = blocks_for((work + kApplyThreads / 32 - 1) / (kApplyThreads / 32));
+  return cxs_host::launch_early("pages apply", apply_kernel<COMPACT>, blocks, kApplyThreads, 0, 0,
+                                stream, c, parents, children, page_bits_of(c));
 }
 
 }  // namespace
@@ -431,9 +429,8 @@ extern "C" int cxs_pages_extend(const cxs_pages_call* call, const int32_t* count
   int status = check_pages(call, "pages extend");
   if (status == CXS_OK) status = check_pointers(call, "pages extend");
   if (status != CXS_OK) return status;
-  extend_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(*call, counts, page_bits_of(*call));
-  CXS_LAUNCH_CHECK("pages extend");
-  return CXS_OK;
+  return cxs_host::launch_early("pages extend", extend_kernel, 1, kPlanThreads, 0, 0,
+                                (cudaStream_t)stream, *call, counts, page_bits_of(*call));
 }
 
 extern "C" int cxs_pages_fork(const cxs_pages_call* call, const int32_t* parents,
@@ -446,9 +443,10 @@ extern "C" int cxs_pages_fork(const cxs_pages_call* call, const int32_t* parents
   status = check_pointers(call, "pages fork");
   if (status != CXS_OK) return status;
   if (!parents || !children) return set_error(CXS_ERR_INVALID, "pages fork: null parents or children");
-  fork_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(*call, parents, children, count,
-                                                            page_bits_of(*call));
-  CXS_LAUNCH_CHECK("pages fork");
+  status = cxs_host::launch_early("pages fork", fork_kernel, 1, kPlanThreads, 0, 0,
+                                  (cudaStream_t)stream, *call, parents, children, count,
+                                  page_bits_of(*call));
+  if (status != CXS_OK) return status;
   const long long chunks = (call->width + kRowChunk - 1) / kRowChunk;
   const long long runs = (long long)count * call->layers * call->kv_heads * 2;
   return launch_apply<false>(*call, parents, children, runs > count * chunks ? runs : count * chunks,
@@ -465,10 +463,8 @@ extern "C" int cxs_pages_free(const cxs_pages_call* call, const int32_t* sequenc
   if (status != CXS_OK) return status;
   if (!sequences) return set_error(CXS_ERR_INVALID, "pages free: null sequences");
   const long long chunks = (call->width + kApplyThreads - 1) / kApplyThreads;
-  free_kernel<<<blocks_for(count * chunks), kApplyThreads, 0, (cudaStream_t)stream>>>(
-      *call, sequences, count);
-  CXS_LAUNCH_CHECK("pages free");
-  return CXS_OK;
+  return cxs_host::launch_early("pages free", free_kernel, blocks_for(count * chunks), kApplyThreads,
+                                0, 0, (cudaStream_t)stream, *call, sequences, count);
 }
 
 extern "C" int cxs_pages_adopt(const cxs_pages_call* call, const int32_t* table,
@@ -495,7 +491,8 @@ extern "C" int cxs_pages_compact(const cxs_pages_call* call, int32_t* live, void
   int status = check_pages(call, "pages compact");
   if (status == CXS_OK) status = check_pointers(call, "pages compact");
   if (status != CXS_OK) return status;
-  compact_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(*call, live);
-  CXS_LAUNCH_CHECK("pages compact");
+  status = cxs_host::launch_early("pages compact", compact_kernel, 1, kPlanThreads, 0, 0,
+                                  (cudaStream_t)stream, *call, live);
+  if (status != CXS_OK) return status;
   return launch_apply<true>(*call, nullptr, nullptr, 1ll << 30, (cudaStream_t)stream);
 }

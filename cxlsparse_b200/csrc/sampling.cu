@@ -638,6 +638,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   const int r = blockIdx.x / ctas, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   Row<T> row((const T*)a.logits + r * a.row_stride, a.vocab, rank, ctas);
   constexpr int kVector = Row<T>::kVector;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0;
+  static_assert(kPowers == kThreads, "a power a thread");
+  s.powers[threadIdx.x] = power_of(threadIdx.x);
+  if (threadIdx.x == 0) s.wanted = 0;
+  // (The next call's CTAs come when these have ended, not before: beside them they
+  // would sit two to an SM, 64 rows of 32000 in 21.5 us against 17.)
+  cxs::after_earlier();
   Settings set{a.temperature ? a.temperature[r] : a.temperature_all,
                a.top_p ? a.top_p[r] : a.top_p_all, a.min_p ? a.min_p[r] : a.min_p_all,
                a.top_k ? a.top_k[r] : a.top_k_all};
@@ -646,10 +653,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
   const bool greedy = set.temperature == 0.f || set.top_k == 1;
   const bool listed = greedy || (set.top_k > 0 && set.top_k <= kMostListed &&
                                  set.top_k <= ctas * kThreads / 2);
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.counts[i] = 0;
-  static_assert(kPowers == kThreads, "a power a thread");
-  s.powers[threadIdx.x] = power_of(threadIdx.x);
-  if (threadIdx.x == 0) s.wanted = 0;
 
   // The largest logit, of the thread and of the row; the run into shared memory.
   float mine = -kInf;
@@ -949,20 +952,8 @@ int launch(const cxs_sample_call& a, cudaStream_t stream) {
   const long long vectors = ((long long)a.vocab * sizeof(T) + 15) / 16 + 1;
   const long long bytes = (vectors + ctas - 1) / ctas * 16;
   const int slice = bytes <= kSliceBytes ? (int)bytes : 0;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(a.rows * ctas);
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = slice;
-  config.stream = stream;
-  cudaLaunchAttribute cluster = {};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = ctas;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  CXS_CUDA(cudaLaunchKernelEx(&config, sample_kernel<T>, a, slice));
-  CXS_LAUNCH_CHECK("sample");
-  return CXS_OK;
+  return cxs_host::launch_early("sample", sample_kernel<T>, dim3(a.rows * ctas), kThreads, slice,
+                                ctas, stream, a, slice);
 }
 
 }  // namespace
