@@ -126,7 +126,7 @@ class PageTable:
     def compact(self):
         """Move pages, in every layer, until the n pages in use are the first n;
         returns n as an int32 tensor [1]. The rest of the pool holds nothing."""
-        live = torch.empty(1, dtype=torch.int32, device=self.device)
+        live = self.lengths.new_empty(1)
         self._run(_lib.packed().cxs_pages_compact, live.data_ptr())
         return live
 

@@ -16,7 +16,7 @@ TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _setting(name, value, dtype, rows, device):
     """(pointer or 0, value for all rows) of a number or a [rows] tensor."""
-    if not torch.is_tensor(value):
+    if not isinstance(value, torch.Tensor):
         return 0, value
     if value.shape != (rows,) or value.dtype != dtype or not value.is_contiguous() \
             or value.device != device:
@@ -42,12 +42,11 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
 
     With ``return_logprobs`` also the tokens' log softmax(logits), fp32, with no
     temperature and nothing cut (-infinity where the token is -1)."""
-    if logits.ndim != 2 or logits.dtype not in TYPES or logits.shape[1] < 1 \
-            or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    device, shape, size, strides = logits.device, uniforms.shape, logits.shape, logits.stride()
+    if len(size) != 2 or logits.dtype not in TYPES or size[1] < 1 \
+            or (strides[1] != 1 and size[1] > 1):
         raise ValueError("logits must be [rows, vocab] in bf16, fp16 or fp32 with contiguous rows")
-    rows, vocab = logits.shape
-    device = logits.device
-    shape = uniforms.shape
+    rows, vocab = size
     if len(shape) not in (1, 2) or shape[0] != rows \
             or uniforms.dtype not in (torch.float32, torch.float64) \
             or not uniforms.is_contiguous() or uniforms.device != device:
@@ -61,12 +60,12 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     min_at, least = _setting("min_p", min_p, torch.float32, rows, device)
     if not 0 <= heat < math.inf or not 0 <= k or not p >= 0 or not 0 <= least <= 1:
         raise ValueError("temperature, top_k and top_p must not be negative, min_p be 0 .. 1")
-    tokens = torch.empty(shape, dtype=torch.int64, device=device)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=device) if return_logprobs else None
+    tokens = uniforms.new_empty(shape, dtype=torch.int64)
+    logprobs = uniforms.new_empty(shape, dtype=torch.float32) if return_logprobs else None
     call = _lib.pack_sample_call(
         logits.data_ptr(), uniforms.data_ptr(), tokens.data_ptr(),
         0 if logprobs is None else logprobs.data_ptr(), heat_at, k_at, p_at, min_at,
-        logits.stride(0), rows, vocab, 1 if len(shape) == 1 else shape[1], TYPES[logits.dtype],
+        strides[0], rows, vocab, 1 if len(shape) == 1 else shape[1], TYPES[logits.dtype],
         uniforms.dtype == torch.float64, heat, min(int(k), vocab), p, least)
     _lib.on_device(device.index, _lib.packed().cxs_sample, call)
     return (tokens, logprobs) if return_logprobs else tokens
