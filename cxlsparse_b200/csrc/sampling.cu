@@ -41,7 +41,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kBinsPerOctave = 32;   // of the weight: 64 octaves in all
+constexpr float kCountBins = 32;     // bins of counts for an octave of the weight
 constexpr int kPowers = 512;         // of two, in a table
 constexpr int kFew = 512;            // tokens whose ranks are counted one by one
 constexpr int kList = kThreads;      // tokens that are gathered for a small top_k
@@ -311,8 +311,8 @@ struct Weigh {
   __device__ __forceinline__ float octaves(float x) const {
     return x == top ? 0.f : (top - x) * rate32;
   }
-  __device__ __forceinline__ int bin(float x) const {
-    const float t = octaves(x) * kBinsPerOctave;
+  __device__ __forceinline__ int bin(float x, float per_octave) const {
+    const float t = octaves(x) * per_octave;
     return t < kBins - 1 ? (int)t : kBins - 1;  // (what is not a number, too)
   }
   // The weight added to `sum`, top being finite: what is far below it, -infinity
@@ -461,6 +461,11 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
                            float share) {
   const int lane = threadIdx.x % 32, ctas = cluster.num_blocks();
   const Cut cut(cut_key);
+  // All tokens of t octaves below M have less than vocab 2^-t of the mass: its border
+  // lies above, and bins may be the narrower (131072 tokens: 80 an octave, so that
+  // those of one are few enough in the first round: 8 rows of 131071 57 -> 38 us). Counts'
+  // borders may lie anywhere. The last bin has what is below.
+  const float per_octave = MASS ? kBins / (40.f - __clz(row.vocab)) : kCountBins;
   uint64_t low = 0, high = ~0ull;      // keys still looked at, from the second round on
   int shift = 0, coarse_bin = -1;
   unsigned long long before = 0;       // of the tokens ahead of them
@@ -472,7 +477,7 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
     __syncthreads();
     row.each_value([&](float x, int i) {
       if (!cut.keeps(x, i)) return;
-      int bin = weigh.bin(x);
+      int bin = weigh.bin(x, per_octave);
       if (round > 0) {
         const uint64_t key = key_of(x, i);
         if (bin != coarse_bin || key < low || key > high) return;
@@ -504,7 +509,7 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
       // Keys of the bin: the bounds of what is there.
       uint64_t least = ~0ull, most = 0;
       row.each_value([&](float x, int i) {
-        if (!cut.keeps(x, i) || weigh.bin(x) != coarse_bin) return;
+        if (!cut.keeps(x, i) || weigh.bin(x, per_octave) != coarse_bin) return;
         const uint64_t key = key_of(x, i);
         least = key < least ? key : least;
         most = key > most ? key : most;
@@ -542,7 +547,7 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
   }
   // Few enough: a list of them all, the rank of each.
   row.each_value([&](float x, int i) {
-    if (!cut.keeps(x, i) || weigh.bin(x) != coarse_bin) return;
+    if (!cut.keeps(x, i) || weigh.bin(x, per_octave) != coarse_bin) return;
     const uint64_t key = key_of(x, i);
     if (key >= low && key <= high) s.list[atomicAdd(&s.listed, 1)] = key;
   });
@@ -564,13 +569,22 @@ __device__ uint64_t border(cg::cluster_group& cluster, Shared& s, const Row<T>& 
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t key = s.all[i];
-    unsigned long long ahead = before;
-    for (int j = 0; j < n; ++j) ahead += s.all[j] > key ? s.weights[j] : 0;
-    if (ahead < target && ahead + s.weights[i] >= target) s.cut = key;
+  // (Each CTA's share of them, as many lanes a token as there are.)
+  const int rank = cluster.block_rank(), share_of = (n + ctas - 1) / ctas;
+  const int stop = min(n, share_of * (rank + 1));
+  int lanes = 1;
+  while (lanes < 32 && 2 * lanes * share_of <= kThreads) lanes *= 2;
+  for (int i0 = share_of * rank; i0 < stop; i0 += kThreads / lanes) {
+    const int i = i0 + threadIdx.x / lanes;
+    const uint64_t key = i < stop ? s.all[i] : ~0ull;
+    unsigned long long ahead = 0;
+    for (int j = threadIdx.x % lanes; j < n; j += lanes) ahead += s.all[j] > key ? s.weights[j] : 0;
+    for (int o = lanes / 2; o; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    ahead += before;
+    if (i < stop && threadIdx.x % lanes == 0 && ahead < target && ahead + s.weights[i] >= target)
+      for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&s, c)->cut = key;
   }
-  cluster.sync();  // (the lists have been read)
+  cluster.sync();  // (the lists have been read, the border is there)
   return s.cut;
 }
 
@@ -690,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
       // At least 1 / ctas of top_k tokens of this CTA lie in the bins that as many
       // of its threads' maxima reach; the least of these maxima bounds them.
       const Weigh local(s.powers, top, kLog2e / set.temperature, a.vocab);
-      const int bin = mine > -kInf ? local.bin(mine) : kBins;
+      const int bin = mine > -kInf ? local.bin(mine, kCountBins) : kBins;
       if (bin < kBins) atomicAdd(&s.counts[bin], 1u);
       __syncthreads();
       const uint4 n = *reinterpret_cast<const uint4*>(&s.counts[4 * threadIdx.x]);
