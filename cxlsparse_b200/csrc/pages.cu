@@ -121,7 +121,8 @@ __device__ __forceinline__ int pages_for(long long tokens, int page_bits) {
 }
 
 // Room for counts[b] more tokens of every sequence (null: one each). Latency:
-// a chain of loads and four barriers a scan, about 3 us however few.
+// a chain of loads and four barriers a scan: 2 us in a graph for 10 to 260 sequences,
+// 3 for 2000.
 __global__ void __launch_bounds__(kPlanThreads)
     extend_kernel(const cxs_pages_call c, const int* counts, int page_bits) {
   const Work w = work_of(c);
@@ -174,6 +175,9 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // What forking does: a fresh page for each child whose parent ends inside a page.
+// With the launch that copies, in a graph: 8 children of 16 layers (2 heads of 64
+// channels) 9 us, 256 of 4 layers (8 of 128) 13, 2000 of one 19. (In one CTA because
+// the lowest free ids, which every child's page depends on, are a scan over all.)
 __global__ void __launch_bounds__(kPlanThreads)
     fork_kernel(const cxs_pages_call c, const int* parents, const int* children, int n,
                 int page_bits) {
@@ -237,7 +241,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
 }
 
-// The live pages past the first `live` ids go to the free ones among those.
+// The live pages past the first `live` ids go to the free ones among those. 16384
+// references a round of each search; nothing to move: 5 us with the second launch.
 __global__ void __launch_bounds__(kPlanThreads)
     compact_kernel(const cxs_pages_call c, int* live_out) {
   const Work w = work_of(c);
@@ -266,7 +271,9 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // Page contents of all layers, a warp for each page's K or V of a head; then the
-// rows: of the children (their parents' full pages), or all, with new ids.
+// rows: of the children (their parents' full pages), or all, with new ids. Bound by
+// HBM: eight 16-byte loads a lane in flight, 570 MB of a pool in 88 us, 0.98 of the
+// copy rate.
 template <bool COMPACT>
 __global__ void __launch_bounds__(kApplyThreads)
     apply_kernel(const cxs_pages_call c, const int* parents, const int* children, int page_bits) {

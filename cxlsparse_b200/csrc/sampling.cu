@@ -293,7 +293,7 @@ struct Cut {
 // table of 32 bits, and 1 - 2^-r, at most 2^-9.5, from its Taylor polynomial in
 // fp32, whose rounding errors are then 2^-33 of the weight. Instructions bound the
 // pass over all tokens: 97 a token with a polynomial in fp64, 44 now (256 rows of
-// 128000 tokens 218 -> 76 us).
+// 128000 tokens 218 -> 74 us).
 struct Weigh {
   float top;       // largest logit
   float least;     // below it a weight is nothing
@@ -940,11 +940,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const cxs_sample_ca
 }
 
 // CTAs of a row's cluster: as many as still have an SM each and kLeast values.
-// Measured for 1, 2, 4, 8 and 16 of them (us): one row of 32000 16.6 / 14.4 / 12.5 /
-// 13.1 / 14.5, 64 rows of 32000 25 / 21 / 27 / 39 / 68, 8 rows of 131071 (fp32, top_p)
-// 191 / 107 / 66 / 42 / 41, 256 rows of 128000 78 / 84 / 94 / 127 / 259.
+// Measured for 1, 2, 4, 8 and 16 of them (us, in a graph, with log-probabilities):
+// few rows, bf16, top_k 50 and top_p of 4000 tokens 9.8 / 10.7 / 10.7 / 10.9 / 12.2, of
+// 8000 10.9 / 10.0 / 10.6 / 10.9 / 12.1, of 16000 12.1 / 11.2 / 10.0 / 10.9 / 12.2, of
+// 32000 14.7 / 12.8 / 11.1 / 10.5 / 12.4, of 64000 20.6 / 15.2 / 12.4 / 11.5 / 11.7
+// (top_p alone 89 / 52 / 34 / 26 / 24); 64 rows of 32000 14.8 / 13.1 / 14.5 / 25 / 54, 8
+// rows of 131071 (fp32, top_p) 184 / 101 / 59 / 38 / 36, 256 rows of 128000 70 / 77 / 89 /
+// 122 / 248.
 int ctas_of(const cxs_sample_call& a) {
-  constexpr int kAtOnce = 148, kLeast = 4096;
+  constexpr int kAtOnce = 148, kLeast = 3000;
   int ctas = 1;
   while (ctas < kMostCtas && (long long)a.rows * ctas * 2 <= kAtOnce && a.vocab >= 2 * kLeast * ctas)
     ctas *= 2;
