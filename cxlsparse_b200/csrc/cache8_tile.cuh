@@ -246,7 +246,8 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
 
 // An item and where its tiles lie among all tiles of the launch.
 struct Item {
-  int user, tile_row, kv_head;   // rows kTileRows * tile_row .. (SHARED: of the group's first user)
+  int user, tile_row, kv_head;   // rows kTileRows * tile_row .. (SHARED: of the group; the
+                                 // common tokens are in that user's pages)
   long long begin, end;
   long long index;               // among all items
   Span span;

@@ -219,9 +219,10 @@ class QuantizedCache:
         [count + 1]`` int32, ascending from 0 to all users) are group g; their
         first shared[g] tokens (``shared [count]`` int32) are the same, codes and
         scales, in whichever pages. A user alone is a group of its own, with 0
-        shared tokens if need be. Groups that do not ascend are an error that
-        ``check`` raises (rows are 0); calls with few rows are computed user by
-        user and do not look at them."""
+        shared tokens if need be; one without rows may hold other tokens, or none.
+        Groups that do not ascend are an error that ``check`` raises (rows are
+        0); calls with few rows are computed user by user and do not look at
+        them."""
         tokens, heads, stride, scale = self._queries(q, scale)
         common = self._call(table, lengths, offsets, tokens, max_tokens, TYPES[q.dtype])
         users, count = common[12], shared.shape[0] if shared.ndim == 1 else -1
